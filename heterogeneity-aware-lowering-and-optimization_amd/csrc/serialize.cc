@@ -363,7 +363,11 @@ odla_status deserialize(const uint8_t* data, size_t size, _odla_computation* c) 
   char magic[8];
   r.raw(magic, 8);
   Options& o = c->opts;
-  o.fp16 = r.i64() != 0; o.bf16 = (odla_bf16_mode)r.i64(); o.int8 = r.i64() != 0; o.raw_acc = r.i64() != 0;
+  o.fp16 = r.i64() != 0;
+  const int64_t bf16 = r.i64();
+  if (bf16 < BF16_DISABLE || bf16 > BF16_AUTO_MODE) return ODLA_INVALID_PARAM;   // checked before the number becomes an enumerator
+  o.bf16 = (odla_bf16_mode)bf16;
+  o.int8 = r.i64() != 0; o.raw_acc = r.i64() != 0;
   c->dynamic_batch = r.i64() != 0;
   c->min_batch = (int)r.i64(); c->max_batch = (int)r.i64(); c->opt_batch = (int)r.i64();
   if (!r.ok || c->min_batch < 0 || c->max_batch < 0 || c->opt_batch < 0) return ODLA_INVALID_PARAM;
@@ -392,7 +396,15 @@ odla_status deserialize(const uint8_t* data, size_t size, _odla_computation* c) 
     }
     Shape s;
     s.rank = (int)rank;
-    for (int i = 0; i < s.rank; ++i) s.d[i] = r.i64();
+    int64_t elements = 1;   // (bounded before anything multiplies the extents)
+    for (int i = 0; i < s.rank; ++i) {
+      s.d[i] = r.i64();
+      if (!r.ok || s.d[i] <= 0 || s.d[i] >= (1ll << 40) || elements > (1ll << 48) / s.d[i]) {
+        OHIP_ERR("stored computation rejected: value %lld has extent %lld", (long long)k, (long long)s.d[i]);
+        return ODLA_INVALID_PARAM;
+      }
+      elements *= s.d[i];
+    }
     const std::string name = r.str();
     _odla_value* v = new_value(c, (_odla_value::Kind)kind, (odla_element_type)et, s,
                                name.empty() ? nullptr : reinterpret_cast<odla_value_id>(const_cast<char*>(name.c_str())));
