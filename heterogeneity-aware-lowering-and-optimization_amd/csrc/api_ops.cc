@@ -26,6 +26,10 @@
 //   TOPK       i0 K, i1 largest, i2 axis; out = values, out2 = indices
 //   LRN        i0 layout, i1 window; f0 alpha, f1 beta, f2 bias
 //   ROWNORM    i0 layout; f0 eps, f1 scalar scale, f2 scalar offset; in = {x, scale?, offset?}
+//   BLOCKQUANT in = {x}; out = 8-bit values, out2 = scales
+//   BLOCKGEMM  in = {A, A scale, B, B scale}
+//   EXPERTS    i0 top k, i1 renormalise; f0 scaling; in = {x, router, gate and up, its scale?, down, its scale?}
+//   SAMPLE     in = {logits, temperature?, top k?, top p?, min p?, uniform}
 #include <climits>
 #include <cmath>
 #include <cstring>
@@ -52,6 +56,14 @@ Node* add_node(_odla_computation* c, OpKind op, std::vector<odla_value> in, odla
   for (const odla_value v : in) {
     if (v != nullptr && v->comp != c) {
       OHIP_ERR("odla_%s: operand '%s' belongs to another computation", op_name(op), v->name.c_str());
+      return nullptr;
+    }
+  }
+  if (!op_knows_float8(op)) {
+    bool f8 = et == ODLA_HIP_FLOAT8_E4M3;
+    for (const odla_value v : in) f8 = f8 || (v != nullptr && v->etype == ODLA_HIP_FLOAT8_E4M3);
+    if (f8) {
+      OHIP_ERR("odla_%s does not take 8-bit floating-point values", op_name(op));
       return nullptr;
     }
   }
@@ -344,6 +356,89 @@ odla_value arg_extreme(bool is_max, odla_value input, odla_int32 axis, odla_bool
 }
 
 }  // namespace
+namespace ohip {
+
+// What the operators of a token step demand of their operands, and their result shapes.  Asked by
+// the builders and for every such node of a loaded computation.
+bool token_op_shapes(OpKind op, const std::vector<_odla_value*>& in, const int64_t* attr, Shape* out, Shape* out2, std::string* why) {
+  auto no = [&](const std::string& s) { *why = s; return false; };
+  const Shape& xs = in[0]->shape;
+  const int64_t last = xs.d[xs.rank - 1], rows = xs.numel() / last;
+  auto blocks = [](int64_t n) { return (n + kScaleBlock - 1) / kScaleBlock; };
+  auto shaped = [](const _odla_value* v, std::initializer_list<int64_t> d) {
+    Shape s;
+    for (int64_t e : d) s.d[s.rank++] = e;
+    return v->shape == s;
+  };
+  constexpr int64_t kMost = 1 << 24;   // of one extent that a kernel counts in 32 bits
+  if (last > kMost || rows > 65535 * 128) return no("operand " + xs.str() + " is too large");
+  switch (op) {
+    case OP_BLOCKQUANT:
+      if (!is_float_type(in[0]->etype)) return no("operand must be a float type");
+      *out = *out2 = xs;
+      out2->d[xs.rank - 1] = blocks(last);
+      return true;
+    case OP_BLOCKGEMM: {
+      const _odla_value *as = in[1], *b = in[2], *bs = in[3];
+      if (in[0]->etype != ODLA_HIP_FLOAT8_E4M3 || b->etype != ODLA_HIP_FLOAT8_E4M3) return no("A and B must be ODLA_HIP_FLOAT8_E4M3");
+      if (as->etype != ODLA_FLOAT32 || bs->etype != ODLA_FLOAT32) return no("scales must be FLOAT32");
+      if (b->shape.rank != 2 || b->shape.d[1] != last) return no("B " + b->shape.str() + " must be [N, K] with the K of A " + xs.str());
+      const int64_t N = b->shape.d[0];
+      if (N > kMost) return no("B " + b->shape.str() + " is too large");
+      Shape s = xs;
+      s.d[xs.rank - 1] = blocks(last);
+      if (as->shape != s) return no("scale of A " + as->shape.str() + " must be " + s.str());
+      if (!shaped(bs, {blocks(N), blocks(last)})) return no("scale of B " + bs->shape.str() + " must have one element per block of 128 x 128");
+      *out = xs;
+      out->d[xs.rank - 1] = N;
+      return true;
+    }
+    case OP_EXPERTS: {
+      const _odla_value *r = in[1], *gu = in[2], *gs = in[3], *dn = in[4], *ds = in[5];
+      const int64_t H = last;
+      if (!is_float_type(in[0]->etype) || r->etype != in[0]->etype) return no("input and router must be of one float type");
+      if (r->shape.rank != 2 || r->shape.d[1] != H) return no("router " + r->shape.str() + " must be [E, H] with the H of the input " + xs.str());
+      const int64_t E = r->shape.d[0];
+      if (E > kMaxExperts) return no("more than 1024 experts");
+      if (rows > kMaxExpertTokens) return no("more than 512 tokens");
+      if (attr[0] < 1 || attr[0] > E || attr[0] > kMaxExpertTopK) return no("top_k must be 1 .. min(E, 32)");
+      if (dn->shape.rank != 3) return no("down " + dn->shape.str() + " must be [E, H, I]");
+      const int64_t I = dn->shape.d[2];
+      if (I > kMost / 2) return no("down " + dn->shape.str() + " is too large");
+      if (!shaped(dn, {E, H, I})) return no("down " + dn->shape.str() + " must be [E, H, I]");
+      if (!shaped(gu, {E, 2 * I, H})) return no("gate_up " + gu->shape.str() + " must be [E, 2 I, H]");
+      const bool f8 = gu->etype == ODLA_HIP_FLOAT8_E4M3;
+      if (gu->etype != dn->etype || (!f8 && gu->etype != in[0]->etype)) return no("gate_up and down must both be of the input's type or both ODLA_HIP_FLOAT8_E4M3");
+      if (f8 != (gs != nullptr) || f8 != (ds != nullptr)) return no("scales belong to 8-bit weights, and to both or none");
+      if (f8) {
+        if (gs->etype != ODLA_FLOAT32 || ds->etype != ODLA_FLOAT32) return no("scales must be FLOAT32");
+        if (!shaped(gs, {E, blocks(2 * I), blocks(H)})) return no("scale of gate_up " + gs->shape.str() + " must have one element per block of 128 x 128");
+        if (!shaped(ds, {E, blocks(H), blocks(I)})) return no("scale of down " + ds->shape.str() + " must have one element per block of 128 x 128");
+      }
+      *out = xs;
+      return true;
+    }
+    case OP_SAMPLE: {
+      if (!is_float_type(in[0]->etype)) return no("logits must be a float type");
+      if (last > kMaxVocabulary) return no("more than 524288 logits in a row");
+      for (int k = 1; k < 6; ++k) {
+        if (in[k] == nullptr) continue;
+        static const char* names[] = {"", "temperature", "top_k", "top_p", "min_p", "uniform"};
+        if (in[k]->etype != (k == 2 ? ODLA_INT32 : ODLA_FLOAT32)) return no(std::string(names[k]) + (k == 2 ? " must be INT32" : " must be FLOAT32"));
+        const int64_t n = in[k]->shape.numel();
+        if (n != 1 && n != rows) return no(std::string(names[k]) + " must have one element, or one for every row of the logits " + xs.str());
+      }
+      *out = Shape();
+      for (int d = 0; d + 1 < xs.rank; ++d) out->d[out->rank++] = xs.d[d];
+      if (out->rank == 0) { out->rank = 1; out->d[0] = 1; }
+      return true;
+    }
+    default:
+      return no("not an operator of a token step");
+  }
+}
+
+}  // namespace ohip
 
 extern "C" {
 
@@ -1400,6 +1495,75 @@ odla_value odla_NMS(odla_value boxes, odla_value scores, odla_uint32 max_num_out
   n->i[0] = max_num_outputs;
   n->f[0] = iou_threshold;
   n->f[1] = score_threshold;
+  return n->out;
+}
+
+// ------------------------------------------- operators of a token step --
+odla_values odla_hip_BlockQuantize(odla_value input, const odla_value_ids value_ids) {
+  odla_values r;
+  r.size = 0;
+  _odla_computation* c = input ? comp_of(input) : nullptr;
+  if (c == nullptr) { OHIP_ERR("odla_hip_BlockQuantize: null operand or no current computation"); return r; }
+  Shape o, o2;
+  std::string why;
+  if (!token_op_shapes(OP_BLOCKQUANT, {input}, nullptr, &o, &o2, &why)) {
+    OHIP_ERR("odla_hip_BlockQuantize: %s", why.c_str());
+    return r;
+  }
+  Node* n = add_node(c, OP_BLOCKQUANT, {input}, ODLA_HIP_FLOAT8_E4M3, o, value_ids.size > 0 ? value_ids.value_ids[0] : nullptr);
+  if (n == nullptr) return r;
+  n->out2 = new_value(c, _odla_value::TEMP, ODLA_FLOAT32, o2, value_ids.size > 1 ? value_ids.value_ids[1] : nullptr);
+  n->out2->producer = n->out->producer;
+  r.size = 2;
+  r.values[0] = n->out;
+  r.values[1] = n->out2;
+  return r;
+}
+
+odla_value odla_hip_BlockGemm(odla_value A, odla_value A_scale, odla_value B, odla_value B_scale,
+                              odla_element_type result_type, const odla_value_id id) {
+  REQUIRE(A && A_scale && B && B_scale, "odla_hip_BlockGemm: null operand");
+  _odla_computation* c = comp_of(A);
+  REQUIRE(c, "odla_hip_BlockGemm: no current computation");
+  REQUIRE(is_float_type(result_type), "odla_hip_BlockGemm: the result must be a float type (got %d)", (int)result_type);
+  Shape o;
+  std::string why;
+  REQUIRE(token_op_shapes(OP_BLOCKGEMM, {A, A_scale, B, B_scale}, nullptr, &o, nullptr, &why), "odla_hip_BlockGemm: %s", why.c_str());
+  Node* n = add_node(c, OP_BLOCKGEMM, {A, A_scale, B, B_scale}, result_type, o, id);
+  if (n == nullptr) return ADD_NODE_FAILED;
+  return n->out;
+}
+
+odla_value odla_hip_MixtureOfExperts(odla_value input, odla_value router, odla_value gate_up, odla_value gate_up_scale,
+                                     odla_value down, odla_value down_scale, odla_uint32 top_k, odla_bool renormalize,
+                                     odla_float32 scaling, const odla_value_id id) {
+  REQUIRE(input && router && gate_up && down, "odla_hip_MixtureOfExperts: null operand");
+  _odla_computation* c = comp_of(input);
+  REQUIRE(c, "odla_hip_MixtureOfExperts: no current computation");
+  const int64_t attr[2] = {(int64_t)top_k, renormalize != 0};
+  Shape o;
+  std::string why;
+  const std::vector<_odla_value*> in = {input, router, gate_up, gate_up_scale, down, down_scale};
+  REQUIRE(token_op_shapes(OP_EXPERTS, in, attr, &o, nullptr, &why), "odla_hip_MixtureOfExperts: %s", why.c_str());
+  Node* n = add_node(c, OP_EXPERTS, in, input->etype, o, id);
+  if (n == nullptr) return ADD_NODE_FAILED;
+  n->i[0] = attr[0];
+  n->i[1] = attr[1];
+  n->f[0] = scaling;
+  return n->out;
+}
+
+odla_value odla_hip_Sample(odla_value logits, odla_value temperature, odla_value top_k, odla_value top_p, odla_value min_p,
+                           odla_value uniform, const odla_value_id id) {
+  REQUIRE(logits && uniform, "odla_hip_Sample: null operand");
+  _odla_computation* c = comp_of(logits);
+  REQUIRE(c, "odla_hip_Sample: no current computation");
+  Shape o;
+  std::string why;
+  const std::vector<_odla_value*> in = {logits, temperature, top_k, top_p, min_p, uniform};
+  REQUIRE(token_op_shapes(OP_SAMPLE, in, nullptr, &o, nullptr, &why), "odla_hip_Sample: %s", why.c_str());
+  Node* n = add_node(c, OP_SAMPLE, in, ODLA_INT32, o, id);
+  if (n == nullptr) return ADD_NODE_FAILED;
   return n->out;
 }
 

@@ -47,9 +47,10 @@ const char* op_name(OpKind k) {
   static const char* names[] = {"Conv", "Gemm", "Binary", "Unary", "BatchNorm", "LayerNorm", "Pool",
                                 "Reduce", "Softmax", "Cast", "Concat", "Gather", "Reshape", "Resize",
                                 "Slice", "Transpose", "Quantize", "Dequantize", "NMS", "Elementwise", "ArgExtreme",
-                                "CopyND", "TopK", "LRN", "RowNorm", "PostProcess", "AxisOp"};
-  static_assert(sizeof(names) / sizeof(names[0]) == (size_t)OP_AXISOP + 1, "one name per OpKind");
-  if ((int)k < 0 || (int)k > (int)OP_AXISOP) return "?";
+                                "CopyND", "TopK", "LRN", "RowNorm", "PostProcess", "AxisOp", "BlockQuantize", "BlockGemm",
+                                "MixtureOfExperts", "Sample"};
+  static_assert(sizeof(names) / sizeof(names[0]) == (size_t)kLastOp + 1, "one name per OpKind");
+  if ((int)k < 0 || (int)k > (int)kLastOp) return "?";
   return names[(int)k];
 }
 
@@ -90,7 +91,7 @@ bool shape_valid(const odla_value_shape& s) {
 }
 
 DType dtype_from_odla(odla_element_type t) {
-  switch (t) {
+  switch ((int)t) {   // (ODLA_HIP_FLOAT8_E4M3 is not an enumerator of the reference's type)
     case ODLA_FLOAT32: return DT_F32;
     case ODLA_FLOAT16: return DT_F16;
     case ODLA_BFLOAT16: return DT_BF16;
@@ -99,6 +100,7 @@ DType dtype_from_odla(odla_element_type t) {
     case ODLA_INT32: case ODLA_QINT32: case ODLA_UINT32: return DT_I32;
     case ODLA_INT64: case ODLA_UINT64: return DT_I64;
     case ODLA_BOOL: return DT_BOOL;
+    case ODLA_HIP_FLOAT8_E4M3: return DT_F8;
     default: return DT_INVALID;
   }
 }

@@ -177,6 +177,27 @@ std::unique_ptr<_odla_computation> clone_for_batch(const _odla_computation& c, i
         // (every image owns max_num_outputs rows of the result, and the image numbers written there
         //  start at the executing context's image_base: a half-batch copy gives the whole batch's rows)
         break;
+      case OP_BLOCKQUANT:
+        if (x->shape.rank < 2) rs.reject(n, "runs along the batch");
+        break;
+      case OP_BLOCKGEMM:
+        if (!rs.carry(n.in[0]) || !rs.carry(n.in[1]) || x->shape.rank < 2) rs.reject(n, "has rows or their scales that do not depend on the batch");
+        if (rs.carry(n.in[2]) || rs.carry(n.in[3])) rs.reject(n, "has a right operand that depends on the batch");
+        break;
+      case OP_EXPERTS:
+        if (!rs.carry(x) || x->shape.rank < 2) rs.reject(n, "has tokens that do not depend on the batch");
+        for (size_t k = 1; k < n.in.size(); ++k)
+          if (rs.carry(n.in[k])) rs.reject(n, "has weights that depend on the batch");
+        break;
+      case OP_SAMPLE:
+        if (!rs.carry(x) || x->shape.rank < 2) rs.reject(n, "has logits that do not depend on the batch");
+        // (a parameter follows the batch with its rows, or is a single one for all of them)
+        for (size_t k = 1; k < n.in.size(); ++k) {
+          const _odla_value* v = n.in[k];
+          if (v == nullptr || (!rs.carry(v) && v->shape.numel() == 1)) continue;
+          if (!rs.carry(v)) rs.reject(n, "has one constant parameter per row");
+        }
+        break;
       case OP_UNARY: case OP_POOL: case OP_CAST: case OP_RESHAPE: case OP_RESIZE: case OP_LRN:
         break;
       default:

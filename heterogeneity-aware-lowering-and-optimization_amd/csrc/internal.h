@@ -36,8 +36,15 @@ enum OpKind : int {
   OP_CONV, OP_GEMM, OP_BINARY, OP_UNARY, OP_BATCHNORM, OP_LAYERNORM, OP_POOL, OP_REDUCE,
   OP_SOFTMAX, OP_CAST, OP_CONCAT, OP_GATHER, OP_RESHAPE, OP_RESIZE, OP_SLICE, OP_TRANSPOSE,
   OP_QUANTIZE, OP_DEQUANTIZE, OP_NMS, OP_EWISE, OP_ARGEXT, OP_COPYND, OP_TOPK, OP_LRN, OP_ROWNORM,
-  OP_POSTPROCESS, OP_AXISOP
+  OP_POSTPROCESS, OP_AXISOP, OP_BLOCKQUANT, OP_BLOCKGEMM, OP_EXPERTS, OP_SAMPLE
 };
+constexpr OpKind kLastOp = OP_SAMPLE;
+// Operators that take or give 8-bit floating-point values (ODLA_HIP_FLOAT8_E4M3): those that
+// compute with them and those that move whole elements whatever they stand for.
+inline bool op_knows_float8(OpKind k) {
+  return k == OP_BLOCKQUANT || k == OP_BLOCKGEMM || k == OP_EXPERTS || k == OP_RESHAPE || k == OP_TRANSPOSE ||
+         k == OP_SLICE || k == OP_CONCAT || k == OP_GATHER;
+}
 // sub-kinds of OP_AXISOP (Node::i[0])
 enum AxisOp : int { AX_GATHER_ELEMENTS = 0, AX_CUMSUM, AX_HARDMAX, AX_COMPRESS };
 const char* op_name(OpKind k);
@@ -220,6 +227,10 @@ void profiler_configure(Options* o);
 // Reads the statistics of one finished execution and appends them to the open run.
 odla_status profiler_collect(const Plan& plan, const char* arena);
 const char* api_op_name(const Node& n);
+
+// Shapes of an operator of a token step (OP_BLOCKQUANT .. OP_SAMPLE); false and a reason when its
+// operands do not fit.  `attr` are the node's integer attributes.
+bool token_op_shapes(OpKind op, const std::vector<_odla_value*>& in, const int64_t* attr, Shape* out, Shape* out2, std::string* why);
 
 DType dtype_from_odla(odla_element_type t);
 int odla_type_size(odla_element_type t);

@@ -1,0 +1,246 @@
+// 8-bit floating point with a scale for each block of 128: rows quantised on the way to a product,
+// and the product itself.
+#include "block_common.h"
+
+namespace ohip {
+namespace {
+
+constexpr float kMostE4m3 = 448.f;
+constexpr float kLeastScale = 1.17549435e-38f;   // 2^-126: x / scale stays finite for blocks of subnormals and zeros
+
+// ------------------------------------------------------------- quantisation --
+// scale = max(max |x| / 448, 2^-126), q = e4m3(x / scale).  Bound by memory: es + 1 bytes per value.
+// Sixteen lanes hold a block, eight values each.
+template <typename T, bool VECTOR>
+__global__ void __launch_bounds__(256) block_quantize_kernel(const T* x, uint8_t* q, float* scale, const int64_t rows, const int len, const int blocks) {
+  const int l16 = threadIdx.x & 15;
+  const int64_t total = rows * blocks, per_pass = (int64_t)gridDim.x * 16;
+  // (whole wavefronts walk on together: group_allreduce reads lanes whatever their EXEC bit)
+  for (int64_t base = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 6 << 2); base < total; base += per_pass) {
+    const int64_t unit = base + (threadIdx.x >> 4 & 3);
+    const bool live = unit < total;
+    const int64_t row = live ? unit / blocks : 0;
+    const int b = live ? (int)(unit - row * blocks) : 0;
+    const int n = live ? min(kScaleBlock, len - b * kScaleBlock) : 0;
+    const int64_t at = row * len + (int64_t)b * kScaleBlock;
+    float v[8];
+    if constexpr (VECTOR) {   // len is a multiple of 8: a lane's eight values are all there or none is
+      const bool in = l16 * 8 < n;
+      constexpr int PER = Vec16<T>::N;
+#pragma unroll
+      for (int h = 0; h < 8 / PER; ++h) {
+        Vec16<T> w;
+        if (in) w.load(x + at + l16 * 8 + h * PER);
+        else w.raw = uintx4{0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int e = 0; e < PER; ++e) v[h * PER + e] = w.get(e);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = l16 + 16 * e < n ? Store<T>::ld(x + at + l16 + 16 * e) : 0.f;
+    }
+    float most = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
+    most = group_allreduce<16>(most, [](float a, float c) { return fmaxf(a, c); });
+    const float s = fmaxf(most / kMostE4m3, kLeastScale);
+    int w0 = 0, w1 = 0;
+#if defined(__HIP_DEVICE_COMPILE__)
+    w0 = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] / s, v[1] / s, w0, false);
+    w0 = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] / s, v[3] / s, w0, true);
+    w1 = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] / s, v[5] / s, w1, false);
+    w1 = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] / s, v[7] / s, w1, true);
+#endif
+    if constexpr (VECTOR) {
+      if (l16 * 8 < n) *reinterpret_cast<uintx2*>(q + at + l16 * 8) = uintx2{(unsigned)w0, (unsigned)w1};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (l16 + 16 * e < n) q[at + l16 + 16 * e] = (uint8_t)((unsigned)(e < 4 ? w0 : w1) >> (8 * (e & 3)));
+    }
+    if (live && l16 == 0) scale[unit] = s;
+  }
+}
+
+template <typename T>
+hipError_t quantize_as(const void* x, void* q, float* scale, int64_t rows, int64_t len, hipStream_t stream) {
+  const int blocks = (int)((len + kScaleBlock - 1) / kScaleBlock);
+  const int grid = grid_for(rows * blocks, 16);
+  if (len % 8 == 0)
+    hipLaunchKernelGGL((block_quantize_kernel<T, true>), dim3(grid), dim3(256), 0, stream, (const T*)x, (uint8_t*)q, scale, rows, (int)len, blocks);
+  else
+    hipLaunchKernelGGL((block_quantize_kernel<T, false>), dim3(grid), dim3(256), 0, stream, (const T*)x, (uint8_t*)q, scale, rows, (int)len, blocks);
+  return hipGetLastError();
+}
+
+// ------------------------------------------------------------------ product --
+// Few rows: y^T tile of 16 columns (rows n of B) x 16 MT rows m of A per workgroup.  The weights are
+// read once, straight into the operand registers; the wavefronts of a workgroup take every
+// blockDim / 64-th block of 128 terms and their sums meet in LDS in wavefront order.  A block's sum is
+// scaled on its way into the accumulator: the scale of row m belongs to a lane (column of the matrix
+// result), that of B to the whole tile.
+template <typename TOut, int MT, bool ALIGNED>
+__global__ void __launch_bounds__(512) block_gemm_rows_kernel(const BlockGemmParams p) {
+  __shared__ floatx4 sums[8][MT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int r = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * MT);
+  const int KB = (p.K + kScaleBlock - 1) / kScaleBlock;
+  const unsigned char* brow = p.b + (int64_t)min(n0 + r, p.N - 1) * p.K;
+  const unsigned char* arow[MT];
+  const float* as[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const int64_t m = min(m0 + 16 * t + r, p.M - 1);
+    arow[t] = p.a + m * p.K;
+    as[t] = p.a_scale + m * KB;
+  }
+  const float* bs = p.b_scale + (int64_t)(n0 / kScaleBlock) * KB;
+  floatx4 acc[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+  for (int kb = wave; kb < KB; kb += waves) {
+    const int64_t k = (int64_t)kb * kScaleBlock + g * 32;
+    const uintx4 w0 = load_row16<ALIGNED>(brow, k, p.K), w1 = load_row16<ALIGNED>(brow, k + 16, p.K);
+    const float sb = bs[kb];
+    uintx4 wv[4];
+    bf16_of_e4m3(w0, w1, wv);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const uintx4 x0 = load_row16<ALIGNED>(arow[t], k, p.K), x1 = load_row16<ALIGNED>(arow[t], k + 16, p.K);
+      uintx4 xv[4];
+      bf16_of_e4m3(x0, x1, xv);
+      const floatx4 part = mma_exact(wv, xv);
+      const float s = as[t][kb] * sb;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf(part[i], s, acc[t][i]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t) sums[wave][t][lane] = acc[t];
+  __syncthreads();
+  for (int t = wave; t < MT; t += waves) {
+    floatx4 v = sums[0][t][lane];
+    for (int w = 1; w < waves; ++w) v += sums[w][t][lane];
+    const int m = m0 + 16 * t + r, n = n0 + 4 * g;
+    if (m < p.M && n < p.N) store4((TOut*)p.y + (int64_t)m * p.N + n, v, p.N - n, (p.N & 3) == 0);
+  }
+}
+
+// Many rows: a workgroup of four wavefronts owns 128 columns n x BM rows m; both operands pass
+// through LDS, 128 terms at a time, the next block's in registers meanwhile.
+template <typename TOut, int BM, bool ALIGNED>
+__global__ void __launch_bounds__(256) block_gemm_tile_kernel(const BlockGemmParams p) {
+  constexpr bool EXACT = sizeof(TOut) == 4;
+  constexpr int BN = 128, PITCH = kScaleBlock + 16;   // (16 bytes more: sixteen rows start in different banks)
+  constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16;
+  constexpr int NB = BN * 8 / 256, NA = BM * 8 / 256;  // 16-byte chunks a thread brings of either
+  __shared__ __attribute__((aligned(16))) unsigned char sa[BM * PITCH], sb[BN * PITCH];
+  __shared__ float ss[BM];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int r = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * BN, m0 = blockIdx.y * BM;
+  const int wn = (wave & 1) * WN, wm = (wave >> 1) * WM;
+  const int KB = (p.K + kScaleBlock - 1) / kScaleBlock;
+  floatx4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  uintx4 ra[NA], rb[NB];
+  float rs = 0.f;
+  auto fetch = [&](const int kb) {
+    const int64_t k = (int64_t)kb * kScaleBlock + (tid & 7) * 16;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) ra[i] = load_row16<ALIGNED>(p.a + (int64_t)min(m0 + (tid >> 3) + 32 * i, p.M - 1) * p.K, k, p.K);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) rb[i] = load_row16<ALIGNED>(p.b + (int64_t)min(n0 + (tid >> 3) + 32 * i, p.N - 1) * p.K, k, p.K);
+    if (tid < BM) rs = p.a_scale[(int64_t)min(m0 + tid, p.M - 1) * KB + kb] * p.b_scale[(int64_t)(n0 / kScaleBlock) * KB + kb];
+  };
+  fetch(0);
+  for (int kb = 0; kb < KB; ++kb) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NA; ++i) *reinterpret_cast<uintx4*>(sa + ((tid >> 3) + 32 * i) * PITCH + (tid & 7) * 16) = ra[i];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) *reinterpret_cast<uintx4*>(sb + ((tid >> 3) + 32 * i) * PITCH + (tid & 7) * 16) = rb[i];
+    if (tid < BM) ss[tid] = rs;
+    __syncthreads();
+    if (kb + 1 < KB) fetch(kb + 1);
+    uintx4 w0[TN], w1[TN], wv[EXACT ? TN : 1][4];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const unsigned char* at = sb + (wn + 16 * j + r) * PITCH + g * 32;
+      w0[j] = *reinterpret_cast<const uintx4*>(at);
+      w1[j] = *reinterpret_cast<const uintx4*>(at + 16);
+      if constexpr (EXACT) bf16_of_e4m3(w0[j], w1[j], wv[j]);
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const unsigned char* at = sa + (wm + 16 * i + r) * PITCH + g * 32;
+      const uintx4 x0 = *reinterpret_cast<const uintx4*>(at), x1 = *reinterpret_cast<const uintx4*>(at + 16);
+      const float s = ss[wm + 16 * i + r];
+      uintx4 xv[4];
+      if constexpr (EXACT) bf16_of_e4m3(x0, x1, xv);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        floatx4 part;
+        if constexpr (EXACT) part = mma_exact(wv[j], xv);
+        else part = mma_e4m3(w0[j], w1[j], x0, x1, floatx4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(part[e], s, acc[i][j][e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int m = m0 + wm + 16 * i + r, n = n0 + wn + 16 * j + 4 * g;
+      if (m < p.M && n < p.N) store4((TOut*)p.y + (int64_t)m * p.N + n, acc[i][j], p.N - n, (p.N & 3) == 0);
+    }
+}
+
+template <typename TOut, int MT, bool ALIGNED>
+hipError_t gemm_rows(const BlockGemmParams& p, hipStream_t stream) {
+  const int KB = (p.K + kScaleBlock - 1) / kScaleBlock;
+  const int waves = KB < 8 ? KB : 8;
+  hipLaunchKernelGGL((block_gemm_rows_kernel<TOut, MT, ALIGNED>), dim3((p.N + 15) / 16, (p.M + 16 * MT - 1) / (16 * MT)), dim3(64 * waves), 0, stream, p);
+  return hipGetLastError();
+}
+template <typename TOut, bool ALIGNED>
+hipError_t gemm_as(const BlockGemmParams& p, hipStream_t stream) {
+  if (p.M <= 16) return gemm_rows<TOut, 1, ALIGNED>(p, stream);
+  if (p.M <= 32) return gemm_rows<TOut, 2, ALIGNED>(p, stream);
+  if (p.M <= 64) return gemm_rows<TOut, 4, ALIGNED>(p, stream);
+  hipLaunchKernelGGL((block_gemm_tile_kernel<TOut, 128, ALIGNED>), dim3((p.N + 127) / 128, (p.M + 127) / 128), dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_block_quantize(const void* x, DType dt, void* q, float* scale, int64_t rows, int64_t len, hipStream_t stream) {
+  if (x == nullptr || q == nullptr || scale == nullptr || rows < 1 || len < 1 || len > (1 << 24)) return hipErrorInvalidValue;
+  switch (dt) {
+    case DT_F32: return quantize_as<float>(x, q, scale, rows, len, stream);
+    case DT_F16: return quantize_as<f16_t>(x, q, scale, rows, len, stream);
+    case DT_BF16: return quantize_as<bf16_t>(x, q, scale, rows, len, stream);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+hipError_t launch_block_gemm(const BlockGemmParams& p, hipStream_t stream) {
+  if (p.a == nullptr || p.b == nullptr || p.a_scale == nullptr || p.b_scale == nullptr || p.y == nullptr) return hipErrorInvalidValue;
+  if (p.M < 1 || p.N < 1 || p.K < 1 || p.N > (1 << 24) || p.K > (1 << 24)) return hipErrorInvalidValue;
+  if (p.M > 65535 * 128) return hipErrorInvalidValue;   // (rows of tiles in one launch)
+  const bool aligned = p.K % 16 == 0;
+  switch (p.out_dt) {
+    case DT_F32: return aligned ? gemm_as<float, true>(p, stream) : gemm_as<float, false>(p, stream);
+    case DT_F16: return aligned ? gemm_as<f16_t, true>(p, stream) : gemm_as<f16_t, false>(p, stream);
+    case DT_BF16: return aligned ? gemm_as<bf16_t, true>(p, stream) : gemm_as<bf16_t, false>(p, stream);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+}  // namespace ohip

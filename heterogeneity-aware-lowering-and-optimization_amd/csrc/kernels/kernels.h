@@ -30,6 +30,7 @@ enum DType : int {
   DT_I32 = 5,
   DT_I64 = 6,
   DT_BOOL = 7,
+  DT_F8 = 8,  // e4m3: 4 exponent bits (bias 7), 3 mantissa bits, no infinity
   DT_INVALID = -1
 };
 
@@ -37,7 +38,7 @@ inline int dtype_size(DType t) {
   switch (t) {
     case DT_F32: case DT_I32: return 4;
     case DT_F16: case DT_BF16: return 2;
-    case DT_I8: case DT_U8: case DT_BOOL: return 1;
+    case DT_I8: case DT_U8: case DT_BOOL: case DT_F8: return 1;
     case DT_I64: return 8;
     default: return 0;
   }
@@ -700,6 +701,60 @@ hipError_t launch_yolo_postprocess(const float* const heads[3], const int dims[3
                                    const int anchors[3][6], const int* img_w, const int* img_h, float iou_thr,
                                    float score_thr, int capacity, float* boxes, float* scores, float* info,
                                    int* num, hipStream_t stream);
+
+// ---------------------------------------------------------------------------
+// Operators of a language model's token step.
+
+// Values that share a scale: 128 of a row, 128 x 128 of a weight matrix.
+constexpr int kScaleBlock = 128;
+
+// q[r][i] = e4m3(x[r][i] / scale[r][i / 128]), scale = max(max |x| / 448, 2^-126) of the block.
+// Reads and writes exactly the elements; bases aligned to 16 bytes.
+hipError_t launch_block_quantize(const void* x, DType dt, void* q, float* scale, int64_t rows, int64_t len, hipStream_t stream);
+
+// y[m][n] = sum over blocks b of 128 k: a_scale[m][b] * b_scale[n / 128][b] * sum a[m][k] b[n][k],
+// a and b in e4m3.  Reads and writes exactly the elements; bases aligned to 16 bytes.
+struct BlockGemmParams {
+  const uint8_t* a = nullptr; const float* a_scale = nullptr;
+  const uint8_t* b = nullptr; const float* b_scale = nullptr;
+  void* y = nullptr;
+  int M = 0, N = 0, K = 0;
+  DType out_dt = DT_F32;
+};
+hipError_t launch_block_gemm(const BlockGemmParams& p, hipStream_t stream);
+
+// A layer of experts for few tokens, in the order of the three launches.
+constexpr int kMaxExperts = 1024, kMaxExpertTokens = 512, kMaxExpertTopK = 32;
+struct ExpertsParams {
+  const void* x = nullptr; const void* router = nullptr;
+  const void* gate_up = nullptr; const float* gate_up_scale = nullptr;   // scales: 8-bit weights only
+  const void* down = nullptr; const float* down_scale = nullptr;
+  void* y = nullptr;
+  void* route = nullptr; void* hidden = nullptr; void* parts = nullptr;  // work space, see experts_space
+  int tokens = 0, E = 0, H = 0, I = 0, top_k = 0;
+  bool renormalize = false;
+  float scaling = 1.f;
+  DType dt = DT_F32, w_dt = DT_F32;
+};
+struct ExpertsSpace { size_t route, hidden, parts; };   // bytes
+ExpertsSpace experts_space(const ExpertsParams& p);
+hipError_t launch_experts_route(const ExpertsParams& p, hipStream_t stream);     // which experts, with which weight
+hipError_t launch_experts_gate_up(const ExpertsParams& p, hipStream_t stream);   // hidden = silu(gate x) * (up x)
+hipError_t launch_experts_down(const ExpertsParams& p, hipStream_t stream);      // y = sum of weight * down hidden
+
+// The next token of each row of logits (see odla_hip_Sample).  step_*: 1 where a parameter has one
+// element per row, 0 where a single one serves all rows; null parameters are off.
+constexpr int kMaxVocabulary = 1 << 19;
+struct SampleParams {
+  const void* logits = nullptr;
+  const float* temperature = nullptr; const int32_t* top_k = nullptr;
+  const float* top_p = nullptr; const float* min_p = nullptr; const float* uniform = nullptr;
+  int32_t* token = nullptr;
+  int rows = 0, V = 0;
+  int step_t = 0, step_k = 0, step_p = 0, step_m = 0, step_u = 0;
+  DType dt = DT_F32;
+};
+hipError_t launch_sample(const SampleParams& p, hipStream_t stream);
 
 }  // namespace ohip
 #endif

@@ -761,6 +761,12 @@ class Planner {
   void lower_argext(int ni);
   void lower_copynd(int ni);
   void lower_topk(int ni);
+  int get_fp32(const _odla_value* v);
+  void lower_blockquant(int ni);
+  void lower_blockgemm(int ni);
+  void lower_experts(int ni);
+  void lower_sample(int ni);
+  std::unordered_map<const _odla_value*, int> fp32_consts_;   // constants that get_fp32 keeps beside the stored form
   void lower_lrn(int ni);
   void lower_rownorm(int ni);
   void lower_postprocess(int ni);
@@ -994,6 +1000,8 @@ void Planner::run() {
         LayoutParams p = lp; p.src = a(e); p.dst = b(e);
         return launch_nhwc_to_nchw(p, st);
       }, kWrites16);
+    } else if (ov->producer >= 0 && comp_->nodes[ov->producer].op == OP_BLOCKQUANT) {
+      t = os.main;   // (scales are fp32 whatever the mode stores)
     } else {
       t = get(ov, L_ROWMAJOR, FORM_FLOAT);
     }
@@ -1130,6 +1138,10 @@ void Planner::lower(int ni) {
     case OP_ROWNORM: lower_rownorm(ni); break;
     case OP_POSTPROCESS: lower_postprocess(ni); break;
     case OP_AXISOP: lower_axisop(ni); break;
+    case OP_BLOCKQUANT: lower_blockquant(ni); break;
+    case OP_BLOCKGEMM: lower_blockgemm(ni); break;
+    case OP_EXPERTS: lower_experts(ni); break;
+    case OP_SAMPLE: lower_sample(ni); break;
   }
 }
 
@@ -4585,6 +4597,142 @@ void Planner::lower_copynd(int ni) {
 }
 
 // ---------------------------------------------------------------- TopK ----
+// `v` as a row-major fp32 tensor, whatever the precision mode stores: scales and sampling parameters
+// keep the bits they were bound, recorded or computed with.
+int Planner::get_fp32(const _odla_value* v) {
+  if (v->kind == _odla_value::CONSTANT && storage_dtype(v) != DT_F32) {
+    auto it = fp32_consts_.find(v);
+    if (it == fp32_consts_.end()) it = fp32_consts_.emplace(v, const_from_host(DT_F32, v->shape, v->host_data, nullptr)).first;
+    return it->second;
+  }
+  VState& s = vs_[v->index];
+  if (s.main < 0 && !settle(v)) materialize_source(v);
+  if (s.main >= 0 && T(s.main).dt == DT_F32 && T(s.main).layout == L_ROWMAJOR && !T(s.main).quant) return s.main;
+  const int t = get(v, L_ROWMAJOR, FORM_FLOAT);
+  if (T(t).dt == DT_F32) return t;
+  const int dst = new_tensor(DT_F32, L_ROWMAJOR, v->shape, 0, SP_ARENA);
+  const DType sdt = T(t).dt;
+  const int64_t n = v->shape.numel();
+  const Ref a = ref(t), b = ref(dst);
+  emit("cast:" + v->name, {t}, {dst}, [=](const ExecEnv& e, hipStream_t st) { return launch_cast(a(e), sdt, b(e), DT_F32, n, st); });
+  return dst;
+}
+
+void Planner::lower_blockquant(int ni) {
+  Node& n = comp_->nodes[ni];
+  const _odla_value* x = n.in[0];
+  const int tx = get(x, L_ROWMAJOR, FORM_FLOAT);
+  const DType dt = T(tx).dt;
+  const int64_t len = x->shape.d[x->shape.rank - 1], rows = x->shape.numel() / len;
+  const int tq = new_tensor(DT_F8, L_ROWMAJOR, n.out->shape, 0, SP_ARENA);
+  const int ts = new_tensor(DT_F32, L_ROWMAJOR, n.out2->shape, 0, SP_ARENA);
+  const Ref a = ref(tx), q = ref(tq), s = ref(ts);
+  emit("blockquant:" + n.out->name, {tx}, {tq, ts}, [=](const ExecEnv& e, hipStream_t st) {
+    return launch_block_quantize(a(e), dt, q(e), (float*)s(e), rows, len, st);
+  }, kReads16 | kWrites16);
+  set_main(n.out, tq);
+  // (where the mode stores FLOAT32 values in 16 bits, other readers than get_fp32 convert)
+  if (storage_dtype(n.out2) == DT_F32) set_main(n.out2, ts);
+  else vs_[n.out2->index].main = ts;
+}
+
+void Planner::lower_blockgemm(int ni) {
+  Node& n = comp_->nodes[ni];
+  const _odla_value *A = n.in[0], *B = n.in[2];
+  const int ta = get(A, L_ROWMAJOR, FORM_FLOAT), tb = get(B, L_ROWMAJOR, FORM_FLOAT);
+  const int tas = get_fp32(n.in[1]), tbs = get_fp32(n.in[3]);
+  const int ty = new_tensor(storage_dtype(n.out), L_ROWMAJOR, n.out->shape, 0, SP_ARENA);
+  BlockGemmParams bp;
+  bp.K = (int)A->shape.d[A->shape.rank - 1];
+  bp.M = (int)(A->shape.numel() / bp.K);
+  bp.N = (int)B->shape.d[0];
+  bp.out_dt = T(ty).dt;
+  const Ref a = ref(ta), as = ref(tas), b = ref(tb), bs = ref(tbs), y = ref(ty);
+  emit("blockgemm:" + n.out->name, {ta, tas, tb, tbs}, {ty}, [=](const ExecEnv& e, hipStream_t st) {
+    BlockGemmParams p = bp;
+    p.a = (const uint8_t*)a(e); p.a_scale = (const float*)as(e);
+    p.b = (const uint8_t*)b(e); p.b_scale = (const float*)bs(e);
+    p.y = y(e);
+    return launch_block_gemm(p, st);
+  }, kReads16 | kWrites16);
+  set_main(n.out, ty);
+}
+
+void Planner::lower_experts(int ni) {
+  Node& n = comp_->nodes[ni];
+  const _odla_value* x = n.in[0];
+  const int tx = get(x, L_ROWMAJOR, FORM_FLOAT), tr = get(n.in[1], L_ROWMAJOR, FORM_FLOAT);
+  const int tg = get(n.in[2], L_ROWMAJOR, FORM_FLOAT), td = get(n.in[4], L_ROWMAJOR, FORM_FLOAT);
+  const bool scaled = n.in[3] != nullptr;
+  const int tgs = scaled ? get_fp32(n.in[3]) : -1, tds = scaled ? get_fp32(n.in[5]) : -1;
+  ExpertsParams ep;
+  ep.H = (int)x->shape.d[x->shape.rank - 1];
+  ep.tokens = (int)(x->shape.numel() / ep.H);
+  ep.E = (int)n.in[1]->shape.d[0];
+  ep.I = (int)n.in[4]->shape.d[2];
+  ep.top_k = (int)n.i[0];
+  ep.renormalize = n.i[1] != 0;
+  ep.scaling = n.f[0];
+  ep.dt = T(tx).dt;
+  ep.w_dt = T(tg).dt;
+  if (T(tr).dt != ep.dt || T(td).dt != ep.w_dt || (!scaled && ep.w_dt != ep.dt))
+    fail(ODLA_UNSUPPORTED_DATATYPE, "odla_hip_MixtureOfExperts '%s': operands are stored in different types", n.out->name.c_str());
+  const ExpertsSpace need = experts_space(ep);
+  const int tl = raw_buffer(need.route, SP_ARENA), th = raw_buffer(need.hidden, SP_ARENA), tp = raw_buffer(need.parts, SP_ARENA);
+  const int ty = new_tensor(ep.dt, L_ROWMAJOR, n.out->shape, 0, SP_ARENA);
+  const Ref rx = ref(tx), rr = ref(tr), rg = ref(tg), rd = ref(td), rgs = ref(scaled ? tgs : tx), rds = ref(scaled ? tds : tx);
+  const Ref rl = ref(tl), rh = ref(th), rp = ref(tp), ry = ref(ty);
+  auto args = [=](const ExecEnv& e) {
+    ExpertsParams p = ep;
+    p.x = rx(e); p.router = rr(e); p.gate_up = rg(e); p.down = rd(e); p.y = ry(e);
+    if (scaled) { p.gate_up_scale = (const float*)rgs(e); p.down_scale = (const float*)rds(e); }
+    p.route = rl(e); p.hidden = rh(e); p.parts = rp(e);
+    return p;
+  };
+  const std::string& name = n.out->name;
+  emit("experts.route:" + name, {tx, tr}, {tl}, [=](const ExecEnv& e, hipStream_t st) { return launch_experts_route(args(e), st); }, kReads16);
+  emit("experts.gate_up:" + name, {tx, tg, tgs, tl}, {th}, [=](const ExecEnv& e, hipStream_t st) { return launch_experts_gate_up(args(e), st); }, kReads16);
+  emit("experts.down:" + name, {td, tds, tl, th}, {tp, ty}, [=](const ExecEnv& e, hipStream_t st) { return launch_experts_down(args(e), st); }, kReads16 | kWrites16);
+  set_main(n.out, ty);
+}
+
+void Planner::lower_sample(int ni) {
+  Node& n = comp_->nodes[ni];
+  const _odla_value* x = n.in[0];
+  const int tx = get(x, L_ROWMAJOR, FORM_FLOAT);
+  SampleParams sp;
+  sp.V = (int)x->shape.d[x->shape.rank - 1];
+  sp.rows = (int)(x->shape.numel() / sp.V);
+  sp.dt = T(tx).dt;
+  int t[6];
+  bool each[6];   // one element per row
+  std::vector<int> reads = {tx};
+  for (int k = 1; k < 6; ++k) {
+    const _odla_value* v = n.in[k];
+    t[k] = v == nullptr ? -1 : k == 2 ? get(v, L_ROWMAJOR, FORM_FLOAT) : get_fp32(v);
+    each[k] = v != nullptr && v->shape.numel() > 1;
+    if (t[k] >= 0) reads.push_back(t[k]);
+  }
+  const int ty = new_tensor(DT_I32, L_ROWMAJOR, n.out->shape, 0, SP_ARENA);
+  const Ref a = ref(tx), y = ref(ty);
+  auto param = [&](int k) { return t[k] >= 0 ? ref(t[k]) : ref(tx); };
+  const Ref r1 = param(1), r2 = param(2), r3 = param(3), r4 = param(4), r5 = param(5);
+  const bool h1 = t[1] >= 0, h2 = t[2] >= 0, h3 = t[3] >= 0, h4 = t[4] >= 0;
+  sp.step_t = each[1]; sp.step_k = each[2]; sp.step_p = each[3]; sp.step_m = each[4]; sp.step_u = each[5];
+  emit_lists("sample:" + n.out->name, reads, {ty}, [=](const ExecEnv& e, hipStream_t st) {
+    SampleParams p = sp;
+    p.logits = a(e);
+    p.temperature = h1 ? (const float*)r1(e) : nullptr;
+    p.top_k = h2 ? (const int32_t*)r2(e) : nullptr;
+    p.top_p = h3 ? (const float*)r3(e) : nullptr;
+    p.min_p = h4 ? (const float*)r4(e) : nullptr;
+    p.uniform = (const float*)r5(e);
+    p.token = (int32_t*)y(e);
+    return launch_sample(p, st);
+  }, kReads16 | kWrites16);
+  set_main(n.out, ty);
+}
+
 void Planner::lower_topk(int ni) {
   Node& n = comp_->nodes[ni];
   const _odla_value* x = n.in[0];

@@ -156,6 +156,10 @@ const char* api_op_name(const Node& n) {
     case OP_LRN: return "odla_LRN";
     case OP_ROWNORM: return "odla_InstanceNormalization";
     case OP_POSTPROCESS: return "odla_PostProcess";
+    case OP_BLOCKQUANT: return "odla_hip_BlockQuantize";
+    case OP_BLOCKGEMM: return "odla_hip_BlockGemm";
+    case OP_EXPERTS: return "odla_hip_MixtureOfExperts";
+    case OP_SAMPLE: return "odla_hip_Sample";
     case OP_AXISOP:
       switch ((AxisOp)n.i[0]) {
         case AX_GATHER_ELEMENTS: return "odla_GatherElements";

@@ -157,6 +157,10 @@ bool op_rule(OpKind op, OpRule* r) {
     case OP_ROWNORM: *r = {3, 3, 0x1, false}; return true;
     case OP_POSTPROCESS: *r = {5, 5, 0x1f, true}; return true;
     case OP_AXISOP: *r = {1, 2, ~0u, false}; return true;
+    case OP_BLOCKQUANT: *r = {1, 1, 0x1, true}; return true;
+    case OP_BLOCKGEMM: *r = {4, 4, ~0u, false}; return true;
+    case OP_EXPERTS: *r = {6, 6, 0x17, false}; return true;
+    case OP_SAMPLE: *r = {6, 6, 0x21, false}; return true;
   }
   return false;
 }
@@ -214,6 +218,17 @@ odla_status validate_loaded(const _odla_computation* c) {
     const _odla_value* x = n.in[0];
     const int xr = x->shape.rank, orank = n.out->shape.rank;
     const size_t niv = n.iv.size();
+    if (!op_knows_float8(n.op)) {
+      for (const _odla_value* v : n.in)
+        LOADED_REQUIRE(v == nullptr || v->etype != ODLA_HIP_FLOAT8_E4M3, "%s node %lld has an 8-bit floating-point operand", name, (long long)k);
+      LOADED_REQUIRE(n.out->etype != ODLA_HIP_FLOAT8_E4M3, "%s node %lld has an 8-bit floating-point result", name, (long long)k);
+    } else if (n.op == OP_RESHAPE || n.op == OP_TRANSPOSE || n.op == OP_SLICE || n.op == OP_CONCAT || n.op == OP_GATHER) {
+      // (these move elements as they are: an 8-bit result has 8-bit sources and the other way round)
+      const size_t moved = n.op == OP_CONCAT ? n.in.size() : 1;
+      for (size_t i = 0; i < moved; ++i)
+        LOADED_REQUIRE((n.in[i]->etype == ODLA_HIP_FLOAT8_E4M3) == (n.out->etype == ODLA_HIP_FLOAT8_E4M3),
+                       "%s node %lld changes the element type", name, (long long)k);
+    }
     switch (n.op) {
       case OP_CONV:
         LOADED_REQUIRE(xr == 4 && n.in[1]->shape.rank == 4 && orank == 4, "Conv node %lld: operands must have rank 4", (long long)k);
@@ -336,6 +351,17 @@ odla_status validate_loaded(const _odla_computation* c) {
         }
         break;
       }
+      case OP_BLOCKQUANT: case OP_BLOCKGEMM: case OP_EXPERTS: case OP_SAMPLE: {
+        Shape o, o2;
+        std::string why;
+        LOADED_REQUIRE(token_op_shapes(n.op, n.in, n.i, &o, &o2, &why), "%s node %lld: %s", name, (long long)k, why.c_str());
+        const odla_element_type ot = n.op == OP_BLOCKQUANT ? ODLA_HIP_FLOAT8_E4M3 : n.op == OP_EXPERTS ? x->etype
+                                   : n.op == OP_SAMPLE ? ODLA_INT32 : n.out->etype;
+        const bool of = n.out->etype == ODLA_FLOAT32 || n.out->etype == ODLA_FLOAT16 || n.out->etype == ODLA_BFLOAT16;
+        LOADED_REQUIRE(n.out->shape == o && n.out->etype == ot && (n.op != OP_BLOCKGEMM || of), "%s node %lld: malformed result", name, (long long)k);
+        LOADED_REQUIRE(n.op != OP_BLOCKQUANT || (n.out2->shape == o2 && n.out2->etype == ODLA_FLOAT32), "%s node %lld: malformed scales", name, (long long)k);
+        break;
+      }
       case OP_TOPK:
         LOADED_REQUIRE(n.i[2] >= 0 && n.i[2] < xr && n.i[0] >= 1 && n.i[0] <= x->shape.d[n.i[2]], "TopK node %lld: bad axis or K", (long long)k);
         break;
@@ -390,7 +416,7 @@ odla_status deserialize(const uint8_t* data, size_t size, _odla_computation* c) 
   for (int64_t k = 0; k < nv; ++k) {
     const int64_t kind = r.i64(), et = r.i64(), rank = r.i64();
     if (!r.ok || rank < 0 || rank > ODLA_MAX_DIMENSION || kind < 0 || kind > 2) return ODLA_INVALID_PARAM;
-    if (et < 0 || et > (int64_t)ODLA_STRING) {   // checked before the number becomes an enumerator
+    if (et < 0 || (et > (int64_t)ODLA_STRING && et != (int64_t)ODLA_HIP_FLOAT8_E4M3)) {   // checked before the number becomes an enumerator
       OHIP_ERR("stored computation rejected: value %lld has element type %lld", (long long)k, (long long)et);
       return ODLA_INVALID_PARAM;
     }
@@ -439,7 +465,7 @@ odla_status deserialize(const uint8_t* data, size_t size, _odla_computation* c) 
   for (int64_t k = 0; k < nn; ++k) {
     Node n;
     const int64_t op = r.i64();
-    if (op < 0 || op > (int64_t)OP_AXISOP) return ODLA_INVALID_PARAM;
+    if (op < 0 || op > (int64_t)kLastOp) return ODLA_INVALID_PARAM;
     n.op = (OpKind)op;
     const int64_t nin = r.i64();
     if (!r.ok || nin < 0 || nin > ODLA_MAX_OUTPUTS) return ODLA_INVALID_PARAM;

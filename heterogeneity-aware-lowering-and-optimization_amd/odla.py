@@ -24,6 +24,7 @@ LIB_PATH = os.environ.get("ODLA_HIP_LIBRARY") or os.path.join(_HERE, "libodla_hi
 (ODLA_INT8, ODLA_INT16, ODLA_INT32, ODLA_INT64, ODLA_UINT8, ODLA_UINT16, ODLA_UINT32, ODLA_UINT64,
  ODLA_QINT8, ODLA_QINT16, ODLA_QINT32, ODLA_QINT64, ODLA_QUINT8, ODLA_QUINT16, ODLA_QUINT32,
  ODLA_QUINT64, ODLA_FLOAT16, ODLA_BFLOAT16, ODLA_FLOAT32, ODLA_FLOAT64, ODLA_BOOL, ODLA_STRING) = range(22)
+ODLA_HIP_FLOAT8_E4M3 = 31
 ODLA_SUCCESS = 0
 ODLA_INVALID_PARAM = 3
 ODLA_COMPUTE_INFERENCE = 1
@@ -51,6 +52,32 @@ _NP_TO_ODLA = {
     np.dtype(np.uint32): ODLA_UINT32, np.dtype(np.uint64): ODLA_UINT64,
 }
 _ODLA_TO_NP = {v: k for k, v in _NP_TO_ODLA.items()}
+
+
+class ElementType:
+    """An element type that numpy lacks: arrays hold the bit patterns in `storage`."""
+
+    def __init__(self, name, odla_type, storage):
+        self.name, self.odla_type, self.storage = name, odla_type, np.dtype(storage)
+
+    def __repr__(self):
+        return self.name
+
+
+BFLOAT16 = ElementType("BFLOAT16", ODLA_BFLOAT16, np.uint16)
+FLOAT8_E4M3 = ElementType("FLOAT8_E4M3", ODLA_HIP_FLOAT8_E4M3, np.uint8)
+for _t in (BFLOAT16, FLOAT8_E4M3):
+    _ODLA_TO_NP[_t.odla_type] = _t.storage
+
+
+def element_type(dtype):
+    """odla_element_type of a numpy type or an ElementType."""
+    return dtype.odla_type if isinstance(dtype, ElementType) else _NP_TO_ODLA[np.dtype(dtype)]
+
+
+def storage_type(dtype):
+    """The numpy type that holds elements of `dtype`."""
+    return dtype.storage if isinstance(dtype, ElementType) else np.dtype(dtype)
 
 
 class ValueShape(ctypes.Structure):
@@ -118,7 +145,7 @@ def undefined_shape():
 
 def make_type(np_dtype, dims):
     t = ValueType()
-    t.element_type = _NP_TO_ODLA[np.dtype(np_dtype)]
+    t.element_type = element_type(np_dtype)
     t.shape = make_shape(dims)
     return t
 
@@ -271,6 +298,10 @@ def load_library(path=None):
     proto("odla_LRN", vp, [vp, i32, i32, f32, f32, f32, cid])
     proto("odla_InstanceNormalization", vp, [vp, i32, f32, vp, vp, f32, f32, cid])
     proto("odla_DeConv", vp, [vp, i32, u32, vp, i32, pu32, pu32, pu32, pu32, vp, S, cid])
+    proto("odla_hip_BlockQuantize", Values, [vp, ValueIds])
+    proto("odla_hip_BlockGemm", vp, [vp, vp, vp, vp, i32, cid])
+    proto("odla_hip_MixtureOfExperts", vp, [vp, vp, vp, vp, vp, vp, u32, u32, f32, cid])
+    proto("odla_hip_Sample", vp, [vp, vp, vp, vp, vp, vp, cid])
     if path == LIB_PATH:
         _lib = L
     return L
@@ -366,14 +397,15 @@ class HipBuilder:
         h = self._ret(self.L.odla_CreateArgument(make_type(dtype, shape), _cid(name)), "odla_CreateArgument")
         if shape and shape[0] < 0:          # the dynamic batch: recorded at the largest one
             shape = (self.max_batch,) + tuple(shape[1:])
-        self.args[name] = (h, tuple(shape), np.dtype(dtype))
+        self.args[name] = (h, tuple(shape), storage_type(dtype))
         return h
 
-    def const(self, name, array):
-        a = np.ascontiguousarray(array)
+    def const(self, name, array, dtype=None):
+        """dtype: the ElementType whose bit patterns `array` holds (default: the array's own type)."""
+        a = np.ascontiguousarray(array, None if dtype is None else storage_type(dtype))
         self._keep.append(a)
         shape = a.shape if a.ndim > 0 else ()
-        return self._ret(self.L.odla_CreateConstant(make_type(a.dtype, shape), a.ctypes.data_as(ctypes.c_void_p),
+        return self._ret(self.L.odla_CreateConstant(make_type(a.dtype if dtype is None else dtype, shape), a.ctypes.data_as(ctypes.c_void_p),
                                                     _cid(name)), "odla_CreateConstant")
 
     def output(self, v, name):
@@ -665,6 +697,29 @@ class HipBuilder:
             od = make_shape([s[0], ws[1] * group, out_hw[0], out_hw[1]])
         return self._ret(self.L.odla_DeConv(x, ODLA_CHANNELS_FIRST, group, w, ODLA_IOS, _u32(stride), _u32((1, 1)),
                                             _u32(pad[:2]), _u32(pad[2:]), bias, od, _cid(name)), "odla_DeConv")
+
+    # -- operators of a token step --
+    def block_quantize(self, x, names=(None, None)):
+        """-> (8-bit values, scale of each block of 128 of a row)."""
+        ids = ValueIds()
+        ids.size = 2
+        for i, n in enumerate(names):
+            ids.value_ids[i] = _cid(n)
+        r = self.L.odla_hip_BlockQuantize(x, ids)
+        if r.size != 2:
+            raise OdlaError("odla_hip_BlockQuantize failed (see the library log)")
+        return r.values[0], r.values[1]
+
+    def block_gemm(self, a, a_scale, b, b_scale, dtype=np.float32, name=None):
+        return self._ret(self.L.odla_hip_BlockGemm(a, a_scale, b, b_scale, element_type(dtype), _cid(name)), "odla_hip_BlockGemm")
+
+    def mixture_of_experts(self, x, router, gate_up, down, top_k, gate_up_scale=None, down_scale=None, renormalize=True,
+                           scaling=1.0, name=None):
+        return self._ret(self.L.odla_hip_MixtureOfExperts(x, router, gate_up, gate_up_scale, down, down_scale, int(top_k),
+                                                          int(renormalize), scaling, _cid(name)), "odla_hip_MixtureOfExperts")
+
+    def sample(self, logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, name=None):
+        return self._ret(self.L.odla_hip_Sample(logits, temperature, top_k, top_p, min_p, uniform, _cid(name)), "odla_hip_Sample")
 
     # -- execution --
     def session(self, use_graph=True):

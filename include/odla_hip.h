@@ -59,6 +59,15 @@ typedef enum {
   ODLA_BOOL, ODLA_STRING
 } odla_element_type;
 
+/* Library-private element type (no counterpart in the reference): 8-bit floating
+ * point with 4 exponent bits (bias 7) and 3 mantissa bits, one byte per element.
+ * No infinity; 0x7f / 0xff are NaN, the largest magnitude is 448, the smallest
+ * 2^-9.  Values of this type are arguments, constants and results of
+ * odla_hip_BlockQuantize; odla_hip_BlockGemm and odla_hip_MixtureOfExperts
+ * compute with them, odla_Reshape, odla_Squeeze, odla_Transpose, odla_Slice,
+ * odla_Concat and odla_Gather move them.  Every other operator refuses them. */
+#define ODLA_HIP_FLOAT8_E4M3 ((odla_element_type)31)
+
 /* Status codes.                           [ref: ODLA/include/ODLA/odla_common.h:140-165] */
 typedef enum {
   ODLA_SUCCESS,
@@ -813,6 +822,74 @@ odla_value odla_DeConv(odla_value input, odla_memory_layout input_layout,
                        const odla_uint32* paddings_back, odla_value bias,
                        odla_value_shape output_dims,
                        const odla_value_id value_id);
+
+/* ------------------------------------------------------------------------ */
+/* Operators of a language model's token step (no counterparts in the         */
+/* reference).                                                                */
+/* ------------------------------------------------------------------------ */
+/* Rows of 8-bit floating-point values with a scale for each block of 128.
+ * `input` is a float value [.., K]; values[0] is ODLA_HIP_FLOAT8_E4M3 of its
+ * shape, values[1] FLOAT32 [.., ceil(K / 128)] (the last block of a row may be
+ * short).  For every block, in 32 bits,
+ *   scale = max(max |x| / 448, 2^-126),   q = x / scale to nearest, ties to even.
+ * A NaN stays NaN and is not counted in the maximum; a block with an infinity
+ * has an infinite scale, so that all its values stand for NaN.  The scales are
+ * kept as fp32 in every precision mode. */
+odla_values odla_hip_BlockQuantize(odla_value input,
+                                   const odla_value_ids value_ids);
+/* Product of 8-bit floating-point matrices with a scale for each block of 128:
+ *   y[m][n] = sum_b A_scale[m][b] * B_scale[n / 128][b]
+ *                   * sum_{128 b <= k < min(128 (b + 1), K)} A[m][k] * B[n][k]
+ * A [.., K] with A_scale [.., ceil(K / 128)] as odla_hip_BlockQuantize makes
+ * them; B [N, K] (one row per result column) with B_scale
+ * [ceil(N / 128), ceil(K / 128)]; both scales FLOAT32.  The result [.., N] is
+ * FLOAT32 (stored as the precision mode says), FLOAT16 or BFLOAT16.  Sums are
+ * kept in 32 bits and rounded once, with one exception: of more than 64 rows with
+ * a result in 16 bits, each eight terms k = 8 i .. 8 i + 7 pass through the 8-bit
+ * matrix instructions, which drop what lies below 2^-13 of the largest product of
+ * the eight. */
+odla_value odla_hip_BlockGemm(odla_value A, odla_value A_scale, odla_value B,
+                              odla_value B_scale, odla_element_type result_type,
+                              const odla_value_id value_id);
+/* A layer of E experts for few tokens.  For every token x of `input` [.., H]
+ * (at most 512 tokens; leading extents are flattened):
+ *   l = router x (router [E, H]); its `top_k` largest entries, ties to the
+ *   lowest index, choose the experts; w = softmax(l) of those, divided by their
+ *   sum if `renormalize` is set, times `scaling`;
+ *   y = sum_j w_j down[e_j] (silu(gate[e_j] x) * (up[e_j] x))
+ * gate_up is [E, 2 I, H] (rows 0 .. I - 1 the gate, I .. 2 I - 1 the other
+ * factor), down [E, H, I].  All float operands are stored in one type.  gate_up
+ * and down may be ODLA_HIP_FLOAT8_E4M3 instead, with FLOAT32 scales for blocks
+ * of 128 x 128: gate_up_scale [E, ceil(2 I / 128), ceil(H / 128)], down_scale
+ * [E, ceil(H / 128), ceil(I / 128)]; otherwise both scales are null.  E <= 1024,
+ * top_k <= min(E, 32).  Sums, the router's logits and the softmax are kept in 32
+ * bits; silu(..) * (..) is rounded to the type of `input`.  A NaN among a token's
+ * logits makes its result NaN. */
+odla_value odla_hip_MixtureOfExperts(odla_value input, odla_value router,
+                                     odla_value gate_up,
+                                     odla_value gate_up_scale, odla_value down,
+                                     odla_value down_scale, odla_uint32 top_k,
+                                     odla_bool renormalize, odla_float32 scaling,
+                                     const odla_value_id value_id);
+/* The next token of every row of `logits` [.., V], V <= 524288: INT32 [..].
+ * temperature, top_p, min_p and uniform are FLOAT32, top_k is INT32, each with
+ * one element per row or a single one; null means 1 / off / off; uniform, the
+ * random number in [0, 1) of the row, is required.
+ *   w_i = exp((l_i - max l) / temperature); tokens are ranked by logit, ties by
+ *   ascending index.  Kept are the first of the ranking as far as all of these
+ *   go: the first top_k (off: <= 0 or > V); the shortest prefix whose sum of w is
+ *   at least top_p times that of the first top_k (off: not < 1); those with w >=
+ *   min_p (off: not > 0).  The first is always kept.  The result is the lowest
+ *   kept index i for which the sum of w over kept indices <= i exceeds uniform
+ *   times the sum over all kept.
+ * A temperature that is not above 0 gives the first of the ranking.  NaN logits
+ * count as -inf; a row with nothing above -inf gives -1.  The weights are
+ * exponentials in 64 bits, held as whole multiples of 2^-44 of the largest, so
+ * that sums do not depend on an order; the parameters are read in their own
+ * type in every precision mode. */
+odla_value odla_hip_Sample(odla_value logits, odla_value temperature,
+                           odla_value top_k, odla_value top_p, odla_value min_p,
+                           odla_value uniform, const odla_value_id value_id);
 
 /* ------------------------------------------------------------------------ */
 /* Stored computations and executables.  What is stored is the recorded       */
