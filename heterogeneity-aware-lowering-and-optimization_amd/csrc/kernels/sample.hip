@@ -8,18 +8,30 @@
 // on the last bits of an exponential.  Weights are exponentials in 64 bits, rounded to whole multiples
 // of 2^-44 of the largest; up to 2^19 of them add up exactly in 64-bit integers, in any order.
 //
-// One workgroup per row; the row is read again by every pass, from L2.  The cut of the ranking is a
-// radix descent over the logits' bits as ordered 32-bit keys (11 + 11 + 10 bits): a pass counts the
-// elements and adds the weights of every digit among those that share the digits found so far.
-#include "device_utils.h"
+// One workgroup per row.  A pass over the row reads it from L2 (the first from memory); what a row
+// costs is its passes and the exponentials in them, so that there are few of either:
+//   1  the largest logit and its index (a greedy row ends here);
+//   2  a histogram over 2048 bins of equal width in (max - l) / T - equal width and not the logits'
+//      leading bits, because those put most of a row into a few bins, whose counters then take turns.
+//      With top-k it counts (no exponentials), otherwise it adds weights; it names the bin where the
+//      ranking is cut;
+//   3  top-k: everything up to that bin goes to a list in LDS (a few more than k elements), where
+//      top-p, min-p and the draw are settled; top-p alone: the elements of the one bin, which give the cut;
+//   4  without a list: the kept weights, added by 64 x 16 bytes of the row (a wavefront's vectors of one
+//      iteration); the part where the sum passes u is looked at once more by one wavefront.
+// Rows whose cut is not found that way (thousands of equal logits, top-k in the thousands) take a
+// radix descent over the logits' bits as ordered 32-bit keys, a pass for each of three digits.
+#include "block_common.h"
 
 namespace ohip {
 namespace {
 
 constexpr int kThreads = 1024, kWavesPerRow = kThreads / 64, kBins = 2048;
+constexpr int kList = 4096;     // candidates that are settled in LDS
+constexpr int kBorder = 1024;   // elements of one bin that are ranked against each other: n / 1024 n steps
 typedef unsigned long long u64;
 
-// Order of floats as unsigned numbers: -inf gives 0x007fffff, everything that can be drawn more.
+// Order of floats as unsigned numbers: -inf and NaN give 0x007fffff, everything that can be drawn more.
 constexpr unsigned kKeyOfMinusInf = 0x007fffffu;
 __device__ __forceinline__ unsigned key_of(const float l) {
   const unsigned u = __float_as_uint(l);
@@ -31,89 +43,149 @@ __device__ __forceinline__ float logit_of(const unsigned k) {
   return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
 }
 
+struct Shared {
+  u64 sum[kBins];
+  unsigned count[kBins];
+  unsigned key[kList];
+  int index[kList];
+  int border[kBorder];
+  double power[64];            // 2^(j / 64)
+  u64 wave_a[kWavesPerRow], wave_b[kWavesPerRow];
+  int listed, bordered, found;
+  // result of find()
+  int bin;
+  u64 before;
+  unsigned cut_key;
+  int cut_at;
+};
+
 struct Row {
   float most;         // the largest logit
-  double per;         // 1 / temperature
+  float per_bin;      // bins per unit of (max - l)
+  double per;         // log2(e) / temperature
+  const double* power;
 };
+// 2^44 exp((l - max) / T) in 64 bits: 2^y = 2^n 2^(j / 64) 2^f with |f| <= 1 / 128, the last as its
+// series, whose terms from f^6 on are below 2^-55.
 __device__ __forceinline__ double weight(const Row& r, const float l) {
-  if (l == r.most) return 1.0;
-  const double x = ((double)l - (double)r.most) * r.per;
-  return x == x ? exp(x) : 0.0;   // (an infinite temperature below an infinite logit)
+  const double y = ((double)l - (double)r.most) * r.per;
+  if (!(y >= -64.0)) return l == r.most ? 17592186044416.0 : 0.0;   // (NaN: infinite logits or temperatures)
+  const double k = rint(y * 64.0), f = y - k * 0.015625;
+  const int i = (int)k;
+  double p = 1.3333558146428443e-3;               // ln(2)^5 / 5!
+  p = __builtin_fma(p, f, 9.6181291076284770e-3);
+  p = __builtin_fma(p, f, 5.5504108664821580e-2);
+  p = __builtin_fma(p, f, 2.4022650695910072e-1);
+  p = __builtin_fma(p, f, 6.9314718055994531e-1);
+  p = __builtin_fma(p, f, 1.0);
+  return __builtin_ldexp(p * r.power[i & 63], (i >> 6) + 44);
 }
-__device__ __forceinline__ u64 fixed(const double w) { return (u64)__double2ull_rn(w * 17592186044416.0); }   // 2^44
+// ... as a whole number: the sum with 2^52 has it in its low bits, rounded to nearest even.
+__device__ __forceinline__ u64 whole(const double w) {
+  return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
+}
+// The histogram's bin, not decreasing as l falls; 0 for the largest.
+__device__ __forceinline__ int bin_of(const Row& r, const float l) {
+  const float x = (r.most - l) * r.per_bin;       // NaN (infinite logits or temperatures) counts as far away
+  return l == r.most ? 0 : (int)fminf(x, (float)(kBins - 1));
+}
 
 __device__ __forceinline__ u64 wave_sum_u64(u64 v) {
   for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
   return v;
 }
-
-// The digit of the ranking where a border falls: walking the bins from the highest, the first whose
-// elements (BY_SUM: whose weights) reach `need` together with those above it.  cnt / sum: what stands
-// above that bin on return.  The border must be reached.
-struct Cut { int bin; unsigned above; u64 above_sum; };
-
-struct Shared {
-  unsigned count[kBins];
-  u64 sum[kBins];
-  u64 wave_a[kWavesPerRow];
-  u64 wave_b[kWavesPerRow];
-  float wave_f[kWavesPerRow];
-  int wave_i[kWavesPerRow];
-  Cut cut;
-  int found;
-};
-
-template <typename T>
-__device__ __forceinline__ float logit_at(const T* row, const int i) { return Store<T>::ld(row + i); }
-
-// Every thread holds two neighbouring bins of the descending order; the border is found by a scan over the threads.
-template <bool BY_SUM>
-__device__ void find_cut(Shared* s, const u64 need) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int b0 = kBins - 1 - 2 * tid, b1 = b0 - 1;   // b0 ranks before b1
-  const u64 v0 = BY_SUM ? s->sum[b0] : s->count[b0], v1 = BY_SUM ? s->sum[b1] : s->count[b1];
-  const unsigned c0 = s->count[b0], c1 = s->count[b1];
-  const u64 w0 = s->sum[b0], w1 = s->sum[b1];
-  u64 v = v0 + v1, c = c0 + c1, w = w0 + w1;
-  for (int d = 1; d < 64; d <<= 1) {
-    const u64 ov = __shfl_up(v, d), oc = __shfl_up(c, d), ow = __shfl_up(w, d);
-    if (lane >= d) { v += ov; c += oc; w += ow; }
-  }
-  __shared__ u64 tv[kWavesPerRow], tc[kWavesPerRow], tw[kWavesPerRow];
-  if (lane == 63) { tv[wave] = v; tc[wave] = c; tw[wave] = w; }
+__device__ __forceinline__ u64 block_sum_u64(u64 v, u64* room) {
+  v = wave_sum_u64(v);
   __syncthreads();
-  u64 bv = 0, bc = 0, bw = 0;
-  for (int i = 0; i < wave; ++i) { bv += tv[i]; bc += tc[i]; bw += tw[i]; }
-  v += bv; c += bc; w += bw;          // inclusive of both bins
-  const u64 before = v - v0 - v1;
-  if (before < need && v >= need) {
-    const bool first = before + v0 >= need;
-    s->cut.bin = first ? b0 : b1;
-    s->cut.above = (unsigned)(c - c0 - c1 + (first ? 0 : c0));
-    s->cut.above_sum = w - w0 - w1 + (first ? 0 : w0);
+  if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0;
+#pragma unroll
+  for (int i = 0; i < kWavesPerRow; ++i) v += room[i];
+  return v;
+}
+
+// s->bin = the first bin whose value together with those in front of it reaches `need` (>= 1), s->before
+// = what stands in front.  Some bin must.
+template <typename N>
+__device__ __forceinline__ void find(Shared* s, const N* bins, const u64 need) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const u64 a = bins[2 * tid], b = bins[2 * tid + 1];
+  u64 v = a + b;
+  for (int d = 1; d < 64; d <<= 1) {
+    const u64 o = __shfl_up(v, d);
+    if (lane >= d) v += o;
+  }
+  if (lane == 63) s->wave_b[wave] = v;
+  __syncthreads();
+  for (int i = 0; i < kWavesPerRow; ++i) v += i < wave ? s->wave_b[i] : 0;
+  const u64 front = v - a - b;
+  if (front < need && v >= need) {
+    const bool first = front + a >= need;
+    s->bin = 2 * tid + (first ? 0 : 1);
+    s->before = front + (first ? 0 : a);
   }
   __syncthreads();
 }
+
+__device__ __forceinline__ void clear(u64* sum) {
+  sum[threadIdx.x] = 0ull;
+  sum[threadIdx.x + kThreads] = 0ull;
+}
+__device__ __forceinline__ void clear(unsigned* count) {
+  count[threadIdx.x] = 0u;
+  count[threadIdx.x + kThreads] = 0u;
+}
+
+// ---- the row in vectors of 16 bytes: vector j * 1024 + tid in iteration j ----
+template <typename T>
+struct RowReader {
+  static constexpr int PER = 16 / sizeof(T);
+  const T* row;
+  int V;
+  // f(index, logit) for every element, four vectors of a thread requested at a time
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    const int full = V / PER;
+    for (int v0 = threadIdx.x; v0 < full; v0 += 4 * kThreads) {
+      Vec16<T> x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (v0 + j * kThreads < full) x[j].raw = reinterpret_cast<const Bytes16*>(row + (int64_t)(v0 + j * kThreads) * PER)->v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (v0 + j * kThreads < full)
+#pragma unroll
+          for (int e = 0; e < PER; ++e) f((v0 + j * kThreads) * PER + e, x[j].get(e));
+    }
+    const int rest = full * PER + (int)threadIdx.x;
+    if (rest < V) f(rest, Store<T>::ld(row + rest));
+  }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) {
   __shared__ Shared s;
   const int row_i = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const T* row = (const T*)p.logits + (int64_t)row_i * p.V;
+  const RowReader<T> row{(const T*)p.logits + (int64_t)row_i * p.V, p.V};
   const int V = p.V;
   const float temperature = p.temperature ? p.temperature[(int64_t)row_i * p.step_t] : 1.f;
   const int top_k = p.top_k ? p.top_k[(int64_t)row_i * p.step_k] : 0;
   const float top_p = p.top_p ? p.top_p[(int64_t)row_i * p.step_p] : 1.f;
   const float min_p = p.min_p ? p.min_p[(int64_t)row_i * p.step_m] : 0.f;
   const float u = p.uniform[(int64_t)row_i * p.step_u];
+  if (tid < 64) s.power[tid] = exp2(tid * 0.015625);
+  if (tid == 0) s.listed = s.bordered = 0;
 
-  // ---- the largest logit and its lowest index ----
+  // ---- 1: the largest logit, its lowest index, and how many can be drawn ----
   unsigned best = 0;
   int at = V;
-  for (int i = tid; i < V; i += kThreads) {
-    const unsigned k = key_of(logit_at(row, i));
-    if (k > best) { best = k; at = i; }
-  }
+  unsigned live = 0;
+  row.each([&](const int i, const float l) {
+    const unsigned k = key_of(l);
+    if (k > best || (k == best && i < at)) { best = k; at = i; }
+    live += k > kKeyOfMinusInf;
+  });
   u64 pair = (u64)best << 32 | (unsigned)~at;
   for (int d = 32; d > 0; d >>= 1) {
     const u64 o = __shfl_xor(pair, d);
@@ -122,158 +194,306 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
   if (lane == 0) s.wave_a[wave] = pair;
   __syncthreads();
   for (int i = 0; i < kWavesPerRow; ++i) pair = s.wave_a[i] > pair ? s.wave_a[i] : pair;
-  __syncthreads();
   const unsigned top_key = (unsigned)(pair >> 32);
   const int first = (int)~(unsigned)pair;
   if (top_key <= kKeyOfMinusInf || !(temperature > 0.f) || top_k == 1 || min_p > 1.f) {   // nothing to draw from, or one token left
     if (tid == 0) p.token[row_i] = top_key <= kKeyOfMinusInf ? -1 : first;
     return;
   }
+  const u64 live_all = block_sum_u64(live, s.wave_b);
   Row r;
   r.most = logit_of(top_key);
-  r.per = 1.0 / (double)temperature;
+  r.per = 1.4426950408889634 / (double)temperature;
+  // (a weight rounds to nothing from (max - l) / T = 45 ln 2 = 31.2 on: the last bin takes all of those)
+  r.per_bin = (float)kBins / 31.25f / temperature;
+  r.power = s.power;
+  const double least = (double)min_p * 17592186044416.0;   // (NaN: nothing is below)
 
-  // ---- the cut: everything above cut_key, and of those equal to it the ones up to index cut_at ----
+  // Of everything at or above the first cut: the elements before and at (cut_key, cut_at) in the ranking are kept.
   unsigned cut_key = kKeyOfMinusInf + 1;
   int cut_at = V;
-  auto descend = [&](auto by_sum, u64 need, const unsigned floor_key, const int floor_at, u64* reached) {
-    constexpr bool BY_SUM = decltype(by_sum)::value;
-    // among elements with key > floor_key, or key == floor_key and index <= floor_at
-    unsigned prefix = 0, fixed_bits = 0;
-    u64 sum_above = 0;
+  auto in_cut = [&](const unsigned k, const int i) { return k > cut_key || (k == cut_key && i <= cut_at); };
+
+  // Radix descent among the elements kept so far: the last that a cut at `need` (elements, or weight) keeps
+  // becomes the new cut; the weight of all that remain is returned.
+  auto descend = [&](const bool by_sum, u64 need) -> u64 {
+    unsigned prefix = 0, known = 0;
+    u64 sum_front = 0;
     for (int level = 0; level < 3; ++level) {
       const int shift = level == 0 ? 21 : level == 1 ? 10 : 0;
-      const unsigned bins_mask = level == 2 ? 1023u : 2047u;
-      for (int i = tid; i < kBins; i += kThreads) { s.count[i] = 0u; s.sum[i] = 0ull; }
+      const unsigned mask = level == 2 ? 1023u : 2047u;
+      clear(s.count);
+      clear(s.sum);
       __syncthreads();
-      for (int i = tid; i < V; i += kThreads) {
-        const float l = logit_at(row, i);
+      row.each([&](const int i, const float l) {
         const unsigned k = key_of(l);
-        if ((k & fixed_bits) != prefix || k < floor_key || (k == floor_key && i > floor_at)) continue;
-        const unsigned b = (k >> shift) & bins_mask;
+        if ((k & known) != prefix || !in_cut(k, i)) return;
+        const unsigned b = mask - ((k >> shift) & mask);    // (the highest digit first)
         atomicAdd(&s.count[b], 1u);
-        const u64 w = fixed(weight(r, l));
+        const u64 w = whole(weight(r, l));
         if (w != 0) atomicAdd(&s.sum[b], w);
-      }
+      });
       __syncthreads();
-      find_cut<BY_SUM>(&s, need);
-      const Cut c = s.cut;
-      need -= BY_SUM ? c.above_sum : c.above;
-      sum_above += c.above_sum;
-      prefix |= (unsigned)c.bin << shift;
-      fixed_bits |= bins_mask << shift;
+      if (by_sum) find(&s, s.sum, need); else find(&s, s.count, need);
+      const int b = s.bin;
+      need -= s.before;
+      u64 front = 0;      // weight of the digits in front
+      for (int i = tid; i < b; i += kThreads) front += s.sum[i];
+      sum_front += block_sum_u64(front, s.wave_a);
+      prefix |= (mask - (unsigned)b) << shift;
+      known |= mask << shift;
       __syncthreads();
     }
     // `need` is what the elements equal to the key still have to give: the first `ties` of them
-    const u64 w = fixed(weight(r, logit_of(prefix)));
-    const u64 ties = BY_SUM ? (w ? (need + w - 1) / w : 1) : need;
+    const u64 w = whole(weight(r, logit_of(prefix)));
+    const u64 ties = by_sum ? (w ? (need + w - 1) / w : 1) : need;
+    // the index of the last of them: ties counted by parts of 2048 / V of the row
+    const int part = (V + kBins - 1) / kBins;
+    clear(s.count);
+    __syncthreads();
+    row.each([&](const int i, const float l) {
+      if (key_of(l) == prefix && in_cut(prefix, i)) atomicAdd(&s.count[i / part], 1u);
+    });
+    __syncthreads();
+    find(&s, s.count, ties);
+    if (tid == 0) {
+      u64 seen = s.before;
+      int i = s.bin * part;
+      for (; i < V; ++i)
+        if (key_of(Store<T>::ld(row.row + i)) == prefix && in_cut(prefix, i) && ++seen == ties) break;
+      s.cut_at = i;
+    }
+    __syncthreads();
     cut_key = prefix;
-    *reached = sum_above + ties * w;
-    // the index of the last tie kept: wavefronts own neighbouring segments
-    const int per = (V + kWavesPerRow - 1) / kWavesPerRow;
-    const int lo = wave * per, hi = min(V, lo + per);
-    unsigned mine = 0;
-    for (int i = lo; i < hi; i += 64) {
-      const bool tie = i + lane < hi && key_of(logit_at(row, i + lane)) == prefix && !(prefix == floor_key && i + lane > floor_at);
-      mine += (unsigned)__popcll(__ballot(tie));
-    }
-    if (lane == 0) s.wave_i[wave] = (int)mine;
-    if (tid == 0) s.found = V;
+    cut_at = s.cut_at;
     __syncthreads();
-    u64 before = 0;
-    for (int i = 0; i < wave; ++i) before += (u64)s.wave_i[i];
-    if (before < ties && before + mine >= ties) {
-      u64 seen = before;
-      for (int i = lo; i < hi; i += 64) {
-        const bool tie = i + lane < hi && key_of(logit_at(row, i + lane)) == prefix && !(prefix == floor_key && i + lane > floor_at);
-        const u64 votes = __ballot(tie);
-        const unsigned here = (unsigned)__popcll(votes);
-        if (seen + here >= ties) {
-          const unsigned rank = (unsigned)__popcll(votes & ((1ull << lane) - 1ull));
-          if (tie && seen + rank + 1 == ties) s.found = i + lane;
-          break;
+    return sum_front + ties * w;
+  };
+
+  bool listed = false;      // the candidates are in s.key / s.index
+  // of them this thread's, strided; weight 0, bin kBins: not kept
+  u64 kept_w[kList / kThreads];
+  unsigned kept_key[kList / kThreads];
+  int kept_i[kList / kThreads], kept_bin[kList / kThreads];
+
+  const bool cut_k = top_k > 0 && (u64)top_k < live_all;
+  if (cut_k) {
+    // ---- 2: where the k-th element stands ----
+    clear(s.count);
+    __syncthreads();
+    row.each([&](const int i, const float l) {
+      if (key_of(l) > kKeyOfMinusInf) atomicAdd(&s.count[bin_of(r, l)], 1u);
+    });
+    __syncthreads();
+    find(&s, s.count, (u64)top_k);
+    const int last = s.bin;
+    const unsigned front = (unsigned)s.before, in_bin = s.count[last];
+    if (front + in_bin <= kList && in_bin <= kBorder) {
+      // ---- 3: those up to its bin, and the elements of the bin against each other ----
+      listed = true;
+      row.each([&](const int i, const float l) {
+        const unsigned k = key_of(l);
+        if (k <= kKeyOfMinusInf) return;
+        const int b = bin_of(r, l);
+        if (b > last) return;
+        const int n = atomicAdd(&s.listed, 1);
+        s.key[n] = k;
+        s.index[n] = i;
+        if (b == last) s.border[atomicAdd(&s.bordered, 1)] = n;
+      });
+      __syncthreads();
+      const int n = s.listed, m = s.bordered;
+      if (tid < m) {
+        const int c = s.border[tid];
+        const unsigned k = s.key[c];
+        const int i = s.index[c];
+        unsigned rank = front;
+        for (int j = 0; j < m; ++j) {
+          const int o = s.border[j];
+          rank += s.key[o] > k || (s.key[o] == k && s.index[o] < i);
         }
-        seen += here;
+        if (rank + 1 == (unsigned)top_k) { s.cut_key = k; s.cut_at = i; }
+      }
+      __syncthreads();
+      cut_key = s.cut_key;
+      cut_at = s.cut_at;
+#pragma unroll
+      for (int j = 0; j < kList / kThreads; ++j) {
+        const int c = tid + j * kThreads;
+        kept_w[j] = 0;
+        kept_key[j] = 0;
+        kept_i[j] = 0;
+        kept_bin[j] = kBins;
+        if (c < n && in_cut(s.key[c], s.index[c])) {
+          kept_key[j] = s.key[c];
+          kept_i[j] = s.index[c];
+          const float l = logit_of(s.key[c]);
+          kept_bin[j] = bin_of(r, l);
+          kept_w[j] = whole(weight(r, l));
+        }
       }
     }
-    __syncthreads();
-    cut_at = s.found;
-    __syncthreads();
-  };
-
-  // how many can be drawn at all, and their weights together
-  unsigned live = 0;
-  u64 total = 0;
-  for (int i = tid; i < V; i += kThreads) {
-    const float l = logit_at(row, i);
-    if (key_of(l) <= kKeyOfMinusInf) continue;
-    ++live;
-    total += fixed(weight(r, l));
   }
-  total = wave_sum_u64(total);
-  u64 live64 = wave_sum_u64(live);
-  if (lane == 0) { s.wave_a[wave] = total; s.wave_b[wave] = live64; }
-  __syncthreads();
-  total = 0; live64 = 0;
-  for (int i = 0; i < kWavesPerRow; ++i) { total += s.wave_a[i]; live64 += s.wave_b[i]; }
-  __syncthreads();
 
-  if (top_k > 0 && (u64)top_k < live64) descend(std::false_type(), (u64)top_k, cut_key, cut_at, &total);
+  u64 total = 0;     // weight of what top-k keeps, where top-p asks for it
+  if (cut_k && !listed) total = descend(false, (u64)top_k);
+
   if (top_p < 1.f) {
+    // ---- 2 and 3 of a cut by weight ----
+    clear(s.sum);
+    if (tid == 0) s.bordered = 0;
+    __syncthreads();
+    if (listed) {
+#pragma unroll
+      for (int j = 0; j < kList / kThreads; ++j)
+        if (kept_w[j] != 0) { total += kept_w[j]; atomicAdd(&s.sum[kept_bin[j]], kept_w[j]); }
+    } else {
+      total = 0;
+      row.each([&](const int i, const float l) {
+        const unsigned k = key_of(l);
+        if (!in_cut(k, i)) return;
+        const u64 w = whole(weight(r, l));
+        if (w != 0) { total += w; atomicAdd(&s.sum[bin_of(r, l)], w); }
+      });
+    }
+    total = block_sum_u64(total, s.wave_a);
     const double want = ceil((double)top_p * (double)total);
-    u64 need = want > 1.0 ? (u64)want : 1ull;
+    const u64 need = want > 1.0 ? (u64)want : 1ull;
     if (need < total) {
-      u64 dropped;
-      descend(std::true_type(), need, cut_key, cut_at, &dropped);
+      find(&s, s.sum, need);
+      const int last = s.bin;
+      const u64 front = s.before;
+      // the elements of that bin, ranked against each other (their keys and indices in s.key / s.index;
+      // s.sum is done with and takes their weights)
+      if (listed) {
+        // (the list itself: positions of its elements)
+#pragma unroll
+        for (int j = 0; j < kList / kThreads; ++j)
+          if (kept_bin[j] == last) {
+            const int n = atomicAdd(&s.bordered, 1);
+            if (n < kBorder) { s.border[n] = tid + j * kThreads; s.sum[n] = kept_w[j]; }
+          }
+      } else {
+        row.each([&](const int i, const float l) {
+          const unsigned k = key_of(l);
+          if (!in_cut(k, i) || bin_of(r, l) != last) return;
+          const int n = atomicAdd(&s.bordered, 1);
+          if (n < kBorder) { s.border[n] = n; s.key[n] = k; s.index[n] = i; s.sum[n] = whole(weight(r, l)); }
+        });
+      }
+      __syncthreads();
+      const int m = s.bordered;
+      if (m <= kBorder) {
+        if (tid < m) {
+          const int c = s.border[tid];
+          const unsigned k = s.key[c];
+          const int i = s.index[c];
+          u64 before = front;
+          for (int j = 0; j < m; ++j) {
+            const int o = s.border[j];
+            before += s.key[o] > k || (s.key[o] == k && s.index[o] < i) ? s.sum[j] : 0;
+          }
+          if (before < need && before + s.sum[tid] >= need) { s.cut_key = k; s.cut_at = i; }
+        }
+        __syncthreads();
+        cut_key = s.cut_key;
+        cut_at = s.cut_at;
+        __syncthreads();
+      } else {
+        __syncthreads();
+        descend(true, need);
+        listed = false;
+      }
     }
   }
 
-  // ---- the draw: wavefronts own neighbouring segments of the row ----
-  auto kept = [&](const int i, u64* w) {
-    const float l = logit_at(row, i);
-    const unsigned k = key_of(l);
-    if (k < cut_key || (k == cut_key && i > cut_at)) return false;
-    const double d = weight(r, l);
-    if (d < (double)min_p) return false;
-    *w = fixed(d);
-    return true;
-  };
-  const int per = ((V + kWavesPerRow - 1) / kWavesPerRow + 63) / 64 * 64;
-  const int lo = min(V, wave * per), hi = min(V, lo + per);
-  u64 mine = 0;
-  for (int i = lo + lane; i < hi; i += 64) {
-    u64 w;
-    if (kept(i, &w)) mine += w;
+  // ---- 4: the draw ----
+  if (listed) {
+    // by parts of the row's indices: the part where the sum passes, then its elements against each other
+    const int part = (V + kBins - 1) / kBins;
+    clear(s.sum);
+    if (tid == 0) s.bordered = 0;
+    __syncthreads();
+    u64 all = 0;
+#pragma unroll
+    for (int j = 0; j < kList / kThreads; ++j) {
+      if (kept_w[j] == 0 || !in_cut(kept_key[j], kept_i[j]) || weight(r, logit_of(kept_key[j])) < least) kept_w[j] = 0;
+      if (kept_w[j] != 0) { all += kept_w[j]; atomicAdd(&s.sum[kept_i[j] / part], kept_w[j]); }
+    }
+    all = block_sum_u64(all, s.wave_a);
+    const double want = floor((double)u * (double)all);
+    u64 target = want > 0.0 ? (u64)want : 0ull;   // the first sum above it
+    if (target >= all) target = all - 1;
+    find(&s, s.sum, target + 1);
+    const int b = s.bin;
+    const u64 front = s.before;
+    // (at most `part` <= 256 elements; s.sum is done with and takes their weights)
+#pragma unroll
+    for (int j = 0; j < kList / kThreads; ++j)
+      if (kept_w[j] != 0 && kept_i[j] / part == b) {
+        const int n = atomicAdd(&s.bordered, 1);
+        s.border[n] = kept_i[j];
+        s.sum[n] = kept_w[j];
+      }
+    __syncthreads();
+    const int m = s.bordered;
+    if (tid < m) {
+      u64 before = front;
+      for (int j = 0; j < m; ++j) before += s.border[j] < s.border[tid] ? s.sum[j] : 0;
+      if (before <= target && before + s.sum[tid] > target) p.token[row_i] = s.border[tid];
+    }
+    return;
   }
-  mine = wave_sum_u64(mine);
-  if (lane == 0) s.wave_a[wave] = mine;
-  if (tid == 0) s.found = -1;
+  constexpr int PER = RowReader<T>::PER;
+  auto kept = [&](const int i, const float l) -> u64 {
+    if (!in_cut(key_of(l), i)) return 0;
+    const double w = weight(r, l);
+    return w < least ? 0 : whole(w);
+  };
+  // a wavefront's vectors of iteration j are part 16 j + wave of the row, 64 x PER elements
+  const int vectors = (V + PER - 1) / PER, parts = (vectors + 63) / 64;
+  clear(s.sum);
   __syncthreads();
-  u64 all = 0, before = 0;
-  for (int i = 0; i < kWavesPerRow; ++i) { if (i < wave) before += s.wave_a[i]; all += s.wave_a[i]; }
+  u64 all = 0;
+  auto vector_sum = [&](const int v, u64 (&w)[PER]) {   // of vector v, and its weights
+    u64 sum = 0;
+    if ((v + 1) * PER <= V) {
+      Vec16<T> x;
+      x.raw = reinterpret_cast<const Bytes16*>(row.row + (int64_t)v * PER)->v;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) sum += w[e] = kept(v * PER + e, x.get(e));
+    } else {
+#pragma unroll
+      for (int e = 0; e < PER; ++e) sum += w[e] = v * PER + e < V ? kept(v * PER + e, Store<T>::ld(row.row + v * PER + e)) : 0;
+    }
+    return sum;
+  };
+  for (int part = wave; part < parts; part += kWavesPerRow) {
+    u64 w[PER];
+    const u64 sum = wave_sum_u64(vector_sum(part * 64 + lane, w));
+    all += sum;
+    if (lane == 0) s.sum[part] = sum;
+  }
+  all = block_sum_u64(lane == 0 ? all : 0, s.wave_a);
   const double want = floor((double)u * (double)all);
-  u64 target = want > 0.0 ? (u64)want : 0ull;   // the first sum above it
+  u64 target = want > 0.0 ? (u64)want : 0ull;
   if (target >= all) target = all - 1;
-  if (before <= target && before + mine > target) {
-    u64 seen = before;
-    for (int i = lo; i < hi; i += 64) {
-      u64 w = 0;
-      if (i + lane < hi && !kept(i + lane, &w)) w = 0;
-      u64 upto = w;
-      for (int d = 1; d < 64; d <<= 1) {
-        const u64 o = __shfl_up(upto, d);
-        if (lane >= d) upto += o;
-      }
-      const u64 here = __shfl(upto, 63);
-      if (seen + here > target) {
-        if (seen + upto > target && seen + upto - w <= target) s.found = i + lane;
-        break;
-      }
-      seen += here;
+  find(&s, s.sum, target + 1);
+  if (wave == 0) {
+    u64 w[PER];
+    const u64 sum = vector_sum(s.bin * 64 + lane, w);
+    u64 upto = sum;
+    for (int d = 1; d < 64; d <<= 1) {
+      const u64 o = __shfl_up(upto, d);
+      if (lane >= d) upto += o;
+    }
+    u64 before = s.before + upto - sum;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      if (before <= target && before + w[e] > target) p.token[row_i] = (s.bin * 64 + lane) * PER + e;
+      before += w[e];
     }
   }
-  __syncthreads();
-  if (tid == 0) p.token[row_i] = s.found;
 }
 
 }  // namespace

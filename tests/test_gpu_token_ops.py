@@ -566,3 +566,27 @@ def test_results_reach_only_their_rows(odla):
     finally:
         hb.destroy()
     check_step(got, d, head, rows)
+
+
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+@pytest.mark.parametrize("spread", [0.0, 1e-6, 0.02, 1.0, 30.0])
+def test_cuts_in_crowded_and_empty_places(odla, kind, spread):
+    """Rows from all equal to far apart, cuts from the first element to the last: few, thousands or all beside the cut."""
+    announce("sampling with spread %g, %s" % (spread, kind))
+    rng = np.random.default_rng(5)
+    v, n = 9001, 36
+    x = 3.0 + spread * rng.standard_normal((n, v))
+    x[1::3, rng.integers(0, v, 40)] += 4.0
+    p = {"temperature": np.tile([0.5, 1.0, 20.0], n // 3), "top_k": np.tile(np.repeat([0, 2, 45, 1500, 4500, 9000], 3), n // 18),
+         "top_p": np.tile([1.0, 0.3, 0.97, 0.9999], n // 4), "min_p": np.tile([0.0, 0.0, 0.001], n // 3), "uniform": rng.random(n)}
+    got, want = run_sample(odla, kind, R.to_bits(x, kind), p)
+    assert np.array_equal(got, want), [(i, int(g), int(w)) for i, (g, w) in enumerate(zip(got, want)) if g != w]
+
+
+def test_the_largest_vocabulary(odla):
+    announce("sampling from 524288 logits")
+    rng = np.random.default_rng(2)
+    x = (rng.standard_normal((6, 1 << 19)) * 2).astype(np.float32)
+    p = {"top_k": [0, 0, 50, 5000, 0, 200000], "top_p": [1.0, 0.9, 0.9, 1.0, 0.999, 0.5], "min_p": [0, 0, 0, 0, 0.01, 0], "uniform": rng.random(6)}
+    got, want = run_sample(odla, "fp32", x, p)
+    assert np.array_equal(got, want)
