@@ -8,17 +8,18 @@
 // on the last bits of an exponential.  Weights are exponentials in 64 bits, rounded to whole multiples
 // of 2^-44 of the largest; up to 2^19 of them add up exactly in 64-bit integers, in any order.
 //
-// One workgroup per row.  A pass over the row reads it from L2 (the first from memory); what a row
-// costs is its passes and the exponentials in them, so that there are few of either:
-//   1  the largest logit and its index (a greedy row ends here);
-//   2  a histogram over 2048 bins of equal width in (max - l) / T - equal width and not the logits'
-//      leading bits, because those put most of a row into a few bins, whose counters then take turns.
-//      With top-k it counts (no exponentials), otherwise it adds weights; it names the bin where the
-//      ranking is cut;
-//   3  top-k: everything up to that bin goes to a list in LDS (a few more than k elements), where
+// One workgroup per row.  A pass over the row reads it from L2 (the first from memory), but what it
+// costs is instructions: one per element is four cycles of a SIMD for 64 of them, an exponential 24,
+// and a wavefront's additions to counters in LDS 36 cycles (32 bits) or 100 (64).  So:
+//   1  the largest logit of every thread (half an instruction per element), and of all;
+//   2  where the ranking is cut, by bins of equal width in (max - l) / T (the logits' leading bits would
+//      put most of a row into a few bins, whose counters then take turns).  Top-k: the k-th of the
+//      threads' largest is a bound, found among those 1024.  Top-p: weights are added by bins, but only of
+//      elements in front of the place behind which too little weight is left;
+//   3  top-k: everything from the bound on goes to a list in LDS (not many more than k), where the cut,
 //      top-p, min-p and the draw are settled; top-p alone: the elements of the one bin, which give the cut;
-//   4  without a list: the kept weights, added by 64 x 16 bytes of the row (a wavefront's vectors of one
-//      iteration); the part where the sum passes u is looked at once more by one wavefront.
+//   4  without a list: the kept weights, added by parts of 256 vectors; the part where the sum passes u is
+//      looked at once more by one wavefront.
 // Rows whose cut is not found that way (thousands of equal logits, top-k in the thousands) take a
 // radix descent over the logits' bits as ordered 32-bit keys, a pass for each of three digits.
 #include "block_common.h"
@@ -29,6 +30,7 @@ namespace {
 constexpr int kThreads = 1024, kWavesPerRow = kThreads / 64, kBins = 2048;
 constexpr int kList = 4096;     // candidates that are settled in LDS
 constexpr int kBorder = 1024;   // elements of one bin that are ranked against each other: n / 1024 n steps
+constexpr double kOne = 17592186044416.0;   // 2^44: the largest weight
 typedef unsigned long long u64;
 
 // Order of floats as unsigned numbers: -inf and NaN give 0x007fffff, everything that can be drawn more.
@@ -42,62 +44,97 @@ __device__ __forceinline__ unsigned key_of(const float l) {
 __device__ __forceinline__ float logit_of(const unsigned k) {
   return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
 }
+// a before b in the ranking
+__device__ __forceinline__ bool before(const float la, const int ia, const float lb, const int ib) { return la > lb || (la == lb && ia < ib); }
 
 struct Shared {
   u64 sum[kBins];
   unsigned count[kBins];
-  unsigned key[kList];
+  float logit[kList];
   int index[kList];
   int border[kBorder];
   double power[64];            // 2^(j / 64)
   u64 wave_a[kWavesPerRow], wave_b[kWavesPerRow];
-  int listed, bordered, found;
-  // result of find()
-  int bin;
-  u64 before;
-  unsigned cut_key;
+  float wave_f[kWavesPerRow];
+  int listed, bordered;
+  int bin;                     // results of find()
+  u64 front;
+  float cut_l;
   int cut_at;
 };
 
 struct Row {
   float most;         // the largest logit
+  float per_f;        // log2(e) / temperature
   float per_bin;      // bins per unit of (max - l)
-  double per;         // log2(e) / temperature
+  double most_d, per; // the first two in 64 bits
   const double* power;
 };
+// a * b + c with c in scalar registers (the compiler's own choice copies it to vector registers for every use).
+__device__ __forceinline__ double fma_c(const double a, const double b, const double c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  double d;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));
+  return d;
+#else
+  return __builtin_fma(a, b, c);
+#endif
+}
 // 2^44 exp((l - max) / T) in 64 bits: 2^y = 2^n 2^(j / 64) 2^f with |f| <= 1 / 128, the last as its
-// series, whose terms from f^6 on are below 2^-55.
+// series, whose terms from f^6 on are below 2^-55.  64 y is rounded by adding 1.5 * 2^52, which leaves it in
+// the sum's low word; 2^n goes straight into the exponent.  Masks, not branches: the elements of a vector
+// fill each other's latencies.
 __device__ __forceinline__ double weight(const Row& r, const float l) {
-  const double y = ((double)l - (double)r.most) * r.per;
-  if (!(y >= -64.0)) return l == r.most ? 17592186044416.0 : 0.0;   // (NaN: infinite logits or temperatures)
-  const double k = rint(y * 64.0), f = y - k * 0.015625;
-  const int i = (int)k;
-  double p = 1.3333558146428443e-3;               // ln(2)^5 / 5!
-  p = __builtin_fma(p, f, 9.6181291076284770e-3);
-  p = __builtin_fma(p, f, 5.5504108664821580e-2);
-  p = __builtin_fma(p, f, 2.4022650695910072e-1);
-  p = __builtin_fma(p, f, 6.9314718055994531e-1);
-  p = __builtin_fma(p, f, 1.0);
-  return __builtin_ldexp(p * r.power[i & 63], (i >> 6) + 44);
+  const bool near = (r.most - l) * r.per_f < 60.f;      // (not for NaN: infinite logits or temperatures)
+  const double y = ((double)(near ? l : r.most) - r.most_d) * r.per;
+  const double t = fma_c(y, 64.0, 6755399441055744.0);
+  const double f = __builtin_fma(t - 6755399441055744.0, -0.015625, y);
+  const int k = (int)(unsigned)(u64)__double_as_longlong(t);
+  double p = fma_c(f, 1.3333558146428443e-3, 9.6181291076284770e-3);   // ln(2)^5 / 5!, ln(2)^4 / 4!
+  p = fma_c(p, f, 5.5504108664821580e-2);
+  p = fma_c(p, f, 2.4022650695910072e-1);
+  p = fma_c(p, f, 6.9314718055994531e-1);
+  p = __builtin_fma(p, f, 1.0) * r.power[k & 63];
+  const u64 bits = (u64)__double_as_longlong(p) + ((u64)(unsigned)(((k >> 6) + 44) << 20) << 32);
+  const u64 in = near ? ~0ull : 0ull, top = l == r.most ? (u64)__double_as_longlong(kOne) : 0ull;
+  return __longlong_as_double((long long)((bits & in) | (top & ~in)));
 }
 // ... as a whole number: the sum with 2^52 has it in its low bits, rounded to nearest even.
 __device__ __forceinline__ u64 whole(const double w) {
   return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
 }
-// The histogram's bin, not decreasing as l falls; 0 for the largest.
+// The histogram's bin, not decreasing as l falls; 0 for the largest, kBins for what lies behind the last.
 __device__ __forceinline__ int bin_of(const Row& r, const float l) {
   const float x = (r.most - l) * r.per_bin;       // NaN (infinite logits or temperatures) counts as far away
-  return l == r.most ? 0 : (int)fminf(x, (float)(kBins - 1));
+  return l == r.most ? 0 : (int)fminf(x, (float)kBins);
 }
 
-__device__ __forceinline__ u64 wave_sum_u64(u64 v) {
-  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+// Sums over the lanes up to one's own, by DPP (no trip through LDS): the shifts inside rows of 16,
+// then the last lane of a row to the next row, and of the first half to the second.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_u64(const u64 v) {
+  const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, ROWS, 0xf, false);
+  const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), CTRL, ROWS, 0xf, false);
+  return (u64)hi << 32 | lo;
+}
+__device__ __forceinline__ u64 scan(u64 v) {
+  v += dpp_u64<0x111, 0xf>(v);
+  v += dpp_u64<0x112, 0xf>(v);
+  v += dpp_u64<0x114, 0xf>(v);
+  v += dpp_u64<0x118, 0xf>(v);
+  v += dpp_u64<0x142, 0xa>(v);
+  v += dpp_u64<0x143, 0xc>(v);
   return v;
 }
+__device__ __forceinline__ u64 last_lane(const u64 v) {
+  const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, 63), hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(v >> 32), 63);
+  return (u64)hi << 32 | lo;
+}
+// Sum over the workgroup; `room` may be in use until the call.
 __device__ __forceinline__ u64 block_sum_u64(u64 v, u64* room) {
-  v = wave_sum_u64(v);
+  v = scan(v);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 63) room[threadIdx.x >> 6] = v;
   __syncthreads();
   v = 0;
 #pragma unroll
@@ -105,27 +142,30 @@ __device__ __forceinline__ u64 block_sum_u64(u64 v, u64* room) {
   return v;
 }
 
-// s->bin = the first bin whose value together with those in front of it reaches `need` (>= 1), s->before
-// = what stands in front.  Some bin must.
+// s->bin = the first bin whose value together with those in front of it reaches `need` (>= 1), s->front
+// = what stands in front.  Returns the sum of all; where that is less than `need` there is no such bin.
 template <typename N>
-__device__ __forceinline__ void find(Shared* s, const N* bins, const u64 need) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+__device__ __forceinline__ u64 find(Shared* s, const N* bins, const u64 need) {
+  const int tid = threadIdx.x, wave = tid >> 6;
   const u64 a = bins[2 * tid], b = bins[2 * tid + 1];
-  u64 v = a + b;
-  for (int d = 1; d < 64; d <<= 1) {
-    const u64 o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
-  if (lane == 63) s->wave_b[wave] = v;
+  u64 v = scan(a + b);
+  if ((tid & 63) == 63) s->wave_b[wave] = v;
   __syncthreads();
-  for (int i = 0; i < kWavesPerRow; ++i) v += i < wave ? s->wave_b[i] : 0;
+  u64 all = 0;
+#pragma unroll
+  for (int i = 0; i < kWavesPerRow; ++i) {
+    const u64 w = s->wave_b[i];
+    v += i < wave ? w : 0;
+    all += w;
+  }
   const u64 front = v - a - b;
   if (front < need && v >= need) {
     const bool first = front + a >= need;
     s->bin = 2 * tid + (first ? 0 : 1);
-    s->before = front + (first ? 0 : a);
+    s->front = front + (first ? 0 : a);
   }
   __syncthreads();
+  return all;
 }
 
 __device__ __forceinline__ void clear(u64* sum) {
@@ -137,35 +177,66 @@ __device__ __forceinline__ void clear(unsigned* count) {
   count[threadIdx.x + kThreads] = 0u;
 }
 
-// ---- the row in vectors of 16 bytes: vector j * 1024 + tid in iteration j ----
+// ---- the row in vectors of 16 bytes ----
 template <typename T>
 struct RowReader {
   static constexpr int PER = 16 / sizeof(T);
   const T* row;
   int V;
-  // f(index, logit) for every element, four vectors of a thread requested at a time
+  __device__ __forceinline__ Vec16<T> whole_vector(const int v) const {
+    Vec16<T> x;
+    x.raw = reinterpret_cast<const Bytes16*>(row + (int64_t)v * PER)->v;
+    return x;
+  }
+  __device__ __forceinline__ Vec16<T> vector(const int v) const {   // -inf behind the row's end
+    if ((v + 1) * PER <= V) return whole_vector(v);
+    Vec16<T> x;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) x.set(e, v * PER + e < V ? Store<T>::ld(row + v * PER + e) : -__builtin_inff());
+    return x;
+  }
+  // f(vector's number, vector, 0 .. 3) for all of the row, four vectors of a thread requested at a time
   template <typename F>
-  __device__ __forceinline__ void each(F f) const {
+  __device__ __forceinline__ void each_vector(F f) const {
     const int full = V / PER;
     for (int v0 = threadIdx.x; v0 < full; v0 += 4 * kThreads) {
       Vec16<T> x[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (v0 + j * kThreads < full) x[j].raw = reinterpret_cast<const Bytes16*>(row + (int64_t)(v0 + j * kThreads) * PER)->v;
+        if (v0 + j * kThreads < full) x[j] = whole_vector(v0 + j * kThreads);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (v0 + j * kThreads < full)
-#pragma unroll
-          for (int e = 0; e < PER; ++e) f((v0 + j * kThreads) * PER + e, x[j].get(e));
+        if (v0 + j * kThreads < full) f(v0 + j * kThreads, x[j], j);
     }
-    const int rest = full * PER + (int)threadIdx.x;
-    if (rest < V) f(rest, Store<T>::ld(row + rest));
+    if (full * PER < V && threadIdx.x == 0) f(full, vector(full), 0);
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {    // f(index, logit)
+    each_vector([&](const int v, const Vec16<T>& x, const int) {
+#pragma unroll
+      for (int e = 0; e < PER; ++e) f(v * PER + e, x.get(e));
+    });
+  }
+  // f(index, logit) for every element of the vectors where some lane has one with test(logit)
+  template <typename P, typename F>
+  __device__ __forceinline__ void each_in(P test, F f) const {
+    each_vector([&](const int v, const Vec16<T>& x, const int) {
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) any = any || test(x.get(e));
+      if (any)
+        for (int e = 0; e < PER; ++e) {
+          const float l = x.get(e);
+          if (test(l)) f(v * PER + e, l);
+        }
+    });
   }
 };
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) {
   __shared__ Shared s;
+  constexpr int PER = RowReader<T>::PER, MINE = kList / kThreads;
   const int row_i = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const RowReader<T> row{(const T*)p.logits + (int64_t)row_i * p.V, p.V};
   const int V = p.V;
@@ -174,51 +245,63 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
   const float top_p = p.top_p ? p.top_p[(int64_t)row_i * p.step_p] : 1.f;
   const float min_p = p.min_p ? p.min_p[(int64_t)row_i * p.step_m] : 0.f;
   const float u = p.uniform[(int64_t)row_i * p.step_u];
-  if (tid < 64) s.power[tid] = exp2(tid * 0.015625);
-  if (tid == 0) s.listed = s.bordered = 0;
 
-  // ---- 1: the largest logit, its lowest index, and how many can be drawn ----
-  unsigned best = 0;
-  int at = V;
-  unsigned live = 0;
-  row.each([&](const int i, const float l) {
-    const unsigned k = key_of(l);
-    if (k > best || (k == best && i < at)) { best = k; at = i; }
-    live += k > kKeyOfMinusInf;
+  // ---- 1: the largest logit, and the vector where it first stands ----
+  // (each_vector's four vectors of a turn apart: four samples of a thread's elements)
+  float own[4] = {-__builtin_inff(), -__builtin_inff(), -__builtin_inff(), -__builtin_inff()};
+  int own_v[4] = {0, 0, 0, 0};
+  row.each_vector([&](const int v, const Vec16<T>& x, const int j) {
+    float m = x.get(0);
+#pragma unroll
+    for (int e = 1; e < PER; ++e) m = fmaxf(m, x.get(e));     // (a NaN is passed over)
+    if (m > own[j]) { own[j] = m; own_v[j] = v; }
   });
-  u64 pair = (u64)best << 32 | (unsigned)~at;
+  float best = own[0];
+  int best_v = own_v[0];
+#pragma unroll
+  for (int j = 1; j < 4; ++j)
+    if (own[j] > best || (own[j] == best && own_v[j] < best_v)) { best = own[j]; best_v = own_v[j]; }
+  u64 pair = (u64)key_of(best) << 32 | (unsigned)~best_v;
   for (int d = 32; d > 0; d >>= 1) {
     const u64 o = __shfl_xor(pair, d);
     pair = o > pair ? o : pair;
   }
   if (lane == 0) s.wave_a[wave] = pair;
+  if (tid < 64) s.power[tid] = exp2(tid * 0.015625);
+  if (tid == 0) s.listed = s.bordered = 0;
   __syncthreads();
+#pragma unroll
   for (int i = 0; i < kWavesPerRow; ++i) pair = s.wave_a[i] > pair ? s.wave_a[i] : pair;
   const unsigned top_key = (unsigned)(pair >> 32);
-  const int first = (int)~(unsigned)pair;
-  if (top_key <= kKeyOfMinusInf || !(temperature > 0.f) || top_k == 1 || min_p > 1.f) {   // nothing to draw from, or one token left
-    if (tid == 0) p.token[row_i] = top_key <= kKeyOfMinusInf ? -1 : first;
-    return;
-  }
-  const u64 live_all = block_sum_u64(live, s.wave_b);
   Row r;
   r.most = logit_of(top_key);
+  if (top_key <= kKeyOfMinusInf || !(temperature > 0.f) || top_k == 1 || min_p > 1.f) {   // nothing to draw from, or one token left
+    if (tid == 0) {
+      const int v = (int)~(unsigned)pair;
+      const Vec16<T> x = row.vector(v);
+      int at = -1;
+#pragma unroll
+      for (int e = PER - 1; e >= 0; --e) at = x.get(e) == r.most ? v * PER + e : at;
+      p.token[row_i] = top_key <= kKeyOfMinusInf ? -1 : at;
+    }
+    return;
+  }
+  r.per_f = 1.4426950408889634f / temperature;
+  r.most_d = (double)r.most;
   r.per = 1.4426950408889634 / (double)temperature;
-  // (a weight rounds to nothing from (max - l) / T = 45 ln 2 = 31.2 on: the last bin takes all of those)
-  r.per_bin = (float)kBins / 31.25f / temperature;
+  r.per_bin = (float)kBins / 45.1f * r.per_f;   // (weights round to nothing behind 2^-45)
   r.power = s.power;
-  const double least = (double)min_p * 17592186044416.0;   // (NaN: nothing is below)
+  const double least = (double)min_p * kOne;    // (NaN: nothing is below)
 
-  // Of everything at or above the first cut: the elements before and at (cut_key, cut_at) in the ranking are kept.
-  unsigned cut_key = kKeyOfMinusInf + 1;
+  // The elements up to (cut_l, cut_at) in the ranking are kept.
+  float cut_l = -3.402823466e38f;
   int cut_at = V;
-  auto in_cut = [&](const unsigned k, const int i) { return k > cut_key || (k == cut_key && i <= cut_at); };
+  auto in_cut = [&](const float l, const int i) { return (bool)((int)(l > cut_l) | ((int)(l == cut_l) & (int)(i <= cut_at))); };
 
   // Radix descent among the elements kept so far: the last that a cut at `need` (elements, or weight) keeps
-  // becomes the new cut; the weight of all that remain is returned.
-  auto descend = [&](const bool by_sum, u64 need) -> u64 {
+  // becomes the new cut.  That much must be there.
+  auto descend = [&](const bool by_sum, u64 need) {
     unsigned prefix = 0, known = 0;
-    u64 sum_front = 0;
     for (int level = 0; level < 3; ++level) {
       const int shift = level == 0 ? 21 : level == 1 ? 10 : 0;
       const unsigned mask = level == 2 ? 1023u : 2047u;
@@ -226,177 +309,216 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
       clear(s.sum);
       __syncthreads();
       row.each([&](const int i, const float l) {
+        if (!in_cut(l, i)) return;
         const unsigned k = key_of(l);
-        if ((k & known) != prefix || !in_cut(k, i)) return;
+        if ((k & known) != prefix) return;
         const unsigned b = mask - ((k >> shift) & mask);    // (the highest digit first)
-        atomicAdd(&s.count[b], 1u);
-        const u64 w = whole(weight(r, l));
-        if (w != 0) atomicAdd(&s.sum[b], w);
+        if (by_sum) atomicAdd(&s.sum[b], whole(weight(r, l)));
+        else atomicAdd(&s.count[b], 1u);
       });
       __syncthreads();
-      if (by_sum) find(&s, s.sum, need); else find(&s, s.count, need);
-      const int b = s.bin;
-      need -= s.before;
-      u64 front = 0;      // weight of the digits in front
-      for (int i = tid; i < b; i += kThreads) front += s.sum[i];
-      sum_front += block_sum_u64(front, s.wave_a);
-      prefix |= (mask - (unsigned)b) << shift;
+      if (by_sum) find(&s, s.sum, need);
+      else find(&s, s.count, need);
+      need -= s.front;
+      prefix |= (mask - (unsigned)s.bin) << shift;
       known |= mask << shift;
       __syncthreads();
     }
-    // `need` is what the elements equal to the key still have to give: the first `ties` of them
-    const u64 w = whole(weight(r, logit_of(prefix)));
+    // `need` is what the elements equal to the key still have to give: the first `ties` of them,
+    // counted by parts of the row
+    const float l0 = logit_of(prefix);
+    const u64 w = whole(weight(r, l0));
     const u64 ties = by_sum ? (w ? (need + w - 1) / w : 1) : need;
-    // the index of the last of them: ties counted by parts of 2048 / V of the row
     const int part = (V + kBins - 1) / kBins;
     clear(s.count);
     __syncthreads();
     row.each([&](const int i, const float l) {
-      if (key_of(l) == prefix && in_cut(prefix, i)) atomicAdd(&s.count[i / part], 1u);
+      if (l == l0 && in_cut(l, i)) atomicAdd(&s.count[i / part], 1u);
     });
     __syncthreads();
     find(&s, s.count, ties);
     if (tid == 0) {
-      u64 seen = s.before;
+      u64 seen = s.front;
       int i = s.bin * part;
       for (; i < V; ++i)
-        if (key_of(Store<T>::ld(row.row + i)) == prefix && in_cut(prefix, i) && ++seen == ties) break;
+        if (Store<T>::ld(row.row + i) == l0 && in_cut(l0, i) && ++seen == ties) break;
       s.cut_at = i;
     }
     __syncthreads();
-    cut_key = prefix;
+    cut_l = l0;
     cut_at = s.cut_at;
     __syncthreads();
-    return sum_front + ties * w;
   };
 
-  bool listed = false;      // the candidates are in s.key / s.index
-  // of them this thread's, strided; weight 0, bin kBins: not kept
-  u64 kept_w[kList / kThreads];
-  unsigned kept_key[kList / kThreads];
-  int kept_i[kList / kThreads], kept_bin[kList / kThreads];
+  bool listed = false;      // the candidates are in s.logit / s.index
+  // of them this thread's, strided; weight 0, bin kBins + 1: not kept
+  u64 kept_w[MINE];
+  float kept_l[MINE];
+  int kept_i[MINE], kept_bin[MINE];
 
-  const bool cut_k = top_k > 0 && (u64)top_k < live_all;
-  if (cut_k) {
-    // ---- 2: where the k-th element stands ----
-    clear(s.count);
-    __syncthreads();
-    row.each([&](const int i, const float l) {
-      if (key_of(l) > kKeyOfMinusInf) atomicAdd(&s.count[bin_of(r, l)], 1u);
-    });
-    __syncthreads();
-    find(&s, s.count, (u64)top_k);
-    const int last = s.bin;
-    const unsigned front = (unsigned)s.before, in_bin = s.count[last];
-    if (front + in_bin <= kList && in_bin <= kBorder) {
-      // ---- 3: those up to its bin, and the elements of the bin against each other ----
-      listed = true;
-      row.each([&](const int i, const float l) {
-        const unsigned k = key_of(l);
-        if (k <= kKeyOfMinusInf) return;
-        const int b = bin_of(r, l);
-        if (b > last) return;
-        const int n = atomicAdd(&s.listed, 1);
-        s.key[n] = k;
-        s.index[n] = i;
-        if (b == last) s.border[atomicAdd(&s.bordered, 1)] = n;
-      });
+  bool cut_k = top_k > 0 && top_k < V;
+  if (cut_k && top_k <= kList / 2) {
+    // ---- 2: a bound that at least top_k elements reach.  The bin of the top_k-th of the threads' largest, and the
+    // least of those up to it (fewer than that exist, or it lies behind the bins: the descent); any, where the
+    // list holds the row ----
+    float bound = -3.402823466e38f;
+    bool bounded = V <= kList;
+    if (!bounded) {
+      clear(s.count);
       __syncthreads();
-      const int n = s.listed, m = s.bordered;
-      if (tid < m) {
-        const int c = s.border[tid];
-        const unsigned k = s.key[c];
-        const int i = s.index[c];
-        unsigned rank = front;
-        for (int j = 0; j < m; ++j) {
-          const int o = s.border[j];
-          rank += s.key[o] > k || (s.key[o] == k && s.index[o] < i);
-        }
-        if (rank + 1 == (unsigned)top_k) { s.cut_key = k; s.cut_at = i; }
+      int own_bin[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        own_bin[j] = own[j] > -__builtin_inff() ? bin_of(r, own[j]) : kBins;
+        if (own_bin[j] < kBins) atomicAdd(&s.count[own_bin[j]], 1u);
       }
       __syncthreads();
-      cut_key = s.cut_key;
-      cut_at = s.cut_at;
+      bounded = find(&s, s.count, (u64)top_k) >= (u64)top_k;
+      if (bounded) {
+        float least_own = r.most;
 #pragma unroll
-      for (int j = 0; j < kList / kThreads; ++j) {
-        const int c = tid + j * kThreads;
-        kept_w[j] = 0;
-        kept_key[j] = 0;
-        kept_i[j] = 0;
-        kept_bin[j] = kBins;
-        if (c < n && in_cut(s.key[c], s.index[c])) {
-          kept_key[j] = s.key[c];
-          kept_i[j] = s.index[c];
-          const float l = logit_of(s.key[c]);
-          kept_bin[j] = bin_of(r, l);
-          kept_w[j] = whole(weight(r, l));
+        for (int j = 0; j < 4; ++j)
+          if (own_bin[j] <= s.bin) least_own = fminf(least_own, own[j]);
+        bound = -block_max<kThreads>(-least_own, s.wave_f);
+      }
+    }
+    if (bounded) {
+      // ---- 3: the candidates, and their bins ----
+      clear(s.count);
+      __syncthreads();
+      row.each_in([&](const float l) { return l >= bound; }, [&](const int i, const float l) {
+        const int n = atomicAdd(&s.listed, 1);
+        if (n < kList) {
+          s.logit[n] = l;
+          s.index[n] = i;
+          const int b = bin_of(r, l);
+          if (b < kBins) atomicAdd(&s.count[b], 1u);
+        }
+      });
+      __syncthreads();
+      const int n = s.listed;
+      const bool cut = n >= top_k;     // (the list may hold a row with fewer)
+      if (n <= kList && (!cut || find(&s, s.count, (u64)top_k) >= (u64)top_k)) {
+        const int edge = cut ? s.bin : kBins + 1;
+        const unsigned front = (unsigned)s.front;
+        if (!cut || s.count[edge] <= kBorder) {
+          listed = true;
+#pragma unroll
+          for (int j = 0; j < MINE; ++j) {
+            const int c = tid + j * kThreads;
+            kept_l[j] = c < n ? s.logit[c] : 0.f;
+            kept_i[j] = c < n ? s.index[c] : 0;
+            kept_bin[j] = c < n ? bin_of(r, kept_l[j]) : kBins + 1;
+            if (cut && kept_bin[j] == edge) s.border[atomicAdd(&s.bordered, 1)] = c;
+          }
+          __syncthreads();
+          const int m = s.bordered;
+          if (tid == 0 && !cut) { s.cut_l = cut_l; s.cut_at = cut_at; }
+          if (tid < m) {     // the elements of that bin against each other
+            const int c = s.border[tid];
+            const float l = s.logit[c];
+            const int i = s.index[c];
+            unsigned rank = front;
+            for (int j = 0; j < m; ++j) rank += before(s.logit[s.border[j]], s.index[s.border[j]], l, i);
+            if (rank + 1 == (unsigned)top_k) { s.cut_l = l; s.cut_at = i; }
+          }
+          __syncthreads();
+          cut_l = s.cut_l;
+          cut_at = s.cut_at;
+#pragma unroll
+          for (int j = 0; j < MINE; ++j) {
+            const bool in = kept_bin[j] <= kBins && in_cut(kept_l[j], kept_i[j]);
+            kept_w[j] = in ? whole(weight(r, kept_l[j])) : 0;
+            if (!in) kept_bin[j] = kBins + 1;
+          }
         }
       }
     }
   }
-
-  u64 total = 0;     // weight of what top-k keeps, where top-p asks for it
-  if (cut_k && !listed) total = descend(false, (u64)top_k);
+  if (cut_k && !listed) {
+    u64 live = 0;
+    row.each([&](const int, const float l) { live += l >= -3.402823466e38f; });
+    cut_k = block_sum_u64(live, s.wave_a) > (u64)top_k;
+    if (cut_k) descend(false, (u64)top_k);
+  }
 
   if (top_p < 1.f) {
     // ---- 2 and 3 of a cut by weight ----
+    u64 total = 0;
     clear(s.sum);
     if (tid == 0) s.bordered = 0;
-    __syncthreads();
     if (listed) {
+      __syncthreads();
 #pragma unroll
-      for (int j = 0; j < kList / kThreads; ++j)
+      for (int j = 0; j < MINE; ++j)
         if (kept_w[j] != 0) { total += kept_w[j]; atomicAdd(&s.sum[kept_bin[j]], kept_w[j]); }
     } else {
-      total = 0;
-      row.each([&](const int i, const float l) {
-        const unsigned k = key_of(l);
-        if (!in_cut(k, i)) return;
-        const u64 w = whole(weight(r, l));
-        if (w != 0) { total += w; atomicAdd(&s.sum[bin_of(r, l)], w); }
+      // Behind 2^-e of the largest weight, e = log2(V / ((1 - p) S)) + 1, all elements together weigh at most half
+      // of (1 - p) S: the cut is in front of it.  For S, the sum of all weights, serves that of the threads' largest.
+      // (After a cut by number that may be too much: the bins then end where weights round to nothing.)
+      float e = 45.1f;
+      if (!cut_k) {
+        float w = __builtin_amdgcn_exp2f((best - r.most) * r.per_f);
+        w = block_sum<kThreads>(w >= 0.f && w <= 1.f ? w : 0.f, s.wave_f);
+        e = fmaxf(1.f, fminf(e, __log2f((float)V / ((1.f - top_p) * fmaxf(w, 1.f))) + 1.01f));
+      }
+      r.per_bin = (float)kBins / e * r.per_f;
+      __syncthreads();
+      row.each_vector([&](const int v, const Vec16<T>& x, const int) {
+        u64 w[PER];
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          const float l = x.get(e);
+          w[e] = whole(weight(r, l)) & ((int)!cut_k | (int)in_cut(l, v * PER + e) ? ~0ull : 0ull);
+          total += w[e];
+        }
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          const int b = bin_of(r, x.get(e));
+          if (b < kBins && w[e] != 0) atomicAdd(&s.sum[b], w[e]);
+        }
       });
     }
     total = block_sum_u64(total, s.wave_a);
     const double want = ceil((double)top_p * (double)total);
     const u64 need = want > 1.0 ? (u64)want : 1ull;
     if (need < total) {
-      find(&s, s.sum, need);
-      const int last = s.bin;
-      const u64 front = s.before;
-      // the elements of that bin, ranked against each other (their keys and indices in s.key / s.index;
+      const bool binned = find(&s, s.sum, need) >= need;
+      const int edge = s.bin;
+      const u64 front = s.front;
+      // the elements of that bin, ranked against each other (their logits and indices in s.logit / s.index;
       // s.sum is done with and takes their weights)
-      if (listed) {
-        // (the list itself: positions of its elements)
+      if (binned && listed) {
 #pragma unroll
-        for (int j = 0; j < kList / kThreads; ++j)
-          if (kept_bin[j] == last) {
+        for (int j = 0; j < MINE; ++j)
+          if (kept_bin[j] == edge) {
             const int n = atomicAdd(&s.bordered, 1);
             if (n < kBorder) { s.border[n] = tid + j * kThreads; s.sum[n] = kept_w[j]; }
           }
-      } else {
-        row.each([&](const int i, const float l) {
-          const unsigned k = key_of(l);
-          if (!in_cut(k, i) || bin_of(r, l) != last) return;
-          const int n = atomicAdd(&s.bordered, 1);
-          if (n < kBorder) { s.border[n] = n; s.key[n] = k; s.index[n] = i; s.sum[n] = whole(weight(r, l)); }
+      } else if (binned) {
+        // (logits beside the middle of the bin by more than half of its width, and a little, are not in it)
+        const float middle = r.most - ((float)edge + 0.5f) / r.per_bin;
+        const float half = 0.5f / r.per_bin + 1e-5f * (fabsf(r.most) + fabsf(middle));
+        row.each_in([&](const float l) { return !(fabsf(l - middle) > half); }, [&](const int i, const float l) {
+          if (l > -__builtin_inff() && bin_of(r, l) == edge && in_cut(l, i)) {
+            const int n = atomicAdd(&s.bordered, 1);
+            if (n < kBorder) { s.border[n] = n; s.logit[n] = l; s.index[n] = i; s.sum[n] = whole(weight(r, l)); }
+          }
         });
       }
       __syncthreads();
       const int m = s.bordered;
-      if (m <= kBorder) {
+      if (binned && m <= kBorder) {
         if (tid < m) {
           const int c = s.border[tid];
-          const unsigned k = s.key[c];
+          const float l = s.logit[c];
           const int i = s.index[c];
-          u64 before = front;
-          for (int j = 0; j < m; ++j) {
-            const int o = s.border[j];
-            before += s.key[o] > k || (s.key[o] == k && s.index[o] < i) ? s.sum[j] : 0;
-          }
-          if (before < need && before + s.sum[tid] >= need) { s.cut_key = k; s.cut_at = i; }
+          u64 ahead = front;
+          for (int j = 0; j < m; ++j) ahead += before(s.logit[s.border[j]], s.index[s.border[j]], l, i) ? s.sum[j] : 0;
+          if (ahead < need && ahead + s.sum[tid] >= need) { s.cut_l = l; s.cut_at = i; }
         }
         __syncthreads();
-        cut_key = s.cut_key;
+        cut_l = s.cut_l;
         cut_at = s.cut_at;
         __syncthreads();
       } else {
@@ -416,8 +538,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
     __syncthreads();
     u64 all = 0;
 #pragma unroll
-    for (int j = 0; j < kList / kThreads; ++j) {
-      if (kept_w[j] == 0 || !in_cut(kept_key[j], kept_i[j]) || weight(r, logit_of(kept_key[j])) < least) kept_w[j] = 0;
+    for (int j = 0; j < MINE; ++j) {
+      if (kept_w[j] == 0 || !in_cut(kept_l[j], kept_i[j]) || weight(r, kept_l[j]) < least) kept_w[j] = 0;
       if (kept_w[j] != 0) { all += kept_w[j]; atomicAdd(&s.sum[kept_i[j] / part], kept_w[j]); }
     }
     all = block_sum_u64(all, s.wave_a);
@@ -426,10 +548,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
     if (target >= all) target = all - 1;
     find(&s, s.sum, target + 1);
     const int b = s.bin;
-    const u64 front = s.before;
+    const u64 front = s.front;
     // (at most `part` <= 256 elements; s.sum is done with and takes their weights)
 #pragma unroll
-    for (int j = 0; j < kList / kThreads; ++j)
+    for (int j = 0; j < MINE; ++j)
       if (kept_w[j] != 0 && kept_i[j] / part == b) {
         const int n = atomicAdd(&s.bordered, 1);
         s.border[n] = kept_i[j];
@@ -438,60 +560,62 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
     __syncthreads();
     const int m = s.bordered;
     if (tid < m) {
-      u64 before = front;
-      for (int j = 0; j < m; ++j) before += s.border[j] < s.border[tid] ? s.sum[j] : 0;
-      if (before <= target && before + s.sum[tid] > target) p.token[row_i] = s.border[tid];
+      u64 ahead = front;
+      for (int j = 0; j < m; ++j) ahead += s.border[j] < s.border[tid] ? s.sum[j] : 0;
+      if (ahead <= target && ahead + s.sum[tid] > target) p.token[row_i] = s.border[tid];
     }
     return;
   }
-  constexpr int PER = RowReader<T>::PER;
   auto kept = [&](const int i, const float l) -> u64 {
-    if (!in_cut(key_of(l), i)) return 0;
     const double w = weight(r, l);
-    return w < least ? 0 : whole(w);
+    return whole(w) & ((int)in_cut(l, i) & (int)!(w < least) ? ~0ull : 0ull);
   };
-  // a wavefront's vectors of iteration j are part 16 j + wave of the row, 64 x PER elements
-  const int vectors = (V + PER - 1) / PER, parts = (vectors + 63) / 64;
+  // a part is 256 neighbouring vectors of the row, four per lane of a wavefront
+  const int vectors = (V + PER - 1) / PER, parts = (vectors + 255) / 256;
   clear(s.sum);
   __syncthreads();
   u64 all = 0;
-  auto vector_sum = [&](const int v, u64 (&w)[PER]) {   // of vector v, and its weights
-    u64 sum = 0;
-    if ((v + 1) * PER <= V) {
-      Vec16<T> x;
-      x.raw = reinterpret_cast<const Bytes16*>(row.row + (int64_t)v * PER)->v;
-#pragma unroll
-      for (int e = 0; e < PER; ++e) sum += w[e] = kept(v * PER + e, x.get(e));
-    } else {
-#pragma unroll
-      for (int e = 0; e < PER; ++e) sum += w[e] = v * PER + e < V ? kept(v * PER + e, Store<T>::ld(row.row + v * PER + e)) : 0;
-    }
-    return sum;
-  };
   for (int part = wave; part < parts; part += kWavesPerRow) {
-    u64 w[PER];
-    const u64 sum = wave_sum_u64(vector_sum(part * 64 + lane, w));
-    all += sum;
-    if (lane == 0) s.sum[part] = sum;
+    Vec16<T> x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = row.vector(part * 256 + j * 64 + lane);
+    u64 sum = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) any = any || x[j].get(e) >= cut_l;
+      if (any)
+#pragma unroll
+        for (int e = 0; e < PER; ++e) sum += kept((part * 256 + j * 64 + lane) * PER + e, x[j].get(e));
+    }
+    sum = scan(sum);
+    if (lane == 63) { s.sum[part] = sum; all += sum; }
   }
-  all = block_sum_u64(lane == 0 ? all : 0, s.wave_a);
+  all = block_sum_u64(all, s.wave_a);
   const double want = floor((double)u * (double)all);
   u64 target = want > 0.0 ? (u64)want : 0ull;
   if (target >= all) target = all - 1;
   find(&s, s.sum, target + 1);
   if (wave == 0) {
-    u64 w[PER];
-    const u64 sum = vector_sum(s.bin * 64 + lane, w);
-    u64 upto = sum;
-    for (int d = 1; d < 64; d <<= 1) {
-      const u64 o = __shfl_up(upto, d);
-      if (lane >= d) upto += o;
-    }
-    u64 before = s.before + upto - sum;
+    u64 ahead = s.front;
+    Vec16<T> x[4];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      if (before <= target && before + w[e] > target) p.token[row_i] = (s.bin * 64 + lane) * PER + e;
-      before += w[e];
+    for (int j = 0; j < 4; ++j) x[j] = row.vector(s.bin * 256 + j * 64 + lane);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int v = s.bin * 256 + j * 64 + lane;
+      u64 w[PER], sum = 0;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) sum += w[e] = kept(v * PER + e, x[j].get(e));
+      const u64 upto = scan(sum);
+      u64 at = ahead + upto - sum;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        if (at <= target && at + w[e] > target) p.token[row_i] = v * PER + e;
+        at += w[e];
+      }
+      ahead += last_lane(upto);
     }
   }
 }
