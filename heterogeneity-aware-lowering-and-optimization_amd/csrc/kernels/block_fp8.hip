@@ -128,12 +128,12 @@ __global__ void __launch_bounds__(512) block_gemm_rows_kernel(const BlockGemmPar
   }
 }
 
-// Many rows: a workgroup of four wavefronts owns 128 columns n x BM rows m; both operands pass
+// More rows: a workgroup of four wavefronts owns BN columns n x BM rows m; both operands pass
 // through LDS, 128 terms at a time, the next block's in registers meanwhile.
-template <typename TOut, int BM, bool ALIGNED>
+template <typename TOut, int BM, int BN, bool ALIGNED>
 __global__ void __launch_bounds__(256) block_gemm_tile_kernel(const BlockGemmParams p) {
   constexpr bool EXACT = sizeof(TOut) == 4;
-  constexpr int BN = 128, PITCH = kScaleBlock + 16;   // (16 bytes more: sixteen rows start in different banks)
+  constexpr int PITCH = kScaleBlock + 16;   // (16 bytes more: sixteen rows start in different banks)
   constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16;
   constexpr int NB = BN * 8 / 256, NA = BM * 8 / 256;  // 16-byte chunks a thread brings of either
   __shared__ __attribute__((aligned(16))) unsigned char sa[BM * PITCH], sb[BN * PITCH];
@@ -202,6 +202,134 @@ __global__ void __launch_bounds__(256) block_gemm_tile_kernel(const BlockGemmPar
     }
 }
 
+// Many rows and columns: 256 x 256 results a workgroup of eight wavefronts, 128 rows m x 64 columns n each.
+// Both operands come by direct-to-LDS loads, 128 terms (64 KiB) at a time into one of two buffers while
+// the other is multiplied: one barrier per block of terms, and every fragment of B stays in registers
+// through the eight of A.  LDS rows are 128 bytes, 16-byte chunk c of row r in slot c ^ (r / 2 & 7): the
+// sixteen rows of a fragment read then lie in different banks.
+constexpr int kBigStage = 512 * kScaleBlock;          // bytes of a buffer: 256 rows of A, 256 of B
+constexpr int kBigLds = 2 * kBigStage + 2 * 512 * 4;  // and the scales of the rows of A (twice: every thread stores one)
+// A wavefront's request i is of rows 64 i + 8 wave .. + 7; what lies behind the operand's end, or in the last
+// block behind the row's, is out of the buffer's range and arrives as zeros.
+struct BigSource {
+  __amdgpu_buffer_rsrc_t a, b;
+  unsigned at;     // this lane's offset in request 0 of a block
+  unsigned step;   // 64 rows
+  int left;        // bytes of a row from this lane's chunk on
+};
+__device__ __forceinline__ void big_request(const BigSource& f, const int kb, unsigned char* to) {
+  using lds_ptr = __attribute__((address_space(3))) void*;
+#if defined(__HIP_DEVICE_COMPILE__)
+  const unsigned at = kb * kScaleBlock < f.left ? f.at : 0xfffffff0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(f.a, (lds_ptr)(to + i * 8192), 16, at, i * f.step + kb * kScaleBlock, 0, 0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(f.b, (lds_ptr)(to + 32768 + i * 8192), 16, at, i * f.step + kb * kScaleBlock, 0, 0);
+#else
+  (void)f; (void)kb; (void)to;
+#endif
+}
+
+// One block of terms: the next one is requested into `next`, the one in `now` multiplied.  The two
+// never overlap (without saying so, every read of LDS would wait for the requests).
+__device__ __forceinline__ void big_block(const BigSource& from, const int kb, unsigned char* __restrict next, const unsigned char* __restrict now,
+                                          const float* __restrict scales, const float sb, const int wm, const int wn, const int lane, const int wave,
+                                          floatx4 (&acc)[8][4]) {
+  big_request(from, kb + 1, next + wave * 1024);   // (behind the last block: zeros)
+  const int r = lane & 15, g = lane >> 4;
+  const int sw = r >> 1;      // (rows of a fragment start at multiples of 16)
+  const int c0 = ((2 * g) ^ sw) * 16, c1 = ((2 * g + 1) ^ sw) * 16;
+  uintx4 w0[4], w1[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const unsigned char* at = now + (256 + wn + 16 * j + r) * kScaleBlock;
+    w0[j] = *reinterpret_cast<const uintx4*>(at + c0);
+    w1[j] = *reinterpret_cast<const uintx4*>(at + c1);
+  }
+  // In turn i the matrix cores multiply fragment i of A, the vector units scale the products of fragment
+  // i - 1, and fragment i + 1 is on its way (left to itself the compiler issues all products of the
+  // block first and spills them).
+  uintx4 x[2][2];
+  floatx4 part[2][4];
+  float s[2];
+  auto fetch = [&](const int i) __attribute__((always_inline)) {
+    const unsigned char* at = now + (wm + 16 * i + r) * kScaleBlock;
+    x[i & 1][0] = *reinterpret_cast<const uintx4*>(at + c0);
+    x[i & 1][1] = *reinterpret_cast<const uintx4*>(at + c1);
+    s[i & 1] = scales[wm + 16 * i + r];
+  };
+  auto scale = [&](const int i, const float by) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(part[i & 1][j][e], by, acc[i][j][e]);
+  };
+  fetch(0);
+  float by = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float mine = s[i & 1] * sb;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) part[i & 1][j] = mma_e4m3(w0[j], w1[j], x[i & 1][0], x[i & 1][1], floatx4{0.f, 0.f, 0.f, 0.f});
+    if (i + 1 < 8) fetch(i + 1);
+    if (i > 0) scale(i - 1, by);
+    by = mine;
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  scale(7, by);
+}
+
+template <typename TOut>
+__global__ void __launch_bounds__(512, 2) block_gemm_big_kernel(const BlockGemmParams p, const int tiles_m, const int tiles_n) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  float* const scales = reinterpret_cast<float*>(smem + 2 * kBigStage);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // Workgroups are dealt round-robin to the 8 XCDs: an XCD takes neighbours of a walk through groups of
+  // eight tiles of rows, so that its workgroups share both operands in its L2.
+  int t = blockIdx.x;
+  {
+    const int per = gridDim.x >> 3;
+    if (t < per << 3) t = (t & 7) * per + (t >> 3);
+  }
+  const int group = t / (8 * tiles_n), rows = min(8, tiles_m - 8 * group), in = t - group * 8 * tiles_n;
+  const int m0 = (8 * group + in % rows) * 256, n0 = in / rows * 256;
+  const int KB = (p.K + kScaleBlock - 1) / kScaleBlock;
+  const int chunk = ((lane & 7) ^ (((8 * wave + (lane >> 3)) >> 1) & 7)) * 16;
+  BigSource from;
+  from.a = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.a) + (int64_t)m0 * p.K, 0, min(256, p.M - m0) * p.K, 0x00020000);
+  from.b = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.b) + (int64_t)n0 * p.K, 0, min(256, p.N - n0) * p.K, 0x00020000);
+  from.at = (8 * wave + (lane >> 3)) * p.K + chunk;
+  from.step = 64u * p.K;
+  from.left = p.K - chunk;
+  const float* arow_scale = p.a_scale + (int64_t)min(m0 + (tid & 255), p.M - 1) * KB;
+  const int wm = (wave & 1) * 128, wn = (wave >> 1) * 64;
+  const float* bs = p.b_scale + (int64_t)min((n0 + wn) / kScaleBlock, (p.N - 1) / kScaleBlock) * KB;
+  floatx4 acc[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  scales[tid] = arow_scale[0];
+  float sb = bs[0];
+  big_request(from, 0, smem + wave * 1024);
+  for (int kb = 0; kb < KB; ++kb) {
+    __syncthreads();     // this block's operands have landed, and everybody has left the other buffer
+    // (both scales of the next block ahead of its operands: a wait for them would wait for those too)
+    const float next_scale = arow_scale[min(kb + 1, KB - 1)], next_sb = bs[min(kb + 1, KB - 1)];
+    big_block(from, kb, smem + (~kb & 1) * kBigStage, smem + (kb & 1) * kBigStage, scales + (kb & 1) * 512, sb, wm, wn, lane, wave, acc);
+    scales[(~kb & 1) * 512 + tid] = next_scale;
+    sb = next_sb;
+  }
+  const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int m = m0 + wm + 16 * i + r, n = n0 + wn + 16 * j + 4 * g;
+      if (m < p.M && n < p.N) store4((TOut*)p.y + (int64_t)m * p.N + n, acc[i][j], p.N - n, (p.N & 3) == 0);
+    }
+}
+
 template <typename TOut, int MT, bool ALIGNED>
 hipError_t gemm_rows(const BlockGemmParams& p, hipStream_t stream) {
   const int KB = (p.K + kScaleBlock - 1) / kScaleBlock;
@@ -214,7 +342,20 @@ hipError_t gemm_as(const BlockGemmParams& p, hipStream_t stream) {
   if (p.M <= 16) return gemm_rows<TOut, 1, ALIGNED>(p, stream);
   if (p.M <= 32) return gemm_rows<TOut, 2, ALIGNED>(p, stream);
   if (p.M <= 64) return gemm_rows<TOut, 4, ALIGNED>(p, stream);
-  hipLaunchKernelGGL((block_gemm_tile_kernel<TOut, 128, ALIGNED>), dim3((p.N + 127) / 128, (p.M + 127) / 128), dim3(256), 0, stream, p);
+  const int64_t tm = (p.M + 255) / 256, tn = (p.N + 255) / 256;
+  if constexpr (ALIGNED && sizeof(TOut) == 2) {
+    if (tm * tn >= 192 && p.K <= 1 << 22) {   // (256 rows of an operand within 2^30 bytes of buffer range)
+      static LdsLimit limit;
+      hipError_t e = limit.raise(reinterpret_cast<const void*>(&block_gemm_big_kernel<TOut>), kBigLds);
+      if (e != hipSuccess) return e;
+      hipLaunchKernelGGL((block_gemm_big_kernel<TOut>), dim3((unsigned)(tm * tn)), dim3(512), kBigLds, stream, p, (int)tm, (int)tn);
+      return hipGetLastError();
+    }
+  }
+  if ((int64_t)((p.M + 127) / 128) * ((p.N + 127) / 128) >= 256)
+    hipLaunchKernelGGL((block_gemm_tile_kernel<TOut, 128, 128, ALIGNED>), dim3((p.N + 127) / 128, (p.M + 127) / 128), dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL((block_gemm_tile_kernel<TOut, 64, 64, ALIGNED>), dim3((p.N + 63) / 64, (p.M + 63) / 64), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 

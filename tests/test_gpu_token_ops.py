@@ -590,3 +590,23 @@ def test_the_largest_vocabulary(odla):
     p = {"top_k": [0, 0, 50, 5000, 0, 200000], "top_p": [1.0, 0.9, 0.9, 1.0, 0.999, 0.5], "min_p": [0, 0, 0, 0, 0.01, 0], "uniform": rng.random(6)}
     got, want = run_sample(odla, "fp32", x, p)
     assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("m,n,k", [(3500, 3500, 400), (4100, 3080, 128), (257, 49000, 272)])
+def test_block_product_of_many_tiles(odla, kind, m, n, k):
+    """Sizes that give every compute unit a large tile; checked on rows and columns across the edges of tiles."""
+    announce("block product %s %d x %d x %d" % (kind, m, n, k))
+    rng = np.random.default_rng(m + n)
+    a = (rng.integers(0, 256, (m, k), dtype=np.uint8) & 0xbf, rng.uniform(0.5, 2, (m, R.blocks(k))).astype(np.float32))
+    b = (rng.integers(0, 256, (n, k), dtype=np.uint8) & 0xbf, rng.uniform(0.001, 0.1, (R.blocks(n), R.blocks(k))).astype(np.float32))
+    got = R.values(run_hip(gemm_graph(odla, kind, a, b), {"a": a[0], "sa": a[1], "b": b[0], "sb": b[1]})["y"], kind)
+    rows = np.unique(np.concatenate([np.arange(0, m, 97), [m - 1, 255, 256], np.arange(120, 136)]))
+    for at in (slice(0, 300), slice(n - 300, n)):
+        cols = np.arange(n)[at]
+        bb = b[0][cols]
+        want = R.row_values(a[0][rows], a[1][rows]) @ (R.e4m3_decode(bb) * np.repeat(b[1][cols // R.BLOCK], R.BLOCK, axis=1)[:, :k]).T
+        big = np.abs(R.row_values(a[0][rows], a[1][rows])) @ np.abs(R.e4m3_decode(bb) * np.repeat(b[1][cols // R.BLOCK], R.BLOCK, axis=1)[:, :k]).T
+        # eight products: all but the largest lose up to 2^-13 of it; sums in fp32; the result's own rounding
+        bound = (7 * 2.0 ** -13 + (R.BLOCK + R.blocks(k) + 3) * R.UNIT) * big + R.EPS[kind] / 2 * np.abs(want) * (1 + 2.0 ** -9)
+        check(got[rows][:, cols], want, bound, "product", kind)
