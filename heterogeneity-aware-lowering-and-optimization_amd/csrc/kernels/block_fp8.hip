@@ -74,19 +74,23 @@ hipError_t quantize_as(const void* x, void* q, float* scale, int64_t rows, int64
 }
 
 // ------------------------------------------------------------------ product --
-// Few rows: y^T tile of 16 columns (rows n of B) x 16 MT rows m of A per workgroup.  The weights are
-// read once, straight into the operand registers; the wavefronts of a workgroup take every
-// blockDim / 64-th block of 128 terms and their sums meet in LDS in wavefront order.  A block's sum is
-// scaled on its way into the accumulator: the scale of row m belongs to a lane (column of the matrix
-// result), that of B to the whole tile.
-template <typename TOut, int MT, bool ALIGNED>
+// Few rows: a workgroup owns 16 NT columns n x 16 MT rows m.  The weights are read once, straight into the
+// operand registers; the wavefronts take every blockDim / 64-th block of 128 terms and their sums meet
+// in LDS in wavefront order.  A block's sum is scaled on its way into the accumulator: the scale of row m
+// belongs to a lane (column of the matrix result), that of B to the whole tile.  Bound by the weights' way
+// from memory for one row; with more, the rows of A come from L2 once per workgroup, so that two tiles
+// of columns share them.  EXACT: through bf16 (see mma_exact).
+template <typename TOut, int MT, int NT, bool EXACT, bool ALIGNED>
 __global__ void __launch_bounds__(512) block_gemm_rows_kernel(const BlockGemmParams p) {
-  __shared__ floatx4 sums[8][MT][64];
+  constexpr int UN = MT == 1 ? 4 : 2;      // blocks of terms requested at a time
+  __shared__ floatx4 sums[8][NT * MT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int r = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * MT);
+  const int n0 = blockIdx.x * (16 * NT), m0 = blockIdx.y * (16 * MT);
   const int KB = (p.K + kScaleBlock - 1) / kScaleBlock;
-  const unsigned char* brow = p.b + (int64_t)min(n0 + r, p.N - 1) * p.K;
+  const unsigned char* brow[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) brow[j] = p.b + (int64_t)min(n0 + 16 * j + r, p.N - 1) * p.K;
   const unsigned char* arow[MT];
   const float* as[MT];
 #pragma unroll
@@ -96,34 +100,64 @@ __global__ void __launch_bounds__(512) block_gemm_rows_kernel(const BlockGemmPar
     as[t] = p.a_scale + m * KB;
   }
   const float* bs = p.b_scale + (int64_t)(n0 / kScaleBlock) * KB;
-  floatx4 acc[MT];
+  floatx4 acc[NT][MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-  for (int kb = wave; kb < KB; kb += waves) {
-    const int64_t k = (int64_t)kb * kScaleBlock + g * 32;
-    const uintx4 w0 = load_row16<ALIGNED>(brow, k, p.K), w1 = load_row16<ALIGNED>(brow, k + 16, p.K);
-    const float sb = bs[kb];
-    uintx4 wv[4];
-    bf16_of_e4m3(w0, w1, wv);
+  for (int j = 0; j < NT; ++j)
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const uintx4 x0 = load_row16<ALIGNED>(arow[t], k, p.K), x1 = load_row16<ALIGNED>(arow[t], k + 16, p.K);
-      uintx4 xv[4];
-      bf16_of_e4m3(x0, x1, xv);
-      const floatx4 part = mma_exact(wv, xv);
-      const float s = as[t][kb] * sb;
+    for (int t = 0; t < MT; ++t) acc[j][t] = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int kb0 = wave; kb0 < KB; kb0 += UN * waves) {
+    uintx4 w[UN][NT][2], x[UN][MT][2];
+    float sa[UN][MT], sb[UN];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf(part[i], s, acc[t][i]);
+    for (int q = 0; q < UN; ++q) {
+      const int kb = kb0 + q * waves;
+      if (kb >= KB) break;
+      const int64_t k = (int64_t)kb * kScaleBlock + g * 32;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int v = 0; v < 2; ++v) w[q][j][v] = load_row16<ALIGNED>(brow[j], k + 16 * v, p.K);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+#pragma unroll
+        for (int v = 0; v < 2; ++v) x[q][t][v] = load_row16<ALIGNED>(arow[t], k + 16 * v, p.K);
+        sa[q][t] = as[t][kb];
+      }
+      sb[q] = bs[kb];
+    }
+#pragma unroll
+    for (int q = 0; q < UN; ++q) {
+      if (kb0 + q * waves >= KB) break;
+      uintx4 wv[EXACT ? NT : 1][4];
+      if constexpr (EXACT) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) bf16_of_e4m3(w[q][j][0], w[q][j][1], wv[j]);
+      }
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        uintx4 xv[4];
+        if constexpr (EXACT) bf16_of_e4m3(x[q][t][0], x[q][t][1], xv);
+        const float s = sa[q][t] * sb[q];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          floatx4 part;
+          if constexpr (EXACT) part = mma_exact(wv[j], xv);
+          else part = mma_e4m3(w[q][j][0], w[q][j][1], x[q][t][0], x[q][t][1], floatx4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[j][t][i] = __builtin_fmaf(part[i], s, acc[j][t][i]);
+        }
+      }
     }
   }
 #pragma unroll
-  for (int t = 0; t < MT; ++t) sums[wave][t][lane] = acc[t];
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) sums[wave][j * MT + t][lane] = acc[j][t];
   __syncthreads();
-  for (int t = wave; t < MT; t += waves) {
-    floatx4 v = sums[0][t][lane];
-    for (int w = 1; w < waves; ++w) v += sums[w][t][lane];
-    const int m = m0 + 16 * t + r, n = n0 + 4 * g;
+  for (int q = wave; q < NT * MT; q += waves) {
+    floatx4 v = sums[0][q][lane];
+    for (int w = 1; w < waves; ++w) v += sums[w][q][lane];
+    const int m = m0 + 16 * (q % MT) + r, n = n0 + 16 * (q / MT) + 4 * g;
     if (m < p.M && n < p.N) store4((TOut*)p.y + (int64_t)m * p.N + n, v, p.N - n, (p.N & 3) == 0);
   }
 }
@@ -333,18 +367,20 @@ __global__ void __launch_bounds__(512, 2) block_gemm_big_kernel(const BlockGemmP
     }
 }
 
-template <typename TOut, int MT, bool ALIGNED>
+template <typename TOut, int MT, int NT, bool EXACT, bool ALIGNED>
 hipError_t gemm_rows(const BlockGemmParams& p, hipStream_t stream) {
   const int KB = (p.K + kScaleBlock - 1) / kScaleBlock;
   const int waves = KB < 8 ? KB : 8;
-  hipLaunchKernelGGL((block_gemm_rows_kernel<TOut, MT, ALIGNED>), dim3((p.N + 15) / 16, (p.M + 16 * MT - 1) / (16 * MT)), dim3(64 * waves), 0, stream, p);
+  hipLaunchKernelGGL((block_gemm_rows_kernel<TOut, MT, NT, EXACT, ALIGNED>), dim3((p.N + 16 * NT - 1) / (16 * NT)), dim3(64 * waves), 0, stream, p);
   return hipGetLastError();
 }
 template <typename TOut, bool ALIGNED>
 hipError_t gemm_as(const BlockGemmParams& p, hipStream_t stream) {
-  if (p.M <= 16) return gemm_rows<TOut, 1, ALIGNED>(p, stream);
-  if (p.M <= 32) return gemm_rows<TOut, 2, ALIGNED>(p, stream);
-  if (p.M <= 64) return gemm_rows<TOut, 4, ALIGNED>(p, stream);
+  constexpr bool EXACT = sizeof(TOut) == 4;
+  if (p.M <= 16) return gemm_rows<TOut, 1, 1, true, ALIGNED>(p, stream);
+  if (p.M <= 32) return gemm_rows<TOut, 2, 2, EXACT, ALIGNED>(p, stream);
+  if (p.M <= 48) return gemm_rows<TOut, 3, 2, EXACT, ALIGNED>(p, stream);
+  if (p.M <= 64) return gemm_rows<TOut, 4, 2, EXACT, ALIGNED>(p, stream);
   const int64_t tm = (p.M + 255) / 256, tn = (p.N + 255) / 256;
   if constexpr (ALIGNED && sizeof(TOut) == 2) {
     if (tm * tn >= 192 && p.K <= 1 << 22) {   // (256 rows of an operand within 2^30 bytes of buffer range)
