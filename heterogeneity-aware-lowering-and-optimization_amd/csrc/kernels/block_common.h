@@ -29,6 +29,14 @@ __device__ __forceinline__ uintx4 load_row16(const unsigned char* row, const int
   }
 }
 
+// The bytes n .. 15 (0 < n < 16) moved to the front, zeros behind them.
+__device__ __forceinline__ uintx4 bytes_down(const uintx4 v, const int n) {
+  const unsigned long long lo = (unsigned long long)v.y << 32 | v.x, hi = (unsigned long long)v.w << 32 | v.z;
+  const int bits = 8 * n;
+  const unsigned long long l = bits >= 64 ? hi >> (bits - 64) : lo >> bits | hi << (63 - bits) << 1, h = bits >= 64 ? 0ull : hi >> bits;
+  return uintx4{(unsigned)l, (unsigned)(l >> 32), (unsigned)h, (unsigned)(h >> 32)};
+}
+
 // c + A B^T for 16 rows of A and 16 of B over 128 e4m3 values: lane l supplies 32 values of row
 // l % 16 of either, those of quarter l / 16 of the 128 (which quarter holds which values does not
 // matter as long as A and B agree).  Result element i of lane l: row 4 * (l / 16) + i of A, row

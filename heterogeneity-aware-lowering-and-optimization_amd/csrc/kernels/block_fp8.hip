@@ -74,104 +74,148 @@ hipError_t quantize_as(const void* x, void* q, float* scale, int64_t rows, int64
 }
 
 // ------------------------------------------------------------------ product --
-// Few rows: a workgroup owns 16 NT columns n x 16 MT rows m.  The weights are read once, straight into the
-// operand registers; the wavefronts take every blockDim / 64-th block of 128 terms and their sums meet
-// in LDS in wavefront order.  A block's sum is scaled on its way into the accumulator: the scale of row m
-// belongs to a lane (column of the matrix result), that of B to the whole tile.  Bound by the weights' way
-// from memory for one row; with more, the rows of A come from L2 once per workgroup, so that two tiles
-// of columns share them.  EXACT: through bf16 (see mma_exact).
-template <typename TOut, int MT, int NT, bool EXACT, bool ALIGNED>
-__global__ void __launch_bounds__(512) block_gemm_rows_kernel(const BlockGemmParams p) {
-  constexpr int UN = MT == 1 ? 4 : 2;      // blocks of terms requested at a time
-  __shared__ floatx4 sums[8][NT * MT][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+// Few tiles: a workgroup owns 16 NT columns n x 16 MT rows m, and its wavefronts share out the blocks of 128
+// terms; their sums meet in LDS in wavefront order.  Every wavefront has LDS of its own and no barrier:
+// eight lanes bring 128 neighbouring bytes of a row, P blocks ahead, and the operand fragments (lane l: row
+// l % 16) are read back from there.  Straight from memory a fragment's neighbouring lanes are rows apart, and
+// a compute unit gets 36 KB/us out of L2 instead of 120 (measured; from memory 26 either way).
+// A block's sum is scaled on its way into the accumulator: the scale of row m belongs to a lane (column of
+// the matrix result), that of B to the whole tile.  EXACT: through bf16 (see mma_exact).
+template <typename TOut, int NT, int MT, int P, bool EXACT, bool ALIGNED>
+__global__ void __launch_bounds__(512) block_gemm_split_kernel(const BlockGemmParams p) {
+  constexpr int ROWS = 16 * (NT + MT);     // of B, then of A
+  constexpr int OWN = ROWS * kScaleBlock;  // bytes of a wavefront's LDS
+  constexpr int NR = ROWS / 8;             // requests of a block: eight rows each
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int r = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * (16 * NT), m0 = blockIdx.y * (16 * MT);
   const int KB = (p.K + kScaleBlock - 1) / kScaleBlock;
-  const unsigned char* brow[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) brow[j] = p.b + (int64_t)min(n0 + 16 * j + r, p.N - 1) * p.K;
-  const unsigned char* arow[MT];
+  unsigned char* const own = smem + wave * OWN;
+  // what this lane brings: 16 bytes at chunk lane % 8 of rows 8 i + lane / 8, of B and then of A (rows
+  // behind the operand's end: nothing); addresses are a wavefront's base and 32 bits of a lane's own
+  const int chunk = lane & 7, l8 = lane >> 3;
+  const unsigned char *const b_tile = p.b + (int64_t)n0 * p.K, *const a_tile = p.a + (int64_t)m0 * p.K;
+  const int b_rows = min(16 * NT, p.N - n0), a_rows = min(16 * MT, p.M - m0);
+  const unsigned lane_row = (unsigned)l8 * p.K;
   const float* as[MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const int64_t m = min(m0 + 16 * t + r, p.M - 1);
-    arow[t] = p.a + m * p.K;
-    as[t] = p.a_scale + m * KB;
-  }
+  for (int t = 0; t < MT; ++t) as[t] = p.a_scale + (int64_t)min(m0 + 16 * t + r, p.M - 1) * KB;
   const float* bs = p.b_scale + (int64_t)(n0 / kScaleBlock) * KB;
   floatx4 acc[NT][MT];
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[j][t] = floatx4{0.f, 0.f, 0.f, 0.f};
-  for (int kb0 = wave; kb0 < KB; kb0 += UN * waves) {
-    uintx4 w[UN][NT][2], x[UN][MT][2];
-    float sa[UN][MT], sb[UN];
+
+  uintx4 in[P][NR];
+  float sa[P][MT], sb[P];
+  // Unaligned rows: 16 bytes that would pass the row's end are its last 16 (moved into place on their way to LDS),
+  // and a row of fewer is read by bytes, one step for the whole product.
+  const bool in_vectors = ALIGNED || p.K >= 16;
+  auto fetch = [&](const int kb, const int q) __attribute__((always_inline)) {
+    if (kb >= KB) return;
+    const int at = kb * kScaleBlock + chunk * 16;
+    const unsigned lane_at = lane_row + (ALIGNED ? at : min(at, p.K - 16));
 #pragma unroll
-    for (int q = 0; q < UN; ++q) {
-      const int kb = kb0 + q * waves;
-      if (kb >= KB) break;
-      const int64_t k = (int64_t)kb * kScaleBlock + g * 32;
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int v = 0; v < 2; ++v) w[q][j][v] = load_row16<ALIGNED>(brow[j], k + 16 * v, p.K);
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-#pragma unroll
-        for (int v = 0; v < 2; ++v) x[q][t][v] = load_row16<ALIGNED>(arow[t], k + 16 * v, p.K);
-        sa[q][t] = as[t][kb];
-      }
-      sb[q] = bs[kb];
+    for (int i = 0; i < NR; ++i) {
+      const bool is_b = i < 2 * NT;
+      const int first = 8 * (is_b ? i : i - 2 * NT);
+      const unsigned char* row = (is_b ? b_tile : a_tile) + (int64_t)first * p.K;
+      in[q][i] = uintx4{0u, 0u, 0u, 0u};
+      if (in_vectors && first + l8 < (is_b ? b_rows : a_rows) && at < p.K)
+        in[q][i] = ALIGNED ? *reinterpret_cast<const uintx4*>(row + lane_at) : reinterpret_cast<const Bytes16*>(row + lane_at)->v;
     }
 #pragma unroll
-    for (int q = 0; q < UN; ++q) {
-      if (kb0 + q * waves >= KB) break;
-      uintx4 wv[EXACT ? NT : 1][4];
-      if constexpr (EXACT) {
+    for (int t = 0; t < MT; ++t) sa[q][t] = as[t][kb];
+    sb[q] = bs[kb];
+  };
 #pragma unroll
-        for (int j = 0; j < NT; ++j) bf16_of_e4m3(w[q][j][0], w[q][j][1], wv[j]);
+  for (int q = 0; q < P; ++q) fetch(wave + q * waves, q);
+  for (int kb0 = wave; kb0 < KB; kb0 += P * waves) {
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+      const int kb = kb0 + q * waves;
+      if (kb >= KB) break;
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_wave_barrier();     // (the fragments of the block before have been read: LDS keeps a wavefront's order)
+      auto place = [&](const int i) { return reinterpret_cast<uintx4*>(own + (8 * i + l8) * kScaleBlock + ((chunk ^ ((8 * i + l8) >> 1 & 7)) << 4)); };
+      if (!ALIGNED && (kb + 1) * kScaleBlock > p.K) {
+        const int behind = kb * kScaleBlock + chunk * 16 + 16 - p.K;     // bytes of this lane's 16 that are not the row's
+        if (in_vectors) {
+          if (behind > 0 && behind < 16) {
+#pragma unroll
+            for (int i = 0; i < NR; ++i) in[q][i] = bytes_down(in[q][i], behind);
+          }
+        } else if (behind < 16) {
+#pragma unroll
+          for (int i = 0; i < NR; ++i) {
+            const bool is_b = i < 2 * NT;
+            const int row = 8 * (is_b ? i : i - 2 * NT) + l8;
+            if (row < (is_b ? b_rows : a_rows)) in[q][i] = load_row16<false>((is_b ? b_tile : a_tile) + (int64_t)row * p.K, chunk * 16, p.K);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NR; ++i) *place(i) = in[q][i];
+      float scale[MT];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) scale[t] = sa[q][t] * sb[q];
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_wave_barrier();
+      fetch(kb + P * waves, q);
+      const int c0 = (g ^ (r >> 1)) << 4, c1 = ((g + 4) ^ (r >> 1)) << 4;
+      uintx4 w[NT][2], wv[EXACT ? NT : 1][4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const unsigned char* at = own + (16 * j + r) * kScaleBlock;
+        w[j][0] = *reinterpret_cast<const uintx4*>(at + c0);
+        w[j][1] = *reinterpret_cast<const uintx4*>(at + c1);
+        if constexpr (EXACT) bf16_of_e4m3(w[j][0], w[j][1], wv[j]);
       }
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
+        const unsigned char* at = own + (16 * (NT + t) + r) * kScaleBlock;
+        const uintx4 x0 = *reinterpret_cast<const uintx4*>(at + c0), x1 = *reinterpret_cast<const uintx4*>(at + c1);
         uintx4 xv[4];
-        if constexpr (EXACT) bf16_of_e4m3(x[q][t][0], x[q][t][1], xv);
-        const float s = sa[q][t] * sb[q];
+        if constexpr (EXACT) bf16_of_e4m3(x0, x1, xv);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           floatx4 part;
           if constexpr (EXACT) part = mma_exact(wv[j], xv);
-          else part = mma_e4m3(w[q][j][0], w[q][j][1], x[q][t][0], x[q][t][1], floatx4{0.f, 0.f, 0.f, 0.f});
+          else part = mma_e4m3(w[j][0], w[j][1], x0, x1, floatx4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[j][t][i] = __builtin_fmaf(part[i], s, acc[j][t][i]);
+          for (int i = 0; i < 4; ++i) acc[j][t][i] = __builtin_fmaf(part[i], scale[t], acc[j][t][i]);
         }
       }
     }
   }
+  // the sums: NT x MT x 64 quads of every wavefront
+  floatx4* const sums = reinterpret_cast<floatx4*>(smem);
+  __syncthreads();
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
-    for (int t = 0; t < MT; ++t) sums[wave][j * MT + t][lane] = acc[j][t];
+    for (int t = 0; t < MT; ++t) sums[(wave * NT * MT + j * MT + t) * 64 + lane] = acc[j][t];
   __syncthreads();
   for (int q = wave; q < NT * MT; q += waves) {
-    floatx4 v = sums[0][q][lane];
-    for (int w = 1; w < waves; ++w) v += sums[w][q][lane];
+    floatx4 v = sums[q * 64 + lane];
+    for (int w = 1; w < waves; ++w) v += sums[(w * NT * MT + q) * 64 + lane];
     const int m = m0 + 16 * (q % MT) + r, n = n0 + 16 * (q / MT) + 4 * g;
     if (m < p.M && n < p.N) store4((TOut*)p.y + (int64_t)m * p.N + n, v, p.N - n, (p.N & 3) == 0);
   }
 }
 
-// More rows: a workgroup of four wavefronts owns BN columns n x BM rows m; both operands pass
-// through LDS, 128 terms at a time, the next block's in registers meanwhile.
+// Many tiles that the kernel below does not take: a workgroup of four wavefronts owns BN columns n x BM rows m;
+// both operands pass through LDS, 128 terms at a time, the next 128 on their way in registers.
 template <typename TOut, int BM, int BN, bool ALIGNED>
 __global__ void __launch_bounds__(256) block_gemm_tile_kernel(const BlockGemmParams p) {
   constexpr bool EXACT = sizeof(TOut) == 4;
   constexpr int PITCH = kScaleBlock + 16;   // (16 bytes more: sixteen rows start in different banks)
   constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16;
   constexpr int NB = BN * 8 / 256, NA = BM * 8 / 256;  // 16-byte chunks a thread brings of either
-  __shared__ __attribute__((aligned(16))) unsigned char sa[BM * PITCH], sb[BN * PITCH];
-  __shared__ float ss[BM];
+  __shared__ __attribute__((aligned(16))) unsigned char lds[(BM + BN) * PITCH];
+  __shared__ float sc[BM];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int r = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * BN, m0 = blockIdx.y * BM;
@@ -182,16 +226,32 @@ __global__ void __launch_bounds__(256) block_gemm_tile_kernel(const BlockGemmPar
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  const unsigned char *arow[NA], *brow[NB];
+#pragma unroll
+  for (int i = 0; i < NA; ++i) arow[i] = p.a + (int64_t)min(m0 + (tid >> 3) + 32 * i, p.M - 1) * p.K;
+#pragma unroll
+  for (int i = 0; i < NB; ++i) brow[i] = p.b + (int64_t)min(n0 + (tid >> 3) + 32 * i, p.N - 1) * p.K;
+  const float* as = p.a_scale + (int64_t)min(m0 + tid % BM, p.M - 1) * KB;
+  const float* bs = p.b_scale + (int64_t)(n0 / kScaleBlock) * KB;
   uintx4 ra[NA], rb[NB];
-  float rs = 0.f;
-  auto fetch = [&](const int kb) {
+  float rs, rt;
+  auto fetch = [&](const int kb) __attribute__((always_inline)) {
     const int64_t k = (int64_t)kb * kScaleBlock + (tid & 7) * 16;
+    if (ALIGNED || kb + 1 < KB) {      // (a row's last block may end inside a vector)
 #pragma unroll
-    for (int i = 0; i < NA; ++i) ra[i] = load_row16<ALIGNED>(p.a + (int64_t)min(m0 + (tid >> 3) + 32 * i, p.M - 1) * p.K, k, p.K);
+      for (int i = 0; i < NA; ++i) ra[i] = ALIGNED ? load_row16<ALIGNED>(arow[i], k, p.K) : reinterpret_cast<const Bytes16*>(arow[i] + k)->v;
 #pragma unroll
-    for (int i = 0; i < NB; ++i) rb[i] = load_row16<ALIGNED>(p.b + (int64_t)min(n0 + (tid >> 3) + 32 * i, p.N - 1) * p.K, k, p.K);
-    if (tid < BM) rs = p.a_scale[(int64_t)min(m0 + tid, p.M - 1) * KB + kb] * p.b_scale[(int64_t)(n0 / kScaleBlock) * KB + kb];
+      for (int i = 0; i < NB; ++i) rb[i] = ALIGNED ? load_row16<ALIGNED>(brow[i], k, p.K) : reinterpret_cast<const Bytes16*>(brow[i] + k)->v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < NA; ++i) ra[i] = load_row16<ALIGNED>(arow[i], k, p.K);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) rb[i] = load_row16<ALIGNED>(brow[i], k, p.K);
+    }
+    rs = as[kb];
+    rt = bs[kb];     // (multiplied where they are stored: here that would wait for the whole request)
   };
+  unsigned char *const sa = lds, *const sb = lds + BM * PITCH;
   fetch(0);
   for (int kb = 0; kb < KB; ++kb) {
     __syncthreads();
@@ -199,7 +259,7 @@ __global__ void __launch_bounds__(256) block_gemm_tile_kernel(const BlockGemmPar
     for (int i = 0; i < NA; ++i) *reinterpret_cast<uintx4*>(sa + ((tid >> 3) + 32 * i) * PITCH + (tid & 7) * 16) = ra[i];
 #pragma unroll
     for (int i = 0; i < NB; ++i) *reinterpret_cast<uintx4*>(sb + ((tid >> 3) + 32 * i) * PITCH + (tid & 7) * 16) = rb[i];
-    if (tid < BM) ss[tid] = rs;
+    if (tid < BM) sc[tid] = rs * rt;
     __syncthreads();
     if (kb + 1 < KB) fetch(kb + 1);
     uintx4 w0[TN], w1[TN], wv[EXACT ? TN : 1][4];
@@ -214,7 +274,7 @@ __global__ void __launch_bounds__(256) block_gemm_tile_kernel(const BlockGemmPar
     for (int i = 0; i < TM; ++i) {
       const unsigned char* at = sa + (wm + 16 * i + r) * PITCH + g * 32;
       const uintx4 x0 = *reinterpret_cast<const uintx4*>(at), x1 = *reinterpret_cast<const uintx4*>(at + 16);
-      const float s = ss[wm + 16 * i + r];
+      const float s = sc[wm + 16 * i + r];
       uintx4 xv[4];
       if constexpr (EXACT) bf16_of_e4m3(x0, x1, xv);
 #pragma unroll
@@ -367,20 +427,25 @@ __global__ void __launch_bounds__(512, 2) block_gemm_big_kernel(const BlockGemmP
     }
 }
 
-template <typename TOut, int MT, int NT, bool EXACT, bool ALIGNED>
-hipError_t gemm_rows(const BlockGemmParams& p, hipStream_t stream) {
+template <typename TOut, int NT, int MT, int P, bool ALIGNED>
+hipError_t gemm_split(const BlockGemmParams& p, hipStream_t stream) {
+  constexpr bool EXACT = sizeof(TOut) == 4 || MT == 1;
+  constexpr int kOwn = 16 * (NT + MT) * kScaleBlock, kSums = NT * MT * 64 * 16;   // bytes of a wavefront: operands, sums
   const int KB = (p.K + kScaleBlock - 1) / kScaleBlock;
-  const int waves = KB < 8 ? KB : 8;
-  hipLaunchKernelGGL((block_gemm_rows_kernel<TOut, MT, NT, EXACT, ALIGNED>), dim3((p.N + 16 * NT - 1) / (16 * NT)), dim3(64 * waves), 0, stream, p);
+  const int waves = KB < 8 ? KB : 8, lds = waves * (kOwn > kSums ? kOwn : kSums);
+  static LdsLimit limit;
+  hipError_t e = limit.raise(reinterpret_cast<const void*>(&block_gemm_split_kernel<TOut, NT, MT, P, EXACT, ALIGNED>), 8 * (kOwn > kSums ? kOwn : kSums));
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((block_gemm_split_kernel<TOut, NT, MT, P, EXACT, ALIGNED>), dim3((p.N + 16 * NT - 1) / (16 * NT), (p.M + 16 * MT - 1) / (16 * MT)),
+                     dim3(64 * waves), lds, stream, p);
   return hipGetLastError();
 }
 template <typename TOut, bool ALIGNED>
 hipError_t gemm_as(const BlockGemmParams& p, hipStream_t stream) {
-  constexpr bool EXACT = sizeof(TOut) == 4;
-  if (p.M <= 16) return gemm_rows<TOut, 1, 1, true, ALIGNED>(p, stream);
-  if (p.M <= 32) return gemm_rows<TOut, 2, 2, EXACT, ALIGNED>(p, stream);
-  if (p.M <= 48) return gemm_rows<TOut, 3, 2, EXACT, ALIGNED>(p, stream);
-  if (p.M <= 64) return gemm_rows<TOut, 4, 2, EXACT, ALIGNED>(p, stream);
+  // Two tiles of columns a workgroup where that still leaves one for most of the compute units.
+  if (p.M <= 16) return gemm_split<TOut, 1, 1, 4, ALIGNED>(p, stream);
+  if (p.M <= 32) return p.N > 32 * 192 ? gemm_split<TOut, 2, 2, 2, ALIGNED>(p, stream) : gemm_split<TOut, 1, 2, 2, ALIGNED>(p, stream);
+  if (p.M <= 64) return p.N > 32 * 192 ? gemm_split<TOut, 2, 4, 1, ALIGNED>(p, stream) : gemm_split<TOut, 1, 4, 2, ALIGNED>(p, stream);
   const int64_t tm = (p.M + 255) / 256, tn = (p.N + 255) / 256;
   if constexpr (ALIGNED && sizeof(TOut) == 2) {
     if (tm * tn >= 192 && p.K <= 1 << 22) {   // (256 rows of an operand within 2^30 bytes of buffer range)
@@ -391,10 +456,14 @@ hipError_t gemm_as(const BlockGemmParams& p, hipStream_t stream) {
       return hipGetLastError();
     }
   }
-  if ((int64_t)((p.M + 127) / 128) * ((p.N + 127) / 128) >= 256)
-    hipLaunchKernelGGL((block_gemm_tile_kernel<TOut, 128, 128, ALIGNED>), dim3((p.N + 127) / 128, (p.M + 127) / 128), dim3(256), 0, stream, p);
-  else
-    hipLaunchKernelGGL((block_gemm_tile_kernel<TOut, 64, 64, ALIGNED>), dim3((p.N + 63) / 64, (p.M + 63) / 64), dim3(256), 0, stream, p);
+  // Too few of the tiles below for every compute unit: 64 x 64 results (64 rows x 32 columns where even those are
+  // few).  N = K = 4096: a tile below takes 47 us however few there are; here 512 rows take 27 us, 256 14.5.
+  if ((int64_t)((p.M + 127) / 128) * ((p.N + 127) / 128) < 256) {
+    if ((int64_t)((p.M + 63) / 64) * ((p.N + 31) / 32) <= 320) return gemm_split<TOut, 2, 4, 1, ALIGNED>(p, stream);
+    if constexpr (sizeof(TOut) == 2) return gemm_split<TOut, 4, 4, 1, ALIGNED>(p, stream);
+    else return gemm_split<TOut, 2, 4, 1, ALIGNED>(p, stream);      // (bf16 copies of four tiles do not fit in registers)
+  }
+  hipLaunchKernelGGL((block_gemm_tile_kernel<TOut, 128, 128, ALIGNED>), dim3((p.N + 127) / 128, (p.M + 127) / 128), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 
