@@ -14,6 +14,14 @@ typedef int intx8 __attribute__((ext_vector_type(8)));
 // 16 bytes from an address of any alignment (one global_load_dwordx4: gfx950 takes them unaligned).
 struct __attribute__((packed, aligned(1))) Bytes16 { uintx4 v; };
 
+// The bytes n .. 15 (0 < n < 16) moved to the front, zeros behind them.
+__device__ __forceinline__ uintx4 bytes_down(const uintx4 v, const int n) {
+  const unsigned long long lo = (unsigned long long)v.y << 32 | v.x, hi = (unsigned long long)v.w << 32 | v.z;
+  const int bits = 8 * n;
+  const unsigned long long l = bits >= 64 ? hi >> (bits - 64) : lo >> bits | hi << (63 - bits) << 1, h = bits >= 64 ? 0ull : hi >> bits;
+  return uintx4{(unsigned)l, (unsigned)(l >> 32), (unsigned)h, (unsigned)(h >> 32)};
+}
+
 // Bytes at .. at + 15 of a row of `len` bytes; zero behind its end.  Never reads outside the row.
 // ALIGNED: rows start on 16-byte boundaries and are whole 16-byte vectors.
 template <bool ALIGNED>
@@ -21,20 +29,20 @@ __device__ __forceinline__ uintx4 load_row16(const unsigned char* row, const int
   if constexpr (ALIGNED) {
     return at < len ? *reinterpret_cast<const uintx4*>(row + at) : uintx4{0u, 0u, 0u, 0u};
   } else {
-    if (at + 16 <= len) return reinterpret_cast<const Bytes16*>(row + at)->v;
-    unsigned w[4] = {0u, 0u, 0u, 0u};
-    for (int i = 0; i < 16; ++i)
-      if (at + i < len) w[i >> 2] |= (unsigned)row[at + i] << (8 * (i & 3));
-    return uintx4{w[0], w[1], w[2], w[3]};
+    if (len >= 16) {      // (16 bytes that would pass the end are the last 16)
+      const int64_t from = at + 16 <= len ? at : len - 16;
+      const uintx4 v = reinterpret_cast<const Bytes16*>(row + from)->v;
+      return at == from ? v : at >= len ? uintx4{0u, 0u, 0u, 0u} : bytes_down(v, (int)(at - from));
+    }
+    unsigned long long lo = 0, hi = 0;
+#pragma unroll 1
+    for (int i = 0; at + i < len; ++i) {
+      const unsigned long long b = row[at + i];
+      if (i < 8) lo |= b << 8 * i;
+      else hi |= b << 8 * (i - 8);
+    }
+    return uintx4{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)};
   }
-}
-
-// The bytes n .. 15 (0 < n < 16) moved to the front, zeros behind them.
-__device__ __forceinline__ uintx4 bytes_down(const uintx4 v, const int n) {
-  const unsigned long long lo = (unsigned long long)v.y << 32 | v.x, hi = (unsigned long long)v.w << 32 | v.z;
-  const int bits = 8 * n;
-  const unsigned long long l = bits >= 64 ? hi >> (bits - 64) : lo >> bits | hi << (63 - bits) << 1, h = bits >= 64 ? 0ull : hi >> bits;
-  return uintx4{(unsigned)l, (unsigned)(l >> 32), (unsigned)h, (unsigned)(h >> 32)};
 }
 
 // c + A B^T for 16 rows of A and 16 of B over 128 e4m3 values: lane l supplies 32 values of row
@@ -73,9 +81,9 @@ __device__ __forceinline__ floatx4 mma_vec(const uintx4 w, const uintx4 x, float
   }
 }
 
-// e4m3 values as X, exactly: vector `v` of the 32 values in w (16 / sizeof(X) of them).
+// e4m3 values as X, exactly: vector `v` of the 16 values in w (16 / sizeof(X) of them).
 template <typename X>
-__device__ __forceinline__ uintx4 values_of(const unsigned (&w)[8], const int v) {
+__device__ __forceinline__ uintx4 values_of(const uintx4 w, const int v) {
   uintx4 o = {0u, 0u, 0u, 0u};
 #if defined(__HIP_DEVICE_COMPILE__)
   if constexpr (std::is_same<X, float>::value) {
@@ -102,9 +110,8 @@ __device__ __forceinline__ uintx4 values_of(const unsigned (&w)[8], const int v)
 // exactly, through the 16-bit matrix instructions.  The 8-bit ones align the products of eight
 // neighbouring terms to the largest of them and drop what lies below 2^-13 of it.
 __device__ __forceinline__ void bf16_of_e4m3(const uintx4 w0, const uintx4 w1, uintx4 (&v)[4]) {
-  const unsigned b[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = values_of<bf16_t>(b, i);
+  for (int i = 0; i < 4; ++i) v[i] = values_of<bf16_t>(i < 2 ? w0 : w1, i & 1);
 }
 __device__ __forceinline__ floatx4 mma_exact(const uintx4 (&a)[4], const uintx4 (&b)[4]) {
   floatx4 c = {0.f, 0.f, 0.f, 0.f};

@@ -4691,7 +4691,7 @@ void Planner::lower_experts(int ni) {
   };
   const std::string& name = n.out->name;
   emit("experts.route:" + name, {tx, tr}, {tl}, [=](const ExecEnv& e, hipStream_t st) { return launch_experts_route(args(e), st); }, kReads16);
-  emit("experts.gate_up:" + name, {tx, tg, tgs, tl}, {th}, [=](const ExecEnv& e, hipStream_t st) { return launch_experts_gate_up(args(e), st); }, kReads16);
+  emit("experts.gate_up:" + name, {tx, tg, tgs, tl}, {tl, th}, [=](const ExecEnv& e, hipStream_t st) { return launch_experts_gate_up(args(e), st); }, kReads16);
   emit("experts.down:" + name, {td, tds, tl, th}, {tp, ty}, [=](const ExecEnv& e, hipStream_t st) { return launch_experts_down(args(e), st); }, kReads16 | kWrites16);
   set_main(n.out, ty);
 }
