@@ -203,11 +203,22 @@ struct Staging {
   static constexpr int BYTES = 4096 + XR * 1024;                  // of a wavefront
   static_assert(BYTES >= 2 * ((C + 15) / 16) * 1024, "the sums take the operands' place");
 };
+// 16 bytes at `at`; zeros where that is not within `size` bytes from `base` on.
+constexpr unsigned kOutside = 0xfffffff0u;
+__device__ __forceinline__ uintx4 load_within(const unsigned char* base, const unsigned size, const unsigned at, const unsigned uniform) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(base), 0, size, 0x00020000);
+  return __builtin_bit_cast(uintx4, __builtin_amdgcn_raw_buffer_load_b128(r, at, uniform, 0));
+#else
+  (void)base; (void)size; (void)at; (void)uniform;
+  return uintx4{0u, 0u, 0u, 0u};
+#endif
+}
 template <bool GATED>
 __host__ __device__ inline int tile_rows(const ExpertsParams& p) { return GATED ? (p.I + 15) / 16 : (p.H + 31) / 32; }
 
 template <typename X, typename W, int C, int P, bool ALIGNED, bool GATED>
-__global__ void __launch_bounds__(512, C > 8 || sizeof(X) > 2 * sizeof(W) ? 1 : sizeof(X) == sizeof(W) ? 4 : 3) experts_product_kernel(const ExpertsParams p, const bool choice) {
+__global__ void __launch_bounds__(512, C > 8 || sizeof(X) > 2 * sizeof(W) ? 1 : sizeof(X) == sizeof(W) || ALIGNED ? 4 : 3) experts_product_kernel(const ExpertsParams p, const bool choice) {
   using S = Staging<X, W, C>;
   constexpr int MT = (C + 15) / 16;    // (eight columns: the others of a tile repeat them)
   constexpr int PLANES = S::PLANES, XR = S::XR, NR = 4 + XR;
@@ -244,37 +255,31 @@ __global__ void __launch_bounds__(512, C > 8 || sizeof(X) > 2 * sizeof(W) ? 1 : 
   int w_rows[2] = {};
   const float* w_scale[3] = {};        // of the first rows, of the second, and of the second from row `cut` on
   int cut = 16;
-  int64_t x_row[C / 8] = {};
+  unsigned x_row[C / 8] = {};
   float weight = 0.f;
   const unsigned char* const xs = (const unsigned char*)(GATED ? p.x : p.hidden);
+  const unsigned xbytes = (unsigned)((GATED ? p.tokens : p.tokens * p.top_k) * xlen);      // (below 2^32: see valid)
   const unsigned lane_row = (unsigned)l8 * wlen;
   const bool in_vectors = ALIGNED || wlen >= 16;     // (a row of fewer bytes: one step, byte by byte)
   uintx4 in[P][NR];
-  float sc[P][3];
+  float sc[3] = {};                    // lane l: of this wavefront's step l (of 64)
   auto fetch = [&](const int s, const int q) __attribute__((always_inline)) {
     if (s >= steps) return;
     const int at = s * 128 + chunk * 16;
-    const unsigned lane_at = lane_row + (ALIGNED ? at : min(at, wlen - 16));
+    const unsigned lane_at = at < wlen ? lane_row + (ALIGNED ? at : min(at, wlen - 16)) : kOutside;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int first = 8 * (i & 1);
-      const unsigned char* row = w_tile[i >> 1] + (int64_t)first * wlen;
-      in[q][i] = uintx4{0u, 0u, 0u, 0u};
-      if (in_vectors && first + l8 < w_rows[i >> 1] && at < wlen)
-        in[q][i] = ALIGNED ? *reinterpret_cast<const uintx4*>(row + lane_at) : reinterpret_cast<const Bytes16*>(row + lane_at)->v;
-    }
+    for (int i = 0; i < 4; ++i) in[q][i] = load_within(w_tile[i >> 1], in_vectors ? w_rows[i >> 1] * wlen : 0, lane_at, 8 * (i & 1) * wlen);
 #pragma unroll
     for (int i = 0; i < XR; ++i) {
-      const int first = 8 * (i / PLANES);
-      const int64_t from = (int64_t)s * (128 * PLANES) + i % PLANES * 128 + chunk * 16;
-      in[q][4 + i] = uintx4{0u, 0u, 0u, 0u};
-      if (first < here && first + l8 < here && from < xlen && (ALIGNED || xlen >= 16))
-        in[q][4 + i] = ALIGNED ? *reinterpret_cast<const uintx4*>(xs + x_row[i / PLANES] + from)
-                               : reinterpret_cast<const Bytes16*>(xs + x_row[i / PLANES] + min(from, xlen - 16))->v;
+      const unsigned from = s * (128 * PLANES) + i % PLANES * 128 + chunk * 16;
+      if (8 * (i / PLANES) < here)
+        in[q][4 + i] = load_within(xs, ALIGNED || xlen >= 16 ? xbytes : 0, 8 * (i / PLANES) + l8 < here && from < (unsigned)xlen ? x_row[i / PLANES] + (ALIGNED ? from : min(from, (unsigned)xlen - 16)) : kOutside, 0);
     }
+  };
+  auto scales_from = [&](const int s) __attribute__((always_inline)) {
     if constexpr (SCALED) {
 #pragma unroll
-      for (int i = 0; i < (GATED ? 3 : 1); ++i) sc[q][i] = w_scale[i][s];
+      for (int i = 0; i < (GATED ? 3 : 1); ++i) sc[i] = w_scale[i][min(s + lane * waves, steps - 1)];
     }
   };
   auto start = [&]() __attribute__((always_inline)) {
@@ -304,9 +309,10 @@ __global__ void __launch_bounds__(512, C > 8 || sizeof(X) > 2 * sizeof(W) ? 1 : 
 #pragma unroll
     for (int i = 0; i < C / 8; ++i) {
       const int pair = 8 * i + l8 < here ? c.pairs[pair0 + 8 * i + l8] : 0;
-      x_row[i] = (int64_t)(GATED ? pair / p.top_k : pair) * xlen;
+      x_row[i] = (unsigned)((GATED ? pair / p.top_k : pair) * xlen);
     }
     if (!GATED) weight = 16 * wave + r < here ? weights[c.pairs[pair0 + 16 * wave + r]] : 0.f;
+    scales_from(wave);
 #pragma unroll
     for (int q = 0; q < P; ++q) fetch(wave + q * waves, q);
   };
@@ -318,7 +324,13 @@ __global__ void __launch_bounds__(512, C > 8 || sizeof(X) > 2 * sizeof(W) ? 1 : 
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int t = 0; t < MT; ++t) acc[j][t] = floatx4{0.f, 0.f, 0.f, 0.f};
-    for (int s0 = wave; s0 < steps; s0 += P * waves) {
+    static_assert(64 % P == 0, "a round of the loop has its scales in one load");
+    int done = 0;
+    for (int s0 = wave; s0 < steps; s0 += P * waves, done += P) {
+      if (SCALED && done == 64) {
+        scales_from(s0);
+        done = 0;
+      }
 #pragma unroll
       for (int q = 0; q < P; ++q) {
         const int s = s0 + q * waves;
@@ -364,16 +376,17 @@ __global__ void __launch_bounds__(512, C > 8 || sizeof(X) > 2 * sizeof(W) ? 1 : 
         float scale[3] = {1.f, 1.f, 1.f};
         if constexpr (SCALED) {
 #pragma unroll
-          for (int i = 0; i < (GATED ? 3 : 1); ++i) scale[i] = sc[q][i];
+          for (int i = 0; i < (GATED ? 3 : 1); ++i) scale[i] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc[i]), done + q));
         }
         asm volatile("" ::: "memory");
         __builtin_amdgcn_wave_barrier();
         fetch(s + P * waves, q);
+        // (8-bit weights: half a step at a time, or operands in 16 bits take the registers of steps under way)
         uintx4 w[2][2];
+        if constexpr (!SCALED || MT > 1) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) w[j][h] = *reinterpret_cast<const uintx4*>(own + (16 * j + r) * 128 + ((g + 4 * h ^ r >> 1) << 4));
+          for (int j = 0; j < 4; ++j) w[j >> 1][j & 1] = *reinterpret_cast<const uintx4*>(own + (16 * (j >> 1) + r) * 128 + ((g + 4 * (j & 1) ^ r >> 1) << 4));
+        }
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
           if (16 * t >= here) break;
@@ -381,13 +394,21 @@ __global__ void __launch_bounds__(512, C > 8 || sizeof(X) > 2 * sizeof(W) ? 1 : 
 #pragma unroll
           for (int j = 0; j < 2; ++j) part[j] = SCALED ? floatx4{0.f, 0.f, 0.f, 0.f} : acc[j][t];
 #pragma unroll
-          for (int v = 0; v < 2 * PLANES; ++v) {
-            const int row = 16 * t + r & C - 1;
-            const uintx4 x = *reinterpret_cast<const uintx4*>(own + 4096 + v % PLANES * (C * 128) + row * 128 + ((g + 4 * (v / PLANES) ^ (row >> 1 & 7)) << 4));
+          for (int h = 0; h < 2; ++h) {
+            if constexpr (SCALED && MT == 1) {
+              __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              if constexpr (SCALED) part[j] = mma_vec<X>(values_of<X>(w[j][v / PLANES], v % PLANES), x, part[j]);
-              else part[j] = mma_vec<X>(w[j][v], x, part[j]);
+              for (int j = 0; j < 2; ++j) w[j][h] = *reinterpret_cast<const uintx4*>(own + (16 * j + r) * 128 + ((g + 4 * h ^ r >> 1) << 4));
+            }
+#pragma unroll
+            for (int v = 0; v < PLANES; ++v) {
+              const int row = 16 * t + r & C - 1;
+              const uintx4 x = *reinterpret_cast<const uintx4*>(own + 4096 + v * (C * 128) + row * 128 + ((g + 4 * h ^ (row >> 1 & 7)) << 4));
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                if constexpr (SCALED) part[j] = mma_vec<X>(values_of<X>(w[j][h], v), x, part[j]);
+                else part[j] = mma_vec<X>(w[j][h], x, part[j]);
+              }
             }
           }
 #pragma unroll
@@ -458,7 +479,7 @@ bool valid(const ExpertsParams& p) {
   return p.x != nullptr && p.router != nullptr && p.gate_up != nullptr && p.down != nullptr && p.y != nullptr && p.route != nullptr &&
          p.hidden != nullptr && p.parts != nullptr && p.tokens >= 1 && p.tokens <= kMaxExpertTokens && p.E >= 1 && p.E <= kMaxExperts &&
          p.H >= 1 && p.H <= (1 << 24) && p.I >= 1 && p.I <= (1 << 23) && p.top_k >= 1 && p.top_k <= p.E && p.top_k <= kMaxExpertTopK &&
-         dtype_is_float(p.dt) && (p.w_dt == p.dt || (p.w_dt == DT_F8 && p.gate_up_scale != nullptr && p.down_scale != nullptr));
+         (int64_t)p.tokens * p.H * 4 < kMaxExpertBytes && (int64_t)p.tokens * p.top_k * p.I * 4 < kMaxExpertBytes && dtype_is_float(p.dt) && (p.w_dt == p.dt || (p.w_dt == DT_F8 && p.gate_up_scale != nullptr && p.down_scale != nullptr));
 }
 // rows of x, hidden and weights are whole 16-byte vectors
 bool whole_vectors(const ExpertsParams& p, const int len) { return (int64_t)len * dtype_size(p.dt) % 16 == 0 && (int64_t)len * dtype_size(p.w_dt) % 16 == 0; }
@@ -498,7 +519,7 @@ hipError_t product_one(const ExpertsParams& p, hipStream_t stream) {
   hipError_t e = limit.raise(reinterpret_cast<const void*>(&experts_product_kernel<X, W, C, P, ALIGNED, GATED>), kLdsOfUnit);
   if (e != hipSuccess) return e;
   const int64_t tiles = (int64_t)slots_of(p.tokens, p.top_k, p.E) * tile_rows<GATED>(p);
-  const int64_t resident = kComputeUnits * std::max<int64_t>(1, std::min<int64_t>(16 / waves, kLdsOfUnit / lds));
+  const int64_t resident = kComputeUnits * std::max<int64_t>(1, std::min<int64_t>((sizeof(X) == sizeof(W) || ALIGNED ? 16 : 12) / waves, kLdsOfUnit / lds));
   hipLaunchKernelGGL((experts_product_kernel<X, W, C, P, ALIGNED, GATED>), dim3((unsigned)std::min(tiles, resident)), dim3(64 * waves), lds, stream, p, choice);
   return hipGetLastError();
 }
@@ -506,8 +527,9 @@ template <typename X, typename W, bool GATED>
 hipError_t product_as(const ExpertsParams& p, hipStream_t stream) {
   constexpr int MANY = sizeof(X) / sizeof(W) == 4 ? 32 : 64;      // (x of a step within LDS)
   const bool a = whole_vectors(p, GATED ? p.H : p.I);
+  constexpr int P = sizeof(X) == sizeof(W) ? 2 : 1;             // (within registers)
   if (few_columns(p)) return a ? product_one<X, W, 8, 2, true, GATED>(p, stream) : product_one<X, W, 8, 2, false, GATED>(p, stream);
-  return a ? product_one<X, W, MANY, 1, true, GATED>(p, stream) : product_one<X, W, MANY, 1, false, GATED>(p, stream);
+  return a ? product_one<X, W, MANY, P, true, GATED>(p, stream) : product_one<X, W, MANY, P, false, GATED>(p, stream);
 }
 template <typename X, typename W>
 hipError_t gate_up_as(const ExpertsParams& p, hipStream_t stream) { return product_as<X, W, true>(p, stream); }

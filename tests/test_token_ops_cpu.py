@@ -104,6 +104,16 @@ def test_refusals_of_the_experts(odla, b):
         b.mixture_of_experts(*many, 33)
 
 
+@pytest.mark.parametrize("tokens,hidden,inner,top_k", [(512, 1 << 21, 4, 1), (512, 4, 1 << 16, 32), (64, 4, 1 << 23, 2)])
+def test_refusal_of_experts_behind_32_bit_offsets(odla, b, tokens, hidden, inner, top_k):
+    def layer(t):
+        b.mixture_of_experts(b.arg(None, (t, hidden)), b.arg(None, (64, hidden)), b.arg(None, (64, 2 * inner, hidden)),
+                             b.arg(None, (64, hidden, inner)), top_k)
+    layer(tokens - 1)
+    with pytest.raises(odla.OdlaError):
+        layer(tokens)
+
+
 def test_refusals_of_the_sampling(odla, b):
     l, u = b.arg("l", (4, 100)), b.arg("u", (4,))
     b.sample(l, u)
