@@ -31,6 +31,8 @@ constexpr int kThreads = 1024, kWavesPerRow = kThreads / 64, kBins = 2048;
 constexpr int kList = 4096;     // candidates that are settled in LDS
 constexpr int kBorder = 1024;   // elements of one bin that are ranked against each other: n / 1024 n steps
 constexpr double kOne = 17592186044416.0;   // 2^44: the largest weight
+constexpr int kPowers = 1024;
+static_assert(kPowers == kThreads, "a thread makes one of the powers");
 typedef unsigned long long u64;
 
 // Order of floats as unsigned numbers: -inf and NaN give 0x007fffff, everything that can be drawn more.
@@ -53,7 +55,7 @@ struct Shared {
   float logit[kList];
   int index[kList];
   int border[kBorder];
-  double power[64];            // 2^(j / 64)
+  double power[kPowers];       // 2^(44 + j / kPowers)
   u64 wave_a[kWavesPerRow], wave_b[kWavesPerRow];
   float wave_f[kWavesPerRow];
   int listed, bordered;
@@ -67,41 +69,35 @@ struct Row {
   float most;         // the largest logit
   float per_f;        // log2(e) / temperature
   float per_bin;      // bins per unit of (max - l)
-  double most_d, per; // the first two in 64 bits
+  double most_d, per; // kPowers of the exponent's units per unit of (l - max), in 64 bits
+  double floor;       // (so many of those units that a weight rounds to nothing)
   const double* power;
 };
-// a * b + c with c in scalar registers (the compiler's own choice copies it to vector registers for every use).
-__device__ __forceinline__ double fma_c(const double a, const double b, const double c) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  double d;
-  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));
-  return d;
-#else
-  return __builtin_fma(a, b, c);
-#endif
-}
-// 2^44 exp((l - max) / T) in 64 bits: 2^y = 2^n 2^(j / 64) 2^f with |f| <= 1 / 128, the last as its
-// series, whose terms from f^6 on are below 2^-55.  64 y is rounded by adding 1.5 * 2^52, which leaves it in
-// the sum's low word; 2^n goes straight into the exponent.  Masks, not branches: the elements of a vector
-// fill each other's latencies.
-__device__ __forceinline__ double weight(const Row& r, const float l) {
-  const bool near = (r.most - l) * r.per_f < 60.f;      // (not for NaN: infinite logits or temperatures)
-  const double y = ((double)(near ? l : r.most) - r.most_d) * r.per;
-  const double t = fma_c(y, 64.0, 6755399441055744.0);
-  const double f = __builtin_fma(t - 6755399441055744.0, -0.015625, y);
+// 2^44 exp((l - max) / T) = 2^n 2^(44 + j / 1024) 2^f with |f| <= 1 / 2048, the last as its series, whose terms
+// from f^4 on are below 2^-50.  1024 y is rounded by adding 1.5 * 2^52, which leaves it in the sum's low
+// word; 2^n goes straight into the exponent of the power from the table.  The product and its rounding to a whole
+// number are one fused operation: the sum with 2^52 has it in its low bits, nearest even.  Nineteen instructions
+// and no branch; NaN (infinities among the operands) weighs nothing.
+struct Factors { double series, power; };
+__device__ __forceinline__ Factors factors(const Row& r, const float l) {
+  const double y = __builtin_fmax(((double)l - r.most_d) * r.per, r.floor);
+  const double t = y + 6755399441055744.0;
+  const double f = y - (t - 6755399441055744.0);
   const int k = (int)(unsigned)(u64)__double_as_longlong(t);
-  double p = fma_c(f, 1.3333558146428443e-3, 9.6181291076284770e-3);   // ln(2)^5 / 5!, ln(2)^4 / 4!
-  p = fma_c(p, f, 5.5504108664821580e-2);
-  p = fma_c(p, f, 2.4022650695910072e-1);
-  p = fma_c(p, f, 6.9314718055994531e-1);
-  p = __builtin_fma(p, f, 1.0) * r.power[k & 63];
-  const u64 bits = (u64)__double_as_longlong(p) + ((u64)(unsigned)(((k >> 6) + 44) << 20) << 32);
-  const u64 in = near ? ~0ull : 0ull, top = l == r.most ? (u64)__double_as_longlong(kOne) : 0ull;
-  return __longlong_as_double((long long)((bits & in) | (top & ~in)));
+  double p = __builtin_fma(f, 5.169222938345892e-11, 2.290978498068816e-7);   // (ln(2) / 1024)^3 / 3!, ^2 / 2!
+  p = __builtin_fma(p, f, 6.769015435155716e-4);
+  p = __builtin_fma(p, f, 1.0);
+  const u64 power = (u64)__double_as_longlong(r.power[k & (kPowers - 1)]);
+  const unsigned hi = (unsigned)(power >> 32) + ((unsigned)(k & -kPowers) << 10);
+  return {p, __longlong_as_double((long long)((u64)hi << 32 | (unsigned)power))};
 }
-// ... as a whole number: the sum with 2^52 has it in its low bits, rounded to nearest even.
-__device__ __forceinline__ u64 whole(const double w) {
-  return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
+__device__ __forceinline__ double weight(const Row& r, const float l) {      // before it is rounded
+  const Factors f = factors(r, l);
+  return f.series * f.power;
+}
+__device__ __forceinline__ u64 whole_weight(const Row& r, const float l) {
+  const Factors f = factors(r, l);
+  return (u64)__double_as_longlong(__builtin_fma(f.series, f.power, 4503599627370496.0)) & 0xfffffffffffffull;
 }
 // The histogram's bin, not decreasing as l falls; 0 for the largest, kBins for what lies behind the last.
 __device__ __forceinline__ int bin_of(const Row& r, const float l) {
@@ -267,7 +263,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
     pair = o > pair ? o : pair;
   }
   if (lane == 0) s.wave_a[wave] = pair;
-  if (tid < 64) s.power[tid] = exp2(tid * 0.015625);
+  s.power[tid] = exp2(44.0 + tid * 0.0009765625);
   if (tid == 0) s.listed = s.bordered = 0;
   __syncthreads();
 #pragma unroll
@@ -287,14 +283,17 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
     return;
   }
   r.per_f = 1.4426950408889634f / temperature;
-  r.most_d = (double)r.most;
-  r.per = 1.4426950408889634 / (double)temperature;
+  // (infinite logits: those alone are kept, and all weigh the same)
+  const bool infinite = r.most == __builtin_inff();
+  r.most_d = infinite ? 0.0 : (double)r.most;
+  r.per = infinite ? 0.0 : 1024.0 * 1.4426950408889634 / (double)temperature;
+  r.floor = infinite ? 0.0 : -60.0 * 1024.0;
   r.per_bin = (float)kBins / 45.1f * r.per_f;   // (weights round to nothing behind 2^-45)
   r.power = s.power;
   const double least = (double)min_p * kOne;    // (NaN: nothing is below)
 
   // The elements up to (cut_l, cut_at) in the ranking are kept.
-  float cut_l = -3.402823466e38f;
+  float cut_l = infinite ? r.most : -3.402823466e38f;
   int cut_at = V;
   auto in_cut = [&](const float l, const int i) { return (bool)((int)(l > cut_l) | ((int)(l == cut_l) & (int)(i <= cut_at))); };
 
@@ -313,7 +312,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
         const unsigned k = key_of(l);
         if ((k & known) != prefix) return;
         const unsigned b = mask - ((k >> shift) & mask);    // (the highest digit first)
-        if (by_sum) atomicAdd(&s.sum[b], whole(weight(r, l)));
+        if (by_sum) atomicAdd(&s.sum[b], whole_weight(r, l));
         else atomicAdd(&s.count[b], 1u);
       });
       __syncthreads();
@@ -327,7 +326,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
     // `need` is what the elements equal to the key still have to give: the first `ties` of them,
     // counted by parts of the row
     const float l0 = logit_of(prefix);
-    const u64 w = whole(weight(r, l0));
+    const u64 w = whole_weight(r, l0);
     const u64 ties = by_sum ? (w ? (need + w - 1) / w : 1) : need;
     const int part = (V + kBins - 1) / kBins;
     clear(s.count);
@@ -425,10 +424,11 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
           __syncthreads();
           cut_l = s.cut_l;
           cut_at = s.cut_at;
+          if (infinite && cut_l != r.most) { cut_l = r.most; cut_at = V; }
 #pragma unroll
           for (int j = 0; j < MINE; ++j) {
             const bool in = kept_bin[j] <= kBins && in_cut(kept_l[j], kept_i[j]);
-            kept_w[j] = in ? whole(weight(r, kept_l[j])) : 0;
+            kept_w[j] = in ? whole_weight(r, kept_l[j]) : 0;
             if (!in) kept_bin[j] = kBins + 1;
           }
         }
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
   }
   if (cut_k && !listed) {
     u64 live = 0;
-    row.each([&](const int, const float l) { live += l >= -3.402823466e38f; });
+    row.each([&](const int i, const float l) { live += in_cut(l, i); });
     cut_k = block_sum_u64(live, s.wave_a) > (u64)top_k;
     if (cut_k) descend(false, (u64)top_k);
   }
@@ -463,13 +463,14 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
         e = fmaxf(1.f, fminf(e, __log2f((float)V / ((1.f - top_p) * fmaxf(w, 1.f))) + 1.01f));
       }
       r.per_bin = (float)kBins / e * r.per_f;
+      const bool whole_row = !cut_k && !infinite;
       __syncthreads();
       row.each_vector([&](const int v, const Vec16<T>& x, const int) {
         u64 w[PER];
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
           const float l = x.get(e);
-          w[e] = whole(weight(r, l)) & ((int)!cut_k | (int)in_cut(l, v * PER + e) ? ~0ull : 0ull);
+          w[e] = whole_weight(r, l) & ((int)whole_row | (int)in_cut(l, v * PER + e) ? ~0ull : 0ull);
           total += w[e];
         }
 #pragma unroll
@@ -502,7 +503,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
         row.each_in([&](const float l) { return !(fabsf(l - middle) > half); }, [&](const int i, const float l) {
           if (l > -__builtin_inff() && bin_of(r, l) == edge && in_cut(l, i)) {
             const int n = atomicAdd(&s.bordered, 1);
-            if (n < kBorder) { s.border[n] = n; s.logit[n] = l; s.index[n] = i; s.sum[n] = whole(weight(r, l)); }
+            if (n < kBorder) { s.border[n] = n; s.logit[n] = l; s.index[n] = i; s.sum[n] = whole_weight(r, l); }
           }
         });
       }
@@ -567,8 +568,11 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
     return;
   }
   auto kept = [&](const int i, const float l) -> u64 {
-    const double w = weight(r, l);
-    return whole(w) & ((int)in_cut(l, i) & (int)!(w < least) ? ~0ull : 0ull);
+    const Factors f = factors(r, l);
+    const u64 w = (u64)__double_as_longlong(__builtin_fma(f.series, f.power, 4503599627370496.0)) & 0xfffffffffffffull;
+    bool in = in_cut(l, i);
+    if (least > 0.0) in = (int)in & (int)!(f.series * f.power < least);
+    return w & (in ? ~0ull : 0ull);
   };
   // a part is 256 neighbouring vectors of the row, four per lane of a wavefront
   const int vectors = (V + PER - 1) / PER, parts = (vectors + 255) / 256;
