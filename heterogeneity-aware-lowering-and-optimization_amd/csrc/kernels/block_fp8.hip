@@ -44,12 +44,28 @@ __global__ void __launch_bounds__(256) block_quantize_kernel(const T* x, uint8_t
     for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
     most = group_allreduce<16>(most, [](float a, float c) { return fmaxf(a, c); });
     const float s = fmaxf(most / kMostE4m3, kLeastScale);
+    // v / s, correctly rounded: from the correctly rounded 1 / s, two steps of quotient += remainder / s with exact
+    // remainders give what the division gives in half of its instructions.  Where a remainder that matters could
+    // underflow, or s is infinite, the division itself.  (The sign is v's: a zero's would be lost.)
+    if (s >= 0x1p-70f && s <= 0x1p120f) {
+      const float by = 1.f / s;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float u = v[e] * by;
+        u = __builtin_fmaf(__builtin_fmaf(-u, s, v[e]), by, u);
+        u = __builtin_fmaf(__builtin_fmaf(-u, s, v[e]), by, u);
+        v[e] = __builtin_copysignf(u, v[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] /= s;
+    }
     int w0 = 0, w1 = 0;
 #if defined(__HIP_DEVICE_COMPILE__)
-    w0 = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] / s, v[1] / s, w0, false);
-    w0 = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] / s, v[3] / s, w0, true);
-    w1 = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] / s, v[5] / s, w1, false);
-    w1 = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] / s, v[7] / s, w1, true);
+    w0 = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], w0, false);
+    w0 = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w0, true);
+    w1 = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], w1, false);
+    w1 = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], w1, true);
 #endif
     if constexpr (VECTOR) {
       if (l16 * 8 < n) *reinterpret_cast<uintx2*>(q + at + l16 * 8) = uintx2{(unsigned)w0, (unsigned)w1};

@@ -149,6 +149,23 @@ def test_a_nan_stays_in_its_row_or_column(odla, m):
     assert np.array_equal(np.isnan(got), nan)
 
 
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+def test_quantized_rows_of_every_magnitude(odla, kind):
+    """Blocks whose scales pass the borders between the two ways of dividing, each with values down to subnormals."""
+    announce("block quantisation of blocks of every magnitude, %s" % kind)
+    rng = np.random.default_rng(21)
+    exponents = np.array([-130, -118, -75, -71, -70, -69, -62, -61, -60, -20, 0, 60, 110, 118, 119, 127])
+    x = (1 + rng.random((len(exponents), 384))) * rng.choice([-1.0, 1.0], (len(exponents), 384)) / 2
+    x *= 2.0 ** rng.choice([0, -1, -5, -9, -12, -40], x.shape)
+    x = np.ldexp(x, exponents[:, None])
+    x[:, 5], x[:, 6], x[:, 130] = -0.0, 0.0, -2.0 ** -149
+    bits = R.to_bits(x, kind)
+    got = run_hip(quantize_graph(odla, kind, x.shape), {"x": bits})
+    q, s = R.quantize_rows(R.values(bits, kind))
+    assert np.array_equal(got["s"], s) and same_codes(got["q"], q)
+
+
+
 @pytest.mark.parametrize("mode", ["fp32", "fp16", "bf16"])
 def test_quantised_in_front_of_a_product(odla, mode):
     """FLOAT32 values as the precision mode stores them; the scales stay fp32 between the two operators."""
