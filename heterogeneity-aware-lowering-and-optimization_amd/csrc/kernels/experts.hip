@@ -103,15 +103,17 @@ __device__ __forceinline__ void choose(const ExpertsParams& p, const int t, cons
   *id = 0;
   for (int j = 0; j < p.top_k; ++j) {
     const unsigned k = wave_largest(best);
-    const int e = (int)~wave_largest(best == k ? ~(unsigned)at : 0u);
+    const unsigned long long some = __ballot(best == k);
+    const int e = (some & (some - 1)) == 0 ? __builtin_amdgcn_readlane(at, __ffsll(some) - 1) : (int)~wave_largest(best == k ? ~(unsigned)at : 0u);
     const float v = expf(number_of(k) - most);
     chosen += v;
     if (lane == j) { mine = v; *id = e; }
     if (lane == (e & 63)) {
       keys[e] = 0;
       best = 0;
-      for (int o = lane; o < p.E; o += 64)
-        if (keys[o] > best) { best = keys[o]; at = o; }
+      if (p.E > 64)
+        for (int o = lane; o < p.E; o += 64)
+          if (keys[o] > best) { best = keys[o]; at = o; }
     }
   }
   // (a NaN among the logits reaches every weight through the whole sum)
