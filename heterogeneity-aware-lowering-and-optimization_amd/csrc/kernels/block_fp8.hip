@@ -10,7 +10,8 @@ constexpr float kLeastScale = 1.17549435e-38f;   // 2^-126: x / scale stays fini
 
 // ------------------------------------------------------------- quantisation --
 // scale = max(max |x| / 448, 2^-126), q = e4m3(x / scale).  Bound by memory: es + 1 bytes per value.
-// Sixteen lanes hold a block, eight values each.
+// Sixteen lanes hold a block, eight values each.  8192 x 7168 bf16: 33 us, 5.3 TB/s read and written (with a
+// division per value 40); 1 x 4096: 2.2 us, a launch.
 template <typename T, bool VECTOR>
 __global__ void __launch_bounds__(256) block_quantize_kernel(const T* x, uint8_t* q, float* scale, const int64_t rows, const int len, const int blocks) {
   const int l16 = threadIdx.x & 15;
@@ -97,6 +98,9 @@ hipError_t quantize_as(const void* x, void* q, float* scale, int64_t rows, int64
 // a compute unit gets 36 KB/us out of L2 instead of 120 (measured; from memory 26 either way).
 // A block's sum is scaled on its way into the accumulator: the scale of row m belongs to a lane (column of
 // the matrix result), that of B to the whole tile.  EXACT: through bf16 (see mma_exact).
+// K = 4096: 1 row x 4096 columns 6.1 us, 64 rows 11.6, 128 rows 11.5, 256 rows 14.6; 48 x 7168 x 2048 6.7 us;
+// 100 x 1000 x 8000 13.5; 509 x 2500 x 1400 (rows that are no whole vectors) 17.  A call's first bytes from memory and
+// the meeting of the sums are 4 to 5 us of that.
 template <typename TOut, int NT, int MT, int P, bool EXACT, bool ALIGNED>
 __global__ void __launch_bounds__(512) block_gemm_split_kernel(const BlockGemmParams p) {
   constexpr int ROWS = 16 * (NT + MT);     // of B, then of A

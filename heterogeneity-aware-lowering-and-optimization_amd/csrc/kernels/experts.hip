@@ -4,9 +4,14 @@
 //   l = router x, top k of l; w = softmax(l) of those (divided by their sum)
 //   h = silu(gate_e x) * (up_e x),   y = sum_j w_j down_ej h_j
 //
-// Few tokens: bound by the weights of the experts that some token chose, which are read once.  Their
-// rows go straight into operand registers of the matrix instructions, sixteen rows a tile; the
-// tokens that chose the expert are the columns (up to sixteen at no further cost).
+// Few tokens: bound by the weights of the experts that some token chose, which are read once: their rows are the
+// rows of a matrix product, the tokens that chose the expert its columns.  Four launches (three where the first
+// product makes the choice itself): logits, choice, first product, second product with its parts, sum.
+//   64 experts of 2048 x 1024, 8 chosen, bf16: 1 token 5 + 17 (100 MB in all) + 9 + 4 us; 32 tokens 7 + 4 + 98 +
+//   51 + 4 us, 5.4 TB/s in the products.  7 tokens, 128 experts of 2624 x 704, 8-bit weights 7 + 30 + 16 + 4 us,
+//   4.5 TB/s; of 2600 x 712, rows that are no whole vectors, 35 + 22.
+// The last of a token's parts adding them up instead of a launch was slower: making parts visible to the
+// other chiplets costs more (a release of the whole L2 in every tile: 52 -> 240 us).
 #include "block_common.h"
 #include "lds_limit.h"
 
@@ -464,7 +469,7 @@ __global__ void __launch_bounds__(512, C > 8 || sizeof(X) > 2 * sizeof(W) ? 1 : 
   }
 }
 
-// ---- y[t][n] = sum of the parts of token t, in the order of its choices ----
+// ---- y[t][n] = sum of the parts of token t, in the order of its choices: a launch's 4 us and little else ----
 template <typename X>
 __global__ void __launch_bounds__(256) experts_sum_kernel(const ExpertsParams p) {
   const int64_t n = (int64_t)p.tokens * p.H;
