@@ -99,7 +99,7 @@ hipError_t quantize_as(const void* x, void* q, float* scale, int64_t rows, int64
 // A block's sum is scaled on its way into the accumulator: the scale of row m belongs to a lane (column of
 // the matrix result), that of B to the whole tile.  EXACT: through bf16 (see mma_exact).
 // K = 4096: 1 row x 4096 columns 6.1 us, 64 rows 11.6, 128 rows 11.5, 256 rows 14.6; 48 x 7168 x 2048 6.7 us;
-// 100 x 1000 x 8000 13.5; 509 x 2500 x 1400 (rows that are no whole vectors) 17.  A call's first bytes from memory and
+// 100 x 1000 x 8000 13.5; 509 x 2500 x 1400 (rows that are no whole vectors) 13.5.  A call's first bytes from memory and
 // the meeting of the sums are 4 to 5 us of that.
 template <typename TOut, int NT, int MT, int P, bool EXACT, bool ALIGNED>
 __global__ void __launch_bounds__(512) block_gemm_split_kernel(const BlockGemmParams p) {
@@ -452,7 +452,11 @@ hipError_t gemm_split(const BlockGemmParams& p, hipStream_t stream) {
   constexpr bool EXACT = sizeof(TOut) == 4 || MT == 1;
   constexpr int kOwn = 16 * (NT + MT) * kScaleBlock, kSums = NT * MT * 64 * 16;   // bytes of a wavefront: operands, sums
   const int KB = (p.K + kScaleBlock - 1) / kScaleBlock;
-  const int waves = KB < 8 ? KB : 8, lds = waves * (kOwn > kSums ? kOwn : kSums);
+  // Eight wavefronts, but four where eight fill a compute unit's LDS and there are more tiles than units: two tiles a
+  // unit then run side by side.  N = K = 4096, 512 rows: 24.4 us (eight: 26.9); 509 x 2500 x 1400 13.5 (18.0).
+  const int64_t tiles = (int64_t)((p.N + 16 * NT - 1) / (16 * NT)) * ((p.M + 16 * MT - 1) / (16 * MT));
+  const int most = tiles > 256 && 8 * kOwn > 80 * 1024 ? 4 : 8;
+  const int waves = KB < most ? KB : most, lds = waves * (kOwn > kSums ? kOwn : kSums);
   static LdsLimit limit;
   hipError_t e = limit.raise(reinterpret_cast<const void*>(&block_gemm_split_kernel<TOut, NT, MT, P, EXACT, ALIGNED>), 8 * (kOwn > kSums ? kOwn : kSums));
   if (e != hipSuccess) return e;
@@ -477,7 +481,7 @@ hipError_t gemm_as(const BlockGemmParams& p, hipStream_t stream) {
     }
   }
   // Too few of the tiles below for every compute unit: 64 x 64 results (64 rows x 32 columns where even those are
-  // few).  N = K = 4096: a tile below takes 47 us however few there are; here 512 rows take 27 us, 256 14.5.
+  // few).  N = K = 4096: a tile below takes 47 us however few there are; here 512 rows take 24 us, 256 14.5.
   if ((int64_t)((p.M + 127) / 128) * ((p.N + 127) / 128) < 256) {
     if ((int64_t)((p.M + 63) / 64) * ((p.N + 31) / 32) <= 320) return gemm_split<TOut, 2, 4, 1, ALIGNED>(p, stream);
     if constexpr (sizeof(TOut) == 2) return gemm_split<TOut, 4, 4, 1, ALIGNED>(p, stream);
