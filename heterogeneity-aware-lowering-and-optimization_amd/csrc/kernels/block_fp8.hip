@@ -316,31 +316,39 @@ __global__ void __launch_bounds__(256) block_gemm_tile_kernel(const BlockGemmPar
     }
 }
 
-// Many rows and columns: 256 x 256 results a workgroup of eight wavefronts, 128 rows m x 64 columns n each.
-// Both operands come by direct-to-LDS loads, 128 terms (64 KiB) at a time into one of two buffers while
+// Many rows and columns: 256 x 256 results a workgroup of eight wavefronts, 128 rows m x 64 columns n each, or
+// 128 x 128 of four, 64 x 64 each, two workgroups a compute unit.
+// Both operands come by direct-to-LDS loads, 128 terms (64 or 32 KiB) at a time into one of two buffers while
 // the other is multiplied: one barrier per block of terms, and every fragment of B stays in registers
-// through the eight of A.  LDS rows are 128 bytes, 16-byte chunk c of row r in slot c ^ (r / 2 & 7), and a
+// through those of A.  LDS rows are 128 bytes, 16-byte chunk c of row r in slot c ^ (r / 2 & 7), and a
 // quarter g of a wavefront takes chunks g and g + 4 (which terms a lane holds does not matter as long as A
 // and B agree): no two of the sixteen lanes that LDS serves at a time share a bank.  With chunks 2 g and
 // 2 g + 1 half of LDS's busy cycles are conflicts (counters: 25 M of 55 M at 8192 x 8192 x 4096).
-constexpr int kBigStage = 512 * kScaleBlock;          // bytes of a buffer: 256 rows of A, 256 of B
-constexpr int kBigLds = 2 * kBigStage + 2 * 512 * 4;  // and the scales of the rows of A (twice: every thread stores one)
-// A wavefront's request i is of rows 64 i + 8 wave .. + 7; what lies behind the operand's end, or in the last
+template <int WAVES>
+struct Big {
+  static constexpr int SIDE = 32 * WAVES;                            // rows of A, of B
+  static constexpr int FM = WAVES;                                   // fragments of a wavefront's rows, of its columns
+  static constexpr int FN = 4;
+  static constexpr int STAGE = 2 * SIDE * kScaleBlock;               // bytes of a buffer
+  static constexpr int LDS = 2 * STAGE + 2 * 64 * WAVES * 4;         // and the scales of the rows of A (twice: every thread stores one)
+};
+// A wavefront's request i is of rows 8 WAVES i + 8 wave .. + 7; what lies behind the operand's end, or in the last
 // block behind the row's, is out of the buffer's range and arrives as zeros.
 struct BigSource {
   __amdgpu_buffer_rsrc_t a, b;
   unsigned at;     // this lane's offset in request 0 of a block
-  unsigned step;   // 64 rows
+  unsigned step;   // 8 WAVES rows
   int left;        // bytes of a row from this lane's chunk on
 };
+template <int WAVES>
 __device__ __forceinline__ void big_request(const BigSource& f, const int kb, unsigned char* to) {
   using lds_ptr = __attribute__((address_space(3))) void*;
 #if defined(__HIP_DEVICE_COMPILE__)
   const unsigned at = kb * kScaleBlock < f.left ? f.at : 0xfffffff0u;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(f.a, (lds_ptr)(to + i * 8192), 16, at, i * f.step + kb * kScaleBlock, 0, 0);
+  for (int i = 0; i < 4; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(f.a, (lds_ptr)(to + i * 1024 * WAVES), 16, at, i * f.step + kb * kScaleBlock, 0, 0);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(f.b, (lds_ptr)(to + 32768 + i * 8192), 16, at, i * f.step + kb * kScaleBlock, 0, 0);
+  for (int i = 0; i < 4; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(f.b, (lds_ptr)(to + Big<WAVES>::SIDE * kScaleBlock + i * 1024 * WAVES), 16, at, i * f.step + kb * kScaleBlock, 0, 0);
 #else
   (void)f; (void)kb; (void)to;
 #endif
@@ -348,17 +356,19 @@ __device__ __forceinline__ void big_request(const BigSource& f, const int kb, un
 
 // One block of terms: the next one is requested into `next`, the one in `now` multiplied.  The two
 // never overlap (without saying so, every read of LDS would wait for the requests).
+template <int WAVES>
 __device__ __forceinline__ void big_block(const BigSource& from, const int kb, unsigned char* __restrict next, const unsigned char* __restrict now,
                                           const float* __restrict scales, const float sb, const int wm, const int wn, const int lane, const int wave,
-                                          floatx4 (&acc)[8][4]) {
-  big_request(from, kb + 1, next + wave * 1024);   // (behind the last block: zeros)
+                                          floatx4 (&acc)[Big<WAVES>::FM][Big<WAVES>::FN]) {
+  constexpr int FM = Big<WAVES>::FM, FN = Big<WAVES>::FN, PRODUCTS = FM * FN;
+  big_request<WAVES>(from, kb + 1, next + wave * 1024);   // (behind the last block: zeros)
   const int r = lane & 15, g = lane >> 4;
   const int sw = r >> 1;      // (rows of a fragment start at multiples of 16)
   const int c0 = (g ^ sw) * 16, c1 = ((g + 4) ^ sw) * 16;
-  uintx4 w0[4], w1[4];
+  uintx4 w0[FN], w1[FN];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const unsigned char* at = now + (256 + wn + 16 * j + r) * kScaleBlock;
+  for (int j = 0; j < FN; ++j) {
+    const unsigned char* at = now + (Big<WAVES>::SIDE + wn + 16 * j + r) * kScaleBlock;
     w0[j] = *reinterpret_cast<const uintx4*>(at + c0);
     w1[j] = *reinterpret_cast<const uintx4*>(at + c1);
   }
@@ -382,22 +392,23 @@ __device__ __forceinline__ void big_block(const BigSource& from, const int kb, u
   };
   fetch(0);
 #pragma unroll
-  for (int n = 0; n < 32; ++n) {
+  for (int n = 0; n < PRODUCTS; ++n) {
     const int i = n >> 2, j = n & 3;
     if (j == 0) by[i & 1] = s[i & 1] * sb;
     part[n % (LAG + 1)] = mma_e4m3(w0[j], w1[j], x[i & 1][0], x[i & 1][1], floatx4{0.f, 0.f, 0.f, 0.f});
-    if (j == 0 && i + 1 < 8) fetch(i + 1);
+    if (j == 0 && i + 1 < FM) fetch(i + 1);
     if (n >= LAG) scale(n - LAG);
     __builtin_amdgcn_sched_barrier(0);
   }
 #pragma unroll
-  for (int n = 32 - LAG; n < 32; ++n) scale(n);
+  for (int n = PRODUCTS - LAG; n < PRODUCTS; ++n) scale(n);
 }
 
-template <typename TOut>
-__global__ void __launch_bounds__(512, 2) block_gemm_big_kernel(const BlockGemmParams p, const int tiles_m, const int tiles_n) {
+template <typename TOut, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, 2) block_gemm_big_kernel(const BlockGemmParams p, const int tiles_m, const int tiles_n) {
+  constexpr int SIDE = Big<WAVES>::SIDE, FM = Big<WAVES>::FM, FN = Big<WAVES>::FN, STAGE = Big<WAVES>::STAGE;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  float* const scales = reinterpret_cast<float*>(smem + 2 * kBigStage);
+  float* const scales = reinterpret_cast<float*>(smem + 2 * STAGE);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // Workgroups are dealt round-robin to the 8 XCDs: an XCD takes neighbours of a walk through groups of
   // eight tiles of rows, so that its workgroups share both operands in its L2.
@@ -407,41 +418,41 @@ __global__ void __launch_bounds__(512, 2) block_gemm_big_kernel(const BlockGemmP
     if (t < per << 3) t = (t & 7) * per + (t >> 3);
   }
   const int group = t / (8 * tiles_n), rows = min(8, tiles_m - 8 * group), in = t - group * 8 * tiles_n;
-  const int m0 = (8 * group + in % rows) * 256, n0 = in / rows * 256;
+  const int m0 = (8 * group + in % rows) * SIDE, n0 = in / rows * SIDE;
   const int KB = (p.K + kScaleBlock - 1) / kScaleBlock;
   const int chunk = ((lane & 7) ^ (((8 * wave + (lane >> 3)) >> 1) & 7)) * 16;
   BigSource from;
-  from.a = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.a) + (int64_t)m0 * p.K, 0, min(256, p.M - m0) * p.K, 0x00020000);
-  from.b = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.b) + (int64_t)n0 * p.K, 0, min(256, p.N - n0) * p.K, 0x00020000);
+  from.a = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.a) + (int64_t)m0 * p.K, 0, min(SIDE, p.M - m0) * p.K, 0x00020000);
+  from.b = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.b) + (int64_t)n0 * p.K, 0, min(SIDE, p.N - n0) * p.K, 0x00020000);
   from.at = (8 * wave + (lane >> 3)) * p.K + chunk;
-  from.step = 64u * p.K;
+  from.step = 8u * WAVES * p.K;
   from.left = p.K - chunk;
-  const float* arow_scale = p.a_scale + (int64_t)min(m0 + (tid & 255), p.M - 1) * KB;
-  const int wm = (wave & 1) * 128, wn = (wave >> 1) * 64;
+  const float* arow_scale = p.a_scale + (int64_t)min(m0 + (tid & (SIDE - 1)), p.M - 1) * KB;
+  const int wm = (wave & 1) * 16 * FM, wn = (wave >> 1) * 16 * FN;
   const float* bs = p.b_scale + (int64_t)min((n0 + wn) / kScaleBlock, (p.N - 1) / kScaleBlock) * KB;
-  floatx4 acc[8][4];
+  floatx4 acc[FM][FN];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < FN; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
   scales[tid] = arow_scale[0];
   float sb = bs[0];
-  big_request(from, 0, smem + wave * 1024);
+  big_request<WAVES>(from, 0, smem + wave * 1024);
   for (int kb = 0; kb < KB; ++kb) {
     __syncthreads();     // this block's operands have landed, and everybody has left the other buffer
     // (both scales of the next block ahead of its operands: a wait for them would wait for those too)
     const float next_scale = arow_scale[min(kb + 1, KB - 1)], next_sb = bs[min(kb + 1, KB - 1)];
     __builtin_amdgcn_sched_barrier(0);
-    big_block(from, kb, smem + (~kb & 1) * kBigStage, smem + (kb & 1) * kBigStage, scales + (kb & 1) * 512, sb, wm, wn, lane, wave, acc);
-    scales[(~kb & 1) * 512 + tid] = next_scale;
+    big_block<WAVES>(from, kb, smem + (~kb & 1) * STAGE, smem + (kb & 1) * STAGE, scales + (kb & 1) * 64 * WAVES, sb, wm, wn, lane, wave, acc);
+    scales[(~kb & 1) * 64 * WAVES + tid] = next_scale;
     sb = next_sb;
   }
   __syncthreads();       // (nothing is under way into LDS when the workgroup ends)
   const int r = lane & 15, g = lane >> 4;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < FN; ++j) {
       const int m = m0 + wm + 16 * i + r, n = n0 + wn + 16 * j + 4 * g;
       if (m < p.M && n < p.N) store4((TOut*)p.y + (int64_t)m * p.N + n, acc[i][j], p.N - n, (p.N & 3) == 0);
     }
@@ -464,20 +475,30 @@ hipError_t gemm_split(const BlockGemmParams& p, hipStream_t stream) {
                      dim3(64 * waves), lds, stream, p);
   return hipGetLastError();
 }
+// From here on 128 x 128 results a workgroup, loaded straight into LDS, beat 64 x 64 with the terms shared out.
+// N = K = 4096: 512 rows (128 tiles) 26.6 us against 24.4, 1024 rows 29.3 against 47 (four times 256 rows' 14.5).
+constexpr int kMiddleTiles = 144;
+template <typename TOut, int WAVES>
+hipError_t gemm_big(const BlockGemmParams& p, hipStream_t stream) {
+  constexpr int SIDE = Big<WAVES>::SIDE, LDS = Big<WAVES>::LDS;
+  const int64_t tm = (p.M + SIDE - 1) / SIDE, tn = (p.N + SIDE - 1) / SIDE;
+  static LdsLimit limit;
+  hipError_t e = limit.raise(reinterpret_cast<const void*>(&block_gemm_big_kernel<TOut, WAVES>), LDS);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((block_gemm_big_kernel<TOut, WAVES>), dim3((unsigned)(tm * tn)), dim3(64 * WAVES), LDS, stream, p, (int)tm, (int)tn);
+  return hipGetLastError();
+}
 template <typename TOut, bool ALIGNED>
 hipError_t gemm_as(const BlockGemmParams& p, hipStream_t stream) {
   // Two tiles of columns a workgroup where that still leaves one for most of the compute units.
   if (p.M <= 16) return gemm_split<TOut, 1, 1, 4, ALIGNED>(p, stream);
   if (p.M <= 32) return p.N > 32 * 192 ? gemm_split<TOut, 2, 2, 2, ALIGNED>(p, stream) : gemm_split<TOut, 1, 2, 2, ALIGNED>(p, stream);
   if (p.M <= 64) return p.N > 32 * 192 ? gemm_split<TOut, 2, 4, 1, ALIGNED>(p, stream) : gemm_split<TOut, 1, 4, 2, ALIGNED>(p, stream);
-  const int64_t tm = (p.M + 255) / 256, tn = (p.N + 255) / 256;
   if constexpr (ALIGNED && sizeof(TOut) == 2) {
-    if (tm * tn >= 192 && p.K <= 1 << 22) {   // (256 rows of an operand within 2^30 bytes of buffer range)
-      static LdsLimit limit;
-      hipError_t e = limit.raise(reinterpret_cast<const void*>(&block_gemm_big_kernel<TOut>), kBigLds);
-      if (e != hipSuccess) return e;
-      hipLaunchKernelGGL((block_gemm_big_kernel<TOut>), dim3((unsigned)(tm * tn)), dim3(512), kBigLds, stream, p, (int)tm, (int)tn);
-      return hipGetLastError();
+    // 256 x 256 for three quarters of the compute units at least: 3000 x 4096 x 4096 72 us; 2048 rows in 128 x 128 47 us.
+    if (p.K <= 1 << 22) {   // (256 rows of an operand within 2^30 bytes of buffer range)
+      if ((int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256) >= 192) return gemm_big<TOut, 8>(p, stream);
+      if ((int64_t)((p.M + 127) / 128) * ((p.N + 127) / 128) >= kMiddleTiles) return gemm_big<TOut, 4>(p, stream);
     }
   }
   // Too few of the tiles below for every compute unit: 64 x 64 results (64 rows x 32 columns where even those are

@@ -610,9 +610,9 @@ def test_the_largest_vocabulary(odla):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp16"])
-@pytest.mark.parametrize("m,n,k", [(3500, 3500, 400), (4100, 3080, 128), (257, 49000, 272)])
+@pytest.mark.parametrize("m,n,k", [(3500, 3500, 400), (4100, 3080, 128), (257, 49000, 272), (1500, 1700, 400), (1161, 2305, 128), (130, 12000, 1040)])
 def test_block_product_of_many_tiles(odla, kind, m, n, k):
-    """Sizes that give every compute unit a large tile; checked on rows and columns across the edges of tiles."""
+    """Sizes that give (most of) the compute units a tile of 256 x 256, or of 128 x 128; checked on rows and columns across the edges of tiles."""
     announce("block product %s %d x %d x %d" % (kind, m, n, k))
     rng = np.random.default_rng(m + n)
     a = (rng.integers(0, 256, (m, k), dtype=np.uint8) & 0xbf, rng.uniform(0.5, 2, (m, R.blocks(k))).astype(np.float32))
