@@ -619,6 +619,7 @@ def test_block_product_of_many_tiles(odla, kind, m, n, k):
     b = (rng.integers(0, 256, (n, k), dtype=np.uint8) & 0xbf, rng.uniform(0.001, 0.1, (R.blocks(n), R.blocks(k))).astype(np.float32))
     got = R.values(run_hip(gemm_graph(odla, kind, a, b), {"a": a[0], "sa": a[1], "b": b[0], "sb": b[1]})["y"], kind)
     rows = np.unique(np.concatenate([np.arange(0, m, 97), [m - 1, 255, 256], np.arange(120, 136)]))
+    rows = rows[rows < m]
     for at in (slice(0, 300), slice(n - 300, n)):
         cols = np.arange(n)[at]
         bb = b[0][cols]
