@@ -256,6 +256,24 @@ def test_experts(odla, kind, weights, t, e, h, i, top_k):
     check(R.values(got, kind), want, bound, "experts")
 
 
+@pytest.mark.parametrize("kind,weights", [("fp32", "fp32"), ("bf16", "bf16"), ("bf16", "fp8"), ("fp32", "fp8")])
+@pytest.mark.parametrize("t,e,h,i,top_k", [(64, 64, 72, 200, 4), (64, 40, 72, 330, 2), (200, 16, 272, 152, 3), (300, 4, 136, 104, 2), (65, 1, 64, 600, 1),
+                                           (2, 2, 33100, 20, 2), (3, 1, 24, 33040, 1), (40, 2, 33040, 10, 2), (8, 1024, 40, 8, 32)])
+def test_experts_of_many_tiles_columns_and_steps(odla, kind, weights, t, e, h, i, top_k):
+    """More tiles than resident workgroups, more columns than a tile has, rows of more than 64 steps a wavefront."""
+    announce("experts %s / %s: %d tokens, %d of %d experts, %d x %d" % (kind, weights, t, top_k, e, h, i))
+    d = expert_operands(t, e, h, i, kind, weights, seed=t + 10 * e + h + i)
+    got = R.values(run_hip(expert_graph(odla, d, top_k, kind, weights), d, repeats=2)["y"], kind)
+    x, router, gate_up, down = expert_values(d, kind, weights)
+    sure = np.ones(t, bool)
+    if top_k < e:       # (tokens whose choice is clear)
+        order = np.sort(x @ router.T, 1)
+        sure = order[:, -top_k] - order[:, -top_k - 1] > 4.1 * (h + 2) * R.UNIT * (np.abs(x) @ np.abs(router).T).max(1)
+        assert sure.sum() >= 0.75 * t
+    want, bound = R.experts(x[sure], router, gate_up, down, top_k, True, 1.0, kind, weights == "fp8")
+    check(got[sure], want, bound, "experts")
+
+
 def test_experts_with_constant_weights_and_leading_extents(odla):
     announce("experts, constants, rank 3")
     d = expert_operands(10, 12, 144, 80, "bf16", "fp8", seed=77)
