@@ -45,6 +45,18 @@ __device__ __forceinline__ uintx4 load_row16(const unsigned char* row, const int
   }
 }
 
+// 16 bytes at base + at + uniform (any alignment); zeros where that is not within `size` bytes from `base` on.
+constexpr unsigned kOutside = 0xfffffff0u;
+__device__ __forceinline__ uintx4 load_within(const unsigned char* base, const unsigned size, const unsigned at, const unsigned uniform) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(base), 0, size, 0x00020000);
+  return __builtin_bit_cast(uintx4, __builtin_amdgcn_raw_buffer_load_b128(r, at, uniform, 0));
+#else
+  (void)base; (void)size; (void)at; (void)uniform;
+  return uintx4{0u, 0u, 0u, 0u};
+#endif
+}
+
 // c + A B^T for 16 rows of A and 16 of B over 128 e4m3 values: lane l supplies 32 values of row
 // l % 16 of either, those of quarter l / 16 of the 128 (which quarter holds which values does not
 // matter as long as A and B agree).  Result element i of lane l: row 4 * (l / 16) + i of A, row

@@ -99,7 +99,7 @@ hipError_t quantize_as(const void* x, void* q, float* scale, int64_t rows, int64
 // A block's sum is scaled on its way into the accumulator: the scale of row m belongs to a lane (column of
 // the matrix result), that of B to the whole tile.  EXACT: through bf16 (see mma_exact).
 // K = 4096: 1 row x 4096 columns 6.1 us, 64 rows 11.6, 128 rows 11.5, 256 rows 14.6; 48 x 7168 x 2048 6.7 us;
-// 100 x 1000 x 8000 13.5; 509 x 2500 x 1400 (rows that are no whole vectors) 13.5.  A call's first bytes from memory and
+// 100 x 1000 x 8000 13.5; 509 x 2500 x 1400 (rows that are no whole vectors) 11.4.  A call's first bytes from memory and
 // the meeting of the sums are 4 to 5 us of that.
 template <typename TOut, int NT, int MT, int P, bool EXACT, bool ALIGNED>
 __global__ void __launch_bounds__(512) block_gemm_split_kernel(const BlockGemmParams p) {
@@ -136,15 +136,18 @@ __global__ void __launch_bounds__(512) block_gemm_split_kernel(const BlockGemmPa
   auto fetch = [&](const int kb, const int q) __attribute__((always_inline)) {
     if (kb >= KB) return;
     const int at = kb * kScaleBlock + chunk * 16;
-    const unsigned lane_at = lane_row + (ALIGNED ? at : min(at, p.K - 16));
+    const unsigned lane_at = ALIGNED ? lane_row + at : at < p.K ? lane_row + min(at, p.K - 16) : kOutside;
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
       const bool is_b = i < 2 * NT;
-      const int first = 8 * (is_b ? i : i - 2 * NT);
-      const unsigned char* row = (is_b ? b_tile : a_tile) + (int64_t)first * p.K;
-      in[q][i] = uintx4{0u, 0u, 0u, 0u};
-      if (in_vectors && first + l8 < (is_b ? b_rows : a_rows) && at < p.K)
-        in[q][i] = ALIGNED ? *reinterpret_cast<const uintx4*>(row + lane_at) : reinterpret_cast<const Bytes16*>(row + lane_at)->v;
+      const int first = 8 * (is_b ? i : i - 2 * NT), rows = is_b ? b_rows : a_rows;
+      const unsigned char* const tile = is_b ? b_tile : a_tile;
+      if constexpr (ALIGNED) {
+        in[q][i] = uintx4{0u, 0u, 0u, 0u};
+        if (first + l8 < rows && at < p.K) in[q][i] = *reinterpret_cast<const uintx4*>(tile + (int64_t)first * p.K + lane_at);
+      } else {            // (a load with a range: fewer registers)
+        in[q][i] = load_within(tile, in_vectors ? rows * p.K : 0, lane_at, first * p.K);
+      }
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t) sa[q][t] = as[t][kb];
@@ -167,17 +170,21 @@ __global__ void __launch_bounds__(512) block_gemm_split_kernel(const BlockGemmPa
 #pragma unroll
             for (int i = 0; i < NR; ++i) in[q][i] = bytes_down(in[q][i], behind);
           }
-        } else if (behind < 16) {
-#pragma unroll
+        } else {
+#pragma unroll 1
           for (int i = 0; i < NR; ++i) {
             const bool is_b = i < 2 * NT;
             const int row = 8 * (is_b ? i : i - 2 * NT) + l8;
-            if (row < (is_b ? b_rows : a_rows)) in[q][i] = load_row16<false>((is_b ? b_tile : a_tile) + (int64_t)row * p.K, chunk * 16, p.K);
+            uintx4 v = {0u, 0u, 0u, 0u};
+            if (behind < 16 && row < (is_b ? b_rows : a_rows)) v = load_row16<false>((is_b ? b_tile : a_tile) + (int64_t)row * p.K, chunk * 16, p.K);
+            *place(i) = v;
           }
         }
       }
+      if (in_vectors) {
 #pragma unroll
-      for (int i = 0; i < NR; ++i) *place(i) = in[q][i];
+        for (int i = 0; i < NR; ++i) *place(i) = in[q][i];
+      }
       float scale[MT];
 #pragma unroll
       for (int t = 0; t < MT; ++t) scale[t] = sa[q][t] * sb[q];
@@ -464,7 +471,7 @@ hipError_t gemm_split(const BlockGemmParams& p, hipStream_t stream) {
   constexpr int kOwn = 16 * (NT + MT) * kScaleBlock, kSums = NT * MT * 64 * 16;   // bytes of a wavefront: operands, sums
   const int KB = (p.K + kScaleBlock - 1) / kScaleBlock;
   // Eight wavefronts, but four where eight fill a compute unit's LDS and there are more tiles than units: two tiles a
-  // unit then run side by side.  N = K = 4096, 512 rows: 24.4 us (eight: 26.9); 509 x 2500 x 1400 13.5 (18.0).
+  // unit then run side by side.  N = K = 4096, 512 rows: 24.4 us (eight: 26.9); 509 x 2500 x 1400, before its loads had a range, 13.5 (18.0).
   const int64_t tiles = (int64_t)((p.N + 16 * NT - 1) / (16 * NT)) * ((p.M + 16 * MT - 1) / (16 * MT));
   const int most = tiles > 256 && 8 * kOwn > 80 * 1024 ? 4 : 8;
   const int waves = KB < most ? KB : most, lds = waves * (kOwn > kSums ? kOwn : kSums);

@@ -210,17 +210,6 @@ struct Staging {
   static constexpr int BYTES = 4096 + XR * 1024;                  // of a wavefront
   static_assert(BYTES >= 2 * ((C + 15) / 16) * 1024, "the sums take the operands' place");
 };
-// 16 bytes at `at`; zeros where that is not within `size` bytes from `base` on.
-constexpr unsigned kOutside = 0xfffffff0u;
-__device__ __forceinline__ uintx4 load_within(const unsigned char* base, const unsigned size, const unsigned at, const unsigned uniform) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(base), 0, size, 0x00020000);
-  return __builtin_bit_cast(uintx4, __builtin_amdgcn_raw_buffer_load_b128(r, at, uniform, 0));
-#else
-  (void)base; (void)size; (void)at; (void)uniform;
-  return uintx4{0u, 0u, 0u, 0u};
-#endif
-}
 template <bool GATED>
 __host__ __device__ inline int tile_rows(const ExpertsParams& p) { return GATED ? (p.I + 15) / 16 : (p.H + 31) / 32; }
 
