@@ -418,6 +418,28 @@ def test_rows_that_leave_little(odla):
     assert got[0] == -1 and got[1] == -1 and got[2] == 211
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("v", [300, 6001, 70000])
+def test_rows_with_infinite_logits(odla, kind, v):
+    """Only the infinite ones are drawn, alike, whatever the cuts leave of them."""
+    announce("sampling %s from %d logits with infinite ones" % (kind, v))
+    rng = np.random.default_rng(v)
+    p = {n: [] for n in PARAMS}
+    for k in (0, 1, 2, 3, 4, 20, 2500):
+        for top_p in (1.0, 0.6, 0.3):
+            for min_p, temperature in ((0.0, 1.0), (0.5, 0.3), (0.0, np.inf)):
+                for n, a in zip(PARAMS, (temperature, k, top_p, min_p, rng.random())):
+                    p[n].append(a)
+    rows = len(p["top_k"])
+    x = rng.standard_normal((rows, v)) * 4
+    x[:, ::7] = -np.inf
+    x[:, 5] = {"fp32": 3.4028234e38, "fp16": 65504.0, "bf16": 3.3895e38}[kind]
+    for r in range(rows):
+        x[r, rng.choice(v, 3, replace=False)] = np.inf
+    got, want = run_sample(odla, kind, R.to_bits(x, kind), p)
+    assert np.array_equal(got, want), [(i, int(g), int(w)) for i, (g, w) in enumerate(zip(got, want)) if g != w]
+
+
 def test_drawn_frequencies_follow_the_weights(odla):
     """Evenly spaced random numbers hit every token by its share of the sum, to one draw."""
     announce("sampling frequencies")
