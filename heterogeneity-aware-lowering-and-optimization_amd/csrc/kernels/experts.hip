@@ -480,8 +480,10 @@ bool valid(const ExpertsParams& p) {
 // rows of x, hidden and weights are whole 16-byte vectors
 bool whole_vectors(const ExpertsParams& p, const int len) { return (int64_t)len * dtype_size(p.dt) % 16 == 0 && (int64_t)len * dtype_size(p.w_dt) % 16 == 0; }
 
-// Eight columns at a time, unless experts get more than four tokens on average.
-bool few_columns(const ExpertsParams& p) { return p.tokens <= 8 || (int64_t)p.tokens * p.top_k <= 4 * (int64_t)p.E; }
+// Eight columns at a time, unless experts get more than eight tokens on average (an expert with more is read again).
+// 64 experts of 2048 x 1024, 8 chosen, both products in us, eight columns / 64 (bf16) or 32 (8-bit weights):
+//   four tokens an expert 153 / 181, six 161 / 184, eight 179 / 186, twelve 226 / 194;  8-bit: eight 104 / 114, twelve 131 / 124.
+bool few_columns(const ExpertsParams& p) { return p.tokens <= 8 || (int64_t)p.tokens * p.top_k <= 8 * (int64_t)p.E; }
 // Two steps of 128 bytes a wavefront at least, and a wavefront for every sixteen columns.
 template <int C>
 int product_waves(const ExpertsParams& p, const int K) {
@@ -521,11 +523,10 @@ hipError_t product_one(const ExpertsParams& p, hipStream_t stream) {
 }
 template <typename X, typename W, bool GATED>
 hipError_t product_as(const ExpertsParams& p, hipStream_t stream) {
-  constexpr int MANY = sizeof(X) / sizeof(W) == 4 ? 32 : 64;      // (x of a step within LDS)
+  constexpr int MANY = 64 * sizeof(W) / sizeof(X);      // (two steps under way within registers)
   const bool a = whole_vectors(p, GATED ? p.H : p.I);
-  constexpr int P = sizeof(X) == sizeof(W) ? 2 : 1;             // (within registers)
   if (few_columns(p)) return a ? product_one<X, W, 8, 2, true, GATED>(p, stream) : product_one<X, W, 8, 2, false, GATED>(p, stream);
-  return a ? product_one<X, W, MANY, P, true, GATED>(p, stream) : product_one<X, W, MANY, P, false, GATED>(p, stream);
+  return a ? product_one<X, W, MANY, 2, true, GATED>(p, stream) : product_one<X, W, MANY, 2, false, GATED>(p, stream);
 }
 template <typename X, typename W>
 hipError_t gate_up_as(const ExpertsParams& p, hipStream_t stream) { return product_as<X, W, true>(p, stream); }
