@@ -16,6 +16,7 @@
 // other chiplets costs more (a release of the whole L2 in every tile: 52 -> 240 us).
 #include "block_common.h"
 #include "lds_limit.h"
+#include "row_range.h"
 
 namespace ohip {
 namespace {
@@ -290,8 +291,9 @@ __global__ void __launch_bounds__(512, C > 8 || sizeof(X) > 2 * sizeof(W) ? 1 : 
     int row0[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      row0[j] = GATED ? j * p.I + n0 : n0 + 16 * j;
-      w_rows[j] = min(16, GATED ? p.I - n0 : p.H - row0[j]);
+      const RowTile half = expert_rows(GATED, n0, j, p.I, p.H);     // (the last tile's second half may have no rows)
+      row0[j] = half.row0;
+      w_rows[j] = half.rows;
       w_tile[j] = w + (int64_t)row0[j] * wlen;
     }
     if constexpr (SCALED) {
