@@ -405,7 +405,7 @@ bool token_op_shapes(OpKind op, const std::vector<_odla_value*>& in, const int64
       if (dn->shape.rank != 3) return no("down " + dn->shape.str() + " must be [E, H, I]");
       const int64_t I = dn->shape.d[2];
       if (I > kMost / 2) return no("down " + dn->shape.str() + " is too large");
-      if (rows * H * 4 >= kMaxExpertBytes || rows * attr[0] * I * 4 >= kMaxExpertBytes) return no("the tokens or their hidden rows, at four bytes an element, pass 4 GiB");
+      if (rows * H * 4 > kMaxExpertBytes || rows * attr[0] * I * 4 > kMaxExpertBytes) return no("the tokens or their hidden rows, at four bytes an element, pass 4 GiB less 16 bytes");
       if (!shaped(dn, {E, H, I})) return no("down " + dn->shape.str() + " must be [E, H, I]");
       if (!shaped(gu, {E, 2 * I, H})) return no("gate_up " + gu->shape.str() + " must be [E, 2 I, H]");
       const bool f8 = gu->etype == ODLA_HIP_FLOAT8_E4M3;

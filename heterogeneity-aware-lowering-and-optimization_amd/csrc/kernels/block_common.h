@@ -4,6 +4,7 @@
 #define ODLA_HIP_BLOCK_COMMON_H_
 
 #include "device_utils.h"
+#include "row_range.h"
 
 #include <type_traits>
 
@@ -45,14 +46,13 @@ __device__ __forceinline__ uintx4 load_row16(const unsigned char* row, const int
   }
 }
 
-// 16 bytes at base + at + uniform (any alignment); zeros where that is not within `size` bytes from `base` on.
-constexpr unsigned kOutside = 0xfffffff0u;
-__device__ __forceinline__ uintx4 load_within(const unsigned char* base, const unsigned size, const unsigned at, const unsigned uniform) {
+// 16 bytes at range.base + at (any alignment); zeros where that is not within the range.
+__device__ __forceinline__ uintx4 load_within(const RowRange range, const unsigned at) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(base), 0, size, 0x00020000);
-  return __builtin_bit_cast(uintx4, __builtin_amdgcn_raw_buffer_load_b128(r, at, uniform, 0));
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(range.base), 0, range.size, 0x00020000);
+  return __builtin_bit_cast(uintx4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
 #else
-  (void)base; (void)size; (void)at; (void)uniform;
+  (void)range; (void)at;
   return uintx4{0u, 0u, 0u, 0u};
 #endif
 }

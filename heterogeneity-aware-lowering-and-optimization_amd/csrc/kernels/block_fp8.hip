@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(512) block_gemm_split_kernel(const BlockGemmPa
   auto fetch = [&](const int kb, const int q) __attribute__((always_inline)) {
     if (kb >= KB) return;
     const int at = kb * kScaleBlock + chunk * 16;
-    const unsigned lane_at = ALIGNED ? lane_row + at : at < p.K ? lane_row + min(at, p.K - 16) : kOutside;
+    const unsigned lane_at = ALIGNED ? lane_row + at : lane_offset(lane_row, at, p.K, false);
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
       const bool is_b = i < 2 * NT;
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(512) block_gemm_split_kernel(const BlockGemmPa
         in[q][i] = uintx4{0u, 0u, 0u, 0u};
         if (first + l8 < rows && at < p.K) in[q][i] = *reinterpret_cast<const uintx4*>(tile + (int64_t)first * p.K + lane_at);
       } else {            // (a load with a range: fewer registers)
-        in[q][i] = load_within(tile, in_vectors ? rows * p.K : 0, lane_at, first * p.K);
+        in[q][i] = load_within(row_range(tile, in_vectors ? rows : 0, first, 8, p.K), lane_at);
       }
     }
 #pragma unroll
@@ -340,22 +340,24 @@ struct Big {
   static constexpr int LDS = 2 * STAGE + 2 * 64 * WAVES * 4;         // and the scales of the rows of A (twice: every thread stores one)
 };
 // A wavefront's request i is of rows 8 WAVES i + 8 wave .. + 7; what lies behind the operand's end, or in the last
-// block behind the row's, is out of the buffer's range and arrives as zeros.
+// block behind the row's, is out of the request's range and arrives as zeros.
 struct BigSource {
-  __amdgpu_buffer_rsrc_t a, b;
-  unsigned at;     // this lane's offset in request 0 of a block
-  unsigned step;   // 8 WAVES rows
-  int left;        // bytes of a row from this lane's chunk on
+  const unsigned char *a, *b;   // the tile's rows
+  int a_rows, b_rows, len;
+  unsigned row;                 // this lane's row of a request, in bytes
+  int chunk;                    // and its bytes of a block
 };
 template <int WAVES>
 __device__ __forceinline__ void big_request(const BigSource& f, const int kb, unsigned char* to) {
   using lds_ptr = __attribute__((address_space(3))) void*;
 #if defined(__HIP_DEVICE_COMPILE__)
-  const unsigned at = kb * kScaleBlock < f.left ? f.at : 0xfffffff0u;
+  const unsigned at = lane_offset(f.row, kb * kScaleBlock + f.chunk, f.len, true);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(f.a, (lds_ptr)(to + i * 1024 * WAVES), 16, at, i * f.step + kb * kScaleBlock, 0, 0);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(f.b, (lds_ptr)(to + Big<WAVES>::SIDE * kScaleBlock + i * 1024 * WAVES), 16, at, i * f.step + kb * kScaleBlock, 0, 0);
+  for (int i = 0; i < 8; ++i) {
+    const RowRange r = i < 4 ? row_range(f.a, f.a_rows, i * 8 * WAVES, 8 * WAVES, f.len) : row_range(f.b, f.b_rows, (i - 4) * 8 * WAVES, 8 * WAVES, f.len);
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(r.base), 0, r.size, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(to + i * 1024 * WAVES), 16, at, 0, 0, 0);
+  }
 #else
   (void)f; (void)kb; (void)to;
 #endif
@@ -429,11 +431,13 @@ __global__ void __launch_bounds__(64 * WAVES, 2) block_gemm_big_kernel(const Blo
   const int KB = (p.K + kScaleBlock - 1) / kScaleBlock;
   const int chunk = ((lane & 7) ^ (((8 * wave + (lane >> 3)) >> 1) & 7)) * 16;
   BigSource from;
-  from.a = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.a) + (int64_t)m0 * p.K, 0, min(SIDE, p.M - m0) * p.K, 0x00020000);
-  from.b = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.b) + (int64_t)n0 * p.K, 0, min(SIDE, p.N - n0) * p.K, 0x00020000);
-  from.at = (8 * wave + (lane >> 3)) * p.K + chunk;
-  from.step = 8u * WAVES * p.K;
-  from.left = p.K - chunk;
+  from.a = p.a + (int64_t)m0 * p.K;
+  from.b = p.b + (int64_t)n0 * p.K;
+  from.a_rows = rows_within(p.M - m0, SIDE);
+  from.b_rows = rows_within(p.N - n0, SIDE);
+  from.len = p.K;
+  from.row = (unsigned)(8 * wave + (lane >> 3)) * p.K;
+  from.chunk = chunk;
   const float* arow_scale = p.a_scale + (int64_t)min(m0 + (tid & (SIDE - 1)), p.M - 1) * KB;
   const int wm = (wave & 1) * 16 * FM, wn = (wave >> 1) * 16 * FN;
   const float* bs = p.b_scale + (int64_t)min((n0 + wn) / kScaleBlock, (p.N - 1) / kScaleBlock) * KB;

@@ -16,7 +16,6 @@
 // other chiplets costs more (a release of the whole L2 in every tile: 52 -> 240 us).
 #include "block_common.h"
 #include "lds_limit.h"
-#include "row_range.h"
 
 namespace ohip {
 namespace {
@@ -257,7 +256,7 @@ __global__ void __launch_bounds__(512, C > 8 || sizeof(X) > 2 * sizeof(W) ? 1 : 
   unsigned x_row[C / 8] = {};
   float weight = 0.f;
   const unsigned char* const xs = (const unsigned char*)(GATED ? p.x : p.hidden);
-  const unsigned xbytes = (unsigned)((GATED ? p.tokens : p.tokens * p.top_k) * xlen);      // (below 2^32: see valid)
+  const unsigned xbytes = (unsigned)((GATED ? p.tokens : p.tokens * p.top_k) * xlen);      // (at most kOutside: see valid)
   const unsigned lane_row = (unsigned)l8 * wlen;
   const bool in_vectors = ALIGNED || wlen >= 16;     // (a row of fewer bytes: one step, byte by byte)
   uintx4 in[P][NR];
@@ -265,14 +264,14 @@ __global__ void __launch_bounds__(512, C > 8 || sizeof(X) > 2 * sizeof(W) ? 1 : 
   auto fetch = [&](const int s, const int q) __attribute__((always_inline)) {
     if (s >= steps) return;
     const int at = s * 128 + chunk * 16;
-    const unsigned lane_at = at < wlen ? lane_row + (ALIGNED ? at : min(at, wlen - 16)) : kOutside;
+    const unsigned lane_at = lane_offset(lane_row, at, wlen, ALIGNED);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) in[q][i] = load_within(w_tile[i >> 1], in_vectors ? w_rows[i >> 1] * wlen : 0, lane_at, 8 * (i & 1) * wlen);
+    for (int i = 0; i < 4; ++i) in[q][i] = load_within(row_range(w_tile[i >> 1], in_vectors ? w_rows[i >> 1] : 0, 8 * (i & 1), 8, wlen), lane_at);
 #pragma unroll
     for (int i = 0; i < XR; ++i) {
-      const unsigned from = s * (128 * PLANES) + i % PLANES * 128 + chunk * 16;
+      const int from = s * (128 * PLANES) + i % PLANES * 128 + chunk * 16;
       if (8 * (i / PLANES) < here)
-        in[q][4 + i] = load_within(xs, ALIGNED || xlen >= 16 ? xbytes : 0, 8 * (i / PLANES) + l8 < here && from < (unsigned)xlen ? x_row[i / PLANES] + (ALIGNED ? from : min(from, (unsigned)xlen - 16)) : kOutside, 0);
+        in[q][4 + i] = load_within({xs, ALIGNED || xlen >= 16 ? xbytes : 0}, 8 * (i / PLANES) + l8 < here ? lane_offset(x_row[i / PLANES], from, (int)xlen, ALIGNED) : kOutside);
     }
   };
   auto scales_from = [&](const int s) __attribute__((always_inline)) {
@@ -475,11 +474,12 @@ __global__ void __launch_bounds__(256) experts_sum_kernel(const ExpertsParams p)
   }
 }
 
+static_assert(kMaxExpertBytes <= kOutside, "what lies behind a row is asked for outside every range");
 bool valid(const ExpertsParams& p) {
   return p.x != nullptr && p.router != nullptr && p.gate_up != nullptr && p.down != nullptr && p.y != nullptr && p.route != nullptr &&
          p.hidden != nullptr && p.parts != nullptr && p.tokens >= 1 && p.tokens <= kMaxExpertTokens && p.E >= 1 && p.E <= kMaxExperts &&
          p.H >= 1 && p.H <= (1 << 24) && p.I >= 1 && p.I <= (1 << 23) && p.top_k >= 1 && p.top_k <= p.E && p.top_k <= kMaxExpertTopK &&
-         (int64_t)p.tokens * p.H * 4 < kMaxExpertBytes && (int64_t)p.tokens * p.top_k * p.I * 4 < kMaxExpertBytes && dtype_is_float(p.dt) && (p.w_dt == p.dt || (p.w_dt == DT_F8 && p.gate_up_scale != nullptr && p.down_scale != nullptr));
+         (int64_t)p.tokens * p.H * 4 <= kMaxExpertBytes && (int64_t)p.tokens * p.top_k * p.I * 4 <= kMaxExpertBytes && dtype_is_float(p.dt) && (p.w_dt == p.dt || (p.w_dt == DT_F8 && p.gate_up_scale != nullptr && p.down_scale != nullptr));
 }
 // rows of x, hidden and weights are whole 16-byte vectors
 bool whole_vectors(const ExpertsParams& p, const int len) { return (int64_t)len * dtype_size(p.dt) % 16 == 0 && (int64_t)len * dtype_size(p.w_dt) % 16 == 0; }

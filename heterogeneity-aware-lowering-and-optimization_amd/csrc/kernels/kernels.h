@@ -725,7 +725,7 @@ hipError_t launch_block_gemm(const BlockGemmParams& p, hipStream_t stream);
 
 // A layer of experts for few tokens, in the order of the three launches.
 constexpr int kMaxExperts = 1024, kMaxExpertTokens = 512, kMaxExpertTopK = 32;
-constexpr int64_t kMaxExpertBytes = int64_t{1} << 32;   // of all tokens in fp32, and of all choices' hidden rows
+constexpr int64_t kMaxExpertBytes = 0xfffffff0;   // of all tokens in fp32, and of all choices' hidden rows: one buffer range
 struct ExpertsParams {
   const void* x = nullptr; const void* router = nullptr;
   const void* gate_up = nullptr; const float* gate_up_scale = nullptr;   // scales: 8-bit weights only

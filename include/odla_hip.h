@@ -862,9 +862,10 @@ odla_value odla_hip_BlockGemm(odla_value A, odla_value A_scale, odla_value B,
  * and down may be ODLA_HIP_FLOAT8_E4M3 instead, with FLOAT32 scales for blocks
  * of 128 x 128: gate_up_scale [E, ceil(2 I / 128), ceil(H / 128)], down_scale
  * [E, ceil(H / 128), ceil(I / 128)]; otherwise both scales are null.  E <= 1024,
- * top_k <= min(E, 32); tokens * H and tokens * top_k * I below 2^30.  Sums, the router's logits and the softmax are kept in 32
- * bits; silu(..) * (..) is rounded to the type of `input`.  A NaN among a token's
- * logits makes its result NaN. */
+ * top_k <= min(E, 32); tokens * H and tokens * top_k * I at most 2^30 - 4.
+ * Sums, the router's logits and the softmax are kept in 32 bits; silu(..) * (..)
+ * is rounded to the type of `input`.  A NaN among a token's logits makes its
+ * result NaN. */
 odla_value odla_hip_MixtureOfExperts(odla_value input, odla_value router,
                                      odla_value gate_up,
                                      odla_value gate_up_scale, odla_value down,
