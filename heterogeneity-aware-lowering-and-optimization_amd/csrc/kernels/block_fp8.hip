@@ -450,7 +450,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) block_gemm_big_kernel(const Blo
   float sb = bs[0];
   big_request<WAVES>(from, 0, smem + wave * 1024);
   for (int kb = 0; kb < KB; ++kb) {
-    __syncthreads();     // this block's operands have landed, and everybody has left the other buffer
+    // This block's operands have landed, and everybody has left the other buffer.  The scales stored below in the turn
+    // before are waited for here: the barrier comes without a wait for LDS (the compiler takes it away in this loop).
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __syncthreads();
     // (both scales of the next block ahead of its operands: a wait for them would wait for those too)
     const float next_scale = arow_scale[min(kb + 1, KB - 1)], next_sb = bs[min(kb + 1, KB - 1)];
     __builtin_amdgcn_sched_barrier(0);

@@ -1,5 +1,6 @@
 """Properties of the compiled gfx950 code of the kernels over 8-bit blocks, experts' weights and logits that their
-correctness relies on: buffer loads whose range check needs nothing but a lane's offset."""
+correctness relies on: buffer loads whose range check needs nothing but a lane's offset, and nothing on its way
+into LDS where wavefronts meet."""
 import os
 import re
 import subprocess
@@ -49,3 +50,71 @@ def test_ranges_are_checked_against_lane_offsets_alone(bodies):
                 seen += 1
                 assert re.search(r", s\[\d+:\d+\], 0 offen\b", l), (name, l)
     assert seen > 500
+
+
+def is_lds_write(op, l):
+    return op.startswith("ds_") and ("write" in op or "add" in op or "append" in op)
+
+
+def is_load_into_lds(op, l):
+    return op.startswith(("buffer_load", "global_load")) and bool(re.search(r"\blds\b|_lds_", l))
+
+
+def unsettled_barrier(body, starts=is_lds_write, counter="lgkmcnt"):
+    """The first s_barrier that some path reaches with what `starts` names not waited for, or None.  (Only a wait for 0
+    settles the last of them.)"""
+    labels = {l[:-1]: i for i, l in enumerate(body) if l.endswith(":")}
+    wait = re.compile(r"s_waitcnt\b.*%s\(0\)" % counter)
+    dirty_at = [None] * len(body)      # whether a write may be under way in front of instruction i: unknown, False or True
+    todo = [(0, False)]
+    while todo:
+        i, dirty = todo.pop()
+        while i < len(body):
+            if dirty_at[i] is not None and (dirty_at[i] or not dirty):
+                break
+            dirty_at[i] = dirty
+            l = body[i]
+            op = l.split()[0]
+            if wait.match(l) or l.strip() == "s_waitcnt 0":
+                dirty = False
+            elif starts(op, l):
+                dirty = True
+            elif op == "s_barrier" and dirty:
+                return i
+            if op == "s_endpgm":
+                break
+            if op.startswith("s_cbranch") or op == "s_branch":
+                target = labels[l.split()[1]]
+                todo.append((target, dirty))
+                if op == "s_branch":
+                    break
+            i += 1
+    return None
+
+
+def test_the_walk_over_barriers():
+    assert unsettled_barrier(["ds_write_b32 v0, v1", "s_barrier", "s_endpgm"]) == 1
+    assert unsettled_barrier(["ds_write_b32 v0, v1", "s_waitcnt vmcnt(0) lgkmcnt(0)", "s_barrier", "s_endpgm"]) is None
+    loop = [".LBB0_1:", "s_waitcnt vmcnt(0)", "s_barrier", "ds_write_b32 v0, v1", "s_cbranch_scc0 .LBB0_1", "s_endpgm"]
+    assert unsettled_barrier(loop) == 2                      # (the write of the turn before)
+    assert unsettled_barrier(loop[:4] + ["s_waitcnt lgkmcnt(0)"] + loop[4:]) is None
+    direct = ["buffer_load_dwordx4 v1, s[4:7], 0 offen lds", "s_waitcnt lgkmcnt(0)", "s_barrier", "s_endpgm"]
+    assert unsettled_barrier(direct, is_load_into_lds, "vmcnt") == 2 and unsettled_barrier(direct) is None
+
+
+def test_lds_writes_are_settled_in_front_of_every_barrier(bodies):
+    barriers = 0
+    for name, body in bodies.items():
+        barriers += sum(l == "s_barrier" for l in body)
+        at = unsettled_barrier(body)
+        assert at is None, (name, body[max(0, at - 8):at + 1])
+    assert barriers > 300
+
+
+def test_loads_into_lds_are_settled_in_front_of_every_barrier(bodies):
+    loads = 0
+    for name, body in bodies.items():
+        loads += sum(is_load_into_lds(l.split()[0], l) for l in body)
+        at = unsettled_barrier(body, is_load_into_lds, "vmcnt")
+        assert at is None, (name, body[max(0, at - 8):at + 1])
+    assert loads >= 4 * 8
