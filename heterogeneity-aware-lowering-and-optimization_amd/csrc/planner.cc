@@ -298,6 +298,48 @@ class Planner {
     if (d == DT_F32) return cdt_;
     return d;
   }
+  // FLOAT32 values that stay fp32 where the mode stores 16 bits: scales, sampling parameters, and what moves their
+  // elements on the way from where they are bound, recorded or computed.  (Their fp32 tensor is the value's main one
+  // and fills no slot: readers of any other kind convert it.)
+  bool kept_fp32(const _odla_value* v) const { return v != nullptr && kept_fp32_[v->index] != 0; }
+  static bool reads_fp32(const Node& n, size_t operand) {
+    return (n.op == OP_BLOCKGEMM && (operand == 1 || operand == 3)) || (n.op == OP_EXPERTS && (operand == 3 || operand == 5)) ||
+           (n.op == OP_SAMPLE && operand >= 1 && operand != 2);
+  }
+  // How many of the node's operands, from the first on, it moves the elements of and does nothing else with.
+  static size_t moved_operands(const Node& n) {
+    switch (n.op) {
+      case OP_RESHAPE: case OP_TRANSPOSE: case OP_SLICE: case OP_GATHER: case OP_COPYND: return 1;
+      case OP_CONCAT: return n.in.size();
+      case OP_AXISOP: return n.i[0] == AX_GATHER_ELEMENTS || n.i[0] == AX_COMPRESS ? 1 : 0;
+      default: return 0;
+    }
+  }
+  void find_kept_fp32() {
+    kept_fp32_.assign(comp_->values.size(), 0);
+    if (cdt_ == DT_F32) return;      // (everything is)
+    auto keep = [&](const _odla_value* v) {
+      if (v != nullptr && dtype_from_odla(v->etype) == DT_F32) kept_fp32_[v->index] = 1;
+    };
+    for (const Node& n : comp_->nodes) {
+      if (n.op == OP_BLOCKQUANT) keep(n.out2);
+      for (size_t k = 0; k < moved_operands(n); ++k)
+        if (kept_fp32(n.in[k])) keep(n.out);
+    }
+    for (size_t j = comp_->nodes.size(); j-- > 0;) {
+      const Node& n = comp_->nodes[j];
+      for (size_t k = 0; k < n.in.size(); ++k)
+        if (reads_fp32(n, k) || (k < moved_operands(n) && kept_fp32(n.out))) keep(n.in[k]);
+    }
+  }
+  void set_kept(const _odla_value* v, int t) {
+    if (kept_fp32(v) && T(t).dt == DT_F32) vs_[v->index].main = t;
+    else set_main(v, t);
+  }
+  // The row-major tensor that a moving operator with the result `out` takes its operand from.
+  int get_to_move(const _odla_value* v, const _odla_value* out) {
+    return kept_fp32(out) ? get_fp32(v) : get_moved(v, L_ROWMAJOR);
+  }
   // Type of the tensor a Conv / Gemm reads for a FLOAT32 operand.
   DType mm_dtype(const _odla_value* v) const {
     const DType d = dtype_from_odla(v->etype);
@@ -587,7 +629,7 @@ class Planner {
     if (calib_ || comp_->opts.int8 || v->is_output || v->shape.rank != 4 || consumers_[v->index].size() != 1) return -1;
     const int ci = consumers_[v->index][0];
     const Node& c = comp_->nodes[ci];
-    if (c.op != OP_CONCAT || c.absorbed || c.i[0] != 1 || c.out->shape.rank != 4 || storage_dtype(c.out) != dt || storage_dtype(v) != dt) return -1;
+    if (c.op != OP_CONCAT || c.absorbed || c.i[0] != 1 || c.out->shape.rank != 4 || storage_dtype(c.out) != dt || storage_dtype(v) != dt || kept_fp32(c.out)) return -1;
     int64_t off = 0;
     for (const _odla_value* part : c.in) {
       if (part == v) break;
@@ -610,7 +652,7 @@ class Planner {
     if (calib_ || comp_->opts.int8 || v->is_output || v->shape.rank > 3 || consumers_[v->index].size() != 1) return -1;
     const int ci = consumers_[v->index][0];
     const Node& c = comp_->nodes[ci];
-    if (c.op != OP_CONCAT || c.absorbed || c.out->shape.rank != v->shape.rank || storage_dtype(c.out) != dt) return -1;
+    if (c.op != OP_CONCAT || c.absorbed || c.out->shape.rank != v->shape.rank || storage_dtype(c.out) != dt || kept_fp32(c.out)) return -1;
     for (const _odla_value* part : c.in) if (storage_dtype(part) != dt) return -1;
     int64_t acc = 1;
     for (int i = v->shape.rank - 1; i >= 0; --i) { st[i] = acc; acc *= c.out->shape.d[i]; }
@@ -677,7 +719,7 @@ class Planner {
   struct Strided { int tensor = -1; std::vector<std::pair<int64_t, int64_t>> walk; };
   std::unordered_map<int, Strided> strided_;   // by value index
   bool read_by_groups(const _odla_value* v, int depth = 0) const {
-    if (calib_ || comp_->opts.int8 || v->is_output || depth > 4 || !dtype_is_float(storage_dtype(v)) || consumers_[v->index].empty()) return false;
+    if (kept_fp32(v) || calib_ || comp_->opts.int8 || v->is_output || depth > 4 || !dtype_is_float(storage_dtype(v)) || consumers_[v->index].empty()) return false;
     for (int ci : consumers_[v->index]) {
       const Node& c = comp_->nodes[ci];
       if (c.op == OP_RESHAPE && !c.absorbed) {
@@ -766,6 +808,7 @@ class Planner {
   void lower_blockgemm(int ni);
   void lower_experts(int ni);
   void lower_sample(int ni);
+  std::vector<char> kept_fp32_;   // by value index, see kept_fp32
   std::unordered_map<const _odla_value*, int> fp32_consts_;   // constants that get_fp32 keeps beside the stored form
   void lower_lrn(int ni);
   void lower_rownorm(int ni);
@@ -924,6 +967,7 @@ void Planner::run() {
   for (size_t ni = 0; ni < comp_->nodes.size(); ++ni)
     for (_odla_value* v : comp_->nodes[ni].in)
       if (v != nullptr) consumers_[v->index].push_back((int)ni);
+  find_kept_fp32();
 
   // Arguments: one staging tensor each (declared type, row-major), alive from
   // the start of the execution because the H2D copy precedes every step.
@@ -1000,8 +1044,8 @@ void Planner::run() {
         LayoutParams p = lp; p.src = a(e); p.dst = b(e);
         return launch_nhwc_to_nchw(p, st);
       }, kWrites16);
-    } else if (ov->producer >= 0 && comp_->nodes[ov->producer].op == OP_BLOCKQUANT) {
-      t = os.main;   // (scales are fp32 whatever the mode stores)
+    } else if (ov->producer >= 0 && kept_fp32(ov)) {
+      t = get_fp32(ov);   // (scales are fp32 whatever the mode stores)
     } else {
       t = get(ov, L_ROWMAJOR, FORM_FLOAT);
     }
@@ -2914,7 +2958,7 @@ bool Planner::fuse_candidate(int ni) const {
 bool Planner::fuse_slice_seed(int ni) const {
   const Node& n = comp_->nodes[ni];
   if (n.op != OP_SLICE || n.absorbed || n.out->is_output || consumers_[n.out->index].empty()) return false;
-  if (n.out->shape.rank > 3 || !dtype_is_float(storage_dtype(n.out))) return false;
+  if (n.out->shape.rank > 3 || !dtype_is_float(storage_dtype(n.out)) || kept_fp32(n.out)) return false;
   return fuse_candidate(consumers_[n.out->index][0]);
 }
 
@@ -2933,7 +2977,7 @@ bool Planner::lower_fused_group(int seed, int from) {
   for (int j = from; j < scan_end; ++j) {
     const Node& n = comp_->nodes[j];
     if (n.absorbed) continue;
-    if (n.op == OP_SLICE && n.out->shape.rank <= 3 && !n.out->is_output && storage_dtype(n.out) == dt &&
+    if (n.op == OP_SLICE && n.out->shape.rank <= 3 && !n.out->is_output && storage_dtype(n.out) == dt && !kept_fp32(n.out) &&
         dtype_is_float(dt) && available(n.in[0]) && !consumers_[n.out->index].empty()) {
       bool ok = true;
       for (int c : consumers_[n.out->index]) ok = ok && (comp_->nodes[c].op == OP_UNARY || comp_->nodes[c].op == OP_BINARY);
@@ -3150,7 +3194,7 @@ bool Planner::lower_fused_group(int seed, int from) {
       const Node& cn = comp_->nodes[c];
       if (in_group.count(cn.out) && in_group[cn.out] == c) continue;
       const bool full = v->shape.rank == R && v->shape == S;
-      if (cn.op == OP_CONCAT && !cn.absorbed && full && storage_dtype(cn.out) == dt && cn.out->shape.rank == R) {
+      if (cn.op == OP_CONCAT && !cn.absorbed && full && storage_dtype(cn.out) == dt && !kept_fp32(cn.out) && cn.out->shape.rank == R) {
         bool all = true;
         for (const _odla_value* ci : cn.in) all = all && in_group.count(ci) && ci->shape.rank == R;
         if (all) {
@@ -3171,7 +3215,7 @@ bool Planner::lower_fused_group(int seed, int from) {
       // elements a row apart; beyond a few million elements the tiled copy
       // behind a plain store is several times faster than that - unless the loads
       // come from in front of a Transpose that did the opposite.
-      if (cn.op == OP_TRANSPOSE && !cn.absorbed && full && storage_dtype(cn.out) == dt && (int)cn.iv.size() == R &&
+      if (cn.op == OP_TRANSPOSE && !cn.absorbed && full && storage_dtype(cn.out) == dt && !kept_fp32(cn.out) && (int)cn.iv.size() == R &&
           (cn.iv[R - 1] == R - 1 || S.numel() <= kTransposeSinkMax || (any_strided && all_along && cn.iv[R - 1] == unit_dim))) {
         if (std::find(sink_nodes.begin(), sink_nodes.end(), c) == sink_nodes.end()) {
           sink_nodes.push_back(c);
@@ -3537,7 +3581,7 @@ bool Planner::plane_candidate(const Node& n) const {
       return n.i[0] != ODLA_LINEAR && os.rank == 4 && os.d[0] == xs.d[0] && os.d[1] == xs.d[1] && os.numel() > 0 &&
              os.d[2] * os.d[3] < (1 << 20) && os.d[2] * xs.d[2] < (1 << 20) && (os.d[3] + 4) * xs.d[3] < (1 << 20);
     case OP_REDUCE: return (ReduceKind)n.i[0] == RED_MEAN && n.iv.size() == 2 && n.iv[0] == 2 && n.iv[1] == 3;
-    case OP_CONCAT: return n.i[0] == 1 && os.rank == 4;
+    case OP_CONCAT: return n.i[0] == 1 && os.rank == 4 && !kept_fp32(n.out);
     default: return false;
   }
 }
@@ -4296,7 +4340,7 @@ void Planner::lower_concat(int ni) {
   const Shape& os = n.out->shape;
   const int axis = (int)n.i[0];
   // channel concat of channels-last tensors stays channels-last
-  bool nhwc = os.rank == 4 && axis == 1;
+  bool nhwc = os.rank == 4 && axis == 1 && !kept_fp32(n.out);
   if (nhwc) {
     bool any = false;
     for (_odla_value* v : n.in) {
@@ -4308,7 +4352,7 @@ void Planner::lower_concat(int ni) {
   const Layout lay = nhwc ? L_NHWC : L_ROWMAJOR;
   std::vector<int> tin;
   const auto placed = concat_dst_.find(ni);   // (some parts are stored in the result already)
-  for (_odla_value* v : n.in) tin.push_back(placed_.count(v->index) ? placed->second : get(v, lay, FORM_FLOAT));
+  for (_odla_value* v : n.in) tin.push_back(placed_.count(v->index) ? placed->second : kept_fp32(n.out) ? get_fp32(v) : get(v, lay, FORM_FLOAT));
   const DType dt = T(tin[0]).dt;
   const int es = dtype_size(dt);
   const int ty = placed != concat_dst_.end() ? placed->second : new_tensor(dt, lay, os, nhwc ? (int)os.d[1] : 0, SP_ARENA);
@@ -4352,7 +4396,7 @@ void Planner::lower_concat(int ni) {
     }
     strided_copy_step("concat:" + n.out->name, tin[k], ty, cp);
   }
-  set_main(n.out, ty);
+  set_kept(n.out, ty);
 }
 
 // -------------------------------------------------------------- Gather ----
@@ -4384,7 +4428,7 @@ void Planner::lower_gather(int ni) {
   const _odla_value* x = n.in[0];
   const _odla_value* idx = n.in[1];
   const int axis = (int)n.i[0];
-  const int tx = get(x, L_ROWMAJOR, FORM_FLOAT);
+  const int tx = kept_fp32(n.out) ? get_fp32(x) : get(x, L_ROWMAJOR, FORM_FLOAT);
   const int ti = get(idx, L_ROWMAJOR, FORM_FLOAT);
   const Shape& xs = x->shape;
   int64_t outer = 1, inner = 1;
@@ -4412,7 +4456,7 @@ void Planner::lower_gather(int ni) {
   emit("gather:" + n.out->name, {tx, ti}, {ty}, [=](const ExecEnv& e, hipStream_t st) {
     return launch_gather_rows(a(e), ri(e), idt, b(e), outer, n_src, n_idx, row_bytes, st);
   }, kReads16 | kWrites16);
-  set_main(n.out, ty);
+  set_kept(n.out, ty);
 }
 
 // ------------------------------- GatherElements, CumSum, Hardmax, Compress ----
@@ -4422,7 +4466,7 @@ void Planner::lower_axisop(int ni) {
   const Shape& xs = x->shape;
   const AxisOp op = (AxisOp)n.i[0];
   const int axis = (int)n.i[1];
-  const int tx = get(x, L_ROWMAJOR, FORM_FLOAT);
+  const int tx = moved_operands(n) > 0 && kept_fp32(n.out) ? get_fp32(x) : get(x, L_ROWMAJOR, FORM_FLOAT);
   const DType dt = T(tx).dt;
   int64_t outer = 1, inner = 1;
   for (int i = 0; i < axis; ++i) outer *= xs.d[i];
@@ -4485,7 +4529,7 @@ void Planner::lower_axisop(int ni) {
     default:
       fail(ODLA_INTERNAL_LOGIC_ERR, "unknown axis operator %d", (int)op);
   }
-  set_main(n.out, ty);
+  set_kept(n.out, ty);
 }
 
 // ------------------------------------------------------------- Reshape ----
@@ -4506,9 +4550,9 @@ void Planner::lower_reshape(int ni) {
   if (s.main >= 0 && T(s.main).quant && s.slot[L_ROWMAJOR][FORM_QUANT] >= 0 && qentry(n.out) != nullptr)
     tx = s.slot[L_ROWMAJOR][FORM_QUANT];
   else
-    tx = get_moved(x, L_ROWMAJOR);
+    tx = get_to_move(x, n.out);
   const int ty = alias_tensor(tx, n.out->shape);
-  set_main(n.out, ty);
+  set_kept(n.out, ty);
 }
 
 // -------------------------------------------------------------- Resize ----
@@ -4544,7 +4588,7 @@ void Planner::lower_resize(int ni) {
 void Planner::lower_slice(int ni) {
   Node& n = comp_->nodes[ni];
   const _odla_value* x = n.in[0];
-  const int tx = get(x, L_ROWMAJOR, FORM_FLOAT);
+  const int tx = kept_fp32(n.out) ? get_fp32(x) : get(x, L_ROWMAJOR, FORM_FLOAT);
   const Shape& xs = x->shape;
   const Shape& os = n.out->shape;
   const int r = xs.rank;
@@ -4564,14 +4608,14 @@ void Planner::lower_slice(int ni) {
     sy *= os.d[i];
   }
   strided_copy_step("slice:" + n.out->name, tx, ty, cp);
-  set_main(n.out, ty);
+  set_kept(n.out, ty);
 }
 
 // ------------------------------------- Pad / Tile / broadcast / stuffing ----
 void Planner::lower_copynd(int ni) {
   Node& n = comp_->nodes[ni];
   const _odla_value* x = n.in[0];
-  const int tx = get(x, L_ROWMAJOR, FORM_FLOAT);
+  const int tx = kept_fp32(n.out) ? get_fp32(x) : get(x, L_ROWMAJOR, FORM_FLOAT);
   const DType dt = T(tx).dt;
   const int ty = new_tensor(dt, L_ROWMAJOR, n.out->shape, 0, SP_ARENA);
   const int r = (int)n.iv[0];
@@ -4593,7 +4637,7 @@ void Planner::lower_copynd(int ni) {
     emit("fill:" + n.out->name, {}, {ty}, [=](const ExecEnv& e, hipStream_t st) { return launch_fill_bytes(b(e), bytes, 0u, st); });
   }
   strided_copy_step("copy:" + n.out->name, tx, ty, cp);
-  set_main(n.out, ty);
+  set_kept(n.out, ty);
 }
 
 // ---------------------------------------------------------------- TopK ----
@@ -4631,9 +4675,7 @@ void Planner::lower_blockquant(int ni) {
     return launch_block_quantize(a(e), dt, q(e), (float*)s(e), rows, len, st);
   }, kReads16 | kWrites16);
   set_main(n.out, tq);
-  // (where the mode stores FLOAT32 values in 16 bits, other readers than get_fp32 convert)
-  if (storage_dtype(n.out2) == DT_F32) set_main(n.out2, ts);
-  else vs_[n.out2->index].main = ts;
+  set_kept(n.out2, ts);
 }
 
 void Planner::lower_blockgemm(int ni) {
@@ -4820,11 +4862,11 @@ void Planner::lower_transpose(int ni) {
   // N,C,H,W -> N,H,W,C of a value that already lives channels-last is free
   const VState& s = vs_[x->index];
   if (r == 4 && n.iv[0] == 0 && n.iv[1] == 2 && n.iv[2] == 3 && n.iv[3] == 1 && s.main >= 0 &&
-      T(s.main).layout == L_NHWC && !T(s.main).quant && T(s.main).cs == xs.d[1]) {
+      T(s.main).layout == L_NHWC && !T(s.main).quant && T(s.main).cs == xs.d[1] && !kept_fp32(n.out)) {
     set_main(n.out, alias_tensor(s.main, os));
     return;
   }
-  const int tx = get_moved(x, L_ROWMAJOR);
+  const int tx = get_to_move(x, n.out);
   const DType dt = T(tx).dt;
   int64_t xstr[ODLA_MAX_DIMENSION];
   {
@@ -4856,7 +4898,7 @@ void Planner::lower_transpose(int ni) {
     sy *= os.d[i];
   }
   strided_copy_step("transpose:" + n.out->name, tx, ty, cp);
-  set_main(n.out, ty);
+  set_kept(n.out, ty);
 }
 
 // ------------------------------------------------- Quantize/Dequantize ----

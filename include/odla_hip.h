@@ -834,7 +834,10 @@ odla_value odla_DeConv(odla_value input, odla_memory_layout input_layout,
  *   scale = max(max |x| / 448, 2^-126),   q = x / scale to nearest, ties to even.
  * A NaN stays NaN and is not counted in the maximum; a block with an infinity
  * has an infinite scale, so that all its values stand for NaN.  The scales are
- * kept as fp32 in every precision mode. */
+ * kept as fp32 in every precision mode, also behind operators that only move
+ * elements (odla_Reshape, odla_Squeeze, odla_Transpose, odla_Slice, odla_Concat,
+ * odla_Gather, odla_Tile, ...); what others compute from them is stored as the
+ * mode says. */
 odla_values odla_hip_BlockQuantize(odla_value input,
                                    const odla_value_ids value_ids);
 /* Product of 8-bit floating-point matrices with a scale for each block of 128:
@@ -886,8 +889,9 @@ odla_value odla_hip_MixtureOfExperts(odla_value input, odla_value router,
  * A temperature that is not above 0 gives the first of the ranking.  NaN logits
  * count as -inf; a row with nothing above -inf gives -1.  The weights are
  * exponentials in 64 bits, held as whole multiples of 2^-44 of the largest, so
- * that sums do not depend on an order; the parameters are read in their own
- * type in every precision mode. */
+ * that sums do not depend on an order; the parameters keep
+ * their own type in every precision mode, as the scales of
+ * odla_hip_BlockQuantize do. */
 odla_value odla_hip_Sample(odla_value logits, odla_value temperature,
                            odla_value top_k, odla_value top_p, odla_value min_p,
                            odla_value uniform, const odla_value_id value_id);
