@@ -177,19 +177,24 @@ std::unique_ptr<_odla_computation> clone_for_batch(const _odla_computation& c, i
         // (every image owns max_num_outputs rows of the result, and the image numbers written there
         //  start at the executing context's image_base: a half-batch copy gives the whole batch's rows)
         break;
+      // (No halves where a token hangs on them: the last bits of a product's and of the experts' rows
+      //  depend on how many rows there are, and a context that tries halves would change them between two calls.)
       case OP_BLOCKQUANT:
         if (x->shape.rank < 2) rs.reject(n, "runs along the batch");
         break;
       case OP_BLOCKGEMM:
+        if (rows_apart) rs.reject(n, "gives rows whose last bits depend on how many there are");
         if (!rs.carry(n.in[0]) || !rs.carry(n.in[1]) || x->shape.rank < 2) rs.reject(n, "has rows or their scales that do not depend on the batch");
         if (rs.carry(n.in[2]) || rs.carry(n.in[3])) rs.reject(n, "has a right operand that depends on the batch");
         break;
       case OP_EXPERTS:
+        if (rows_apart) rs.reject(n, "gives rows whose last bits depend on how many there are");
         if (!rs.carry(x) || x->shape.rank < 2) rs.reject(n, "has tokens that do not depend on the batch");
         for (size_t k = 1; k < n.in.size(); ++k)
           if (rs.carry(n.in[k])) rs.reject(n, "has weights that depend on the batch");
         break;
       case OP_SAMPLE:
+        if (rows_apart) rs.reject(n, "draws tokens, which are to be the same in every execution");
         if (!rs.carry(x) || x->shape.rank < 2) rs.reject(n, "has logits that do not depend on the batch");
         // (a parameter follows the batch with its rows, or is a single one for all of them)
         for (size_t k = 1; k < n.in.size(); ++k) {
