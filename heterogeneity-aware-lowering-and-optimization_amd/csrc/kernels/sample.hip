@@ -79,7 +79,8 @@ struct Row {
 // from f^4 on are below 2^-50.  1024 y is rounded by adding 1.5 * 2^52, which leaves it in the sum's low
 // word; 2^n goes straight into the exponent of the power from the table.  The product and its rounding to a whole
 // number are one fused operation: the sum with 2^52 has it in its low bits, nearest even.  Nineteen instructions
-// and no branch; NaN (infinities among the operands) weighs nothing.
+// and no branch.  NaN weighs what `floor` does: nothing, but all of it in a row with infinite logits, where `floor` is 0
+// and everything weighs the same: there the cut leaves out what is not infinite.
 struct Factors { double series, power; };
 __device__ __forceinline__ Factors factors(const Row& r, const float l) {
   const double y = __builtin_fmax(((double)l - r.most_d) * r.per, r.floor);
@@ -105,6 +106,13 @@ __device__ __forceinline__ u64 whole_weight(const Row& r, const float l) {
 __device__ __forceinline__ int bin_of(const Row& r, const float l) {
   const float x = (r.most - l) * r.per_bin;       // NaN (infinite logits or temperatures) counts as far away
   return l == r.most ? 0 : (int)fminf(x, (float)kBins);
+}
+
+// What bin_of gives may lie behind the last bin and still have a weight: max - l beyond fp32, or so low a
+// temperature that log2(e) / T is.  Nothing is added then; a cut that the bins do not hold is found by descent.
+template <typename N>
+__device__ __forceinline__ void add_to_bin(N* bins, const int b, const N n) {
+  if (b < kBins) atomicAdd(&bins[b], n);
 }
 
 // Sums over the lanes up to one's own, by DPP (no trip through LDS): the shifts inside rows of 16,
@@ -371,7 +379,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         own_bin[j] = own[j] > -__builtin_inff() ? bin_of(r, own[j]) : kBins;
-        if (own_bin[j] < kBins) atomicAdd(&s.count[own_bin[j]], 1u);
+        add_to_bin(s.count, own_bin[j], 1u);
       }
       __syncthreads();
       bounded = find(&s, s.count, (u64)top_k) >= (u64)top_k;
@@ -392,8 +400,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
         if (n < kList) {
           s.logit[n] = l;
           s.index[n] = i;
-          const int b = bin_of(r, l);
-          if (b < kBins) atomicAdd(&s.count[b], 1u);
+          add_to_bin(s.count, bin_of(r, l), 1u);
         }
       });
       __syncthreads();
@@ -453,7 +460,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < MINE; ++j)
-        if (kept_w[j] != 0) { total += kept_w[j]; atomicAdd(&s.sum[kept_bin[j]], kept_w[j]); }
+        if (kept_w[j] != 0) {
+          total += kept_w[j];
+          add_to_bin(s.sum, kept_bin[j], kept_w[j]);
+        }
     } else {
       // Behind 2^-e of the largest weight, e = log2(V / ((1 - p) S)) + 1, all elements together weigh at most half
       // of (1 - p) S: the cut is in front of it.  For S, the sum of all weights, serves that of the threads' largest.
@@ -478,7 +488,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
           const int b = bin_of(r, x.get(e));
-          if (b < kBins && w[e] != 0) atomicAdd(&s.sum[b], w[e]);
+          if (w[e] != 0) add_to_bin(s.sum, b, w[e]);
         }
       });
     }
