@@ -10,8 +10,9 @@ constexpr float kLeastScale = 1.17549435e-38f;   // 2^-126: x / scale stays fini
 
 // ------------------------------------------------------------- quantisation --
 // scale = max(max |x| / 448, 2^-126), q = e4m3(x / scale).  Bound by memory: es + 1 bytes per value.
-// Sixteen lanes hold a block, eight values each.  8192 x 7168 bf16: 33 us, 5.3 TB/s read and written (with a
-// division per value 40); 1 x 4096: 2.2 us, a launch.
+// Sixteen lanes hold a block, eight values each.  8192 x 7168 bf16: 32 us, 5.5 TB/s read and written (with a
+// division per value 40); 1 x 4096: 2.1 us, a launch.  Rows whose length is no multiple of 8 go element by element:
+// 8192 x 7001 50 us.
 template <typename T, bool VECTOR>
 __global__ void __launch_bounds__(256) block_quantize_kernel(const T* x, uint8_t* q, float* scale, const int64_t rows, const int len, const int blocks) {
   const int l16 = threadIdx.x & 15;
@@ -98,7 +99,7 @@ hipError_t quantize_as(const void* x, void* q, float* scale, int64_t rows, int64
 // a compute unit gets 36 KB/us out of L2 instead of 120 (measured; from memory 26 either way).
 // A block's sum is scaled on its way into the accumulator: the scale of row m belongs to a lane (column of
 // the matrix result), that of B to the whole tile.  EXACT: through bf16 (see mma_exact).
-// K = 4096: 1 row x 4096 columns 6.1 us, 64 rows 11.6, 128 rows 11.5, 256 rows 14.6; 48 x 7168 x 2048 6.7 us;
+// K = 4096: 1 row x 4096 columns 5.3 us, 64 rows 11.0, 128 rows 11.3, 256 rows 14.4; 48 x 7168 x 2048 6.9 us;
 // 100 x 1000 x 8000 13.5; 509 x 2500 x 1400 (rows that are no whole vectors) 11.4.  A call's first bytes from memory and
 // the meeting of the sums are 4 to 5 us of that.
 template <typename TOut, int NT, int MT, int P, bool EXACT, bool ALIGNED>
@@ -235,6 +236,8 @@ __global__ void __launch_bounds__(512) block_gemm_split_kernel(const BlockGemmPa
 
 // Many tiles that the kernel below does not take: a workgroup of four wavefronts owns BN columns n x BM rows m;
 // both operands pass through LDS, 128 terms at a time, the next 128 on their way in registers.
+// 8192 x 8192 x 4096 with fp32 results (bf16 matrix instructions) 614 us, x 4090 with bf16 results 573; 2048 x 4096 x
+// 4096 82 and 83.
 template <typename TOut, int BM, int BN, bool ALIGNED>
 __global__ void __launch_bounds__(256) block_gemm_tile_kernel(const BlockGemmParams p) {
   constexpr bool EXACT = sizeof(TOut) == 4;
@@ -490,7 +493,7 @@ hipError_t gemm_split(const BlockGemmParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 // From here on 128 x 128 results a workgroup, loaded straight into LDS, beat 64 x 64 with the terms shared out.
-// N = K = 4096: 512 rows (128 tiles) 26.6 us against 24.4, 1024 rows 29.3 against 47 (four times 256 rows' 14.5).
+// N = K = 4096: 512 rows (128 tiles) 26.6 us against 24.4, 1024 rows 33 against 47 (four times 256 rows' 14.4).
 constexpr int kMiddleTiles = 144;
 template <typename TOut, int WAVES>
 hipError_t gemm_big(const BlockGemmParams& p, hipStream_t stream) {
@@ -509,7 +512,7 @@ hipError_t gemm_as(const BlockGemmParams& p, hipStream_t stream) {
   if (p.M <= 32) return p.N > 32 * 192 ? gemm_split<TOut, 2, 2, 2, ALIGNED>(p, stream) : gemm_split<TOut, 1, 2, 2, ALIGNED>(p, stream);
   if (p.M <= 64) return p.N > 32 * 192 ? gemm_split<TOut, 2, 4, 1, ALIGNED>(p, stream) : gemm_split<TOut, 1, 4, 2, ALIGNED>(p, stream);
   if constexpr (ALIGNED && sizeof(TOut) == 2) {
-    // 256 x 256 for three quarters of the compute units at least: 3000 x 4096 x 4096 72 us; 2048 rows in 128 x 128 47 us.
+    // 256 x 256 for three quarters of the compute units at least: 3000 x 4096 x 4096 73 us; 2048 rows in 128 x 128 50 us.
     if (p.K <= 1 << 22) {   // (256 rows of an operand within 2^30 bytes of buffer range)
       if ((int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256) >= 192) return gemm_big<TOut, 8>(p, stream);
       if ((int64_t)((p.M + 127) / 128) * ((p.N + 127) / 128) >= kMiddleTiles) return gemm_big<TOut, 4>(p, stream);

@@ -7,9 +7,9 @@
 // Few tokens: bound by the weights of the experts that some token chose, which are read once: their rows are the
 // rows of a matrix product, the tokens that chose the expert its columns.  Five launches (four where the first
 // product makes the choice itself): logits, choice, first product, second product with its parts, sum.
-//   64 experts of 2048 x 1024, 8 chosen, bf16: 1 token 5 + 17 (100 MB in all) + 9 + 4 us; 32 tokens 7 + 4 + 98 +
-//   51 + 4 us, 5.4 TB/s in the products.  7 tokens, 128 experts of 2624 x 704, 8-bit weights 7 + 30 + 16 + 4 us,
-//   4.6 TB/s; of 2600 x 712, rows that are no whole vectors, 35 + 18.
+//   64 experts of 2048 x 1024, 8 chosen, bf16: 1 token 5 + 17 (100 MB in all) + 8 + 4 us; 32 tokens 7 + 4 + 102 +
+//   53 + 4 us, 5.2 TB/s in the products.  7 tokens, 128 experts of 2624 x 704, 8-bit weights 7 + 30 + 15 + 4 us,
+//   4.6 TB/s; of 2600 x 712, rows that are no whole vectors, 33 + 17.
 // Logits, softmax, sums and parts are fp32.  hidden is rounded to the input's type: it is an operand of the second
 // product's matrix instructions, which take that type.
 // The last of a token's parts adding them up instead of a launch was slower: making parts visible to the

@@ -723,7 +723,7 @@ struct BlockGemmParams {
 };
 hipError_t launch_block_gemm(const BlockGemmParams& p, hipStream_t stream);
 
-// A layer of experts for few tokens, in the order of the three launches.
+// A layer of experts for few tokens, in three steps.
 constexpr int kMaxExperts = 1024, kMaxExpertTokens = 512, kMaxExpertTopK = 32;
 constexpr int64_t kMaxExpertBytes = 0xfffffff0;   // of all tokens in fp32, and of all choices' hidden rows: one buffer range
 struct ExpertsParams {
