@@ -68,3 +68,54 @@ def test_moved_parameters_reach_the_sampling(odla, mode):
     got = run_hip(build, {"p": p, "l": logits}, **MODES[mode])["t"]
     want = [R.sample_row(logits[0], 1.0, 0, p[2, i], 0.0, p[0, i]) for i in range(n)]
     assert np.array_equal(got, want) and len(set(want)) > 1
+
+
+MOVED_PARAMETERS = {
+    "tile": lambda b, a, n: b.tile(b.slice(a, (n // 2,), (n // 2 + 1,)), (n,)),
+    "broadcast": lambda b, a, n: b.broadcast_to(b.slice(a, (1,), (2,)), (n,)),
+    "pad": lambda b, a, n: b.pad(b.slice(a, (0,), (n - 3,)), (1,), (2,)),
+    "gather_elements": lambda b, a, n: b.gather_elements(a, b.const(None, np.arange(n, dtype=np.int32)[::-1].copy()), 0),
+    "compress": lambda b, a, n: b.slice(b.compress(b.concat([a, a], 0), b.const(None, np.arange(2 * n) % 2 == 1), 0, (2 * n,)), (0,), (n,)),
+}
+
+
+@pytest.mark.parametrize("mode", list(MODES))
+@pytest.mark.parametrize("move", list(MOVED_PARAMETERS))
+def test_random_numbers_keep_their_bits_on_the_way(odla, move, mode):
+    announce("random numbers behind %s, %s mode" % (move, mode))
+    n = 64
+    u = np.float32(0.5) + (np.arange(n) - n // 2 - 0.5).astype(np.float32) * np.float32(2.0 ** -20)
+    at = {"tile": np.full(n, n // 2), "broadcast": np.full(n, 1), "pad": np.clip(np.arange(n) - 1, 0, None), "gather_elements": np.arange(n)[::-1],
+          "compress": np.concatenate([np.arange(1, n, 2)] * 2)}[move]
+    moved = u[at].copy()
+    if move == "pad":
+        moved[[0, n - 2, n - 1]] = 0.0
+    logits = np.full((n, 64), -np.inf, np.float32)
+    logits[:, [3, 40]] = 1.0
+
+    def build(b):
+        b.output(b.sample(b.arg("l", logits.shape, np.float16), MOVED_PARAMETERS[move](b, b.arg("u", (n,)), n), name="t"), "t")
+    got = run_hip(build, {"u": u, "l": logits.astype(np.float16)}, **MODES[mode])["t"]
+    want = np.where(moved < 0.5, 3, 40)
+    assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("mode", list(MODES))
+def test_scales_joined_with_computed_ones(odla, mode):
+    """A Concat of moved scales, which stay fp32, and of ones that a group of element-wise operators made as the mode stores them."""
+    announce("moved and computed scales in one Concat, %s mode" % mode)
+    x, w, ws = G.moved_operands()
+
+    def build(b):
+        q, s = b.block_quantize(b.arg("x", x.shape, np.float16))
+        made = b.mul(b.mul(b.slice(s, (0, 1), (6, 3)), b.const(None, np.array([[2.0]], np.float32))), b.const(None, np.array([[0.25]], np.float32)))
+        sa = b.concat([b.slice(s, (0, 0), (6, 1)), made], 1)
+        b.output(b.block_gemm(q, sa, b.const("w", w, odla.FLOAT8_E4M3), b.const("ws", ws), np.float16, name="y"), "y")
+        b.output(sa, "sa")
+    got = run_hip(build, {"x": x}, **MODES[mode])
+    q, s = R.quantize_rows(x)
+    want = s.copy()
+    want[:, 1:] = R.values(R.to_bits(s[:, 1:].astype(np.float64), mode), mode) / 2      # (factors of two: one rounding)
+    assert np.array_equal(got["sa"], want)
+    y, bound = R.block_gemm(q, want, w, ws, "fp16")
+    check(got["y"], y, bound, "product", "fp16")
