@@ -30,6 +30,9 @@
 //   BLOCKGEMM  in = {A, A scale, B, B scale}
 //   EXPERTS    i0 top k, i1 renormalise; f0 scaling; in = {x, router, gate and up, its scale?, down, its scale?}
 //   SAMPLE     in = {logits, temperature?, top k?, top p?, min p?, uniform}
+//   RMSNORM    i0 8-bit result; f0 eps; in = {x, residual?, weight?}; results = normalised, scales (8-bit), sum (residual)
+//   PAGEDATTENTION i0 window (0: none); f0 scale; in = {query, key?, value?, key cache, value cache, page table, cached, starts?}
+//   LOGPROBS   i0 top; in = {logits, tokens}; results = log probabilities, entropies, top log probabilities, top tokens (top > 0)
 #include <climits>
 #include <cmath>
 #include <cstring>
@@ -432,6 +435,92 @@ bool token_op_shapes(OpKind op, const std::vector<_odla_value*>& in, const int64
       *out = Shape();
       for (int d = 0; d + 1 < xs.rank; ++d) out->d[out->rank++] = xs.d[d];
       if (out->rank == 0) { out->rank = 1; out->d[0] = 1; }
+      return true;
+    }
+    default:
+      return no("not an operator of a token step");
+  }
+}
+
+bool token_op_results(OpKind op, const std::vector<_odla_value*>& in, const int64_t* attr, std::vector<ResultType>* results, std::string* why) {
+  auto no = [&](const std::string& s) { *why = s; return false; };
+  results->clear();
+  const Shape& xs = in[0]->shape;
+  const int64_t last = xs.d[xs.rank - 1], rows = xs.numel() / last;
+  constexpr int64_t kMost = 1 << 24;
+  if (last > kMost || rows > 65535 * 128) return no("operand " + xs.str() + " is too large");
+  if (!is_float_type(in[0]->etype)) return no("operand must be a float type");
+  switch (op) {
+    case OP_RMSNORM: {
+      const _odla_value *r = in[1], *w = in[2];
+      if (r != nullptr && (r->etype != in[0]->etype || r->shape != xs)) return no("residual must have the type and the shape of the input " + xs.str());
+      if (w != nullptr) {
+        if (w->etype != ODLA_FLOAT32 && w->etype != in[0]->etype) return no("weight must be FLOAT32 or of the input's type");
+        if (w->shape.numel() != last) return no("weight " + w->shape.str() + " must have one element per column of the input " + xs.str());
+      }
+      results->push_back({attr[0] ? ODLA_HIP_FLOAT8_E4M3 : in[0]->etype, xs});
+      if (attr[0]) {
+        Shape s = xs;
+        s.d[xs.rank - 1] = (last + kScaleBlock - 1) / kScaleBlock;
+        results->push_back({ODLA_FLOAT32, s});
+      }
+      if (r != nullptr) results->push_back({in[0]->etype, xs});
+      return true;
+    }
+    case OP_PAGEDATTENTION: {
+      const _odla_value *k = in[1], *v = in[2], *kc = in[3], *vc = in[4], *table = in[5], *cached = in[6], *starts = in[7];
+      if (kc->kind != _odla_value::ARG || vc->kind != _odla_value::ARG || kc->eager || vc->eager) return no("caches must be arguments");
+      if (kc == vc) return no("key and value cache must be two arguments");
+      if (kc->shape.rank != 4 || vc->shape != kc->shape) return no("caches " + kc->shape.str() + " and " + vc->shape.str() + " must both be [pages, page size, heads, head size]");
+      if (kc->etype != in[0]->etype || vc->etype != in[0]->etype) return no("caches must be of the query's type");
+      const int64_t pages = kc->shape.d[0], page = kc->shape.d[1], heads = kc->shape.d[2], d = kc->shape.d[3];
+      if (d % 8 != 0 || d > kMaxHeadSize) return no("head size must be a multiple of 8 up to 256");
+      if (pages > INT32_MAX || page > INT32_MAX || pages * page > INT32_MAX) return no("caches " + kc->shape.str() + " have 2^31 tokens or more");
+      if (xs.rank != 2 && xs.rank != 3) return no("query " + xs.str() + " must be [tokens, heads, head size] or [tokens, heads * head size]");
+      const int64_t tokens = xs.d[0], wide = xs.numel() / tokens;
+      if (xs.rank == 3 && last != d) return no("query " + xs.str() + " must have the head size of the caches " + kc->shape.str());
+      if (wide % (heads * d) != 0) return no("query " + xs.str() + " must have a multiple of the heads of the caches " + kc->shape.str());
+      const int64_t group = wide / (heads * d);
+      if (heads > 65535 || group > 65535 || tokens * heads * group > INT32_MAX / 2) return no("query " + xs.str() + " is too large");
+      if ((k == nullptr) != (v == nullptr)) return no("key and value belong together");
+      for (const _odla_value* n : {k, v}) {
+        if (n == nullptr) continue;
+        if (n->etype != in[0]->etype) return no("key and value must be of the query's type");
+        if (n->shape.rank < 2 || n->shape.rank > 3 || n->shape.d[0] != tokens || n->shape.numel() != tokens * heads * d || (n->shape.rank == 3 && n->shape.d[2] != d))
+          return no("key and value must be [tokens, heads, head size] with the query's tokens and the caches' heads (got " + n->shape.str() + ")");
+      }
+      for (const _odla_value* n : {table, cached, starts})
+        if (n != nullptr && n->etype != ODLA_INT32) return no("page table, cached lengths and starts must be INT32");
+      if (table->shape.rank != 2) return no("page table " + table->shape.str() + " must be [sequences, pages]");
+      const int64_t seqs = table->shape.d[0];
+      if (seqs > kMaxSequences) return no("more than 65536 sequences");
+      if (table->shape.d[1] > INT32_MAX || table->shape.d[1] * page > (1 << 30)) return no("page table " + table->shape.str() + " reaches beyond 2^30 tokens");
+      if (cached->shape.numel() != seqs) return no("cached lengths " + cached->shape.str() + " must have one element per sequence");
+      if (starts != nullptr && starts->shape.numel() != seqs + 1) return no("starts " + starts->shape.str() + " must have one element more than there are sequences");
+      if (starts == nullptr && tokens % seqs != 0) return no("without starts every sequence has the same number of tokens");
+      if (attr[0] < 0 || attr[0] > INT32_MAX) return no("window must not be negative");
+      results->push_back({in[0]->etype, xs});
+      return true;
+    }
+    case OP_LOGPROBS: {
+      const _odla_value* t = in[1];
+      if (last > kMaxVocabulary) return no("more than 524288 logits in a row");
+      if (t->etype != ODLA_INT32) return no("tokens must be INT32");
+      const int64_t n = t->shape.numel();
+      if (n % rows != 0 || n / rows > kMaxTokensPerRow) return no("tokens " + t->shape.str() + " must be 1 .. 64 for every row of the logits " + xs.str());
+      if (attr[0] < 0 || attr[0] > last || attr[0] > kMaxAlternatives) return no("top must be 0 .. min(V, 32)");
+      Shape lead;
+      for (int d = 0; d + 1 < xs.rank; ++d) lead.d[lead.rank++] = xs.d[d];
+      Shape top = lead;
+      if (lead.rank == 0) { lead.rank = 1; lead.d[0] = 1; }
+      results->push_back({ODLA_FLOAT32, t->shape});
+      results->push_back({ODLA_FLOAT32, lead});
+      if (attr[0] > 0) {
+        if (top.rank >= ODLA_MAX_DIMENSION) return no("logits of rank " + std::to_string(xs.rank));
+        top.d[top.rank++] = attr[0];
+        results->push_back({ODLA_FLOAT32, top});
+        results->push_back({ODLA_INT32, top});
+      }
       return true;
     }
     default:
@@ -1500,6 +1589,40 @@ odla_value odla_NMS(odla_value boxes, odla_value scores, odla_uint32 max_num_out
 }
 
 // ------------------------------------------- operators of a token step --
+static odla_values no_values() {
+  odla_values r;
+  r.size = 0;
+  return r;
+}
+
+// Records an operator of OP_RMSNORM .. OP_LOGPROBS with all its results; `required`: bit k, operand k must be there.
+static odla_values add_token_node(const char* what, OpKind op, const std::vector<odla_value>& in, unsigned required, int64_t i0, float f0,
+                                  const odla_value_ids& ids) {
+  odla_values r = no_values();
+  for (size_t k = 0; k < in.size(); ++k) {
+    if ((required >> k & 1) && in[k] == nullptr) { OHIP_ERR("%s: null operand", what); return r; }
+  }
+  _odla_computation* c = comp_of(in[0]);
+  if (c == nullptr) { OHIP_ERR("%s: no current computation", what); return r; }
+  std::vector<ResultType> results;
+  std::string why;
+  if (!token_op_results(op, in, &i0, &results, &why)) { OHIP_ERR("%s: %s", what, why.c_str()); return r; }
+  auto id = [&](size_t k) { return k < ids.size ? ids.value_ids[k] : nullptr; };
+  Node* n = add_node(c, op, in, results[0].etype, results[0].shape, id(0));
+  if (n == nullptr) return r;
+  n->i[0] = i0;
+  n->f[0] = f0;
+  r.values[r.size++] = n->out;
+  for (size_t k = 1; k < results.size(); ++k) {
+    odla_value v = new_value(c, _odla_value::TEMP, results[k].etype, results[k].shape, id(k));
+    v->producer = n->out->producer;
+    if (k == 1) n->out2 = v;
+    else n->more.push_back(v);
+    r.values[r.size++] = v;
+  }
+  return r;
+}
+
 odla_values odla_hip_BlockQuantize(odla_value input, const odla_value_ids value_ids) {
   odla_values r;
   r.size = 0;
@@ -1566,6 +1689,35 @@ odla_value odla_hip_Sample(odla_value logits, odla_value temperature, odla_value
   Node* n = add_node(c, OP_SAMPLE, in, ODLA_INT32, o, id);
   if (n == nullptr) return ADD_NODE_FAILED;
   return n->out;
+}
+
+odla_values odla_hip_RmsNorm(odla_value input, odla_value residual, odla_value weight, odla_float32 epsilon,
+                             odla_element_type result_type, const odla_value_ids value_ids) {
+  if (input != nullptr && result_type != input->etype && result_type != ODLA_HIP_FLOAT8_E4M3) {
+    OHIP_ERR("odla_hip_RmsNorm: the result must be of the input's type or ODLA_HIP_FLOAT8_E4M3 (got %d)", (int)result_type);
+    return no_values();
+  }
+  if (!(epsilon >= 0.f) || std::isinf(epsilon)) {
+    OHIP_ERR("odla_hip_RmsNorm: epsilon must be a finite number from 0 on (got %g)", (double)epsilon);
+    return no_values();
+  }
+  return add_token_node("odla_hip_RmsNorm", OP_RMSNORM, {input, residual, weight}, 0x1, result_type == ODLA_HIP_FLOAT8_E4M3, epsilon, value_ids);
+}
+
+odla_value odla_hip_PagedAttention(odla_value query, odla_value key, odla_value value, odla_value key_cache, odla_value value_cache,
+                                   odla_value page_table, odla_value cached, odla_value starts, odla_float32 scale, odla_uint32 window,
+                                   const odla_value_id id) {
+  REQUIRE(std::isfinite(scale), "odla_hip_PagedAttention: the scale must be finite");
+  odla_value_ids ids;
+  ids.size = 1;
+  ids.value_ids[0] = id;
+  const odla_values r = add_token_node("odla_hip_PagedAttention", OP_PAGEDATTENTION, {query, key, value, key_cache, value_cache, page_table, cached, starts},
+                                       0x79, window, scale, ids);
+  return r.size == 1 ? r.values[0] : nullptr;
+}
+
+odla_values odla_hip_LogProbs(odla_value logits, odla_value tokens, odla_uint32 top, const odla_value_ids value_ids) {
+  return add_token_node("odla_hip_LogProbs", OP_LOGPROBS, {logits, tokens}, 0x3, top, 0.f, value_ids);
 }
 
 }  // extern "C"

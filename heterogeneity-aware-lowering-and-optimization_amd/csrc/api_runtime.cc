@@ -48,7 +48,7 @@ const char* op_name(OpKind k) {
                                 "Reduce", "Softmax", "Cast", "Concat", "Gather", "Reshape", "Resize",
                                 "Slice", "Transpose", "Quantize", "Dequantize", "NMS", "Elementwise", "ArgExtreme",
                                 "CopyND", "TopK", "LRN", "RowNorm", "PostProcess", "AxisOp", "BlockQuantize", "BlockGemm",
-                                "MixtureOfExperts", "Sample"};
+                                "MixtureOfExperts", "Sample", "RmsNorm", "PagedAttention", "LogProbs"};
   static_assert(sizeof(names) / sizeof(names[0]) == (size_t)kLastOp + 1, "one name per OpKind");
   if ((int)k < 0 || (int)k > (int)kLastOp) return "?";
   return names[(int)k];
@@ -308,15 +308,41 @@ odla_status run_steps(_odla_context* ctx, const Plan& plan, char* arena, const s
   return ODLA_SUCCESS;
 }
 
+// Whether a cache bound at `p` can be extended there: 16-byte aligned memory of the current device that
+// no other cache of the computation (entered in `ext` already) overlaps.
+bool cache_is_usable(const Plan& plan, const std::vector<const char*>& ext, const size_t k, const void* p) {
+  const char* name = plan.inputs[k].v->name.c_str();
+  hipPointerAttribute_t attr;
+  int device = -1;
+  if (hipPointerGetAttributes(&attr, p) != hipSuccess || attr.type != hipMemoryTypeDevice) {
+    (void)hipGetLastError();
+    OHIP_ERR("cache '%s' must be bound to device memory: it is extended in place", name);
+    return false;
+  }
+  if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0 || hipGetDevice(&device) != hipSuccess || attr.device != device) {
+    OHIP_ERR("cache '%s' must be 16-byte aligned memory of the current device", name);
+    return false;
+  }
+  const char* a = static_cast<const char*>(p);
+  for (size_t j = 0; j < k; ++j) {
+    if (!plan.inputs[j].caller_only || ext[j] == nullptr) continue;
+    if (a < ext[j] + plan.inputs[j].bytes && ext[j] < a + plan.inputs[k].bytes) {
+      OHIP_ERR("caches '%s' and '%s' overlap", plan.inputs[j].v->name.c_str(), name);
+      return false;
+    }
+  }
+  return true;
+}
+
 // Copies the bound arguments into their staging tensors.  With `ext`, an argument
 // that lives in device memory and that the plan can read in place is not copied:
 // its buffer is entered in (*ext)[k] instead (nullptr for the copied ones).  With `wait`
 // (nothing of an earlier execution is still under way) small pageable arguments pass
 // through host_stage; where the plan cannot read them there, they are entered behind the results
-// in *ext, and the first launches of run_steps copy them.
-odla_status stage_inputs(_odla_context* ctx, const Plan& plan, char* arena, std::vector<const char*>* ext = nullptr,
-                         const bool wait = false) {
-  if (ext != nullptr) ext->assign(2 * plan.inputs.size() + plan.outputs.size(), nullptr);
+// in *ext, and the first launches of run_steps copy them.  Caches are never copied, also not without `in_place`.
+odla_status stage_inputs(_odla_context* ctx, const Plan& plan, char* arena, std::vector<const char*>* ext,
+                         const bool wait = false, const bool in_place = true) {
+  ext->assign(2 * plan.inputs.size() + plan.outputs.size(), nullptr);
   for (size_t k = 0; k < plan.inputs.size(); ++k) {
     const Plan::IO& io = plan.inputs[k];
     auto it = ctx->bound_in.find(io.v);
@@ -324,7 +350,12 @@ odla_status stage_inputs(_odla_context* ctx, const Plan& plan, char* arena, std:
       OHIP_ERR("argument '%s' is not bound", io.v->name.c_str());
       return ODLA_INVALID_PARAM;
     }
-    if (ext != nullptr && io.in_place_ok && !ctx->in_place_off && in_place_args_enabled() &&
+    if (io.caller_only) {
+      if (!cache_is_usable(plan, *ext, k, it->second)) return ODLA_INVALID_PARAM;
+      (*ext)[k] = static_cast<const char*>(it->second);
+      continue;
+    }
+    if (in_place && io.in_place_ok && !ctx->in_place_off && in_place_args_enabled() &&
         (!io.align16 || (reinterpret_cast<uintptr_t>(it->second) & 15u) == 0) && is_device_memory(it->second)) {
       (*ext)[k] = static_cast<const char*>(it->second);
       OHIP_DEBUG("argument '%s' is read in place", io.v->name.c_str());
@@ -332,7 +363,7 @@ odla_status stage_inputs(_odla_context* ctx, const Plan& plan, char* arena, std:
     }
     char* dst = arena + plan.tensors[io.tensor].offset;
     const void* src = it->second;
-    char* const room = ext != nullptr && wait && is_pageable_memory(src) ? host_stage(ctx, plan, k) : nullptr;
+    char* const room = in_place && wait && is_pageable_memory(src) ? host_stage(ctx, plan, k) : nullptr;
     if (room != nullptr) {
       memcpy(room, src, io.bytes);
       if (io.host_ok && !ctx->in_place_off && in_place_args_enabled()) {
@@ -1140,9 +1171,10 @@ odla_status odla_hip_ExecuteComputationStatic(odla_computation comp, odla_contex
     return ODLA_MEM_ERROR;
   }
   char* arena = static_cast<char*>(base);
-  odla_status st = stage_inputs(ctx, plan, arena);
+  std::vector<const char*> ext;   // (caches alone)
+  odla_status st = stage_inputs(ctx, plan, arena, &ext, /*wait=*/false, /*in_place=*/false);
   if (st != ODLA_SUCCESS) return st;
-  st = run_steps(ctx, plan, arena);
+  st = run_steps(ctx, plan, arena, &ext);
   if (st != ODLA_SUCCESS) return st;
   return fetch_outputs(ctx, plan, arena);
 }
@@ -1185,8 +1217,10 @@ odla_status odla_hip_ProfileSteps(odla_context ctx, odla_int32 iters, odla_hip_s
   env.base[SP_ARENA] = ctx->arena;
   env.base[SP_CONST] = plan.const_pool;
   odla_status st = ODLA_SUCCESS;
+  std::vector<const char*> ext;
   for (int it = 0; it < iters && st == ODLA_SUCCESS; ++it) {
-    st = stage_inputs(ctx, plan, ctx->arena);
+    st = stage_inputs(ctx, plan, ctx->arena, &ext, /*wait=*/false, /*in_place=*/false);
+    env.ext = ext.data();
     for (int i = 0; i < n && st == ODLA_SUCCESS; ++i) {
       (void)hipEventRecord(ev[2 * i], ctx->stream);
       if (plan.steps[i].fn(env, ctx->stream) != hipSuccess) st = ODLA_FAILURE;

@@ -203,13 +203,32 @@ std::unique_ptr<_odla_computation> clone_for_batch(const _odla_computation& c, i
           if (!rs.carry(v)) rs.reject(n, "has one constant parameter per row");
         }
         break;
+      case OP_RMSNORM:
+        if (!rs.carry(x) || x->shape.rank < 2) rs.reject(n, "has rows that do not depend on the batch");
+        if (n.in[1] != nullptr && !rs.carry(n.in[1])) rs.reject(n, "has a residual that does not depend on the batch");
+        if (rs.carry(n.in[2])) rs.reject(n, "has a weight that depends on the batch");
+        break;
+      case OP_PAGEDATTENTION:
+        // (the batch is the sequences, each with the same number of new tokens; its caches are whole in every batch)
+        if (rows_apart) rs.reject(n, "extends caches that all sequences share");
+        if (n.in[7] != nullptr) rs.reject(n, "has sequences of different lengths");
+        if (!rs.carry(x) || !rs.carry(n.in[5]) || !rs.carry(n.in[6]) || (n.in[1] != nullptr && (!rs.carry(n.in[1]) || !rs.carry(n.in[2]))))
+          rs.reject(n, "has tokens, page tables or lengths that do not depend on the batch");
+        if (rs.carry(n.in[3]) || rs.carry(n.in[4])) rs.reject(n, "has caches that depend on the batch");
+        break;
+      case OP_LOGPROBS:
+        if (rows_apart) rs.reject(n, "gives rows whose last bits depend on how many there are");
+        if (!rs.carry(x) || x->shape.rank < 2 || !rs.carry(n.in[1])) rs.reject(n, "has logits or tokens that do not depend on the batch");
+        break;
       case OP_UNARY: case OP_POOL: case OP_CAST: case OP_RESHAPE: case OP_RESIZE: case OP_LRN:
         break;
       default:
         rs.reject(n, "is not known to keep the batch in the leading extent");
         break;
     }
-    for (const _odla_value* o : {n.out, n.out2}) {
+    std::vector<const _odla_value*> results = {n.out, n.out2};
+    results.insert(results.end(), n.more.begin(), n.more.end());
+    for (const _odla_value* o : results) {
       if (o == nullptr) continue;
       if (!rs.scalable(o->shape.d[0])) rs.reject(n, "has a result whose leading extent is not a multiple of the batch");
       rs.carries[o->index] = 1;
@@ -235,6 +254,7 @@ std::unique_ptr<_odla_computation> clone_for_batch(const _odla_computation& c, i
     for (auto& v : n.in) v = map(v);
     n.out = map(n.out);
     n.out2 = map(n.out2);
+    for (auto& v : n.more) v = map(v);
     n.iv = new_iv[ni];
     d->nodes.push_back(std::move(n));
   }

@@ -36,14 +36,15 @@ enum OpKind : int {
   OP_CONV, OP_GEMM, OP_BINARY, OP_UNARY, OP_BATCHNORM, OP_LAYERNORM, OP_POOL, OP_REDUCE,
   OP_SOFTMAX, OP_CAST, OP_CONCAT, OP_GATHER, OP_RESHAPE, OP_RESIZE, OP_SLICE, OP_TRANSPOSE,
   OP_QUANTIZE, OP_DEQUANTIZE, OP_NMS, OP_EWISE, OP_ARGEXT, OP_COPYND, OP_TOPK, OP_LRN, OP_ROWNORM,
-  OP_POSTPROCESS, OP_AXISOP, OP_BLOCKQUANT, OP_BLOCKGEMM, OP_EXPERTS, OP_SAMPLE
+  OP_POSTPROCESS, OP_AXISOP, OP_BLOCKQUANT, OP_BLOCKGEMM, OP_EXPERTS, OP_SAMPLE,
+  OP_RMSNORM, OP_PAGEDATTENTION, OP_LOGPROBS
 };
-constexpr OpKind kLastOp = OP_SAMPLE;
+constexpr OpKind kLastOp = OP_LOGPROBS;
 // Operators that take or give 8-bit floating-point values (ODLA_HIP_FLOAT8_E4M3): those that
 // compute with them and those that move whole elements whatever they stand for.
 inline bool op_knows_float8(OpKind k) {
   return k == OP_BLOCKQUANT || k == OP_BLOCKGEMM || k == OP_EXPERTS || k == OP_RESHAPE || k == OP_TRANSPOSE ||
-         k == OP_SLICE || k == OP_CONCAT || k == OP_GATHER;
+         k == OP_SLICE || k == OP_CONCAT || k == OP_GATHER || k == OP_RMSNORM;
 }
 // sub-kinds of OP_AXISOP (Node::i[0])
 enum AxisOp : int { AX_GATHER_ELEMENTS = 0, AX_CUMSUM, AX_HARDMAX, AX_COMPRESS };
@@ -99,6 +100,7 @@ struct Node {
   std::vector<_odla_value*> in;  // nullptr entries allowed for optional operands
   _odla_value* out = nullptr;
   _odla_value* out2 = nullptr;  // second result (TopK indices)
+  std::vector<_odla_value*> more;  // third result and further ones
   // attributes (meaning depends on op; see api_ops.cc)
   int64_t i[24] = {0};
   float f[8] = {0};
@@ -193,6 +195,8 @@ struct Plan {
     // arguments: the one launch that reads the tensor reads every element once;
     // results: no launch reads the tensor.  Page-locked host memory then serves as well as device memory.
     bool host_ok = false;
+    // an argument that launches extend in place (a cache): device memory of the caller's, never copied
+    bool caller_only = false;
   };
   std::vector<IO> inputs, outputs;
   std::unordered_map<const _odla_value*, int> final_tensor;  // for odla_GetValueData
@@ -231,6 +235,13 @@ const char* api_op_name(const Node& n);
 // Shapes of an operator of a token step (OP_BLOCKQUANT .. OP_SAMPLE); false and a reason when its
 // operands do not fit.  `attr` are the node's integer attributes.
 bool token_op_shapes(OpKind op, const std::vector<_odla_value*>& in, const int64_t* attr, Shape* out, Shape* out2, std::string* why);
+// The same for OP_RMSNORM .. OP_LOGPROBS: types and shapes of all results (out, out2, more).
+struct ResultType { odla_element_type etype; Shape shape; };
+bool token_op_results(OpKind op, const std::vector<_odla_value*>& in, const int64_t* attr, std::vector<ResultType>* results, std::string* why);
+// Nodes of this operator may have more than two results.
+inline bool has_more(OpKind k) { return k == OP_RMSNORM || k == OP_LOGPROBS; }
+// Operand `k` of the node is a cache: an argument that its launches extend in the caller's buffer.
+inline bool is_cache_operand(const Node& n, size_t k) { return n.op == OP_PAGEDATTENTION && (k == 3 || k == 4); }
 
 DType dtype_from_odla(odla_element_type t);
 int odla_type_size(odla_element_type t);

@@ -74,6 +74,37 @@ __device__ __forceinline__ floatx4 mma_e4m3(const uintx4 a0, const uintx4 a1, co
 
 struct f8_t { uint8_t bits; };
 
+// The scale of a block with the largest magnitude `most`, and eight of its values v divided by it as e4m3 bytes.
+constexpr float kMostE4m3 = 448.f;
+constexpr float kLeastScale = 1.17549435e-38f;   // 2^-126: x / scale stays finite for blocks of subnormals and zeros
+__device__ __forceinline__ float e4m3_scale(const float most) { return fmaxf(most / kMostE4m3, kLeastScale); }
+__device__ __forceinline__ uintx2 e4m3_of(float (&v)[8], const float s) {
+  // v / s, correctly rounded: from the correctly rounded 1 / s, two steps of quotient += remainder / s with exact
+  // remainders give what the division gives in half of its instructions.  Where a remainder that matters could
+  // underflow, or s is infinite, the division itself.  (The sign is v's: a zero's would be lost.)
+  if (s >= 0x1p-70f && s <= 0x1p120f) {
+    const float by = 1.f / s;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float u = v[e] * by;
+      u = __builtin_fmaf(__builtin_fmaf(-u, s, v[e]), by, u);
+      u = __builtin_fmaf(__builtin_fmaf(-u, s, v[e]), by, u);
+      v[e] = __builtin_copysignf(u, v[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] /= s;
+  }
+  int w0 = 0, w1 = 0;
+#if defined(__HIP_DEVICE_COMPILE__)
+  w0 = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], w0, false);
+  w0 = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w0, true);
+  w1 = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], w1, false);
+  w1 = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], w1, true);
+#endif
+  return uintx2{(unsigned)w0, (unsigned)w1};
+}
+
 // c + W X^T over the elements of one 16-byte vector of X per lane (16 rows of either).
 template <typename X>
 __device__ __forceinline__ floatx4 mma_vec(const uintx4 w, const uintx4 x, floatx4 c) {
@@ -142,6 +173,49 @@ __device__ __forceinline__ void store4(T* y, const floatx4 v, const int n, const
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (i < n) Store<T>::st(y + i, v[i]);
+  }
+}
+
+struct __attribute__((packed, aligned(1))) Bytes8 { uintx2 v; };
+
+// Values at .. at + 7 of a row of `len`, zeros behind its end; VECTOR: rows are whole 16-byte aligned groups of eight.
+// (Other rows: one load of any alignment per 16 bytes; the last group of a row comes value by value.)
+template <typename T, bool VECTOR>
+__device__ __forceinline__ void load8(const T* row, const int at, const int len, float (&v)[8]) {
+  constexpr int PER = Vec16<T>::N;
+  if (at + 8 <= len) {
+#pragma unroll
+    for (int h = 0; h < 8 / PER; ++h) {
+      Vec16<T> w;
+      if constexpr (VECTOR) w.load(row + at + h * PER);
+      else w.raw = reinterpret_cast<const Bytes16*>(row + at + h * PER)->v;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) v[h * PER + e] = w.get(e);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = !VECTOR && at + e < len ? Store<T>::ld(row + at + e) : 0.f;
+  }
+}
+template <typename T, bool VECTOR>
+__device__ __forceinline__ void store8(T* row, const int at, const int len, const float (&v)[8]) {
+  if (at + 8 <= len) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uintx4 w = {__float_as_uint(v[4 * h]), __float_as_uint(v[4 * h + 1]), __float_as_uint(v[4 * h + 2]), __float_as_uint(v[4 * h + 3])};
+        if constexpr (VECTOR) *reinterpret_cast<uintx4*>(row + at + 4 * h) = w;
+        else reinterpret_cast<Bytes16*>(row + at + 4 * h)->v = w;
+      }
+    } else {
+      const uintx4 w = pack8_rne<T>(v);
+      if constexpr (VECTOR) *reinterpret_cast<uintx4*>(row + at) = w;
+      else reinterpret_cast<Bytes16*>(row + at)->v = w;
+    }
+  } else if (!VECTOR) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (at + e < len) Store<T>::st(row + at + e, v[e]);
   }
 }
 

@@ -5,9 +5,6 @@
 namespace ohip {
 namespace {
 
-constexpr float kMostE4m3 = 448.f;
-constexpr float kLeastScale = 1.17549435e-38f;   // 2^-126: x / scale stays finite for blocks of subnormals and zeros
-
 // ------------------------------------------------------------- quantisation --
 // scale = max(max |x| / 448, 2^-126), q = e4m3(x / scale).  Bound by memory: es + 1 bytes per value.
 // Sixteen lanes hold a block, eight values each.  8192 x 7168 bf16: 32 us, 5.5 TB/s read and written (with a
@@ -45,36 +42,14 @@ __global__ void __launch_bounds__(256) block_quantize_kernel(const T* x, uint8_t
 #pragma unroll
     for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
     most = group_allreduce<16>(most, [](float a, float c) { return fmaxf(a, c); });
-    const float s = fmaxf(most / kMostE4m3, kLeastScale);
-    // v / s, correctly rounded: from the correctly rounded 1 / s, two steps of quotient += remainder / s with exact
-    // remainders give what the division gives in half of its instructions.  Where a remainder that matters could
-    // underflow, or s is infinite, the division itself.  (The sign is v's: a zero's would be lost.)
-    if (s >= 0x1p-70f && s <= 0x1p120f) {
-      const float by = 1.f / s;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float u = v[e] * by;
-        u = __builtin_fmaf(__builtin_fmaf(-u, s, v[e]), by, u);
-        u = __builtin_fmaf(__builtin_fmaf(-u, s, v[e]), by, u);
-        v[e] = __builtin_copysignf(u, v[e]);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] /= s;
-    }
-    int w0 = 0, w1 = 0;
-#if defined(__HIP_DEVICE_COMPILE__)
-    w0 = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], w0, false);
-    w0 = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w0, true);
-    w1 = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], w1, false);
-    w1 = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], w1, true);
-#endif
+    const float s = e4m3_scale(most);
+    const uintx2 w = e4m3_of(v, s);
     if constexpr (VECTOR) {
-      if (l16 * 8 < n) *reinterpret_cast<uintx2*>(q + at + l16 * 8) = uintx2{(unsigned)w0, (unsigned)w1};
+      if (l16 * 8 < n) *reinterpret_cast<uintx2*>(q + at + l16 * 8) = w;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (l16 + 16 * e < n) q[at + l16 + 16 * e] = (uint8_t)((unsigned)(e < 4 ? w0 : w1) >> (8 * (e & 3)));
+        if (l16 + 16 * e < n) q[at + l16 + 16 * e] = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
     }
     if (live && l16 == 0) scale[unit] = s;
   }

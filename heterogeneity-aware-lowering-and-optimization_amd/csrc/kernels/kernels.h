@@ -757,5 +757,54 @@ struct SampleParams {
 };
 hipError_t launch_sample(const SampleParams& p, hipStream_t stream);
 
+// Rows normalised by their root mean square (see odla_hip_RmsNorm): s = x + residual (where there is one),
+// y = s / sqrt(mean s^2 + eps) * weight, in y_dt (dt, or DT_F8 with a scale for each block of 128 of a row); sum = s.
+// Reads and writes exactly the elements; bases aligned to 16 bytes.
+struct RmsNormParams {
+  const void* x = nullptr; const void* residual = nullptr; const void* weight = nullptr;   // (null: none)
+  void* y = nullptr; float* scale = nullptr; void* sum = nullptr;
+  int64_t rows = 0;
+  int len = 0;
+  float eps = 0.f;
+  DType dt = DT_F32, w_dt = DT_F32;
+  bool quantize = false;
+};
+hipError_t launch_rms_norm(const RmsNormParams& p, hipStream_t stream);
+
+// Attention of new tokens over a paged cache (see odla_hip_PagedAttention).
+constexpr int kMaxHeadSize = 256, kMaxSequences = 65536;
+struct PagedAttentionParams {
+  const void* q = nullptr;                              // [tokens][kv_heads * group][d]
+  const void* k = nullptr; const void* v = nullptr;     // [tokens][kv_heads][d] (null: in the caches already)
+  void* k_cache = nullptr; void* v_cache = nullptr;     // [pages][page][kv_heads][d]
+  const int32_t* table = nullptr;                       // [seqs][table_width]
+  const int32_t* cached = nullptr; const int32_t* starts = nullptr;
+  void* y = nullptr;
+  void* work = nullptr;                                 // paged_attention_space(p) bytes
+  int tokens = 0, seqs = 0, kv_heads = 0, group = 0, d = 0, page = 0, pages = 0, table_width = 0, window = 0;
+  float scale = 1.f;
+  DType dt = DT_F32;
+};
+size_t paged_attention_space(const PagedAttentionParams& p);
+hipError_t launch_cache_write(const PagedAttentionParams& p, hipStream_t stream);        // the new keys and values into their pages
+hipError_t launch_paged_attention(const PagedAttentionParams& p, hipStream_t stream);    // y, or parts of it in the work space
+hipError_t launch_attention_join(const PagedAttentionParams& p, hipStream_t stream);     // y from the parts; rows of no sequence zero
+
+// Log probabilities, entropy and the best alternatives of rows of logits (see odla_hip_LogProbs).
+constexpr int kMaxAlternatives = 32, kMaxTokensPerRow = 64;
+struct LogProbsParams {
+  const void* logits = nullptr;
+  const int32_t* tokens = nullptr;                      // [rows][per_row]
+  float* log_prob = nullptr; float* entropy = nullptr;  // [rows][per_row], [rows]
+  float* top_log_prob = nullptr; int32_t* top_token = nullptr;   // [rows][top]
+  void* work = nullptr;                                 // log_probs_space(p) bytes
+  int rows = 0, V = 0, per_row = 1, top = 0;
+  DType dt = DT_F32;
+};
+int log_probs_parts(const LogProbsParams& p);           // workgroups that share a row
+size_t log_probs_space(const LogProbsParams& p);
+hipError_t launch_log_probs(const LogProbsParams& p, hipStream_t stream);
+hipError_t launch_log_probs_join(const LogProbsParams& p, hipStream_t stream);   // where log_probs_parts is above 1
+
 }  // namespace ohip
 #endif

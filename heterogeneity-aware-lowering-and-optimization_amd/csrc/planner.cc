@@ -322,7 +322,13 @@ class Planner {
       if (v != nullptr && dtype_from_odla(v->etype) == DT_F32) kept_fp32_[v->index] = 1;
     };
     for (const Node& n : comp_->nodes) {
-      if (n.op == OP_BLOCKQUANT) keep(n.out2);
+      if (n.op == OP_BLOCKQUANT || (n.op == OP_RMSNORM && n.i[0] != 0)) keep(n.out2);
+      if (n.op == OP_PAGEDATTENTION) keep(n.out);     // (of fp32 caches, which stay fp32)
+      if (n.op == OP_LOGPROBS) {
+        keep(n.out);
+        keep(n.out2);
+        if (!n.more.empty()) keep(n.more[0]);
+      }
       for (size_t k = 0; k < moved_operands(n); ++k)
         if (kept_fp32(n.in[k])) keep(n.out);
     }
@@ -808,6 +814,9 @@ class Planner {
   void lower_blockgemm(int ni);
   void lower_experts(int ni);
   void lower_sample(int ni);
+  void lower_rmsnorm(int ni);
+  void lower_pagedattention(int ni);
+  void lower_logprobs(int ni);
   std::vector<char> kept_fp32_;   // by value index, see kept_fp32
   std::unordered_map<const _odla_value*, int> fp32_consts_;   // constants that get_fp32 keeps beside the stored form
   void lower_lrn(int ni);
@@ -827,6 +836,8 @@ class Planner {
   std::vector<char> no_fuse_;                        // nodes of an element-wise group that was given up
   void emit_stats(const _odla_value* v, const char* op_type, int forced_axis, const Node* producer);
   bool calib_ = false;
+  std::unordered_set<const _odla_value*> caches_;
+  bool is_cache(const _odla_value* v) const { return caches_.count(v) != 0; }
   struct SoftmaxAdd { const _odla_value* x; const _odla_value* mask; int64_t div; };
   std::unordered_map<int, SoftmaxAdd> softmax_add_;  // index of a folded Add's result -> its operands
 
@@ -968,6 +979,15 @@ void Planner::run() {
     for (_odla_value* v : comp_->nodes[ni].in)
       if (v != nullptr) consumers_[v->index].push_back((int)ni);
   find_kept_fp32();
+  // Caches are extended in the caller's buffers: nothing else may read them (a copy in another form would go stale).
+  for (const Node& n : comp_->nodes)
+    for (size_t k = 0; k < n.in.size(); ++k)
+      if (is_cache_operand(n, k)) caches_.insert(n.in[k]);
+  for (const Node& n : comp_->nodes)
+    for (size_t k = 0; k < n.in.size(); ++k)
+      if (is_cache(n.in[k]) && !is_cache_operand(n, k)) fail(ODLA_UNSUPPORTED_OP, "%s reads the cache '%s'; only odla_hip_PagedAttention does", api_op_name(n), n.in[k]->name.c_str());
+  for (const _odla_value* v : comp_->outputs)
+    if (is_cache(v)) fail(ODLA_UNSUPPORTED_OP, "the cache '%s' is an output; it is extended in the caller's buffer", v->name.c_str());
 
   // Arguments: one staging tensor each (declared type, row-major), alive from
   // the start of the execution because the H2D copy precedes every step.
@@ -981,6 +1001,7 @@ void Planner::run() {
     io.tensor = t;
     io.bytes = T(t).bytes;
     plan_->inputs.push_back(io);
+    if (is_cache(a)) T(t).bytes = 0;   // (no room in the arena)
     VState& s = vs_[a->index];
     s.main = t;
     if (d == storage_dtype(a)) {
@@ -990,7 +1011,8 @@ void Planner::run() {
   }
 
   if (calib_) {
-    for (_odla_value* a : comp_->args) emit_stats(a, a->eager ? "odla_SetValueData" : "odla_CreateArgument", -1, nullptr);
+    for (_odla_value* a : comp_->args)
+      if (!is_cache(a)) emit_stats(a, a->eager ? "odla_SetValueData" : "odla_CreateArgument", -1, nullptr);
     if (!o.calib_skip_weights) {
       // kernels of convolutions get one range per output channel whatever the channel axis is
       std::unordered_map<const _odla_value*, int> kernel_axis;
@@ -1021,6 +1043,7 @@ void Planner::run() {
       const Node& n = comp_->nodes[ni];
       emit_stats(n.out, api_op_name(n), -1, &n);
       if (n.out2 != nullptr) emit_stats(n.out2, api_op_name(n), -1, &n);
+      for (const _odla_value* v : n.more) emit_stats(v, api_op_name(n), -1, &n);
     }
   }
 
@@ -1100,6 +1123,11 @@ void Planner::run() {
   for (size_t k = 0; k < plan_->inputs.size(); ++k) {
     Plan::IO& io = plan_->inputs[k];
     const int r = root(io.tensor);
+    if (is_cache(io.v)) {
+      io.in_place_ok = io.caller_only = io.align16 = true;
+      T(r).ext_slot = (int)k;
+      continue;
+    }
     bool ok = !calib_ && r == io.tensor && T(r).space == SP_ARENA && T(r).last_step >= 0 && !arena_only_.count(r) && !written_.count(r);
     for (const Plan::IO& o : plan_->outputs) ok = ok && root(o.tensor) != r;
     for (const auto& ft : plan_->final_tensor) ok = ok && root(ft.second) != r;
@@ -1186,6 +1214,9 @@ void Planner::lower(int ni) {
     case OP_BLOCKGEMM: lower_blockgemm(ni); break;
     case OP_EXPERTS: lower_experts(ni); break;
     case OP_SAMPLE: lower_sample(ni); break;
+    case OP_RMSNORM: lower_rmsnorm(ni); break;
+    case OP_PAGEDATTENTION: lower_pagedattention(ni); break;
+    case OP_LOGPROBS: lower_logprobs(ni); break;
   }
 }
 
@@ -4773,6 +4804,123 @@ void Planner::lower_sample(int ni) {
     return launch_sample(p, st);
   }, kReads16 | kWrites16);
   set_main(n.out, ty);
+}
+
+void Planner::lower_rmsnorm(int ni) {
+  Node& n = comp_->nodes[ni];
+  const _odla_value *x = n.in[0], *r = n.in[1], *w = n.in[2];
+  RmsNormParams rp;
+  rp.len = (int)x->shape.d[x->shape.rank - 1];
+  rp.rows = x->shape.numel() / rp.len;
+  rp.eps = n.f[0];
+  rp.quantize = n.i[0] != 0;
+  const int tx = get(x, L_ROWMAJOR, FORM_FLOAT);
+  const int tr = r != nullptr ? get(r, L_ROWMAJOR, FORM_FLOAT) : -1, tw = w != nullptr ? get(w, L_ROWMAJOR, FORM_FLOAT) : -1;
+  rp.dt = T(tx).dt;
+  rp.w_dt = tw >= 0 ? T(tw).dt : rp.dt;
+  if (tr >= 0 && T(tr).dt != rp.dt) fail(ODLA_UNSUPPORTED_DATATYPE, "odla_hip_RmsNorm '%s': input and residual are stored in different types", n.out->name.c_str());
+  const int ty = new_tensor(rp.quantize ? DT_F8 : rp.dt, L_ROWMAJOR, n.out->shape, 0, SP_ARENA);
+  const _odla_value* sum = r == nullptr ? nullptr : rp.quantize ? n.more[0] : n.out2;
+  // (a sum that nothing reads is not written)
+  const bool wanted = sum != nullptr && (sum->is_output || !consumers_[sum->index].empty() || (calib_ && !sum->name.empty()));
+  const int ts = rp.quantize ? new_tensor(DT_F32, L_ROWMAJOR, n.out2->shape, 0, SP_ARENA) : -1;
+  const int tz = wanted ? new_tensor(rp.dt, L_ROWMAJOR, sum->shape, 0, SP_ARENA) : -1;
+  const Ref rx = ref(tx), rr = ref(tr >= 0 ? tr : tx), rw = ref(tw >= 0 ? tw : tx), ry = ref(ty), rs = ref(ts >= 0 ? ts : ty), rz = ref(tz >= 0 ? tz : ty);
+  const bool hr = tr >= 0, hw = tw >= 0, hz = tz >= 0;
+  emit_lists("rmsnorm:" + n.out->name, {tx, tr, tw}, {ty, ts, tz}, [=](const ExecEnv& e, hipStream_t st) {
+    RmsNormParams p = rp;
+    p.x = rx(e); p.y = ry(e);
+    if (hr) p.residual = rr(e);
+    if (hw) p.weight = rw(e);
+    if (p.quantize) p.scale = (float*)rs(e);
+    if (hz) p.sum = rz(e);
+    return launch_rms_norm(p, st);
+  }, kReads16 | kWrites16);
+  set_main(n.out, ty);
+  if (ts >= 0) set_kept(n.out2, ts);
+  if (tz >= 0) set_main(sum, tz);
+}
+
+void Planner::lower_pagedattention(int ni) {
+  Node& n = comp_->nodes[ni];
+  const _odla_value *q = n.in[0], *kc = n.in[3], *table = n.in[5], *starts = n.in[7];
+  const int tkc = vs_[kc->index].main, tvc = vs_[n.in[4]->index].main;
+  PagedAttentionParams ap;
+  ap.dt = T(tkc).dt;   // (caches keep their declared type in every precision mode)
+  auto operand = [&](const _odla_value* v) { return v == nullptr ? -1 : ap.dt == DT_F32 ? get_fp32(v) : get(v, L_ROWMAJOR, FORM_FLOAT); };
+  const int tq = operand(q), tk = operand(n.in[1]), tv = operand(n.in[2]);
+  const int tt = get(table, L_ROWMAJOR, FORM_FLOAT), tc = get(n.in[6], L_ROWMAJOR, FORM_FLOAT), ts = starts != nullptr ? get(starts, L_ROWMAJOR, FORM_FLOAT) : -1;
+  for (int t : {tq, tk, tv})
+    if (t >= 0 && T(t).dt != ap.dt) fail(ODLA_UNSUPPORTED_DATATYPE, "odla_hip_PagedAttention '%s': operands are stored in different types", n.out->name.c_str());
+  ap.tokens = (int)q->shape.d[0];
+  ap.pages = (int)kc->shape.d[0];
+  ap.page = (int)kc->shape.d[1];
+  ap.kv_heads = (int)kc->shape.d[2];
+  ap.d = (int)kc->shape.d[3];
+  ap.group = (int)(q->shape.numel() / ap.tokens / ap.kv_heads / ap.d);
+  ap.seqs = (int)table->shape.d[0];
+  ap.table_width = (int)table->shape.d[1];
+  ap.window = (int)n.i[0];
+  ap.scale = n.f[0];
+  const int ty = new_tensor(ap.dt, L_ROWMAJOR, n.out->shape, 0, SP_ARENA);
+  const int tw = raw_buffer(paged_attention_space(ap), SP_ARENA);
+  const Ref rq = ref(tq), rk = ref(tk >= 0 ? tk : tq), rv = ref(tv >= 0 ? tv : tq), rkc = ref(tkc), rvc = ref(tvc), rt = ref(tt), rc = ref(tc), rs = ref(ts >= 0 ? ts : tc);
+  const Ref ry = ref(ty), rw = ref(tw);
+  const bool fresh = tk >= 0, ragged = ts >= 0;
+  auto args = [=](const ExecEnv& e) {
+    PagedAttentionParams p = ap;
+    p.q = rq(e);
+    if (fresh) { p.k = rk(e); p.v = rv(e); }
+    p.k_cache = rkc(e); p.v_cache = rvc(e);
+    p.table = (const int32_t*)rt(e); p.cached = (const int32_t*)rc(e);
+    if (ragged) p.starts = (const int32_t*)rs(e);
+    p.y = ry(e); p.work = rw(e);
+    return p;
+  };
+  const std::string& name = n.out->name;
+  if (fresh)
+    emit("attend.write:" + name, {tk, tv, tt, tc, ts}, {tkc, tvc}, [=](const ExecEnv& e, hipStream_t st) { return launch_cache_write(args(e), st); }, kReads16 | kWrites16);
+  emit("attend:" + name, {tq, tkc, tvc, tt, tc, ts}, {tw, ty}, [=](const ExecEnv& e, hipStream_t st) { return launch_paged_attention(args(e), st); }, kReads16 | kWrites16);
+  emit("attend.join:" + name, {tw, tt, tc, ts}, {ty}, [=](const ExecEnv& e, hipStream_t st) { return launch_attention_join(args(e), st); }, kReads16 | kWrites16);
+  set_kept(n.out, ty);
+}
+
+void Planner::lower_logprobs(int ni) {
+  Node& n = comp_->nodes[ni];
+  const _odla_value* x = n.in[0];
+  const int tx = get(x, L_ROWMAJOR, FORM_FLOAT), tt = get(n.in[1], L_ROWMAJOR, FORM_FLOAT);
+  LogProbsParams lp;
+  lp.V = (int)x->shape.d[x->shape.rank - 1];
+  lp.rows = (int)(x->shape.numel() / lp.V);
+  lp.per_row = (int)(n.in[1]->shape.numel() / lp.rows);
+  lp.top = (int)n.i[0];
+  lp.dt = T(tx).dt;
+  const bool top = lp.top > 0;
+  const int tl = new_tensor(DT_F32, L_ROWMAJOR, n.out->shape, 0, SP_ARENA), te = new_tensor(DT_F32, L_ROWMAJOR, n.out2->shape, 0, SP_ARENA);
+  const int ta = top ? new_tensor(DT_F32, L_ROWMAJOR, n.more[0]->shape, 0, SP_ARENA) : -1;
+  const int ti = top ? new_tensor(DT_I32, L_ROWMAJOR, n.more[1]->shape, 0, SP_ARENA) : -1;
+  const int parts = log_probs_parts(lp);
+  const int tw = parts > 1 ? raw_buffer(log_probs_space(lp), SP_ARENA) : -1;
+  const Ref rx = ref(tx), rt = ref(tt), rl = ref(tl), re = ref(te), ra = ref(top ? ta : tl), ri = ref(top ? ti : tl), rw = ref(tw >= 0 ? tw : tl);
+  auto args = [=](const ExecEnv& e) {
+    LogProbsParams p = lp;
+    p.logits = rx(e);
+    p.tokens = (const int32_t*)rt(e);
+    p.log_prob = (float*)rl(e); p.entropy = (float*)re(e);
+    if (top) { p.top_log_prob = (float*)ra(e); p.top_token = (int32_t*)ri(e); }
+    if (parts > 1) p.work = rw(e);
+    return p;
+  };
+  const std::string& name = n.out->name;
+  if (parts > 1) {
+    emit_lists("logprobs:" + name, {tx}, {tw}, [=](const ExecEnv& e, hipStream_t st) { return launch_log_probs(args(e), st); }, kReads16 | kWrites16);
+    emit_lists("logprobs.join:" + name, {tx, tt, tw}, {tl, te, ta, ti}, [=](const ExecEnv& e, hipStream_t st) { return launch_log_probs_join(args(e), st); }, kReads16 | kWrites16);
+  } else {
+    emit_lists("logprobs:" + name, {tx, tt}, {tl, te, ta, ti}, [=](const ExecEnv& e, hipStream_t st) { return launch_log_probs(args(e), st); }, kReads16 | kWrites16);
+  }
+  set_kept(n.out, tl);
+  set_kept(n.out2, te);
+  if (top) { set_kept(n.more[0], ta); set_main(n.more[1], ti); }
 }
 
 void Planner::lower_topk(int ni) {

@@ -160,6 +160,9 @@ const char* api_op_name(const Node& n) {
     case OP_BLOCKGEMM: return "odla_hip_BlockGemm";
     case OP_EXPERTS: return "odla_hip_MixtureOfExperts";
     case OP_SAMPLE: return "odla_hip_Sample";
+    case OP_RMSNORM: return "odla_hip_RmsNorm";
+    case OP_PAGEDATTENTION: return "odla_hip_PagedAttention";
+    case OP_LOGPROBS: return "odla_hip_LogProbs";
     case OP_AXISOP:
       switch ((AxisOp)n.i[0]) {
         case AX_GATHER_ELEMENTS: return "odla_GatherElements";

@@ -15,6 +15,8 @@
 // passes the hash is still checked record by record (validate_loaded): shapes,
 // element types and, per operator, the operands and attributes the planner
 // will index.
+#include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <memory>
@@ -111,6 +113,10 @@ odla_status serialize(_odla_computation* c, std::vector<uint8_t>* out) {
     for (int i = 0; i < 8; ++i) w.f32(n.f[i]);
     w.i64((int64_t)n.iv.size());
     for (int64_t v : n.iv) w.i64(v);
+    if (has_more(n.op)) {
+      w.i64((int64_t)n.more.size());
+      for (const _odla_value* v : n.more) w.i64(v->index);
+    }
   }
   const uint64_t h = fnv1a(w.buf.data(), w.buf.size());
   w.raw(&h, 8);
@@ -161,6 +167,9 @@ bool op_rule(OpKind op, OpRule* r) {
     case OP_BLOCKGEMM: *r = {4, 4, ~0u, false}; return true;
     case OP_EXPERTS: *r = {6, 6, 0x17, false}; return true;
     case OP_SAMPLE: *r = {6, 6, 0x21, false}; return true;
+    case OP_RMSNORM: *r = {3, 3, 0x1, false}; return true;
+    case OP_PAGEDATTENTION: *r = {8, 8, 0x79, false}; return true;
+    case OP_LOGPROBS: *r = {2, 2, 0x3, true}; return true;
   }
   return false;
 }
@@ -185,7 +194,7 @@ odla_status validate_loaded(const _odla_computation* c) {
     if (v.kind == _odla_value::TEMP) {
       LOADED_REQUIRE(v.producer >= 0 && v.producer < nn, "value %d names producer %d", v.index, v.producer);
       const Node& p = c->nodes[(size_t)v.producer];
-      LOADED_REQUIRE(p.out == &v || p.out2 == &v, "value %d is not a result of its producer", v.index);
+      LOADED_REQUIRE(p.out == &v || p.out2 == &v || std::count(p.more.begin(), p.more.end(), &v) != 0, "value %d is not a result of its producer", v.index);
     } else {
       LOADED_REQUIRE(v.producer == -1, "argument / constant %d has a producer", v.index);
     }
@@ -362,6 +371,22 @@ odla_status validate_loaded(const _odla_computation* c) {
         LOADED_REQUIRE(n.op != OP_BLOCKQUANT || (n.out2->shape == o2 && n.out2->etype == ODLA_FLOAT32), "%s node %lld: malformed scales", name, (long long)k);
         break;
       }
+      case OP_RMSNORM: case OP_PAGEDATTENTION: case OP_LOGPROBS: {
+        std::vector<ResultType> want;
+        std::string why;
+        LOADED_REQUIRE(token_op_results(n.op, n.in, n.i, &want, &why), "%s node %lld: %s", name, (long long)k, why.c_str());
+        LOADED_REQUIRE(n.op != OP_RMSNORM || ((n.i[0] == 0 || n.i[0] == 1) && n.f[0] >= 0.f && !std::isinf(n.f[0])), "%s node %lld: malformed attributes", name, (long long)k);
+        LOADED_REQUIRE(n.op != OP_PAGEDATTENTION || std::isfinite(n.f[0]), "%s node %lld: malformed attributes", name, (long long)k);
+        std::vector<const _odla_value*> have = {n.out};
+        if (n.out2 != nullptr) have.push_back(n.out2);
+        have.insert(have.end(), n.more.begin(), n.more.end());
+        LOADED_REQUIRE(have.size() == want.size(), "%s node %lld has %zu results", name, (long long)k, have.size());
+        for (size_t j = 0; j < have.size(); ++j)
+          LOADED_REQUIRE(have[j]->shape == want[j].shape && have[j]->etype == want[j].etype && have[j]->producer == k && have[j]->kind == _odla_value::TEMP &&
+                             std::count(have.begin(), have.end(), have[j]) == 1,
+                         "%s node %lld: malformed result %zu", name, (long long)k, j);
+        break;
+      }
       case OP_TOPK:
         LOADED_REQUIRE(n.i[2] >= 0 && n.i[2] < xr && n.i[0] >= 1 && n.i[0] <= x->shape.d[n.i[2]], "TopK node %lld: bad axis or K", (long long)k);
         break;
@@ -481,6 +506,15 @@ odla_status deserialize(const uint8_t* data, size_t size, _odla_computation* c) 
     const int64_t niv = r.i64();
     if (!r.ok || niv < 0 || (size_t)niv > (r.n - r.pos) / 8) return ODLA_INVALID_PARAM;
     for (int64_t i = 0; i < niv; ++i) n.iv.push_back(r.i64());
+    if (has_more(n.op)) {
+      const int64_t nm = r.i64();
+      if (!r.ok || nm < 0 || nm > ODLA_MAX_OUTPUTS) return ODLA_INVALID_PARAM;
+      for (int64_t i = 0; i < nm; ++i) {
+        _odla_value* v = value_at(r.i64());
+        if (!r.ok || v == nullptr) return ODLA_INVALID_PARAM;
+        n.more.push_back(v);
+      }
+    }
     if (!r.ok || n.out == nullptr) return ODLA_INVALID_PARAM;
     c->nodes.push_back(std::move(n));
   }

@@ -302,6 +302,9 @@ def load_library(path=None):
     proto("odla_hip_BlockGemm", vp, [vp, vp, vp, vp, i32, cid])
     proto("odla_hip_MixtureOfExperts", vp, [vp, vp, vp, vp, vp, vp, u32, u32, f32, cid])
     proto("odla_hip_Sample", vp, [vp, vp, vp, vp, vp, vp, cid])
+    proto("odla_hip_RmsNorm", Values, [vp, vp, vp, f32, i32, ValueIds])
+    proto("odla_hip_PagedAttention", vp, [vp, vp, vp, vp, vp, vp, vp, vp, f32, u32, cid])
+    proto("odla_hip_LogProbs", Values, [vp, vp, u32, ValueIds])
     if path == LIB_PATH:
         _lib = L
     return L
@@ -721,6 +724,37 @@ class HipBuilder:
     def sample(self, logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, name=None):
         return self._ret(self.L.odla_hip_Sample(logits, temperature, top_k, top_p, min_p, uniform, _cid(name)), "odla_hip_Sample")
 
+    def _named(self, names):
+        ids = ValueIds()
+        ids.size = len(names)
+        for i, n in enumerate(names):
+            ids.value_ids[i] = _cid(n)
+        return ids
+
+    def _results(self, r, what):
+        if r.size == 0:
+            raise OdlaError("%s failed (see the library log)" % what)
+        return tuple(r.values[i] for i in range(r.size))
+
+    def rms_norm(self, x, weight=None, residual=None, epsilon=1e-6, dtype=None, names=()):
+        """-> (normalised,) or, with dtype FLOAT8_E4M3, (8-bit values, scales); with a residual x + residual as the last one.
+        dtype: the input's (default) or FLOAT8_E4M3."""
+        t = ValueType()
+        _check(self.L.odla_GetValueType(x, ctypes.byref(t)), "odla_GetValueType")
+        kind = t.element_type if dtype is None else element_type(dtype)
+        return self._results(self.L.odla_hip_RmsNorm(x, residual, weight, epsilon, kind, self._named(names)), "odla_hip_RmsNorm")
+
+    def paged_attention(self, query, key, value, key_cache, value_cache, page_table, cached, starts=None, scale=None, window=0, name=None):
+        """scale: 1 / sqrt(head size) unless given.  The caches are arguments, bound to device memory (see DeviceArray)."""
+        if scale is None:
+            scale = self.shape_of(key_cache)[0][-1] ** -0.5
+        return self._ret(self.L.odla_hip_PagedAttention(query, key, value, key_cache, value_cache, page_table, cached, starts, scale,
+                                                        int(window), _cid(name)), "odla_hip_PagedAttention")
+
+    def log_probs(self, logits, tokens, top=0, names=()):
+        """-> (log probabilities of the tokens, entropies) and, with top > 0, (.., top log probabilities, top tokens)."""
+        return self._results(self.L.odla_hip_LogProbs(logits, tokens, int(top), self._named(names)), "odla_hip_LogProbs")
+
     # -- execution --
     def session(self, use_graph=True):
         return Session(self, use_graph)
@@ -737,6 +771,28 @@ class HipBuilder:
         if self.comp:
             self.L.odla_DestroyComputation(self.comp)
             self.comp = None
+
+
+class DeviceArray:
+    """Device memory that holds a numpy array: what a cache is bound to.  In the feeds of a Session it is bound as it is."""
+
+    def __init__(self, array, lib=None):
+        a = np.ascontiguousarray(array)
+        self.L = lib or load_library()
+        self.shape, self.dtype, self.nbytes = a.shape, a.dtype, a.nbytes
+        self.ptr = ctypes.c_void_p()
+        _check(self.L.odla_AllocateDeviceMemory(ctypes.byref(self.ptr), a.nbytes), "odla_AllocateDeviceMemory")
+        _check(self.L.odla_CopyMemory(self.ptr, a.ctypes.data_as(ctypes.c_void_p), a.nbytes, ODLA_MEMCPY_H2D), "odla_CopyMemory")
+
+    def get(self):
+        o = np.empty(self.shape, self.dtype)
+        _check(self.L.odla_CopyMemory(o.ctypes.data_as(ctypes.c_void_p), self.ptr, self.nbytes, ODLA_MEMCPY_D2H), "odla_CopyMemory")
+        return o
+
+    def close(self):
+        if self.ptr:
+            self.L.odla_FreeDeviceMemory(self.ptr)
+            self.ptr = None
 
 
 class Session:
@@ -764,9 +820,14 @@ class Session:
         return tuple(s.dims[:s.size])
 
     def run(self, feeds):
-        """feeds: name -> numpy array.  Returns name -> numpy array."""
+        """feeds: name -> numpy array or DeviceArray.  Returns name -> numpy array."""
         keep = []
         for name, (h, shape, dt) in self.b.args.items():
+            if isinstance(feeds[name], DeviceArray):
+                d = feeds[name]
+                assert d.shape == self.runtime_shape(h) and d.dtype == dt, (name, d.shape, d.dtype)
+                _check(self.L.odla_BindToArgument(h, d.ptr, self.ctx), "odla_BindToArgument")
+                continue
             a = np.ascontiguousarray(feeds[name], dtype=dt)
             assert tuple(a.shape) == self.runtime_shape(h), (name, a.shape, self.runtime_shape(h))
             keep.append(a)

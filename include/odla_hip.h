@@ -63,8 +63,8 @@ typedef enum {
  * point with 4 exponent bits (bias 7) and 3 mantissa bits, one byte per element.
  * No infinity; 0x7f / 0xff are NaN, the largest magnitude is 448, the smallest
  * 2^-9.  Values of this type are arguments, constants and results of
- * odla_hip_BlockQuantize; odla_hip_BlockGemm and odla_hip_MixtureOfExperts
- * compute with them, odla_Reshape, odla_Squeeze, odla_Transpose, odla_Slice,
+ * odla_hip_BlockQuantize and odla_hip_RmsNorm; odla_hip_BlockGemm and
+ * odla_hip_MixtureOfExperts compute with them, odla_Reshape, odla_Squeeze, odla_Transpose, odla_Slice,
  * odla_Concat and odla_Gather move them.  Every other operator refuses them. */
 #define ODLA_HIP_FLOAT8_E4M3 ((odla_element_type)31)
 
@@ -895,6 +895,84 @@ odla_value odla_hip_MixtureOfExperts(odla_value input, odla_value router,
 odla_value odla_hip_Sample(odla_value logits, odla_value temperature,
                            odla_value top_k, odla_value top_p, odla_value min_p,
                            odla_value uniform, const odla_value_id value_id);
+/* Rows normalised by their root mean square.  For every row of `input` [.., K]
+ *   s = input + residual (null: input alone),
+ *   y = s / sqrt(mean of s^2 + epsilon) * weight (null: ones).
+ * residual has the input's type and shape; weight has K elements, FLOAT32 or of
+ * the input's type.  result_type is the input's type, or ODLA_HIP_FLOAT8_E4M3:
+ * then y is quantised as odla_hip_BlockQuantize does, without being rounded to
+ * another type before.  Results in this order: y (or its 8-bit values, then their
+ * scales, FLOAT32 [.., ceil(K / 128)]), then, with a residual, s in the input's
+ * type.  Sums are kept in 32 bits and s is not rounded before it is normalised.
+ * epsilon is finite and not negative; a row of zeros with epsilon 0 gives NaN,
+ * as the formula does, and so does a row with a NaN.  An infinity gives NaN in its
+ * place and zeros beside it; so do, without the NaN, values whose squares add up
+ * beyond the range of 32 bits.  The weight is stored as the precision mode says,
+ * the scales are kept as fp32 as those of odla_hip_BlockQuantize are. */
+odla_values odla_hip_RmsNorm(odla_value input, odla_value residual,
+                             odla_value weight, odla_float32 epsilon,
+                             odla_element_type result_type,
+                             const odla_value_ids value_ids);
+/* Attention of new tokens over keys and values in pages of a cache, which it
+ * extends by the new tokens' own.
+ *   query      [T, Hq, D] or [T, Hq * D]: T new tokens, those of sequence 0 first
+ *   key, value [T, H, D] or [T, H * D], H a divisor of Hq: query head h reads
+ *              head h / (Hq / H)
+ *   key_cache, value_cache [pages, page size, H, D]: two arguments
+ *   page_table INT32 [B, P]: token p of sequence b lies in page
+ *              page_table[b][p / page size], at p % page size
+ *   cached     INT32 [B]: tokens of sequence b in the caches before the call
+ *   starts     INT32 [B + 1], not decreasing: sequence b has the new tokens
+ *              starts[b] .. starts[b + 1] - 1; null: T / B tokens each
+ * New token i of sequence b has place p = cached[b] + i.  Its key and value are
+ * written to that place of the caches, and
+ *   y = sum_j softmax_j(scale * query . key_j) value_j over places j <= p, with
+ *   window > 0 over the last `window` of them alone.
+ * The result has the shape and type of the query; all float operands are of one
+ * type.  D is a multiple of 8 up to 256, a page may have any size, B <= 65536,
+ * P * page size <= 2^30, pages * page size < 2^31.
+ * key and value may both be null: the new tokens' own are in the caches already
+ * (written by another operator of the computation, or by an earlier call).
+ * The caches are extended where the caller has them: both are bound to 16-byte
+ * aligned memory of the current device (host memory is refused by the execution),
+ * may be operands of odla_hip_PagedAttention only, several of them if wanted, and
+ * are no outputs; they keep their declared type in every precision mode.  What no
+ * new token is written to stays as it was.  Two executions that write the same
+ * pages at the same time race; no page may be in two places that one execution
+ * writes.
+ * Nothing outside the operands is read or written whatever they hold: a page
+ * outside 0 .. pages - 1, or a place that the page table does not reach, is
+ * neither written nor seen; cached is clamped to 0 .. P * page size and starts to
+ * 0 .. T (decreasing ones give results without meaning).  Tokens of no sequence, and
+ * those that see no place at all, give zeros.  Keys and values in places that a
+ * token does not see have no influence, whatever they hold.
+ * Scores, softmax and sums are kept in 32 bits; with 16-bit operands the weights
+ * are rounded to their type before they meet the values.  The last bits of a row
+ * depend on the sizes of the call; the same operands give the same bits on every
+ * run. */
+odla_value odla_hip_PagedAttention(odla_value query, odla_value key,
+                                   odla_value value, odla_value key_cache,
+                                   odla_value value_cache,
+                                   odla_value page_table, odla_value cached,
+                                   odla_value starts, odla_float32 scale,
+                                   odla_uint32 window,
+                                   const odla_value_id value_id);
+/* Log probabilities of given tokens, with the entropy and the best alternatives,
+ * for every row of `logits` [.., V], V <= 524288:
+ *   log p_i = l_i - log sum_j exp(l_j),   entropy = - sum_i p_i log p_i.
+ * tokens: INT32, n = 1 .. 64 for every row (its element count is n times the
+ * rows).  Results: log p of the tokens, FLOAT32 in their shape; the entropies,
+ * FLOAT32 [..]; and, with top > 0 (at most min(V, 32)), the log p of the `top`
+ * largest logits, FLOAT32 [.., top], and their indices, INT32 [.., top], best
+ * first, equal logits by ascending index.
+ * A token outside 0 .. V - 1 has log p = -inf.  NaN logits count as -inf; a row
+ * with nothing above -inf has log p = -inf throughout, entropy 0 and indices -1;
+ * in a row with infinite logits those share the probability.  An alternative
+ * with logit -inf has log p = -inf and index -1.  Sums are kept in 32 bits without
+ * the largest term, which is 1, so that log p of nearly certain tokens keeps its
+ * digits; results are FLOAT32 in every precision mode. */
+odla_values odla_hip_LogProbs(odla_value logits, odla_value tokens,
+                              odla_uint32 top, const odla_value_ids value_ids);
 
 /* ------------------------------------------------------------------------ */
 /* Stored computations and executables.  What is stored is the recorded       */

@@ -1,0 +1,426 @@
+"""odla_hip_PagedAttention against the formula in 64 bits: head layouts, lengths, page sizes, windows, odd operands; the
+caches as they are afterwards; captured and replayed, stored, in the precision modes."""
+import numpy as np
+import pytest
+
+import layer_ops_ref as L
+import token_ops_ref as R
+from test_gpu_token_ops import np_kind
+from util import announce
+
+pytestmark = pytest.mark.gpu
+
+KINDS = ["fp32", "fp16", "bf16"]
+
+
+class Case:
+    """Operands of a call; garbage wherever no token of a sequence lies."""
+
+    def __init__(self, kind, new, cached, heads=2, group=2, d=32, page=16, spare=2, seed=0, starts=True, fresh=True, tail=0, window=0, scale=None, junk=None):
+        rng = np.random.default_rng(seed)
+        self.kind, self.window, self.fresh = kind, window, fresh
+        self.scale = d ** -0.5 if scale is None else scale
+        new, cached = list(new), list(cached)
+        b, t = len(new), sum(new) + tail
+        owned = [-(-(n + c) // page) for n, c in zip(new, cached)]
+        pages = max(1, sum(owned) + spare)
+        order = rng.permutation(pages)
+        self.table = np.full((b, max(owned + [1]) + 1), -1, np.int32)
+        ends = np.cumsum([0] + owned)
+        for i, n in enumerate(owned):
+            self.table[i, :n] = order[ends[i]:ends[i] + n]
+        bits = lambda *shape: R.to_bits(rng.standard_normal(shape), kind)
+        self.q, self.k, self.v = bits(t, heads * group, d), bits(t, heads, d), bits(t, heads, d)
+        self.kc, self.vc = bits(pages, page, heads, d), bits(pages, page, heads, d)
+        self.cached = np.array(cached, np.int32)
+        self.starts = np.cumsum([0] + new).astype(np.int32) if starts else None
+        if not fresh:      # the new tokens lie in the caches already
+            for i, (n, c) in enumerate(zip(new, cached)):
+                for j in range(n):
+                    at = (self.table[i, (c + j) // page], (c + j) % page)
+                    self.kc[at], self.vc[at] = self.k[sum(new[:i]) + j], self.v[sum(new[:i]) + j]
+        if junk is not None:   # places that no sequence owns
+            mine = np.zeros((pages, page), bool)
+            for i, (n, c) in enumerate(zip(new, cached)):
+                for p in range(c + n):
+                    mine[self.table[i, p // page], p % page] = True
+            for cache in (self.kc, self.vc):
+                cache[~mine] = R.to_bits(np.full(cache[~mine].shape, junk), kind)
+
+    def record(self, odla, b, mode_kind=None):
+        kind = np_kind(odla, mode_kind or self.kind)
+        args = {"q": self.q, "k": self.k, "v": self.v, "kc": self.kc, "vc": self.vc}
+        h = {n: b.arg(n, a.shape, kind) for n, a in args.items() if self.fresh or n not in "kv"}
+        return b.paged_attention(h["q"], h.get("k"), h.get("v"), h["kc"], h["vc"], b.arg("pt", self.table.shape, np.int32), b.arg("n", self.cached.shape, np.int32),
+                                 None if self.starts is None else b.arg("s", self.starts.shape, np.int32), self.scale, self.window, "y")
+
+    def feeds(self, odla):
+        f = {"q": self.q, "pt": self.table, "n": self.cached, "kc": odla.DeviceArray(self.kc), "vc": odla.DeviceArray(self.vc)}
+        if self.fresh:
+            f.update(k=self.k, v=self.v)
+        if self.starts is not None:
+            f["s"] = self.starts
+        return f
+
+    def written(self):
+        """Both caches' bits afterwards: what no token is written to stays as it was."""
+        kc, vc = self.kc.copy(), self.vc.copy()
+        pages, page = kc.shape[:2]
+        starts = np.arange(len(self.cached) + 1) * (len(self.q) // len(self.cached)) if self.starts is None else self.starts
+        for i, row in enumerate(self.table):
+            before = min(max(int(self.cached[i]), 0), len(row) * page)
+            for j in range(starts[i], starts[i + 1]):
+                place = before + j - starts[i]
+                if self.fresh and place < len(row) * page and 0 <= row[place // page] < pages:
+                    kc[row[place // page], place % page], vc[row[place // page], place % page] = self.k[j], self.v[j]
+        return kc, vc
+
+    def want(self):
+        v = lambda a: R.values(a, self.kind)
+        return L.paged_attention(v(self.q), v(self.k) if self.fresh else None, v(self.v), v(self.kc), v(self.vc), self.table, self.cached, self.starts,
+                                 self.scale, self.window, self.kind)
+
+
+def run(odla, c, repeats=1, **mode):
+    """Result bits and both caches' bits; executed `repeats` times (the same tokens to the same places)."""
+    b = odla.HipBuilder(**mode)
+    feeds = c.feeds(odla)
+    try:
+        b.output(c.record(odla, b), "y")
+        s = b.session()
+        try:
+            first = None
+            for _ in range(repeats):
+                y = s.run(feeds)["y"]
+                assert first is None or np.array_equal(y, first)
+                first = y
+        finally:
+            s.close()
+        return y, feeds["kc"].get(), feeds["vc"].get()
+    finally:
+        feeds["kc"].close()
+        feeds["vc"].close()
+        b.destroy()
+
+
+def check(odla, c, **kw):
+    y, kc, vc = run(odla, c, **kw)
+    want, bound, _, _ = c.want()
+    kc_want, vc_want = c.written()
+    assert np.array_equal(kc.view(np.uint8), kc_want.view(np.uint8)) and np.array_equal(vc.view(np.uint8), vc_want.view(np.uint8))
+    have = R.values(y, c.kind)
+    with np.errstate(invalid="ignore"):
+        off = np.abs(have - want)
+    assert np.all((off <= bound) | (have == want)), "%d of %d off, worst %g of its bound" % (np.sum(off > bound), off.size, np.nanmax(off / np.maximum(bound, 1e-300)))
+    return y
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("d", [8, 64, 72, 128, 136, 256])
+@pytest.mark.parametrize("heads,group", [(1, 1), (2, 4), (1, 16), (3, 5), (2, 20)])
+def test_heads(odla, kind, d, heads, group):
+    announce("paged attention %s heads %d x %d of %d" % (kind, heads, group, d))
+    check(odla, Case(kind, [1, 3, 1], [40, 0, 75], heads, group, d, seed=d + group))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("page", [1, 3, 16, 20, 64, 1000])
+def test_pages(odla, kind, page):
+    announce("paged attention %s pages of %d" % (kind, page))
+    check(odla, Case(kind, [1, 9, 2, 1], [130, 33, 0, 64], page=page, seed=page, d=64))
+
+
+LENGTHS = [([1], [0]), ([1], [1]), ([1], [31]), ([1], [32]), ([1], [4095]), ([2], [15]), ([16], [0]), ([17], [0]), ([33], [100]), ([64], [0]), ([65], [63]),
+           ([129], [0]), ([300], [500]), ([1, 1, 1, 1], [5, 2000, 0, 300]), ([40, 1, 1, 7], [0, 900, 33, 256]), ([0, 5, 0, 0, 1, 0], [10, 20, 0, 700, 3, 0])]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new,cached", LENGTHS)
+def test_lengths(odla, kind, new, cached):
+    announce("paged attention %s new %s cached %s" % (kind, new, cached))
+    check(odla, Case(kind, new, cached, 2, 4, 64, seed=sum(new) + sum(cached)))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("window", [1, 2, 31, 32, 100, 1000, 2 ** 31 - 1])
+def test_windows(odla, kind, window):
+    announce("paged attention %s window %d" % (kind, window))
+    check(odla, Case(kind, [1, 50, 150, 1], [300, 0, 40, 2000], 1, 3, 64, page=20, window=window, seed=window % 1000))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_many_sequences(odla, kind):
+    """More than a wavefront has lanes, some of them without new tokens."""
+    announce("paged attention %s of 150 sequences" % kind)
+    rng = np.random.default_rng(4)
+    check(odla, Case(kind, rng.integers(0, 4, 150), rng.integers(0, 200, 150), 2, 2, 16, page=7, seed=9))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_long_sequences_are_cut(odla, kind):
+    announce("paged attention %s over 20000 places" % kind)
+    check(odla, Case(kind, [1, 2], [20000, 7000], 1, 4, 64, page=32, seed=3), repeats=2)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_equal_sequences_need_no_starts(odla, kind):
+    announce("paged attention %s without starts" % kind)
+    check(odla, Case(kind, [3, 3, 3, 3], [0, 100, 7, 64], starts=False, seed=1))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new,cached", [([1, 1], [70, 400]), ([40, 3], [0, 50])])
+def test_keys_that_lie_in_the_cache_already(odla, kind, new, cached):
+    announce("paged attention %s without new keys" % kind)
+    check(odla, Case(kind, new, cached, fresh=False, seed=2))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new", [[1, 1], [3, 40], [150, 1]])
+def test_tokens_of_no_sequence_give_zeros(odla, kind, new):
+    announce("paged attention %s with tokens behind the last sequence" % kind)
+    c = Case(kind, new, [30, 5], tail=6, seed=2)
+    y = check(odla, c)
+    assert not np.any(R.values(y[sum(new):], kind))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("junk", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("new,window", [([1, 1, 2], 0), ([30, 5, 1], 0), ([140, 1, 1], 60)])
+def test_what_no_token_owns_has_no_influence(odla, kind, junk, new, window):
+    announce("paged attention %s beside %s" % (kind, junk))
+    check(odla, Case(kind, new, [40, 3, 0], 1, 4, 64, junk=junk, window=window, seed=5))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [12, 150])
+@pytest.mark.parametrize("window", [0, 5])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_keys_and_values_reach_the_tokens_that_see_them_alone(odla, kind, n, window, bad):
+    """An infinite or missing value (or key) of one token: tokens in front of it, and those whose window has left it behind,
+    are as if it were not there."""
+    announce("paged attention %s, %d tokens, window %d, one %s" % (kind, n, window, bad))
+    for part in ("v", "k"):
+        c = Case(kind, [n], [3], 1, 2, 64, window=window, seed=6)
+        at = n // 2
+        getattr(c, part)[at, 0, 7] = R.to_bits(np.full(1, bad), kind)[0]
+        y, kc, vc = run(odla, c)
+        with np.errstate(invalid="ignore"):
+            want, bound, _, _ = c.want()
+        have = R.values(y, kind)
+        sees = np.zeros(n, bool)
+        sees[at:at + window if window else n] = True
+        assert np.all(np.abs(have[~sees] - want[~sees]) <= bound[~sees]), part
+        if part == "v":
+            assert not np.any(np.isfinite(have[sees][:, :, 7]))
+            if np.isinf(bad):
+                assert np.all(have[sees][:, :, 7] == np.inf)
+            rest = [i for i in range(64) if i != 7]
+            assert np.all(np.abs(have[sees][:, :, rest] - want[sees][:, :, rest]) <= bound[sees][:, :, rest])
+        elif np.isnan(bad):
+            assert np.all(np.isnan(have[sees]))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new", [[1, 1, 1], [20, 140, 1]])
+def test_pages_that_do_not_exist_are_neither_written_nor_seen(odla, kind, new):
+    announce("paged attention %s with pages out of range" % kind)
+    c = Case(kind, new, [70, 40, 9], 1, 4, 64, seed=8)
+    pages = c.kc.shape[0]
+    c.table[0, 1] = pages
+    c.table[0, 3] = -5
+    c.table[1, 0] = 2 ** 31 - 1
+    c.table[1, 4] = -2 ** 31
+    c.table[2] = -1                       # nothing of the last sequence exists
+    y = check(odla, c)
+    assert not np.any(R.values(y[sum(new[:2]):], kind))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_lengths_beyond_the_table(odla, kind):
+    """Places that the page table does not reach are neither written nor seen, negative lengths are none."""
+    announce("paged attention %s with lengths out of range" % kind)
+    c = Case(kind, [2, 3, 1], [30, 0, 60], 1, 2, 32, seed=8)
+    reach = c.table.shape[1] * 16
+    c.table[:] = np.random.default_rng(1).permutation(c.kc.shape[0])[np.arange(c.table.size) % c.kc.shape[0]].reshape(c.table.shape)
+    for i in range(3):                    # a page in one sequence each
+        c.table[i] = np.where(np.arange(c.table.size).reshape(c.table.shape)[i] < c.kc.shape[0], c.table[i], -1)
+    c.cached[:] = [reach - 1, -7, 2 ** 31 - 1]
+    check(odla, c)
+
+
+def test_starts_out_of_range_stay_inside(odla):
+    """Starts are clamped to the tokens that there are; what decreasing ones give has no meaning, but every launch ends inside
+    its operands."""
+    announce("paged attention with starts out of range")
+    c = Case("bf16", [4, 4], [20, 3], 1, 2, 32, seed=8)
+    c.starts = np.array([-3, 4, 1000], np.int32)
+    y = run(odla, c)[0]
+    c.starts = np.array([0, 4, 8], np.int32)
+    assert np.array_equal(y, run(odla, c)[0])
+    for odd in ([5, 2, 7], [8, 8, 0], [2 ** 31 - 1, -2 ** 31, 4]):
+        c.starts = np.array(odd, np.int32)
+        run(odla, c)
+
+
+def test_scales(odla):
+    announce("paged attention with other scales")
+    for scale in (0.0, -0.3, 1.0, 30.0):
+        check(odla, Case("fp32", [1, 5], [60, 3], d=16, scale=scale, seed=2))
+        check(odla, Case("bf16", [1, 50], [60, 3], d=16, scale=scale, seed=2))
+
+
+def test_captured_and_replayed(odla):
+    """Graphs of several sets of buffers in turn, each with its own caches."""
+    announce("paged attention captured for three sets of caches")
+    cases = [Case("bf16", [1, 1, 4], [100, 7, 30], seed=s) for s in range(3)]
+    b = odla.HipBuilder()
+    feeds = [c.feeds(odla) for c in cases]
+    b.output(cases[0].record(odla, b), "y")
+    s = b.session()
+    for k in (0, 1, 0, 2, 1, 2, 0):
+        f = dict(feeds[k], pt=cases[k].table)
+        have = R.values(s.run(f)["y"], "bf16")
+        want, bound, kc, vc = cases[k].want()
+        assert np.all(np.abs(have - want) <= bound), k
+        assert np.array_equal(R.values(f["kc"].get(), "bf16"), kc)
+    s.close()
+    b.destroy()
+    for f in feeds:
+        f["kc"].close()
+        f["vc"].close()
+
+
+def test_a_sequence_grows(odla):
+    """A prompt, then token after token, each execution extending the cache of the last: as one attention over all of them."""
+    announce("paged attention, a prompt and twelve tokens behind it")
+    kind, n, more, h, g, d, page = "fp32", 21, 12, 2, 3, 32, 4
+    whole = Case(kind, [n + more], [0], h, g, d, page, seed=7)
+    want, bound, kc, vc = whole.want()
+    kc0, vc0 = odla.DeviceArray(whole.kc), odla.DeviceArray(whole.vc)
+    got = []
+    for first, t in [(0, n)] + [(n + i, 1) for i in range(more)]:
+        part = Case(kind, [t], [first], h, g, d, page, seed=1)
+        part.q, part.k, part.v = (a[first:first + t] for a in (whole.q, whole.k, whole.v))
+        part.kc, part.vc, part.table = whole.kc, whole.vc, whole.table
+        b = odla.HipBuilder()
+        b.output(part.record(odla, b), "y")
+        s = b.session()
+        got.append(s.run({"q": part.q, "k": part.k, "v": part.v, "kc": kc0, "vc": vc0, "pt": part.table, "n": part.cached, "s": part.starts})["y"])
+        s.close()
+        b.destroy()
+    assert np.all(np.abs(np.concatenate(got) - want) <= bound)
+    assert np.array_equal(kc0.get(), kc) and np.array_equal(vc0.get(), vc)
+    kc0.close()
+    vc0.close()
+
+
+@pytest.mark.parametrize("mode", [{"fp16": True}, {"bf16": True}, {"bf16": "accuracy"}])
+def test_precision_modes_leave_caches_as_they_are_declared(odla, mode):
+    """FLOAT32 caches stay fp32 in the modes that store other values in 16 bits, and bf16 ones bf16."""
+    announce("paged attention, FLOAT32 caches, %s" % mode)
+    kind = "fp16" if "fp16" in mode else "bf16"
+    c = Case("fp32", [1, 6], [50, 3], seed=3)
+    for n in "qkv":
+        setattr(c, n, R.values(R.to_bits(getattr(c, n), kind), kind).astype(np.float32))     # (values that the mode's type holds)
+    check(odla, c, **mode)
+    check(odla, Case("bf16", [1, 6], [50, 3], seed=3), **mode)
+
+
+def test_two_attentions_share_a_cache(odla):
+    """The second reads what the first has written."""
+    announce("two attentions over one cache")
+    c = Case("bf16", [2, 1], [20, 40], seed=3)
+    b = odla.HipBuilder()
+    y = c.record(odla, b)
+    b.output(y, "y")
+    q2 = R.to_bits(np.random.default_rng(8).standard_normal(c.q.shape), "bf16")
+    h = lambda n: b.args[n][0]
+    b.output(b.paged_attention(b.arg("q2", q2.shape, odla.BFLOAT16), None, None, h("kc"), h("vc"), h("pt"), h("n"), h("s"), c.scale, name="y2"), "y2")
+    feeds = dict(c.feeds(odla), q2=q2)
+    s = b.session()
+    got = s.run(feeds)
+    s.close()
+    b.destroy()
+    want, bound, _, _ = c.want()
+    assert np.all(np.abs(R.values(got["y"], "bf16") - want) <= bound)
+    c.q = q2
+    want, bound, _, _ = c.want()
+    assert np.all(np.abs(R.values(got["y2"], "bf16") - want) <= bound)
+    feeds["kc"].close()
+    feeds["vc"].close()
+
+
+def test_caches_that_cannot_be_extended_are_refused(odla):
+    """Host memory, an address that is not aligned, and one buffer for both."""
+    announce("caches that are refused")
+    c = Case("bf16", [1], [5], seed=3)
+    b = odla.HipBuilder()
+    b.L.odla_SetLogLevel(0)
+    b.output(c.record(odla, b), "y")
+    s = b.session()
+    feeds = c.feeds(odla)
+    good = dict(feeds)
+    import ctypes
+    off = odla.DeviceArray(np.zeros(c.kc.nbytes + 64, np.uint8))
+    try:
+        for bad in (c.kc, feeds["vc"]):
+            with pytest.raises(odla.OdlaError):
+                s.run(dict(feeds, kc=bad))
+        s.run(good)
+        assert b.L.odla_BindToArgument(b.args["kc"][0], ctypes.c_void_p(off.ptr.value + 8), s.ctx) == 0
+        with pytest.raises(odla.OdlaError):
+            s.execute()
+        s.run(good)
+    finally:
+        b.L.odla_SetLogLevel(2)
+        s.close()
+        b.destroy()
+        off.close()
+        feeds["kc"].close()
+        feeds["vc"].close()
+
+
+def test_static_execution(odla):
+    """odla_hip_ExecuteComputationStatic extends the caches in place too."""
+    announce("paged attention through the static entry point")
+    c = Case("bf16", [1, 3], [50, 3], seed=3)
+    b = odla.HipBuilder()
+    b.output(c.record(odla, b), "y")
+    s = b.session()
+    feeds = c.feeds(odla)
+    y = s.run(feeds)["y"]
+    out = np.zeros_like(y)
+    assert b.L.odla_BindToOutput(b.outs["y"][0], out.ctypes.data, s.ctx) == 0
+    held = [np.ascontiguousarray(a) for a in (c.q, c.k, c.v, c.table, c.cached, c.starts)]
+    for n, a in zip(("q", "k", "v", "pt", "n", "s"), held):
+        assert b.L.odla_BindToArgument(b.args[n][0], a.ctypes.data, s.ctx) == 0
+    assert s.execute_static() == 0
+    assert np.array_equal(out, y)
+    s.close()
+    b.destroy()
+    feeds["kc"].close()
+    feeds["vc"].close()
+
+
+@pytest.mark.parametrize("batch", [1, 3, 8])
+def test_dynamic_batch(odla, batch):
+    announce("paged attention at batch %d of up to 8" % batch)
+    whole = Case("bf16", [1] * 8, [5, 60, 0, 33, 200, 1, 16, 15], starts=False, seed=3)
+    b = odla.HipBuilder(max_batch=8)
+    kind = odla.BFLOAT16
+    row = lambda n, a, t=kind: b.arg(n, (-1,) + a.shape[1:], t)
+    b.output(b.paged_attention(row("q", whole.q), row("k", whole.k), row("v", whole.v), b.arg("kc", whole.kc.shape, kind), b.arg("vc", whole.vc.shape, kind),
+                               row("pt", whole.table, np.int32), row("n", whole.cached, np.int32), scale=whole.scale), "y")
+    s = b.session()
+    s.set_batch(batch)
+    feeds = whole.feeds(odla)
+    for n in ("q", "k", "v", "pt", "n"):
+        feeds[n] = feeds[n][:batch]
+    got = R.values(s.run(feeds)["y"], "bf16")
+    want, bound, _, _ = whole.want()
+    assert np.all(np.abs(got - want[:batch]) <= bound[:batch])
+    s.close()
+    b.destroy()
+    feeds["kc"].close()
+    feeds["vc"].close()
