@@ -42,18 +42,34 @@ OHIP_HD int cache_row(const int page_index, const int in_page, const int page, c
   return page_index >= 0 && page_index < pages ? page_index * page + in_page : -1;
 }
 
-// A call's pieces: the tiles of `rows` rows of every sequence, each with the keys cut into stretches of `stretch`
-// tiles.  `target` stretches at most come from cutting: stretch >= work / target.
-constexpr int kTargetPieces = 1024;
-OHIP_HD int row_tiles(const SeqSpan& s, const int rows, const int group) { return (int)(((long long)s.n * group + rows - 1) / rows); }
-OHIP_HD int stretch_of(const float work, const int least) { return at_least((int)(work / (float)kTargetPieces) + 1, least); }
-OHIP_HD int stretches(const int tiles, const int stretch) { return tiles > 0 ? (tiles - 1) / stretch + 1 : 1; }
-// Bounds over all calls of one size: pieces in all, and pieces of tiles that are cut (their parts have a slot each).
-// (Cut: a tile of k > stretch key tiles gives at most 2 k / stretch parts.  An eighth on top: `work` is a sum in fp32.)
-OHIP_HD long long most_units(const int tokens, const int seqs, const int heads, const int group, const int rows) {
-  return (long long)heads * (at_most(seqs, tokens) + (long long)tokens * group / rows);
+// A call's pieces.  A sequence is cut one of two ways, by how many rows a head of keys has in it: into tiles of `rows`
+// rows, each with its keys in stretches of a number of key tiles of `keys` places that follows from the lengths of all
+// sequences of its way: `target` pieces at most come from cutting (stretch >= work / target), none shorter than `least`.
+struct Way { int rows, keys, least, target; };
+OHIP_HD int row_tiles(const SeqSpan& s, const Way& w, const int group) { return (int)(((long long)s.n * group + w.rows - 1) / w.rows); }
+OHIP_HD int key_tiles(const SeqSpan& s, const Way& w, const int group, const int window) { return most_key_tiles(s, w.rows, group, window, w.keys); }
+OHIP_HD float work_of(const SeqSpan& s, const Way& w, const int group, const int heads, const int window) {
+  return (float)row_tiles(s, w, group) * (float)heads * (float)key_tiles(s, w, group, window);
 }
-constexpr int kMostCutPieces = kTargetPieces + kTargetPieces / 8, kMostSlots = 2 * kMostCutPieces;
+OHIP_HD int stretch_of(const float work, const Way& w) { return at_least((int)(work / (float)w.target) + 1, w.least); }
+OHIP_HD int stretches(const int tiles, const int stretch) { return tiles > 0 ? (tiles - 1) / stretch + 1 : 1; }
+// Bounds over all calls of one size: pieces that come from cutting, and pieces of tiles that are cut (their parts have
+// a slot each).  (Cut: a tile of k > stretch key tiles gives at most 2 k / stretch parts.  An eighth on top: the work
+// is a sum in fp32.)
+OHIP_HD int most_cut_pieces(const Way& w) { return w.target + w.target / 8; }
+OHIP_HD int most_slots(const Way& w) { return 2 * most_cut_pieces(w); }
+
+// Sequences of up to kFewRows rows go in tiles of 16, others in tiles of 128 (16-bit types; fp32: all in tiles of 16).
+constexpr int kFewRows = 32;
+constexpr Way kFew16 = {16, 32, 8, 1024}, kFew32 = {16, 16, 16, 1024}, kMany = {128, 64, 8, 256}, kManyWide = {128, 32, 16, 256};   // (wide: heads above 128)
+OHIP_HD bool is_many(const SeqSpan& s, const int group) { return (long long)s.n * group > kFewRows; }
+OHIP_HD long long most_few_units(const int tokens, const int seqs, const int heads, const int group, const bool all) {
+  const long long each = at_most(seqs, tokens);
+  return heads * (all ? each + (long long)tokens * group / 16 : each * (kFewRows / 16));
+}
+OHIP_HD long long most_many_units(const int tokens, const int seqs, const int heads, const int group) {
+  return (long long)tokens * group <= kFewRows ? 0 : heads * (at_most(seqs, tokens) + (long long)tokens * group / 128);
+}
 
 }  // namespace ohip
 #endif

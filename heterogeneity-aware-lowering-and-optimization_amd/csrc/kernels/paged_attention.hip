@@ -11,6 +11,8 @@
 #include "block_common.h"
 #include "attention_pieces.h"
 
+#include <algorithm>
+
 namespace ohip {
 namespace {
 
@@ -19,6 +21,7 @@ constexpr float kLog2e = 1.44269504f;
 struct Args : PagedAttentionParams {
   unsigned page_magic; int page_shift;
   int reach;          // places of a row of the page table
+  int few_slots, many_slots;
 };
 
 template <int CTRL, int ROWS>
@@ -54,54 +57,91 @@ __device__ __forceinline__ SeqSpan span_from_lane(const SeqSpan& s, const int la
   return {__builtin_amdgcn_readlane(s.first, lane), __builtin_amdgcn_readlane(s.n, lane), __builtin_amdgcn_readlane(s.cached, lane), __builtin_amdgcn_readlane(s.len, lane)};
 }
 
+// The two ways of a type (fp32 has one).
+template <typename T, bool WIDE> struct Ways {
+  static constexpr bool kTwo = sizeof(T) == 2;
+  static constexpr Way few = kTwo ? kFew16 : kFew32, many = WIDE ? kManyWide : kMany;
+};
+
 // A sequence, how its tiles are cut, and where its pieces and the slots of its parts begin.
-struct Found { int seq, cuts, stretch, tiles, piece0, slot0; SeqSpan span; };
+struct Found { int seq, cuts, stretch, tiles, piece0, slot0; bool many; SeqSpan span; };
+constexpr Found kNowhere = {-1, 1, 0, 0, 0, 0, false, {0, 0, 0, 0}};
 // The sequence with piece `key` (or, BY_TOKEN, with the new token `key`), by all lanes of a wavefront together; seq < 0: none.
-template <int R, int KT, int LEAST, bool BY_TOKEN>
+// Pieces of the sequences with many rows, which take longest, come first.
+template <typename T, bool WIDE, bool BY_TOKEN>
 __device__ __forceinline__ Found find(const Args& a, const int key) {
+  using W = Ways<T, WIDE>;
   const int lane = threadIdx.x & 63;
-  float work = 0.f;
+  SeqSpan s = span_of(a, lane);      // (of the first 64: kept)
+  float work[2] = {0.f, 0.f};        // few, many
   for (int b0 = 0; b0 < a.seqs; b0 += 64) {
-    const SeqSpan s = span_of(a, b0 + lane);
-    work += wave_sum((float)row_tiles(s, R, a.group) * (float)a.kv_heads * (float)most_key_tiles(s, R, a.group, a.window, KT));
+    const SeqSpan t = b0 == 0 ? s : span_of(a, b0 + lane);
+    const bool many = W::kTwo && is_many(t, a.group);
+    work[0] += wave_sum(many ? 0.f : work_of(t, W::few, a.group, a.kv_heads, a.window));
+    if (W::kTwo) work[1] += wave_sum(many ? work_of(t, W::many, a.group, a.kv_heads, a.window) : 0.f);
   }
-  const int stretch = stretch_of(work, LEAST);
-  int piece0 = 0, slot0 = 0;
-  for (int b0 = 0; b0 < a.seqs; b0 += 64) {
-    const SeqSpan s = span_of(a, b0 + lane);
-    const int cuts = stretches(most_key_tiles(s, R, a.group, a.window, KT), stretch);
-    const int pieces = row_tiles(s, R, a.group) * a.kv_heads * cuts, slots = cuts > 1 ? pieces : 0;
-    const int piece_end = piece0 + wave_scan(pieces), slot_end = slot0 + wave_scan(slots);
-    const unsigned long long here = BY_TOKEN ? __ballot(key >= s.first && key < s.first + s.n) : __ballot(key < piece_end);
-    if (here != 0) {
-      const int at = __builtin_ctzll(here);
-      Found f;
-      f.seq = b0 + at;
-      f.span = span_from_lane(s, at);
-      f.cuts = __builtin_amdgcn_readlane(cuts, at);
-      f.stretch = stretch;
-      f.tiles = row_tiles(f.span, R, a.group);
-      f.piece0 = __builtin_amdgcn_readlane(piece_end - pieces, at);
-      f.slot0 = __builtin_amdgcn_readlane(slot_end - slots, at);
-      return f;
+  int piece0 = 0;
+  for (int way = W::kTwo ? 1 : 0; way >= 0; --way) {
+    const Way w = way ? W::many : W::few;
+    const int stretch = stretch_of(work[way], w);
+    int slot0 = 0;
+    for (int b0 = 0; b0 < a.seqs; b0 += 64) {
+      const SeqSpan t = b0 == 0 ? s : span_of(a, b0 + lane);
+      const bool mine = !W::kTwo || is_many(t, a.group) == (way == 1);
+      const int cuts = stretches(key_tiles(t, w, a.group, a.window), stretch);
+      const int pieces = mine ? row_tiles(t, w, a.group) * a.kv_heads * cuts : 0, slots = cuts > 1 ? pieces : 0;
+      const int piece_end = piece0 + wave_scan(pieces), slot_end = slot0 + wave_scan(slots);
+      const unsigned long long here = BY_TOKEN ? __ballot(mine && key >= t.first && key < t.first + t.n) : __ballot(key < piece_end);
+      if (here != 0) {
+        const int at = __builtin_ctzll(here);
+        Found f;
+        f.seq = b0 + at;
+        f.many = way == 1;
+        f.span = span_from_lane(t, at);
+        f.cuts = __builtin_amdgcn_readlane(cuts, at);
+        f.stretch = stretch;
+        f.tiles = row_tiles(f.span, w, a.group);
+        f.piece0 = __builtin_amdgcn_readlane(piece_end - pieces, at);
+        f.slot0 = __builtin_amdgcn_readlane(slot_end - slots, at);
+        return f;
+      }
+      piece0 = __builtin_amdgcn_readlane(piece_end, 63);
+      slot0 = __builtin_amdgcn_readlane(slot_end, 63);
     }
-    piece0 = __builtin_amdgcn_readlane(piece_end, 63);
-    slot0 = __builtin_amdgcn_readlane(slot_end, 63);
   }
-  return {-1, 1, stretch, 0, 0, 0, {0, 0, 0, 0}};
+  return kNowhere;
 }
 // Pieces of a sequence: heads side by side (their keys are neighbours in memory), then stretches, then tiles of rows from
 // the last one on, which sees the most keys.
-__device__ __forceinline__ int piece_of(const Found& f, const int heads, const int tile, const int head, const int cut) {
-  return ((f.tiles - 1 - tile) * f.cuts + cut) * heads + head;
+struct Piece { int head, cut, tile, slot; };
+__device__ __forceinline__ Piece piece_at(const Found& f, const int heads, const int in_seq) {
+  const int rest = in_seq / heads;
+  return {in_seq - rest * heads, rest % f.cuts, f.tiles - 1 - rest / f.cuts, f.slot0 + in_seq};
+}
+__device__ __forceinline__ int slot_of(const Found& f, const int heads, const int tile, const int head, const int cut) {
+  return f.slot0 + ((f.tiles - 1 - tile) * f.cuts + cut) * heads + head;
 }
 
-// Work space: m and l of every row of every slot, then their o.
-template <int R> __device__ __forceinline__ float* slot_sums(const Args& a, const int slot, const int row) {
-  return reinterpret_cast<float*>(a.work) + ((int64_t)slot * R + row) * 2;
+// Work space: m and l of every row of every slot, then their o; slots of the one way, then those of the other.
+struct Parts {
+  float* base;
+  int slots, rows, d;
+  __host__ __device__ int64_t floats() const { return (int64_t)slots * rows * (d + 2); }
+  __device__ float* sums(const int slot, const int row) const { return base + ((int64_t)slot * rows + row) * 2; }
+  __device__ float* values(const int slot, const int row) const { return base + (int64_t)slots * rows * 2 + ((int64_t)slot * rows + row) * d; }
+};
+template <typename T, bool WIDE>
+__host__ __device__ __forceinline__ Parts parts_of(const Args& a, const bool many) {
+  using W = Ways<T, WIDE>;
+  Parts p = {reinterpret_cast<float*>(a.work), a.few_slots, W::few.rows, a.d};
+  if (many) p = {p.base + p.floats(), a.many_slots, W::many.rows, a.d};
+  return p;
 }
-template <int R> __device__ __forceinline__ float* slot_rows(const Args& a, const int slot, const int row) {
-  return reinterpret_cast<float*>(a.work) + (int64_t)kMostSlots * R * 2 + ((int64_t)slot * R + row) * a.d;
+// Where a row's result goes.
+template <typename T>
+__device__ __forceinline__ T* result_row(const Args& a, const SeqSpan& s, const int head, const int row) {
+  const int token = row / a.group;
+  return reinterpret_cast<T*>(a.y) + ((int64_t)(s.first + token) * a.kv_heads * a.group + (int64_t)head * a.group + (row - token * a.group)) * a.d;
 }
 
 // ------------------------------------------------------------ the new tokens --
@@ -142,7 +182,7 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const Args a, const in
 }
 
 // ------------------------------------------------------------------ few rows --
-// Tiles of 16 RB rows; the four wavefronts take every fourth tile of KT keys each and meet in LDS at the end.  Nothing
+// Tiles of 16 rows; the four wavefronts take every fourth tile of KT keys each and meet in LDS at the end.  Nothing
 // passes through LDS on the way: keys come from memory as operand fragments (lane l: key l % 16, 16 bytes of it), and the
 // values as VE neighbouring elements of a key a lane (l % 16: which), which are operand fragments once the
 // elements of eight keys have changed places inside the lane.  Which key a place of the product's inner axis has
@@ -151,7 +191,6 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const Args a, const in
 //   o       C[d][row]:   lane l has row l % 16, d = (4 (l / 16) + i) VE + e
 template <typename T> struct Few {
   static constexpr int BLOCKS = sizeof(T) == 4 ? 1 : 2, KEYS = 4 * BLOCKS, KT = 16 * BLOCKS;   // blocks and keys a lane of a tile
-  static constexpr int LEAST = 256 / KT;                    // tiles of the shortest stretch
 };
 template <typename T, int DP> struct FewShape {
   static constexpr int VE = DP / 16;                        // elements of a value that a lane has
@@ -178,52 +217,76 @@ __device__ __forceinline__ void load_part(const T* row, const int at, const int 
   }
 }
 
-// Whether one of the two 16-bit elements of a dword (or the fp32 element) is infinite or NaN.
+// A row's weight for a key that it does not see is zero, and zero times an infinite or missing value is none.  Where a
+// tile has such weights, such values leave it; whoever found one looks at all values of its piece once more in the end and adds
+// those to the rows that see them (what else a row's sum holds, and the weight, make no difference then).
 template <typename T> __device__ __forceinline__ bool not_finite(const unsigned w) {
   if constexpr (sizeof(T) == 4) return (w & 0x7f800000u) == 0x7f800000u;
   constexpr unsigned m = std::is_same<T, f16_t>::value ? 0x7c00u : 0x7f80u;
   return (w & m) == m || (w >> 16 & m) == m;
 }
-template <typename T> __device__ __forceinline__ float element(const unsigned w, const int half) {
-  if constexpr (sizeof(T) == 4) return __uint_as_float(w);
-  else if constexpr (std::is_same<T, f16_t>::value) return f16_to_f32((uint16_t)(half ? w >> 16 : w));
-  else return bf16_to_f32((uint16_t)(half ? w >> 16 : w));
+template <typename T> __device__ __forceinline__ unsigned finite_part(const unsigned w) {
+  if constexpr (sizeof(T) == 4) return not_finite<T>(w) ? 0u : w;
+  constexpr unsigned m = std::is_same<T, f16_t>::value ? 0x7c00u : 0x7f80u;
+  return ((w & m) == m ? 0u : w & 0xffffu) | ((w >> 16 & m) == m ? 0u : w & 0xffff0000u);
+}
+// o: this lane's columns `column(i)` .. + 3 of its row, N times four; rows_of(t): as in the kernels, KT keys a tile.
+template <typename T, int KT, int N, typename RowsOf, typename Column, typename Add>
+__device__ __forceinline__ void add_odd_values(const Args a, const char* vc, const int64_t row_bytes, const int t_begin, const int t_end, const int step, const int last, RowsOf rows_of,
+                                            Column column, Add add) {
+#pragma unroll 1
+  for (int t = t_begin; t < t_end; t += step) {
+    const int rows_ = rows_of(t);
+#pragma unroll 1
+    for (int k = 0; k < KT; ++k) {
+      const int row = __shfl(rows_, k), place = t * KT + k;
+      if (row < 0 || place > last || (a.window != 0 && place <= last - a.window)) continue;
+      const T* v = reinterpret_cast<const T*>(vc + row * row_bytes);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (column(i) >= a.d) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x = Store<T>::ld(v + column(i) + j);
+          if (!__builtin_isfinite(x)) add(i, j, x);
+        }
+      }
+    }
+  }
 }
 
-template <typename T, int DP, int RB>
-__global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attend_few_kernel(const Args a) {
+template <typename T, int DP> constexpr int kFewLds = (4 * 16 * (DP + 4) + 2 * 4 * 16) * (int)sizeof(float);
+template <typename T, int DP>
+__device__ __forceinline__ void attend_few(const Args& a, const Found& f, unsigned char* smem) {
   using F = Few<T>;
   using S = FewShape<T, DP>;
-  constexpr int R = 16 * RB, KEYS = F::KEYS, KT = F::KT, VE = S::VE, VW = S::VW, KC = S::KC;
-  __shared__ __attribute__((aligned(16))) float part[4][16][DP + 4];
-  __shared__ float part_m[4][16], part_l[4][16];
-  const Found f = find<R, KT, F::LEAST, false>(a, blockIdx.x);
-  if (f.seq < 0) return;
+  constexpr bool WIDE = DP > 128;
+  constexpr int R = 16, KEYS = F::KEYS, KT = F::KT, VE = S::VE, VW = S::VW, KC = S::KC;
+  static_assert(R == Ways<T, WIDE>::few.rows && KT == Ways<T, WIDE>::few.keys, "as the pieces are cut");
+  auto part = reinterpret_cast<float (*)[16][DP + 4]>(smem);
+  auto part_m = reinterpret_cast<float (*)[16]>(smem + sizeof(float) * 4 * 16 * (DP + 4));
+  auto part_l = part_m + 4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, g = lane >> 4;
-  const int in_seq = blockIdx.x - f.piece0, rest = in_seq / a.kv_heads;
-  const int head = in_seq - rest * a.kv_heads, cut = rest % f.cuts, tile = f.tiles - 1 - rest / f.cuts;
-  const int r0 = tile * R, rows = min(R, f.span.n * a.group - r0);
+  const Piece piece = piece_at(f, a.kv_heads, blockIdx.x - f.piece0);
+  const int head = piece.head, r0 = piece.tile * R, rows = min(R, f.span.n * a.group - r0);
   const KeyRange seen = keys_of_rows(f.span, r0, R, a.group, a.window);
-  const int t_begin = seen.lo / KT + cut * f.stretch, t_end = min((seen.hi + KT - 1) / KT, f.cuts > 1 ? t_begin + f.stretch : INT32_MAX);
+  const int t_begin = seen.lo / KT + piece.cut * f.stretch, t_end = min((seen.hi + KT - 1) / KT, f.cuts > 1 ? t_begin + f.stretch : INT32_MAX);
   const int64_t row_bytes = (int64_t)a.kv_heads * a.d * (int)sizeof(T);
   const char* kc = reinterpret_cast<const char*>(a.k_cache) + (int64_t)head * a.d * (int)sizeof(T);
   const char* vc = reinterpret_cast<const char*>(a.v_cache) + (int64_t)head * a.d * (int)sizeof(T);
   const int32_t* table = a.table + (int64_t)f.seq * a.table_width;
 
-  // queries: this lane's row of each block, and the last place that it sees
-  uintx4 q[RB][KC];
-  int last[RB];
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    const int r = min(r0 + 16 * b + l16, r0 + rows - 1), token = r / a.group;
+  // queries: this lane's row, and the last place that it sees
+  uintx4 q[KC];
+  const int r = min(r0 + l16, r0 + rows - 1), token = r / a.group, last = f.span.cached + token;
+  {
     const T* row = reinterpret_cast<const T*>(a.q) + ((int64_t)(f.span.first + token) * a.kv_heads * a.group + (int64_t)head * a.group + (r - token * a.group)) * a.d;
-    last[b] = f.span.cached + token;
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
       unsigned w[4];
       load_part<T, 4>(row, (4 * c + g) * (16 / (int)sizeof(T)), a.d, w);
-      q[b][c] = uintx4{w[0], w[1], w[2], w[3]};
+      q[c] = uintx4{w[0], w[1], w[2], w[3]};
     }
   }
   // the rows of the cache that hold a tile's keys, lane l: key l % KT (-1: not there)
@@ -258,15 +321,11 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attend_few_kernel(cons
     }
   };
 
-  float m[RB], l[RB];
-  floatx4 o[RB][VE];
+  float m = -INFINITY, l = 0.f;
+  bool odd = false;
+  floatx4 o[VE];
 #pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    m[b] = -INFINITY;
-    l[b] = 0.f;
-#pragma unroll
-    for (int e = 0; e < VE; ++e) o[b][e] = floatx4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int e = 0; e < VE; ++e) o[e] = floatx4{0.f, 0.f, 0.f, 0.f};
   const float to_log2 = a.scale * kLog2e;
   int here = rows_of(t_begin + wave), next = rows_of(t_begin + wave + 4);
   if (t_begin + wave < t_end) {
@@ -276,192 +335,442 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attend_few_kernel(cons
   // (a wavefront's requests for a tile are on their way while the one before is used)
 #pragma unroll 1
   for (int t = t_begin + wave; t < t_end; t += 4) {
-    floatx4 s[RB][F::BLOCKS];
+    floatx4 s[F::BLOCKS];
 #pragma unroll
-    for (int b = 0; b < RB; ++b)
+    for (int k = 0; k < F::BLOCKS; ++k) {
+      s[k] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < F::BLOCKS; ++k) {
-        s[b][k] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < KC; ++c) s[b][k] = mma_vec<T>(kf[k][c], q[b][c], s[b][k]);
-      }
+      for (int c = 0; c < KC; ++c) s[k] = mma_vec<T>(kf[k][c], q[c], s[k]);
+    }
     if (t + 4 < t_end) load_keys(next);
     const int after = rows_of(t + 8);
-    bool there[KEYS];
-    bool all_there = true;
+    float p[KEYS], most = -INFINITY;
+    bool masked = false;
 #pragma unroll
     for (int j = 0; j < KEYS; ++j) {
-      there[j] = __shfl(here, key_of_slot(j)) >= 0;
-      all_there = all_there && there[j];
+      const int place = t * KT + key_of_slot(j);
+      const bool sees = __shfl(here, key_of_slot(j)) >= 0 && place <= last && (a.window == 0 || place > last - a.window);
+      masked = masked || !sees;
+      p[j] = sees ? s[j >> 2][j & 3] * to_log2 : -INFINITY;
+      most = fmaxf(most, p[j]);
     }
-    // values that are not there weigh nothing, whatever lies in their stead
-    if (!__all(all_there)) {
+    most = fmaxf(m, over_row(most, [](float x, float y) { return fmaxf(x, y); }));
+    const float base = most == -INFINITY ? 0.f : most;
+    const float shrink = __builtin_amdgcn_exp2f(m - base);
+    m = most;
+    l *= shrink;
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j) {
+      p[j] = __builtin_amdgcn_exp2f(p[j] - base);
+      l += p[j];
+    }
+#pragma unroll
+    for (int e = 0; e < VE; ++e) o[e] *= shrink;
+    // element e of this lane's keys, as an operand
+    auto column = [&](const int e, unsigned (&v)[4]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = sizeof(T) == 4 ? vf[j][e] : __builtin_amdgcn_perm(vf[2 * j + 1 & KEYS - 1][e / 2], vf[2 * j & KEYS - 1][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+    };
+    uintx4 weights;
+    if constexpr (sizeof(T) == 4) weights = uintx4{__float_as_uint(p[0]), __float_as_uint(p[1]), __float_as_uint(p[2]), __float_as_uint(p[3])};
+    else weights = pack8_rne<T>(p);
+    if (__any(masked)) {
+      bool found = false;
 #pragma unroll
       for (int j = 0; j < KEYS; ++j)
 #pragma unroll
-        for (int w = 0; w < VW; ++w) vf[j][w] = there[j] ? vf[j][w] : 0u;
-    }
-    float p[RB][KEYS];
-    bool mixed = false;      // a key that one row sees and another does not
+        for (int w = 0; w < VW; ++w) found = found || not_finite<T>(vf[j][w]);
+      if (__any(found)) {
+        odd = true;
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      float most = -INFINITY;
+        for (int j = 0; j < KEYS; ++j)
 #pragma unroll
-      for (int j = 0; j < KEYS; ++j) {
-        const int place = t * KT + key_of_slot(j);
-        const bool sees = there[j] && place <= last[b] && (a.window == 0 || place > last[b] - a.window);
-        mixed = mixed || sees != there[j];
-        p[b][j] = sees ? s[b][j >> 2][j & 3] * to_log2 : -INFINITY;
-        most = fmaxf(most, p[b][j]);
-      }
-      most = fmaxf(m[b], over_row(most, [](float x, float y) { return fmaxf(x, y); }));
-      const float base = most == -INFINITY ? 0.f : most;
-      const float shrink = __builtin_amdgcn_exp2f(m[b] - base);
-      m[b] = most;
-      l[b] *= shrink;
-#pragma unroll
-      for (int j = 0; j < KEYS; ++j) {
-        p[b][j] = __builtin_amdgcn_exp2f(p[b][j] - base);
-        l[b] += p[b][j];
-      }
-#pragma unroll
-      for (int e = 0; e < VE; ++e) o[b][e] *= shrink;
-    }
-    // A row's weight for a key that it does not see is zero, and zero times an infinite or missing value is none: such
-    // values leave the product and are added to the rows that see them one by one.
-    if (__any(mixed)) {
-      bool odd = false;
-#pragma unroll
-      for (int j = 0; j < KEYS; ++j)
-#pragma unroll
-        for (int w = 0; w < VW; ++w) odd = odd || not_finite<T>(vf[j][w]);
-      if (__any(odd)) {
-#pragma unroll
-        for (int j = 0; j < KEYS; ++j) {
-#pragma unroll 1
-          for (int from = 0; from < 4; ++from) {       // the key of slot j in group `from`
-            const int place = t * KT + (j >> 2) * 16 + from * 4 + (j & 3);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-              for (int e = 0; e < VE; ++e) {
-                const unsigned w = (unsigned)__shfl((int)vf[j][e * (int)sizeof(T) / 4], from * 16 + 4 * g + i);
-                const float v = element<T>(w, e & 1);
-                const bool finite = __builtin_isfinite(v);
-#pragma unroll
-                for (int b = 0; b < RB; ++b) {
-                  const float weight = __shfl(p[b][j], from * 16 + l16);
-                  const bool sees = place <= last[b] && (a.window == 0 || place > last[b] - a.window);
-                  if (!finite && sees) o[b][e][i] = __builtin_fmaf(weight, v, o[b][e][i]);
-                }
-              }
-          }
-#pragma unroll
-          for (int w = 0; w < VW; ++w) {
-            if constexpr (sizeof(T) == 4) {
-              vf[j][w] = not_finite<T>(vf[j][w]) ? 0u : vf[j][w];
-            } else {
-              const unsigned lo = __builtin_isfinite(element<T>(vf[j][w], 0)) ? 0xffffu : 0u, hi = __builtin_isfinite(element<T>(vf[j][w], 1)) ? 0xffff0000u : 0u;
-              vf[j][w] &= lo | hi;
-            }
-          }
-        }
+          for (int w = 0; w < VW; ++w) vf[j][w] = finite_part<T>(vf[j][w]);
       }
     }
-    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int e = 0; e < VE; ++e)
-#pragma unroll
-        for (int b = 0; b < RB; ++b)
-#pragma unroll
-          for (int j = 0; j < KEYS; ++j) o[b][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vf[j][e]), p[b][j], o[b][e], 0, 0, 0);
-    } else {
-      uintx4 w[RB];
-#pragma unroll
-      for (int b = 0; b < RB; ++b) w[b] = pack8_rne<T>(p[b]);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        uintx4 column;       // element e of the eight keys
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          column[j] = __builtin_amdgcn_perm(vf[2 * j + 1][e / 2], vf[2 * j][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-        for (int b = 0; b < RB; ++b) o[b][e] = mma_vec<T>(column, w[b], o[b][e]);
-      }
+    for (int e = 0; e < VE; ++e) {
+      unsigned v[4];
+      column(e, v);
+      o[e] = mma_vec<T>(uintx4{v[0], v[1], v[2], v[3]}, weights, o[e]);
     }
     if (t + 4 < t_end) load_values(next);
     here = next;
     next = after;
   }
 
-  // ---- the wavefronts' parts, 16 rows at a time
-  const int mine = threadIdx.x >> 4, column = (threadIdx.x & 15) * VE;
-#pragma unroll 1
-  for (int b = 0; b < RB; ++b) {
-    if (16 * b >= rows) break;
-    if (b > 0) __syncthreads();
+  if (odd)
+    add_odd_values<T, KT, VE>(a, vc, row_bytes, t_begin + wave, t_end, 4, last, rows_of, [&](const int n) { return 4 * (g * VE + n); },
+                              [&](const int n, const int j, const float x) { o[(4 * n + j) % VE][(4 * n + j) / VE] += x; });
+
+  // ---- the wavefronts' parts
+  const int mine = threadIdx.x >> 4, column0 = (threadIdx.x & 15) * VE;
+  const float own_sum = over_row(l, [](float x, float y) { return x + y; });
+  if (g == 0) { part_m[wave][l16] = m; part_l[wave][l16] = own_sum; }
 #pragma unroll
-    for (int k = 0; k < RB; ++k) {
-      if (k != b) continue;
-      const float sum = over_row(l[k], [](float x, float y) { return x + y; });
-      if (g == 0) { part_m[wave][l16] = m[k]; part_l[wave][l16] = sum; }
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+    for (int e = 0; e < VE; ++e) part[wave][l16][(4 * g + i) * VE + e] = o[e][i];
+  __syncthreads();
+  const Parts parts = parts_of<T, WIDE>(a, false);
+  const bool whole = f.cuts == 1;
+  if (mine >= rows || (!whole && piece.slot >= parts.slots)) return;
+  float most = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < VE; ++e) part[wave][l16][(4 * g + i) * VE + e] = o[k][e][i];
+  for (int w = 0; w < 4; ++w) most = fmaxf(most, part_m[w][mine]);
+  float factor[4], sum = 0.f;      // (of a part without keys: 0; of one whose scores are all NaN: NaN)
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    factor[w] = part_m[w][mine] == -INFINITY ? part_l[w][mine] : __builtin_amdgcn_exp2f(part_m[w][mine] - most);
+    sum = __builtin_fmaf(factor[w], part_l[w][mine], sum);
+  }
+  T* y = result_row<T>(a, f.span, head, r0 + mine);
+  float* to = parts.values(piece.slot, mine);
+  const float by = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int e = 0; e < VE; e += 4) {
+    if (column0 + e >= a.d) break;
+    floatx4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const floatx4 x = *reinterpret_cast<const floatx4*>(&part[w][mine][column0 + e]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = factor[w] != 0.f ? __builtin_fmaf(factor[w], x[i], v[i]) : v[i];
     }
-    __syncthreads();
-    const int r = 16 * b + mine;
-    if (r < rows) {
-      float most = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) most = fmaxf(most, part_m[w][mine]);
-      float factor[4], sum = 0.f;      // (of a part without keys: 0; of one whose scores are all NaN: NaN)
+    for (int i = 0; i < 4; ++i) v[i] = by == 0.f ? 0.f : v[i] * by;
+    if (whole) store4<T>(y + column0 + e, v, 4, true);
+    else *reinterpret_cast<floatx4*>(to + column0 + e) = v;
+  }
+  if (!whole && (threadIdx.x & 15) == 0) {
+    float* ml = parts.sums(piece.slot, mine);
+    ml[0] = most;
+    ml[1] = sum;
+  }
+}
+
+// ----------------------------------------------------------------- many rows --
+// Tiles of 128 rows, 32 a wavefront, and of KT keys: keys and values come straight into LDS (one of two buffers, while the other
+// is used) and are read from there by all four wavefronts.  The scores' product gives C[key][row], so that a lane
+// holds, for ITS row, half of the tile's keys: maximum and sum are lane operations and one exchange with lane + 32, and the weights are the
+// operand of the second product as they are (C[d][row], the order of its inner axis being free).  The values'
+// operand has neighbouring keys in a lane: ds_read_b64_tr_b16 reads sixteen columns of four keys that way round.
+// LDS rows keep their 16-byte chunks in other places (key_slot, value_slot), so that what is read at a time lies in different banks.
+// The running maximum follows the true one only when that is 2^8 larger: the sums hold that, and o is seldom rescaled.
+template <int DP> struct Big {
+  static constexpr int KT = DP > 128 ? 32 : 64, BLOCKS = KT / 32;
+  static constexpr int CHUNKS = DP / 8, ROW = DP * 2;                  // 16-byte chunks and bytes of a row
+  static constexpr int TILE = KT * ROW, STAGE = 2 * TILE;              // keys, then values
+  static constexpr int REQUESTS = TILE / 4096, PER = 64 / CHUNKS;      // of a wavefront for each, and rows of one
+  static constexpr int LDS = 2 * STAGE;
+};
+template <int DP> __device__ __forceinline__ int key_slot(const int row, const int chunk) { return chunk ^ (DP == 64 ? row >> 1 & 7 : row & 15); }
+template <int DP> __device__ __forceinline__ int value_slot(const int row, const int chunk) { return chunk ^ (DP == 64 ? (row & 2) << 1 : (row & 3) << 2); }
+
+template <typename T>
+__device__ __forceinline__ floatx16 mma32(const uintx4 a, const uintx4 b, const floatx16 c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  if constexpr (std::is_same<T, f16_t>::value)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(halfx8, a), __builtin_bit_cast(halfx8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+#else
+  (void)a; (void)b;
+  return c;
+#endif
+}
+template <typename Op>
+__device__ __forceinline__ float over_halves(const float v, Op op) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const uintx2 a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return op(__uint_as_float(a.x), __uint_as_float(a.y));
+#else
+  return v;
+#endif
+}
+// Four elements of one column, of the rows that the lanes of its sixteen point to.
+__device__ __forceinline__ uintx2 read_column(const unsigned char* at) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef short shortx4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) shortx4* lds_vec;
+  return __builtin_bit_cast(uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_vec)(at)));
+#else
+  (void)at;
+  return uintx2{0u, 0u};
+#endif
+}
+__device__ __forceinline__ void request16(const char* from, unsigned char* to) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using lds_ptr = __attribute__((address_space(3))) void*;
+  __builtin_amdgcn_global_load_lds(from, (lds_ptr)to, 16, 0, 0);
+#else
+  (void)from; (void)to;
+#endif
+}
+
+// What a wavefront keeps of its 32 rows: lane l has row l % 32.
+template <int DP> struct BigRows {
+  uintx4 q[DP / 16];
+  floatx16 o[DP / 32];
+  float m, l;          // m in units of log 2
+  int last;            // the last place that the row sees
+  bool odd;            // infinite or missing values have left a tile
+};
+
+// One tile of keys, out of `now`; the next one's rows of the cache are requested into `next` meanwhile (the two never
+// overlap: without saying so, every read of LDS would wait for the requests).  valid: bit k, key k is there.
+template <typename T, int DP, bool WHOLE>
+__device__ __forceinline__ void big_tile(const Args& a, unsigned char* __restrict next, unsigned char* __restrict now, const int next_rows, const bool more, const char* kc,
+                                         const char* vc, const int64_t row_bytes, const int place0, const unsigned long long valid, const bool masked, const float mult,
+                                         const int lane, const int wave, BigRows<DP>& w) {
+  using B = Big<DP>;
+  constexpr int BLOCKS = B::BLOCKS;
+  const int l32 = lane & 31, h = lane >> 5;
+  if (more) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        factor[w] = part_m[w][mine] == -INFINITY ? part_l[w][mine] : __builtin_amdgcn_exp2f(part_m[w][mine] - most);
-        sum = __builtin_fmaf(factor[w], part_l[w][mine], sum);
+    for (int i = 0; i < B::REQUESTS; ++i) {
+      const int row = (wave * B::REQUESTS + i) * B::PER + lane / B::CHUNKS, slot = lane % B::CHUNKS;
+      const int64_t at = max(__shfl(next_rows, row), 0) * row_bytes;
+      // (chunks behind the end of a head's row: any of it, they meet zeros of the query or leave columns that are not stored)
+      const int k_chunk = key_slot<DP>(row, slot), v_chunk = value_slot<DP>(row, slot);
+      unsigned char* to = next + (wave * B::REQUESTS + i) * 1024;
+      request16(kc + at + (WHOLE || k_chunk * 8 < a.d ? k_chunk * 16 : 0), to);
+      request16(vc + at + (WHOLE || v_chunk * 8 < a.d ? v_chunk * 16 : 0), to + B::TILE);
+    }
+  }
+  floatx16 s[BLOCKS];
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b) {
+    const unsigned char* row = now + (b * 32 + l32) * B::ROW;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+      if (!WHOLE && c * 16 >= a.d) break;
+      uintx4 k = *reinterpret_cast<const uintx4*>(row + key_slot<DP>(l32, 2 * c + h) * 16);
+      if (!WHOLE && (2 * c + h) * 8 >= a.d) k = uintx4{0u, 0u, 0u, 0u};
+      s[b] = mma32<T>(k, w.q[c], s[b]);
+    }
+  }
+  // element i of block b: place place0 + 32 b + 8 (i / 4) + 4 h + i % 4
+  if (masked) {
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+      const unsigned there = (unsigned)(valid >> (32 * b)) >> (4 * h);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int in = 8 * (i >> 2) + (i & 3), place = place0 + 32 * b + 4 * h + in;
+        const bool sees = (there >> in & 1u) != 0 && place <= w.last && (a.window == 0 || place > w.last - a.window);
+        s[b][i] = sees ? s[b][i] : -INFINITY;
       }
-      const int slot = f.slot0 + in_seq, token = (r0 + r) / a.group;
-      const bool whole = f.cuts == 1;
-      if (whole || slot < kMostSlots) {
-        T* y = reinterpret_cast<T*>(a.y) + ((int64_t)(f.span.first + token) * a.kv_heads * a.group + (int64_t)head * a.group + (r0 + r - token * a.group)) * a.d;
-        float* to = whole ? nullptr : slot_rows<R>(a, slot, r);
-        const float by = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+    }
+  }
+  float most = s[0][0];
 #pragma unroll
-        for (int e = 0; e < VE; e += 4) {
-          if (column + e >= a.d) break;
-          floatx4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const floatx4 x = *reinterpret_cast<const floatx4*>(&part[w][mine][column + e]);
+    for (int i = 0; i < 16; ++i) most = fmaxf(most, s[b][i]);
+  most = over_halves(most, [](float x, float y) { return fmaxf(x, y); }) * mult;
+  const bool grows = most > w.m + 8.f;
+  if (__any(grows)) {
+    const float m = grows ? most : w.m, shrink = grows ? __builtin_amdgcn_exp2f(w.m - m) : 1.f;
+    w.m = m;
+    w.l *= shrink;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = factor[w] != 0.f ? __builtin_fmaf(factor[w], x[i], v[i]) : v[i];
-          }
+    for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = by == 0.f ? 0.f : v[i] * by;
-          if (whole) store4<T>(y + column + e, v, 4, true);
-          else *reinterpret_cast<floatx4*>(to + column + e) = v;
-        }
-        if (!whole && (threadIdx.x & 15) == 0) {
-          float* ml = slot_sums<R>(a, slot, r);
-          ml[0] = most;
-          ml[1] = sum;
-        }
+      for (int i = 0; i < 16; ++i) w.o[d][i] *= shrink;
+  }
+  const float base = w.m == -INFINITY ? 0.f : w.m;
+  uintx4 p[BLOCKS][2];
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][8 * c + i], mult, -base));
+        w.l += e[i];
       }
+      p[b][c] = pack8_rne<T>(e);
+    }
+  unsigned char* values = now + B::TILE;
+  const int from = lane & 15, part = lane >> 4 & 1;
+  // the operand of columns 32 d .. and of half c of block b
+  auto column = [&](const int d, const int b, const int c, unsigned (&v)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int k = 32 * b + 16 * c + 8 * half + 4 * h + (from >> 2), chunk = 4 * d + 2 * part + (from >> 1 & 1);
+      const uintx2 x = read_column(values + k * B::ROW + value_slot<DP>(k, chunk) * 16 + (from & 1) * 8);
+      v[2 * half] = x.x;
+      v[2 * half + 1] = x.y;
+    }
+  };
+  if (masked) {       // (for all four wavefronts, which look at the same values)
+    bool found = false;
+#pragma unroll 4
+    for (int c = lane; c < B::TILE / 16; c += 64) {
+      const uintx4 v = reinterpret_cast<const uintx4*>(values)[c];
+      found = found || not_finite<T>(v.x) || not_finite<T>(v.y) || not_finite<T>(v.z) || not_finite<T>(v.w);
+    }
+    if (__any(found)) {
+      w.odd = true;
+      __syncthreads();
+#pragma unroll 1
+      for (int c = threadIdx.x; c < B::TILE / 16; c += 256) {
+        const uintx4 v = reinterpret_cast<const uintx4*>(values)[c];
+        reinterpret_cast<uintx4*>(values)[c] = uintx4{finite_part<T>(v.x), finite_part<T>(v.y), finite_part<T>(v.z), finite_part<T>(v.w)};
+      }
+      __syncthreads();
+    }
+  }
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) {
+    if (!WHOLE && d * 32 >= a.d) break;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        unsigned v[4];
+        column(d, b, c, v);
+        w.o[d] = mma32<T>(uintx4{v[0], v[1], v[2], v[3]}, p[b][c], w.o[d]);
+      }
+  }
+}
+
+template <typename T, int DP, bool WHOLE>
+__device__ __forceinline__ void attend_many(const Args& a, const Found& f, unsigned char* smem) {
+  using B = Big<DP>;
+  constexpr bool WIDE = DP > 128;
+  constexpr int R = 128, KT = B::KT;
+  static_assert(R == Ways<T, WIDE>::many.rows && KT == Ways<T, WIDE>::many.keys, "as the pieces are cut");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l32 = lane & 31, h = lane >> 5;
+  const Piece piece = piece_at(f, a.kv_heads, blockIdx.x - f.piece0);
+  const int head = piece.head, r0 = piece.tile * R, rows = min(R, f.span.n * a.group - r0);
+  const KeyRange seen = keys_of_rows(f.span, r0, R, a.group, a.window);
+  const int t_begin = seen.lo / KT + piece.cut * f.stretch, t_end = min((seen.hi + KT - 1) / KT, f.cuts > 1 ? t_begin + f.stretch : INT32_MAX);
+  const int64_t row_bytes = (int64_t)a.kv_heads * a.d * 2;
+  const char* kc = reinterpret_cast<const char*>(a.k_cache) + (int64_t)head * a.d * 2;
+  const char* vc = reinterpret_cast<const char*>(a.v_cache) + (int64_t)head * a.d * 2;
+  const int32_t* table = a.table + (int64_t)f.seq * a.table_width;
+  // The scale's sign goes to the queries, and so does a scale of zero: maxima are taken of the products as they are.
+  const float mult = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
+  BigRows<DP> w;
+  const int r = min(wave * 32 + l32, rows - 1), token = (r0 + r) / a.group;
+  {
+    const T* row = reinterpret_cast<const T*>(a.q) + ((int64_t)(f.span.first + token) * a.kv_heads * a.group + (int64_t)head * a.group + (r0 + r - token * a.group)) * a.d;
+    const unsigned flip = a.scale < 0.f ? 0x80008000u : 0u, keep = a.scale == 0.f ? 0u : 0xffffffffu;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+      unsigned x[4];
+      load_part<T, 4>(row, 16 * c + 8 * h, a.d, x);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w.q[c][j] = (x[j] & keep) ^ flip;
+    }
+  }
+  w.last = f.span.cached + token;
+  w.m = -INFINITY;
+  w.l = 0.f;
+  w.odd = false;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w.o[d][i] = 0.f;
+  // what all rows of the tile see
+  const int first_last = f.span.cached + r0 / a.group, last_last = f.span.cached + (r0 + rows - 1) / a.group;
+  auto rows_of = [&](const int t) __attribute__((always_inline)) -> int {
+    const int place = t * KT + (lane & (KT - 1));
+    if (t >= t_end || place >= seen.hi) return -1;
+    const int index = fast_div(place, a.page_magic, a.page_shift);
+    return cache_row(table[index], place - index * a.page, a.page, a.pages);
+  };
+  if (t_begin < t_end) {
+    int here = rows_of(t_begin), next = rows_of(t_begin + 1);
+#pragma unroll
+    for (int i = 0; i < B::REQUESTS; ++i) {
+      const int row = (wave * B::REQUESTS + i) * B::PER + lane / B::CHUNKS, slot = lane % B::CHUNKS;
+      const int64_t at = max(__shfl(here, row), 0) * row_bytes;
+      const int k_chunk = key_slot<DP>(row, slot), v_chunk = value_slot<DP>(row, slot);
+      unsigned char* to = smem + (wave * B::REQUESTS + i) * 1024;
+      request16(kc + at + (WHOLE || k_chunk * 8 < a.d ? k_chunk * 16 : 0), to);
+      request16(vc + at + (WHOLE || v_chunk * 8 < a.d ? v_chunk * 16 : 0), to + B::TILE);
+    }
+#pragma unroll 1
+    for (int t = t_begin; t < t_end; ++t) {
+      // this tile has landed, and everybody has left the other buffer
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __syncthreads();
+      const unsigned long long valid = __ballot(here >= 0), all = KT == 64 ? ~0ull : 0xffffffffull;
+      const bool masked = (valid & all) != all || t * KT + KT - 1 > first_last || (a.window != 0 && t * KT <= last_last - a.window);
+      const int after = rows_of(t + 2), at = (t - t_begin) & 1;
+      big_tile<T, DP, WHOLE>(a, smem + (1 - at) * B::STAGE, smem + at * B::STAGE, next, t + 1 < t_end, kc, vc, row_bytes, t * KT, valid & all, masked, mult, lane, wave, w);
+      here = next;
+      next = after;
+    }
+  }
+  if (w.odd)
+    add_odd_values<T, KT, DP / 8>(a, vc, row_bytes, t_begin, t_end, 1, w.last, rows_of, [&](const int n) { return 8 * n + 4 * h; },
+                                  [&](const int n, const int j, const float x) { w.o[n / 4][n % 4 * 4 + j] += x; });
+  const float sum = over_halves(w.l, [](float x, float y) { return x + y; });
+  if (wave * 32 + l32 >= rows) return;
+  if (f.cuts == 1) {
+    T* y = result_row<T>(a, f.span, head, r0 + r);
+    const float by = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int col = 32 * d + 8 * i + 4 * h;
+        floatx4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = by == 0.f ? 0.f : w.o[d][4 * i + j] * by;
+        if (WHOLE || col < a.d) store4<T>(y + col, v, 4, true);
+      }
+  } else {
+    const Parts parts = parts_of<T, WIDE>(a, true);
+    if (piece.slot >= parts.slots) return;
+    float* to = parts.values(piece.slot, r);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int col = 32 * d + 8 * i + 4 * h;
+        if (WHOLE || col < a.d) *reinterpret_cast<floatx4*>(to + col) = floatx4{w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]};
+      }
+    if (h == 0) {
+      float* ml = parts.sums(piece.slot, r);
+      ml[0] = w.m;
+      ml[1] = sum;
     }
   }
 }
 
+template <typename T, int DP> constexpr int kLds = sizeof(T) == 2 && Big<DP>::LDS > kFewLds<T, DP> ? Big<DP>::LDS : kFewLds<T, DP>;
+template <typename T, int DP, bool WHOLE>
+__global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) attend_kernel(const Args a) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const Found f = find<T, (DP > 128), false>(a, blockIdx.x);
+  if (f.seq < 0) return;
+  if constexpr (sizeof(T) == 2) {
+    if (f.many) {
+      attend_many<T, DP, WHOLE>(a, f, smem);
+      return;
+    }
+  }
+  attend_few<T, DP>(a, f, smem);
+}
+
 // ------------------------------------------------------------------ the parts --
 // A workgroup has a few neighbouring tokens of one head, a wavefront one row after the other.
-template <typename T, int R, int KT, int LEAST>
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) attention_join_kernel(const Args a, const int tokens_each) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int head = blockIdx.x % (unsigned)a.kv_heads, token0 = blockIdx.x / (unsigned)a.kv_heads * tokens_each;
-  Found f = {-1, 1, 0, 0, 0, 0, {0, 0, 0, 0}};
+  Found f = kNowhere;
   for (int token = token0; token < min(token0 + tokens_each, a.tokens); ++token) {
-    if (f.seq < 0 || token < f.span.first || token >= f.span.first + f.span.n) f = find<R, KT, LEAST, true>(a, token);
+    if (f.seq < 0 || token < f.span.first || token >= f.span.first + f.span.n) f = find<T, WIDE, true>(a, token);
     if (f.seq >= 0 && f.cuts == 1) continue;
     for (int q = wave; q < a.group; q += 4) {
       T* y = reinterpret_cast<T*>(a.y) + ((int64_t)token * a.kv_heads * a.group + (int64_t)head * a.group + q) * a.d;
@@ -469,23 +778,24 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const Args a, const
         for (int c = lane * 4; c < a.d; c += 256) store4<T>(y + c, floatx4{0.f, 0.f, 0.f, 0.f}, 4, true);
         continue;
       }
-      const int row = (token - f.span.first) * a.group + q, tile = row / R, r = row - tile * R;
+      const Parts parts = parts_of<T, WIDE>(a, f.many);
+      const int row = (token - f.span.first) * a.group + q, tile = row / parts.rows, r = row - tile * parts.rows;
       float most = -INFINITY;
       for (int cut = 0; cut < f.cuts; ++cut) {
-        const int slot = f.slot0 + piece_of(f, a.kv_heads, tile, head, cut);
-        if (slot < kMostSlots) most = fmaxf(most, slot_sums<R>(a, slot, r)[0]);
+        const int slot = slot_of(f, a.kv_heads, tile, head, cut);
+        if (slot < parts.slots) most = fmaxf(most, parts.sums(slot, r)[0]);
       }
       float sum = 0.f;
       floatx4 v = {0.f, 0.f, 0.f, 0.f};
       for (int cut = 0; cut < f.cuts; ++cut) {
-        const int slot = f.slot0 + piece_of(f, a.kv_heads, tile, head, cut);
-        if (slot >= kMostSlots) continue;
-        const float* ml = slot_sums<R>(a, slot, r);
+        const int slot = slot_of(f, a.kv_heads, tile, head, cut);
+        if (slot >= parts.slots) continue;
+        const float* ml = parts.sums(slot, r);
         if (ml[1] == 0.f) continue;
         const float factor = ml[0] == -INFINITY ? ml[1] : __builtin_amdgcn_exp2f(ml[0] - most);
         sum = __builtin_fmaf(factor, ml[1], sum);
         if (lane * 4 < a.d) {
-          const floatx4 x = *reinterpret_cast<const floatx4*>(slot_rows<R>(a, slot, r) + lane * 4);
+          const floatx4 x = *reinterpret_cast<const floatx4*>(parts.values(slot, r) + lane * 4);
 #pragma unroll
           for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(factor, x[i], v[i]);
         }
@@ -499,44 +809,76 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const Args a, const
   }
 }
 
-Args args_of(const PagedAttentionParams& p) {
+// Slots of a way: none where no sequence can be long enough to be cut.
+int slots_of(const PagedAttentionParams& p, const Way& w, const long long units) {
+  const SeqSpan longest = {0, p.tokens, 0, p.table_width * p.page};
+  const long long most = (long long)key_tiles(longest, w, p.group, std::min(p.window, 1 << 30));
+  return most <= w.least ? 0 : (int)std::min((long long)most_slots(w), units * ((most + w.least - 1) / w.least));
+}
+template <typename T, bool WIDE>
+Args args_as(const PagedAttentionParams& p) {
+  using W = Ways<T, WIDE>;
   Args a;
   static_cast<PagedAttentionParams&>(a) = p;
   div_magic(p.page, &a.page_magic, &a.page_shift);
   a.reach = p.table_width * p.page;
-  a.window = p.window > (1 << 30) ? 1 << 30 : p.window;   // (no place lies further back)
+  a.window = std::min(p.window, 1 << 30);   // (no place lies further back)
+  a.few_slots = slots_of(p, W::few, most_few_units(p.tokens, p.seqs, p.kv_heads, p.group, !W::kTwo));
+  a.many_slots = W::kTwo ? slots_of(p, W::many, most_many_units(p.tokens, p.seqs, p.kv_heads, p.group)) : 0;
   return a;
 }
-constexpr int kRowsFew = 16;
+template <typename T> Args args_of(const PagedAttentionParams& p) { return p.d > 128 ? args_as<T, true>(p) : args_as<T, false>(p); }
+template <typename T> size_t space_of(const PagedAttentionParams& p) {
+  const Args a = args_of<T>(p);
+  const bool wide = p.d > 128;
+  const Parts few = wide ? parts_of<T, true>(a, false) : parts_of<T, false>(a, false);
+  const Parts many = {nullptr, a.many_slots, kMany.rows, p.d};
+  return (size_t)(few.floats() + many.floats() + 4) * sizeof(float);
+}
 
+template <typename T, int DP, bool WHOLE>
+hipError_t attend_with(const Args& a, hipStream_t stream) {
+  using W = Ways<T, (DP > 128)>;
+  long long grid = most_few_units(a.tokens, a.seqs, a.kv_heads, a.group, !W::kTwo) + (a.few_slots > 0 ? most_cut_pieces(W::few) : 0);
+  if (W::kTwo) grid += most_many_units(a.tokens, a.seqs, a.kv_heads, a.group) + (a.many_slots > 0 ? most_cut_pieces(W::many) : 0);
+  static LdsLimit limit;
+  if (kLds<T, DP> > 65536) {
+    const hipError_t e = limit.raise(reinterpret_cast<const void*>(&attend_kernel<T, DP, WHOLE>), kLds<T, DP>);
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL((attend_kernel<T, DP, WHOLE>), dim3((unsigned)grid), dim3(256), (kLds<T, DP>), stream, a);
+  return hipGetLastError();
+}
 template <typename T, int DP>
-void launch_few(const Args& a, hipStream_t stream) {
-  const long long grid = most_units(a.tokens, a.seqs, a.kv_heads, a.group, kRowsFew) + kMostCutPieces;
-  hipLaunchKernelGGL((attend_few_kernel<T, DP, kRowsFew / 16>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+hipError_t attend_wide(const Args& a, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2) {
+    if (a.d == DP) return attend_with<T, DP, true>(a, stream);
+  }
+  return attend_with<T, DP, false>(a, stream);
 }
 template <typename T>
 hipError_t attend_as(const PagedAttentionParams& p, hipStream_t stream) {
-  const Args a = args_of(p);
-  if (p.d <= 64) launch_few<T, 64>(a, stream);
-  else if (p.d <= 128) launch_few<T, 128>(a, stream);
-  else launch_few<T, 256>(a, stream);
-  return hipGetLastError();
+  const Args a = args_of<T>(p);
+  if (p.d <= 64) return attend_wide<T, 64>(a, stream);
+  if (p.d <= 128) return attend_wide<T, 128>(a, stream);
+  return attend_wide<T, 256>(a, stream);
 }
 template <typename T>
 hipError_t join_as(const PagedAttentionParams& p, hipStream_t stream) {
-  const Args a = args_of(p);
+  const Args a = args_of<T>(p);
   const int each = p.group >= 16 ? 1 : 16 / p.group;
-  const unsigned grid = (unsigned)((p.tokens + each - 1) / each) * (unsigned)p.kv_heads;
-  hipLaunchKernelGGL((attention_join_kernel<T, kRowsFew, Few<T>::KT, Few<T>::LEAST>), dim3(grid), dim3(256), 0, stream, a, each);
+  const dim3 grid((unsigned)((p.tokens + each - 1) / each) * (unsigned)p.kv_heads);
+  if (p.d > 128) hipLaunchKernelGGL((attention_join_kernel<T, true>), grid, dim3(256), 0, stream, a, each);
+  else hipLaunchKernelGGL((attention_join_kernel<T, false>), grid, dim3(256), 0, stream, a, each);
   return hipGetLastError();
 }
 
 }  // namespace
 
-size_t paged_attention_space(const PagedAttentionParams& p) { return (size_t)kMostSlots * kRowsFew * (p.d + 2) * sizeof(float); }
+size_t paged_attention_space(const PagedAttentionParams& p) { return p.dt == DT_F32 ? space_of<float>(p) : space_of<bf16_t>(p); }
 
 hipError_t launch_cache_write(const PagedAttentionParams& p, hipStream_t stream) {
-  hipLaunchKernelGGL(cache_write_kernel, dim3((unsigned)((p.tokens + 3) / 4)), dim3(256), 0, stream, args_of(p), p.kv_heads * p.d * dtype_size(p.dt));
+  hipLaunchKernelGGL(cache_write_kernel, dim3((unsigned)((p.tokens + 3) / 4)), dim3(256), 0, stream, args_of<float>(p), p.kv_heads * p.d * dtype_size(p.dt));
   return hipGetLastError();
 }
 

@@ -28,7 +28,7 @@ int main() {
             for (int group = 1; group <= 3; ++group)
               for (int window = 0; window <= 7; ++window)
                 for (int most = 2; most <= 8; most += 3) {
-                  const int tiles = row_tiles(s, most, group);
+                  const int tiles = row_tiles(s, Way{most, 4, 1, 1}, group);
                   if (tiles * most < s.n * group || (tiles - 1) * most >= s.n * group) { printf("tiles\n"); return 1; }
                   for (int tile = 0; tile < tiles; ++tile) {
                     const KeyRange k = keys_of_rows(s, tile * most, most, group, window);
@@ -73,25 +73,28 @@ int main() {
     const int each = rand() % 3 == 0 ? 1 + rand() % 300 : 1;
     for (int b = 0; b < seqs; ++b) starts[b + 1] = starts[b] + rand() % (each + 1);
     const int tokens = starts[seqs] > 0 ? starts[seqs] : 1;
-    for (int big = 0; big < 2; ++big) {
-      const int rows = big ? 128 : 16, kt = big ? 64 : 32, least = 8;
-      SeqSpan s[42];
+    const Way ways[] = {kFew16, kFew32, kMany, kManyWide};
+    SeqSpan spans[42];
+    for (int b = 0; b < seqs; ++b) spans[b] = seq_span(starts[b], starts[b + 1], rand() % (reach + 1), tokens, reach);
+    for (int k = 0; k < 4; ++k) {
+      const Way w = ways[k];
+      auto mine = [&](int b) { return k == 1 || is_many(spans[b], group) == (k >= 2); };   // (fp32: all sequences one way)
       float work = 0.f;
-      for (int b = 0; b < seqs; ++b) {
-        s[b] = seq_span(starts[b], starts[b + 1], rand() % (reach + 1), tokens, reach);
-        work += (float)row_tiles(s[b], rows, group) * (float)heads * (float)most_key_tiles(s[b], rows, group, window, kt);
-      }
-      const int stretch = stretch_of(work, least);
+      for (int b = 0; b < seqs; ++b) work += mine(b) ? work_of(spans[b], w, group, heads, window) : 0.f;
+      const int stretch = stretch_of(work, w);
       long long pieces = 0, slots = 0, units = 0;
       for (int b = 0; b < seqs; ++b) {
-        const int cuts = stretches(most_key_tiles(s[b], rows, group, window, kt), stretch);
-        const long long mine = (long long)row_tiles(s[b], rows, group) * heads * cuts;
-        pieces += mine;
-        units += (long long)row_tiles(s[b], rows, group) * heads;
-        if (cuts > 1) slots += mine;
+        if (!mine(b)) continue;
+        const int cuts = stretches(key_tiles(spans[b], w, group, window), stretch);
+        const long long own = (long long)row_tiles(spans[b], w, group) * heads * cuts;
+        pieces += own;
+        units += (long long)row_tiles(spans[b], w, group) * heads;
+        if (cuts > 1) slots += own;
+        if ((cuts > 1) && stretch < w.least) { printf("stretch\n"); return 1; }
       }
-      if (units > most_units(tokens, seqs, heads, group, rows) || pieces > most_units(tokens, seqs, heads, group, rows) + kMostCutPieces || slots > kMostSlots) {
-        printf("%lld units, %lld pieces, %lld slots\n", units, pieces, slots);
+      const long long most = k >= 2 ? most_many_units(tokens, seqs, heads, group) : most_few_units(tokens, seqs, heads, group, k == 1);
+      if (units > most || pieces > most + most_cut_pieces(w) || slots > most_slots(w)) {
+        printf("way %d: %lld units of %lld, %lld pieces, %lld slots\n", k, units, most, pieces, slots);
         return 1;
       }
     }
