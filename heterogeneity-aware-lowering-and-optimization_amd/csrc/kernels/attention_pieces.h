@@ -61,7 +61,7 @@ OHIP_HD int most_slots(const Way& w) { return 2 * most_cut_pieces(w); }
 
 // Sequences of up to kFewRows rows go in tiles of 16, others in tiles of 128 (16-bit types; fp32: all in tiles of 16).
 constexpr int kFewRows = 32;
-constexpr Way kFew16 = {16, 32, 8, 1024}, kFew32 = {16, 16, 16, 1024}, kMany = {128, 64, 8, 256}, kManyWide = {128, 32, 16, 256};   // (wide: heads above 128)
+constexpr Way kFew16 = {16, 32, 8, 1024}, kFew32 = {16, 16, 16, 1024}, kMany = {128, 64, 8, 512}, kManyWide = {128, 32, 16, 512};   // (wide: heads above 128)
 OHIP_HD bool is_many(const SeqSpan& s, const int group) { return (long long)s.n * group > kFewRows; }
 OHIP_HD long long most_few_units(const int tokens, const int seqs, const int heads, const int group, const bool all) {
   const long long each = at_most(seqs, tokens);

@@ -70,8 +70,42 @@ __device__ __forceinline__ void put_alternative(const LogProbsParams& p, const i
 // Work space: the Sums of every part of every row, then `top` keys for each.
 __host__ __device__ inline int64_t keys_at(const LogProbsParams& p, const int parts) { return (int64_t)p.rows * parts * (int64_t)sizeof(Sums); }
 
+// A thread's 32 logits as they are in memory: group i are those from index first + (i NT + tid) 8 on; -inf behind the end.
+template <typename T> struct Group { unsigned w[2 * sizeof(T)]; };
+template <typename T> __device__ __forceinline__ float logit_at(const Group<T>& g, const int e) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(g.w[e]);
+  else if constexpr (std::is_same<T, f16_t>::value) return f16_to_f32((uint16_t)(g.w[e >> 1] >> (16 * (e & 1))));
+  else return __uint_as_float(e & 1 ? g.w[e >> 1] & 0xffff0000u : g.w[e >> 1] << 16);
+}
+template <typename T, bool VECTOR>
+__device__ __forceinline__ Group<T> load_group(const T* row, const int at, const int end) {
+  Group<T> g;
+  if (at + 8 <= end) {
+#pragma unroll
+    for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
+      uintx4 v;
+      if constexpr (VECTOR) v = *reinterpret_cast<const uintx4*>(row + at + h * (16 / (int)sizeof(T)));
+      else v = reinterpret_cast<const Bytes16*>(row + at + h * (16 / (int)sizeof(T)))->v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) g.w[4 * h + j] = v[j];
+    }
+  } else {
+    constexpr unsigned out = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, f16_t>::value ? 0xfc00u : 0xff80u;
+#pragma unroll
+    for (int j = 0; j < 2 * (int)sizeof(T); ++j) {
+      if constexpr (sizeof(T) == 4) {
+        g.w[j] = at + j < end ? reinterpret_cast<const unsigned*>(row)[at + j] : out;
+      } else {
+        const unsigned lo = at + 2 * j < end ? row[at + 2 * j].bits : out, hi = at + 2 * j + 1 < end ? row[at + 2 * j + 1].bits : out;
+        g.w[j] = lo | hi << 16;
+      }
+    }
+  }
+  return g;
+}
+
 template <int NT> struct Room {
-  float wave[4][NT / 64];
+  Sums wave[NT / 64];
   float group[kGroups];
   float bound;
   int listed;
@@ -79,110 +113,29 @@ template <int NT> struct Room {
   u64 list[kList];
 };
 
-template <typename T, int NT, bool VECTOR>
-__global__ void __launch_bounds__(NT, 4) log_probs_kernel(const LogProbsParams p, const int parts, const int each) {
-  constexpr int WAVES = NT / 64, LPG = NT / kGroups;
-  __shared__ Room<NT> room;
-  const int part = blockIdx.x % (unsigned)parts, row = blockIdx.x / (unsigned)parts;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int first = part * each, end = min(p.V, first + each);
-  const T* logits = reinterpret_cast<const T*>(p.logits) + (int64_t)row * p.V;
-  // logit e of group i: index first + (i NT + tid) 8 + e
-  float l[kEach / 8][8];
-#pragma unroll
-  for (int i = 0; i < kEach / 8; ++i) load8<T, VECTOR>(logits, first + (i * NT + tid) * 8, end, l[i]);
-  float most = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kEach / 8; ++i) {
-    const int at = first + (i * NT + tid) * 8;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      l[i][e] = l[i][e] > -INFINITY && at + e < end ? l[i][e] : -INFINITY;      // (NaN too)
-      most = fmaxf(most, l[i][e]);
-    }
-  }
-  const float mine = most;
-  const float group = group_allreduce<LPG>(mine, [](float a, float b) { return fmaxf(a, b); });
-  if ((tid & (LPG - 1)) == 0) room.group[tid / LPG] = group;
-  if (tid == 0) room.listed = 0;
-  __syncthreads();
-  const float of_group = room.group[lane];
-  most = wave_max(of_group);
-  if (p.top > 0) {
-    // the group whose maximum has top - 1 others in front of it
-#pragma unroll 1
-    for (int j = wave; j < kGroups; j += WAVES) {
-      const float g = room.group[j];
-      const int rank = __popcll(__ballot(of_group > g || (of_group == g && lane < j)));
-      if (rank == p.top - 1 && lane == 0) room.bound = g;
-    }
-  }
-  Sums s = {most, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < kEach / 8; ++i)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      // (a distance of 10^4 weighs nothing; -inf, and everything beside infinite logits, is as far)
-      const float d = fminf(most - l[i][e], 1e4f);
-      const bool top = l[i][e] == most;
-      const float w = top ? 0.f : __builtin_amdgcn_exp2f(d * -kLog2e);
-      s.count += top ? 1.f : 0.f;
-      s.low += w;
-      s.away = __builtin_fmaf(w, d, s.away);
-    }
-  s.count = wave_sum(s.count);
-  s.low = wave_sum(s.low);
-  s.away = wave_sum(s.away);
-  if (lane == 0) { room.wave[0][wave] = s.count; room.wave[1][wave] = s.low; room.wave[2][wave] = s.away; }
-  __syncthreads();
-  s.count = s.low = s.away = 0.f;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) { s.count += room.wave[0][w]; s.low += room.wave[1][w]; s.away += room.wave[2][w]; }
-  RowResult r = {0.f, 0.f};
-  Sums* sums = reinterpret_cast<Sums*>(p.work) + (int64_t)row * parts + part;
-  if (parts == 1) r = finish_row(p, row, s);
-  else if (tid == 0) *sums = s;
-  if (p.top == 0) return;
+// Sums of parts (lane l has one; `n` of them, the first lanes), in every lane.
+__device__ __forceinline__ Sums joined(Sums s, const bool have) {
+  if (!have) s = {-INFINITY, 0.f, 0.f, 0.f};
+  const float most = wave_max(s.most);
+  const bool top = s.most == most;
+  const float d = fminf(most - s.most, 1e4f), f = top ? 1.f : __builtin_amdgcn_exp2f(d * -kLog2e), all = s.count + s.low;
+  return {most, wave_sum(top ? s.count : 0.f), wave_sum(top ? s.low : f * all), wave_sum(top ? s.away : f * __builtin_fmaf(d, all, s.away))};
+}
 
-  u64* keys = reinterpret_cast<u64*>(reinterpret_cast<char*>(p.work) + keys_at(p, parts)) + ((int64_t)row * parts + part) * p.top;
-  auto put = [&](const int place, const u64 key) {
-    if (parts == 1) put_alternative(p, row, place, key, r);
-    else keys[place] = key;
-  };
-  const float bound = room.bound;
-  if (mine >= bound && mine > -INFINITY) {
-#pragma unroll
-    for (int i = 0; i < kEach / 8; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (l[i][e] >= bound && l[i][e] > -INFINITY) {
-          const int at = atomicAdd(&room.listed, 1);
-          if (at < kList) room.list[at] = key_of(l[i][e], first + (i * NT + tid) * 8 + e);
-        }
-  }
-  __syncthreads();
-  const int n = room.listed;
-  if (n <= kList) {
-    for (int c = tid; c < n; c += NT) {
-      const u64 key = room.list[c];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += room.list[j] > key;
-      if (rank < p.top) put(rank, key);
-    }
-    for (int place = n + tid; place < p.top; place += NT) put(place, 0);
-    return;
-  }
+// The `top` best of a part whose logits reach the bound too often: the largest behind the last one, again and again.
+template <typename T, int NT>
+__device__ __noinline__ void best_by_rounds(const T* logits, const int first, const int end, const int top, Room<NT>& room, u64* keys) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   u64 last = ~0ull;
 #pragma unroll 1
-  for (int place = 0; place < p.top; ++place) {
+  for (int place = 0; place < top; ++place) {
     u64 best = 0;
-#pragma unroll
-    for (int i = 0; i < kEach / 8; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const u64 key = key_of(l[i][e], first + (i * NT + tid) * 8 + e);
-        if (l[i][e] > -INFINITY && key < last && key > best) best = key;
-      }
+#pragma unroll 1
+    for (int i = first + (int)threadIdx.x; i < end; i += NT) {
+      const float l = Store<T>::ld(logits + i);
+      const u64 key = key_of(l, i);
+      if (l > -INFINITY && key < last && key > best) best = key;
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
       const u64 other = __shfl_xor(best, o);
@@ -192,10 +145,104 @@ __global__ void __launch_bounds__(NT, 4) log_probs_kernel(const LogProbsParams p
     if (lane == 0) room.best[wave] = best;
     __syncthreads();
     best = room.best[0];
-#pragma unroll
-    for (int w = 1; w < WAVES; ++w) best = room.best[w] > best ? room.best[w] : best;
-    if (tid == 0) put(place, best);
+#pragma unroll 1
+    for (int w = 1; w < NT / 64; ++w) best = room.best[w] > best ? room.best[w] : best;
+    if (threadIdx.x == 0) keys[place] = best;
     last = best;
+  }
+}
+
+// Sums are of a wavefront's logits around its own largest, so that nothing is waited for before they are complete.
+// Per logit: widen, maximum, difference, its bound, exponent, exponential (four times the others), the largest's
+// exclusion (two) and two sums.
+template <typename T, int NT, bool VECTOR, bool TOP>
+__global__ void __launch_bounds__(NT, NT == kWide ? 8 : 6) log_probs_kernel(const LogProbsParams p, const int parts, const int each) {
+  constexpr int WAVES = NT / 64, LPG = NT / kGroups;
+  __shared__ Room<NT> room;
+  const int part = blockIdx.x % (unsigned)parts, row = blockIdx.x / (unsigned)parts;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int first = part * each, end = min(p.V, first + each);
+  const T* logits = reinterpret_cast<const T*>(p.logits) + (int64_t)row * p.V;
+  Group<T> l[kEach / 8];
+#pragma unroll
+  for (int i = 0; i < kEach / 8; ++i) l[i] = load_group<T, VECTOR>(logits, first + (i * NT + tid) * 8, end);
+  float mine = -INFINITY;       // (NaN is no maximum)
+#pragma unroll
+  for (int i = 0; i < kEach / 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) mine = fmaxf(mine, logit_at<T>(l[i], e));
+  if constexpr (TOP) {
+    const float group = group_allreduce<LPG>(mine, [](float a, float b) { return fmaxf(a, b); });
+    if ((tid & (LPG - 1)) == 0) room.group[tid / LPG] = group;
+    if (tid == 0) room.listed = 0;
+  }
+  Sums s = {wave_max(mine), 0.f, 0.f, 0.f};
+  int equal = 0;
+#pragma unroll
+  for (int i = 0; i < kEach / 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      // (a distance of 10^4 weighs nothing; -inf, NaN, and everything beside infinite logits, is as far)
+      const float x = logit_at<T>(l[i], e), d = fminf(s.most - x, 1e4f);
+      const bool top = x == s.most;
+      equal += __popcll(__ballot(top));
+      const float w = top ? 0.f : __builtin_amdgcn_exp2f(d * -kLog2e);
+      s.low += w;
+      s.away = __builtin_fmaf(w, d, s.away);
+    }
+  s.count = (float)equal;
+  s.low = wave_sum(s.low);
+  s.away = wave_sum(s.away);
+  if (lane == 0) room.wave[wave] = s;
+  __syncthreads();
+  s = joined(room.wave[lane & (WAVES - 1)], lane < WAVES);
+  if constexpr (TOP) {
+    // the group whose maximum has top - 1 others in front of it
+    const float of_group = room.group[lane];
+#pragma unroll 1
+    for (int j = wave; j < kGroups; j += WAVES) {
+      const float g = room.group[j];
+      const int rank = __popcll(__ballot(of_group > g || (of_group == g && lane < j)));
+      if (rank == p.top - 1 && lane == 0) room.bound = g;
+    }
+  }
+  RowResult r = {0.f, 0.f};
+  if (parts == 1) r = finish_row(p, row, s);
+  else if (tid == 0) reinterpret_cast<Sums*>(p.work)[(int64_t)row * parts + part] = s;
+  if constexpr (TOP) {
+    u64* keys = reinterpret_cast<u64*>(reinterpret_cast<char*>(p.work) + keys_at(p, parts)) + ((int64_t)row * parts + part) * p.top;
+    auto put = [&](const int place, const u64 key) {
+      if (parts == 1) put_alternative(p, row, place, key, r);
+      else keys[place] = key;
+    };
+    __syncthreads();
+    const float bound = room.bound;
+    if (mine >= bound && mine > -INFINITY) {
+#pragma unroll
+      for (int i = 0; i < kEach / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = logit_at<T>(l[i], e);
+          if (x >= bound && x > -INFINITY) {
+            const int at = atomicAdd(&room.listed, 1);
+            if (at < kList) room.list[at] = key_of(x, first + (i * NT + tid) * 8 + e);
+          }
+        }
+    }
+    __syncthreads();
+    int n = room.listed;
+    if (n > kList) {
+      best_by_rounds<T, NT>(logits, first, end, p.top, room, room.list);
+      __syncthreads();
+      n = p.top;
+    }
+    for (int c = tid; c < n; c += NT) {
+      const u64 key = room.list[c];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += room.list[j] > key || (room.list[j] == key && j < c);      // (places without a logit are alike)
+      if (rank < p.top) put(rank, key);
+    }
+    for (int place = n + tid; place < p.top; place += NT) put(place, 0);
   }
 }
 
@@ -207,21 +254,8 @@ __global__ void __launch_bounds__(256) log_probs_join_kernel(const LogProbsParam
   const u64* keys = reinterpret_cast<const u64*>(reinterpret_cast<const char*>(p.work) + keys_at(p, parts)) + (int64_t)row * n;
   for (int c = threadIdx.x; c < n; c += 256) list[c] = keys[c];
   const Sums* sums = reinterpret_cast<const Sums*>(p.work) + (int64_t)row * parts;
-  Sums s = {-INFINITY, 0.f, 0.f, 0.f};
-  for (int k = 0; k < parts; ++k) s.most = fmaxf(s.most, sums[k].most);
-  for (int k = 0; k < parts; ++k) {
-    const Sums a = sums[k];
-    if (!(a.most > -INFINITY)) continue;
-    if (a.most == s.most) {
-      s.count += a.count;
-      s.low += a.low;
-      s.away += a.away;
-    } else {
-      const float d = fminf(s.most - a.most, 1e4f), f = __builtin_amdgcn_exp2f(d * -kLog2e), w = a.count + a.low;
-      s.low = __builtin_fmaf(f, w, s.low);
-      s.away = __builtin_fmaf(f, __builtin_fmaf(d, w, a.away), s.away);
-    }
-  }
+  const int lane = threadIdx.x & 63;
+  const Sums s = joined(sums[min(lane, parts - 1)], lane < parts);
   __syncthreads();
   const RowResult r = finish_row(p, row, s);
   for (int c = threadIdx.x; c < n; c += 256) {
@@ -237,13 +271,19 @@ hipError_t log_probs_as(const LogProbsParams& p, const int parts, hipStream_t st
   // (parts begin at whole groups of eight, so at 16-byte boundaries where rows do)
   const int each = ((p.V + parts - 1) / parts + 7) / 8 * 8;
   const dim3 grid((unsigned)p.rows * parts);
+#define OHIP_LOG_PROBS(NT, VECTOR)                                                                                                   \
+  do {                                                                                                                             \
+    if (p.top > 0) hipLaunchKernelGGL((log_probs_kernel<T, NT, VECTOR, true>), grid, dim3(NT), 0, stream, p, parts, each);          \
+    else hipLaunchKernelGGL((log_probs_kernel<T, NT, VECTOR, false>), grid, dim3(NT), 0, stream, p, parts, each);                   \
+  } while (0)
   if (p.V <= kNarrow * kEach) {
-    if (p.V % 8 == 0) hipLaunchKernelGGL((log_probs_kernel<T, kNarrow, true>), grid, dim3(kNarrow), 0, stream, p, parts, each);
-    else hipLaunchKernelGGL((log_probs_kernel<T, kNarrow, false>), grid, dim3(kNarrow), 0, stream, p, parts, each);
+    if (p.V % 8 == 0) OHIP_LOG_PROBS(kNarrow, true);
+    else OHIP_LOG_PROBS(kNarrow, false);
   } else {
-    if (p.V % 8 == 0) hipLaunchKernelGGL((log_probs_kernel<T, kWide, true>), grid, dim3(kWide), 0, stream, p, parts, each);
-    else hipLaunchKernelGGL((log_probs_kernel<T, kWide, false>), grid, dim3(kWide), 0, stream, p, parts, each);
+    if (p.V % 8 == 0) OHIP_LOG_PROBS(kWide, true);
+    else OHIP_LOG_PROBS(kWide, false);
   }
+#undef OHIP_LOG_PROBS
   return hipGetLastError();
 }
 

@@ -2,7 +2,8 @@
 //
 // Rows are the queries that share a head of keys: row r of a sequence is query r % group of its token r / group, so that
 // a tile of rows reads each key once for all of them.  Softmax in one pass: per row the running maximum m and
-// the sum l of exp(s - m), and o = sum exp(s - m) v rescaled when m grows.
+// the sum l of exp(s - m), and o = sum exp(s - m) v, rescaled when m grows.  m follows the true maximum only when that is 2^8
+// times larger: the sums hold that, and o is seldom rescaled.
 //
 // Lengths are on the device, so the launch cannot be cut to them: every workgroup finds its piece - a tile of rows, a head
 // and a stretch of the keys - from the lengths itself (attention_pieces.h).  Long sequences with few rows are cut
@@ -112,11 +113,13 @@ __device__ __forceinline__ Found find(const Args& a, const int key) {
   return kNowhere;
 }
 // Pieces of a sequence: heads side by side (their keys are neighbours in memory), then stretches, then tiles of rows from
-// the last one on, which sees the most keys.
+// the last one on, which sees the most keys.  Neighbouring workgroups are on different XCDs, and a head's keys lie in few
+// channels of an XCD's L2 (every heads * head size elements): from one stretch or tile to the next the heads move on by
+// a place or two, so that each XCD has all of them.
 struct Piece { int head, cut, tile, slot; };
 __device__ __forceinline__ Piece piece_at(const Found& f, const int heads, const int in_seq) {
-  const int rest = in_seq / heads;
-  return {in_seq - rest * heads, rest % f.cuts, f.tiles - 1 - rest / f.cuts, f.slot0 + in_seq};
+  const int rest = in_seq / heads, head = (int)((unsigned)(in_seq + f.seq + rest + (rest >> 1) + (rest >> 2) + (rest >> 3)) % (unsigned)heads);
+  return {head, rest % f.cuts, f.tiles - 1 - rest / f.cuts, f.slot0 + rest * heads + head};
 }
 __device__ __forceinline__ int slot_of(const Found& f, const int heads, const int tile, const int head, const int cut) {
   return f.slot0 + ((f.tiles - 1 - tile) * f.cuts + cut) * heads + head;
@@ -198,48 +201,53 @@ template <typename T, int DP> struct FewShape {
   static constexpr int KC = DP * sizeof(T) / 64;            // 16-byte vectors of a key that a lane has
 };
 
-// 16 bytes (or 8) of a row from element `at` on; zeros behind its d elements.
-template <typename T, int W>
+// 16 bytes (or 8) of a row from element `at` on; behind its d elements any of it.  No branch: a load that is not taken by all
+// lanes would be waited for where the lanes meet again, and everything requested before it.
+template <typename T, int W, bool WHOLE>
 __device__ __forceinline__ void load_part(const T* row, const int at, const int d, unsigned* to) {
-  constexpr int PER = W * 4 / (int)sizeof(T);
   static_assert(W == 2 || W == 4, "8 or 16 bytes");
-  if (at + PER <= d) {
-    if constexpr (W == 4) {
-      const uintx4 v = *reinterpret_cast<const uintx4*>(row + at);
-      to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
-    } else {
-      const uintx2 v = *reinterpret_cast<const uintx2*>(row + at);
-      to[0] = v.x; to[1] = v.y;
-    }
+  const T* from = row + (WHOLE || at < d ? at : 0);
+  if constexpr (W == 4) {
+    const uintx4 v = *reinterpret_cast<const uintx4*>(from);
+    to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
   } else {
-#pragma unroll
-    for (int i = 0; i < W; ++i) to[i] = 0u;
+    const uintx2 v = *reinterpret_cast<const uintx2*>(from);
+    to[0] = v.x; to[1] = v.y;
   }
 }
 
 // A row's weight for a key that it does not see is zero, and zero times an infinite or missing value is none.  Where a
 // tile has such weights, such values leave it; whoever found one looks at all values of its piece once more in the end and adds
 // those to the rows that see them (what else a row's sum holds, and the weight, make no difference then).
-template <typename T> __device__ __forceinline__ bool not_finite(const unsigned w) {
-  if constexpr (sizeof(T) == 4) return (w & 0x7f800000u) == 0x7f800000u;
-  constexpr unsigned m = std::is_same<T, f16_t>::value ? 0x7c00u : 0x7f80u;
-  return (w & m) == m || (w >> 16 & m) == m;
+template <typename T> constexpr unsigned kExponent = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, f16_t>::value ? 0x7c00u : 0x7f80u;
+// The largest exponents of a dword's elements so far, and whether one says infinite or missing.
+template <typename T> __device__ __forceinline__ unsigned with_exponents(const unsigned most, const unsigned w) {
+  if constexpr (sizeof(T) == 4) {
+    return max(most, w & kExponent<T>);
+  } else {
+    typedef unsigned short ushortx2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(ushortx2, most), __builtin_bit_cast(ushortx2, w & (kExponent<T> << 16 | kExponent<T>))));
+  }
+}
+template <typename T> __device__ __forceinline__ bool not_finite(const unsigned most) {
+  if constexpr (sizeof(T) == 4) return most == kExponent<T>;
+  else return (most & 0xffffu) == kExponent<T> || most >> 16 == kExponent<T>;
 }
 template <typename T> __device__ __forceinline__ unsigned finite_part(const unsigned w) {
-  if constexpr (sizeof(T) == 4) return not_finite<T>(w) ? 0u : w;
-  constexpr unsigned m = std::is_same<T, f16_t>::value ? 0x7c00u : 0x7f80u;
-  return ((w & m) == m ? 0u : w & 0xffffu) | ((w >> 16 & m) == m ? 0u : w & 0xffff0000u);
+  constexpr unsigned m = kExponent<T>;
+  if constexpr (sizeof(T) == 4) return (w & m) == m ? 0u : w;
+  else return ((w & m) == m ? 0u : w & 0xffffu) | ((w >> 16 & m) == m ? 0u : w & 0xffff0000u);
 }
-// o: this lane's columns `column(i)` .. + 3 of its row, N times four; rows_of(t): as in the kernels, KT keys a tile.
-template <typename T, int KT, int N, typename RowsOf, typename Column, typename Add>
+// column(i): this lane's columns of its row, N times four; rows_of, row_at: as in the kernels, KT keys a tile.
+template <typename T, int KT, int N, typename RowsOf, typename RowAt, typename Column, typename Add>
 __device__ __forceinline__ void add_odd_values(const Args a, const char* vc, const int64_t row_bytes, const int t_begin, const int t_end, const int step, const int last, RowsOf rows_of,
-                                            Column column, Add add) {
+                                            RowAt row_at, Column column, Add add) {
 #pragma unroll 1
   for (int t = t_begin; t < t_end; t += step) {
-    const int rows_ = rows_of(t);
+    const auto rows_ = rows_of(t);
 #pragma unroll 1
     for (int k = 0; k < KT; ++k) {
-      const int row = __shfl(rows_, k), place = t * KT + k;
+      const int row = row_at(rows_, t, k), place = t * KT + k;
       if (row < 0 || place > last || (a.window != 0 && place <= last - a.window)) continue;
       const T* v = reinterpret_cast<const T*>(vc + row * row_bytes);
 #pragma unroll
@@ -256,12 +264,12 @@ __device__ __forceinline__ void add_odd_values(const Args a, const char* vc, con
 }
 
 template <typename T, int DP> constexpr int kFewLds = (4 * 16 * (DP + 4) + 2 * 4 * 16) * (int)sizeof(float);
-template <typename T, int DP>
+template <typename T, int DP, bool WHOLE, bool TWO>
 __device__ __forceinline__ void attend_few(const Args& a, const Found& f, unsigned char* smem) {
   using F = Few<T>;
   using S = FewShape<T, DP>;
   constexpr bool WIDE = DP > 128;
-  constexpr int R = 16, KEYS = F::KEYS, KT = F::KT, VE = S::VE, VW = S::VW, KC = S::KC;
+  constexpr int R = 16, KEYS = F::KEYS, KT = F::KT, VE = S::VE, VW = S::VW, KC = S::KC, PER = 16 / (int)sizeof(T);
   static_assert(R == Ways<T, WIDE>::few.rows && KT == Ways<T, WIDE>::few.keys, "as the pieces are cut");
   auto part = reinterpret_cast<float (*)[16][DP + 4]>(smem);
   auto part_m = reinterpret_cast<float (*)[16]>(smem + sizeof(float) * 4 * 16 * (DP + 4));
@@ -285,39 +293,66 @@ __device__ __forceinline__ void attend_few(const Args& a, const Found& f, unsign
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
       unsigned w[4];
-      load_part<T, 4>(row, (4 * c + g) * (16 / (int)sizeof(T)), a.d, w);
-      q[c] = uintx4{w[0], w[1], w[2], w[3]};
+      load_part<T, 4, WHOLE>(row, (4 * c + g) * PER, a.d, w);
+      q[c] = WHOLE || (4 * c + g) * PER < a.d ? uintx4{w[0], w[1], w[2], w[3]} : uintx4{0u, 0u, 0u, 0u};
     }
   }
-  // the rows of the cache that hold a tile's keys, lane l: key l % KT (-1: not there)
-  auto rows_of = [&](const int t) __attribute__((always_inline)) -> int {
-    const int place = t * KT + (lane & (KT - 1));
-    if (t >= t_end || place >= seen.hi) return -1;
-    const int index = fast_div(place, a.page_magic, a.page_shift);
-    return cache_row(table[index], place - index * a.page, a.page, a.pages);
+  // Where the keys of a tile lie.  TWO: in two pages at most, whose numbers come by scalar loads; otherwise lane l looks up key
+  // l % KT.  A number is looked at one tile after it was requested: vector loads return in order, and whoever waits for one
+  // waits for all keys and values requested before it.
+  struct Where { int first, second, edge; };      // rows of place 0 of either page, if it went on that way, and where the second begins
+  constexpr int kNone = INT32_MIN;
+  const int end = at_least(seen.hi, 1) - 1;       // (lookups stay in front of it)
+  auto look_up = [&](const int t) __attribute__((always_inline)) -> Where {
+    if constexpr (TWO) {
+      const int index = fast_div(at_most(t * KT, end), a.page_magic, a.page_shift), next = at_most(index + 1, fast_div(end, a.page_magic, a.page_shift));
+      const auto numbers = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)table;
+      return {numbers[index], numbers[next], (index + 1) * a.page};
+    } else {
+      return {table[fast_div(at_most(t * KT + (lane & (KT - 1)), end), a.page_magic, a.page_shift)], 0, 0};
+    }
   };
+  auto found = [&](const Where& w, const int t) __attribute__((always_inline)) -> Where {
+    if constexpr (TWO) {
+      const int p = t < t_end ? cache_row(w.first, 0, a.page, a.pages) : -1, q = t < t_end ? cache_row(w.second, 0, a.page, a.pages) : -1;
+      return {p < 0 ? kNone : p - (w.edge - a.page), q < 0 ? kNone : q - w.edge, w.edge};
+    } else {
+      const int place = t * KT + (lane & (KT - 1));
+      const int row = cache_row(w.first, place - fast_div(place, a.page_magic, a.page_shift) * a.page, a.page, a.pages);
+      return {t < t_end && place < seen.hi ? row : -1, 0, 0};
+    }
+  };
+  auto row_at = [&](const Where& w, const int t, const int key) __attribute__((always_inline)) -> int {      // -1: not there
+    if constexpr (TWO) {
+      const int place = t * KT + key, base = place < w.edge ? w.first : w.second;
+      return place < seen.hi && base != kNone ? base + place : -1;
+    } else {
+      return __shfl(w.first, key);
+    }
+  };
+  auto rows_of = [&](const int t) { return found(look_up(t), t); };
   auto key_of_slot = [&](const int j) { return (j >> 2) * 16 + g * 4 + (j & 3); };
   uintx4 kf[F::BLOCKS][KC];
-  auto load_keys = [&](const int rows_) __attribute__((always_inline)) {
+  auto load_keys = [&](const Where& rows_, const int t) __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < F::BLOCKS; ++b) {
-      const T* row = reinterpret_cast<const T*>(kc + max(__shfl(rows_, 16 * b + l16), 0) * row_bytes);
+      const T* row = reinterpret_cast<const T*>(kc + max(row_at(rows_, t, 16 * b + l16), 0) * row_bytes);
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
         unsigned w[4];
-        load_part<T, 4>(row, (4 * c + g) * (16 / (int)sizeof(T)), a.d, w);
+        load_part<T, 4, WHOLE>(row, (4 * c + g) * PER, a.d, w);
         kf[b][c] = uintx4{w[0], w[1], w[2], w[3]};
       }
     }
   };
   unsigned vf[KEYS][VW];
-  auto load_values = [&](const int rows_) __attribute__((always_inline)) {
+  auto load_values = [&](const Where& rows_, const int t) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < KEYS; ++j) {
-      const T* row = reinterpret_cast<const T*>(vc + max(__shfl(rows_, key_of_slot(j)), 0) * row_bytes);
-      constexpr int W = VW < 4 ? 2 : 4, PER = W * 4 / (int)sizeof(T);
+      const T* row = reinterpret_cast<const T*>(vc + max(row_at(rows_, t, key_of_slot(j)), 0) * row_bytes);
+      constexpr int W = VW < 4 ? 2 : 4;
 #pragma unroll
-      for (int w = 0; w < VW / W; ++w) load_part<T, W>(row, l16 * VE + w * PER, a.d, &vf[j][w * W]);
+      for (int w = 0; w < VW / W; ++w) load_part<T, W, WHOLE>(row, l16 * VE + w * (W * 4 / (int)sizeof(T)), a.d, &vf[j][w * W]);
     }
   };
 
@@ -327,45 +362,59 @@ __device__ __forceinline__ void attend_few(const Args& a, const Found& f, unsign
 #pragma unroll
   for (int e = 0; e < VE; ++e) o[e] = floatx4{0.f, 0.f, 0.f, 0.f};
   const float to_log2 = a.scale * kLog2e;
-  int here = rows_of(t_begin + wave), next = rows_of(t_begin + wave + 4);
-  if (t_begin + wave < t_end) {
-    load_keys(here);
-    load_values(here);
-  }
-  // (a wavefront's requests for a tile are on their way while the one before is used)
+  const int window = a.window == 0 ? 1 << 30 : a.window;      // (no place lies further back)
+  const int first_last = f.span.cached + r0 / a.group, last_last = f.span.cached + (r0 + rows - 1) / a.group;
+  // A wavefront's requests are one tile ahead of their use (keys behind the scores' product, values behind the other), the
+  // rows that they are for one more.  All are made, also those behind the last tile (of the cache's first row): where some paths
+  // have fewer requests, waits are for all of them.
+  Where here = found(look_up(t_begin + wave), t_begin + wave), ahead = look_up(t_begin + wave + 4);      // (ahead: numbers as they come)
+  load_keys(here, t_begin + wave);
+  load_values(here, t_begin + wave);
 #pragma unroll 1
   for (int t = t_begin + wave; t < t_end; t += 4) {
+    const Where next = found(ahead, t + 4);
+    ahead = look_up(t + 8);
     floatx4 s[F::BLOCKS];
 #pragma unroll
     for (int k = 0; k < F::BLOCKS; ++k) {
       s[k] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < KC; ++c) s[k] = mma_vec<T>(kf[k][c], q[c], s[k]);
+      for (int c = 0; c < KC; ++c) s[k] = mma_vec<T>(WHOLE || (4 * c + g) * PER < a.d ? kf[k][c] : uintx4{0u, 0u, 0u, 0u}, q[c], s[k]);
     }
-    if (t + 4 < t_end) load_keys(next);
-    const int after = rows_of(t + 8);
+    load_keys(next, t + 4);
+    // what all rows see needs no mask
+    bool there = true;
+    if constexpr (TWO) there = here.first != kNone && (here.second != kNone || here.edge >= t * KT + KT);
+    else there = __all(here.first >= 0);
+    const bool masked = !there || t * KT + KT > min(first_last + 1, seen.hi) || t * KT <= last_last - window;
     float p[KEYS], most = -INFINITY;
-    bool masked = false;
 #pragma unroll
-    for (int j = 0; j < KEYS; ++j) {
-      const int place = t * KT + key_of_slot(j);
-      const bool sees = __shfl(here, key_of_slot(j)) >= 0 && place <= last && (a.window == 0 || place > last - a.window);
-      masked = masked || !sees;
-      p[j] = sees ? s[j >> 2][j & 3] * to_log2 : -INFINITY;
-      most = fmaxf(most, p[j]);
+    for (int j = 0; j < KEYS; ++j) p[j] = s[j >> 2][j & 3] * to_log2;
+    if (masked) {
+#pragma unroll
+      for (int j = 0; j < KEYS; ++j) {
+        const int place = t * KT + key_of_slot(j);
+        const bool sees = (row_at(here, t, key_of_slot(j)) >= 0) & (place <= last) & (place > last - window);
+        p[j] = sees ? p[j] : -INFINITY;
+      }
     }
-    most = fmaxf(m, over_row(most, [](float x, float y) { return fmaxf(x, y); }));
-    const float base = most == -INFINITY ? 0.f : most;
-    const float shrink = __builtin_amdgcn_exp2f(m - base);
-    m = most;
-    l *= shrink;
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j) most = fmaxf(most, p[j]);
+    most = over_row(most, [](float x, float y) { return fmaxf(x, y); });
+    const bool grows = most > m + 8.f;
+    if (__any(grows)) {
+      const float now = grows ? most : m, shrink = grows ? __builtin_amdgcn_exp2f(m - now) : 1.f;
+      m = now;
+      l *= shrink;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) o[e] *= shrink;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int j = 0; j < KEYS; ++j) {
       p[j] = __builtin_amdgcn_exp2f(p[j] - base);
       l += p[j];
     }
-#pragma unroll
-    for (int e = 0; e < VE; ++e) o[e] *= shrink;
     // element e of this lane's keys, as an operand
     auto column = [&](const int e, unsigned (&v)[4]) __attribute__((always_inline)) {
 #pragma unroll
@@ -374,13 +423,13 @@ __device__ __forceinline__ void attend_few(const Args& a, const Found& f, unsign
     uintx4 weights;
     if constexpr (sizeof(T) == 4) weights = uintx4{__float_as_uint(p[0]), __float_as_uint(p[1]), __float_as_uint(p[2]), __float_as_uint(p[3])};
     else weights = pack8_rne<T>(p);
-    if (__any(masked)) {
-      bool found = false;
+    if (masked) {
+      unsigned most = 0;
 #pragma unroll
       for (int j = 0; j < KEYS; ++j)
 #pragma unroll
-        for (int w = 0; w < VW; ++w) found = found || not_finite<T>(vf[j][w]);
-      if (__any(found)) {
+        for (int w = 0; w < VW; ++w) most = with_exponents<T>(most, vf[j][w]);
+      if (__any(not_finite<T>(most))) {
         odd = true;
 #pragma unroll
         for (int j = 0; j < KEYS; ++j)
@@ -394,13 +443,12 @@ __device__ __forceinline__ void attend_few(const Args& a, const Found& f, unsign
       column(e, v);
       o[e] = mma_vec<T>(uintx4{v[0], v[1], v[2], v[3]}, weights, o[e]);
     }
-    if (t + 4 < t_end) load_values(next);
+    load_values(next, t + 4);
     here = next;
-    next = after;
   }
 
   if (odd)
-    add_odd_values<T, KT, VE>(a, vc, row_bytes, t_begin + wave, t_end, 4, last, rows_of, [&](const int n) { return 4 * (g * VE + n); },
+    add_odd_values<T, KT, VE>(a, vc, row_bytes, t_begin + wave, t_end, 4, last, rows_of, row_at, [&](const int n) { return 4 * (g * VE + n); },
                               [&](const int n, const int j, const float x) { o[(4 * n + j) % VE][(4 * n + j) / VE] += x; });
 
   // ---- the wavefronts' parts
@@ -456,7 +504,6 @@ __device__ __forceinline__ void attend_few(const Args& a, const Found& f, unsign
 // operand of the second product as they are (C[d][row], the order of its inner axis being free).  The values'
 // operand has neighbouring keys in a lane: ds_read_b64_tr_b16 reads sixteen columns of four keys that way round.
 // LDS rows keep their 16-byte chunks in other places (key_slot, value_slot), so that what is read at a time lies in different banks.
-// The running maximum follows the true one only when that is 2^8 larger: the sums hold that, and o is seldom rescaled.
 template <int DP> struct Big {
   static constexpr int KT = DP > 128 ? 32 : 64, BLOCKS = KT / 32;
   static constexpr int CHUNKS = DP / 8, ROW = DP * 2;                  // 16-byte chunks and bytes of a row
@@ -554,13 +601,14 @@ __device__ __forceinline__ void big_tile(const Args& a, unsigned char* __restric
   }
   // element i of block b: place place0 + 32 b + 8 (i / 4) + 4 h + i % 4
   if (masked) {
+    const int from_place = a.window == 0 ? -1 : w.last - a.window;
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) {
       const unsigned there = (unsigned)(valid >> (32 * b)) >> (4 * h);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int in = 8 * (i >> 2) + (i & 3), place = place0 + 32 * b + 4 * h + in;
-        const bool sees = (there >> in & 1u) != 0 && place <= w.last && (a.window == 0 || place > w.last - a.window);
+        const bool sees = ((there >> in & 1u) != 0) & (place <= w.last) & (place > from_place);
         s[b][i] = sees ? s[b][i] : -INFINITY;
       }
     }
@@ -608,13 +656,14 @@ __device__ __forceinline__ void big_tile(const Args& a, unsigned char* __restric
     }
   };
   if (masked) {       // (for all four wavefronts, which look at the same values)
-    bool found = false;
+    unsigned most = 0;
 #pragma unroll 4
     for (int c = lane; c < B::TILE / 16; c += 64) {
       const uintx4 v = reinterpret_cast<const uintx4*>(values)[c];
-      found = found || not_finite<T>(v.x) || not_finite<T>(v.y) || not_finite<T>(v.z) || not_finite<T>(v.w);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) most = with_exponents<T>(most, v[j]);
     }
-    if (__any(found)) {
+    if (__any(not_finite<T>(most))) {
       w.odd = true;
       __syncthreads();
 #pragma unroll 1
@@ -665,9 +714,9 @@ __device__ __forceinline__ void attend_many(const Args& a, const Found& f, unsig
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
       unsigned x[4];
-      load_part<T, 4>(row, 16 * c + 8 * h, a.d, x);
+      load_part<T, 4, WHOLE>(row, 16 * c + 8 * h, a.d, x);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w.q[c][j] = (x[j] & keep) ^ flip;
+      for (int j = 0; j < 4; ++j) w.q[c][j] = WHOLE || 16 * c + 8 * h < a.d ? (x[j] & keep) ^ flip : 0u;
     }
   }
   w.last = f.span.cached + token;
@@ -680,14 +729,19 @@ __device__ __forceinline__ void attend_many(const Args& a, const Found& f, unsig
     for (int i = 0; i < 16; ++i) w.o[d][i] = 0.f;
   // what all rows of the tile see
   const int first_last = f.span.cached + r0 / a.group, last_last = f.span.cached + (r0 + rows - 1) / a.group;
-  auto rows_of = [&](const int t) __attribute__((always_inline)) -> int {
-    const int place = t * KT + (lane & (KT - 1));
-    if (t >= t_end || place >= seen.hi) return -1;
-    const int index = fast_div(place, a.page_magic, a.page_shift);
-    return cache_row(table[index], place - index * a.page, a.page, a.pages);
+  // (a number is looked at one tile after it was requested: what is on its way into LDS would be waited for with it)
+  const int end = at_least(seen.hi, 1) - 1;
+  auto look_up = [&](const int t) __attribute__((always_inline)) -> int {
+    return table[fast_div(at_most(t * KT + (lane & (KT - 1)), end), a.page_magic, a.page_shift)];
   };
+  auto found = [&](const int number, const int t) __attribute__((always_inline)) -> int {
+    const int place = t * KT + (lane & (KT - 1));
+    const int row = cache_row(number, place - fast_div(place, a.page_magic, a.page_shift) * a.page, a.page, a.pages);
+    return t < t_end && place < seen.hi ? row : -1;
+  };
+  auto rows_of = [&](const int t) { return found(look_up(t), t); };
   if (t_begin < t_end) {
-    int here = rows_of(t_begin), next = rows_of(t_begin + 1);
+    int here = rows_of(t_begin), number = look_up(t_begin + 1);
 #pragma unroll
     for (int i = 0; i < B::REQUESTS; ++i) {
       const int row = (wave * B::REQUESTS + i) * B::PER + lane / B::CHUNKS, slot = lane % B::CHUNKS;
@@ -704,14 +758,14 @@ __device__ __forceinline__ void attend_many(const Args& a, const Found& f, unsig
       __syncthreads();
       const unsigned long long valid = __ballot(here >= 0), all = KT == 64 ? ~0ull : 0xffffffffull;
       const bool masked = (valid & all) != all || t * KT + KT - 1 > first_last || (a.window != 0 && t * KT <= last_last - a.window);
-      const int after = rows_of(t + 2), at = (t - t_begin) & 1;
+      const int next = found(number, t + 1), at = (t - t_begin) & 1;
+      number = look_up(t + 2);
       big_tile<T, DP, WHOLE>(a, smem + (1 - at) * B::STAGE, smem + at * B::STAGE, next, t + 1 < t_end, kc, vc, row_bytes, t * KT, valid & all, masked, mult, lane, wave, w);
       here = next;
-      next = after;
     }
   }
   if (w.odd)
-    add_odd_values<T, KT, DP / 8>(a, vc, row_bytes, t_begin, t_end, 1, w.last, rows_of, [&](const int n) { return 8 * n + 4 * h; },
+    add_odd_values<T, KT, DP / 8>(a, vc, row_bytes, t_begin, t_end, 1, w.last, rows_of, [](const int rows_, int, const int k) { return __shfl(rows_, k); }, [&](const int n) { return 8 * n + 4 * h; },
                                   [&](const int n, const int j, const float x) { w.o[n / 4][n % 4 * 4 + j] += x; });
   const float sum = over_halves(w.l, [](float x, float y) { return x + y; });
   if (wave * 32 + l32 >= rows) return;
@@ -759,53 +813,79 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) attend_kernel(const Arg
       return;
     }
   }
-  attend_few<T, DP>(a, f, smem);
+  constexpr int KT = Few<T>::KT;
+  if (a.page >= KT || 2 * a.page == KT) attend_few<T, DP, WHOLE, true>(a, f, smem);      // (tiles begin at multiples of KT)
+  else attend_few<T, DP, WHOLE, false>(a, f, smem);
 }
 
 // ------------------------------------------------------------------ the parts --
-// A workgroup has a few neighbouring tokens of one head, a wavefront one row after the other.
+// A workgroup has `each` neighbouring rows of the result, its wavefronts one after the other.  Lanes first bring m and l of
+// up to 64 parts at once, then, a group of lanes a part, their rows.
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(256) attention_join_kernel(const Args a, const int tokens_each) {
+__global__ void __launch_bounds__(256) attention_join_kernel(const Args a, const int each) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int head = blockIdx.x % (unsigned)a.kv_heads, token0 = blockIdx.x / (unsigned)a.kv_heads * tokens_each;
+  const int q_heads = a.kv_heads * a.group;
+  const int end = min((int)(blockIdx.x + 1) * each, a.tokens * q_heads);
+  const int lanes = a.d <= 64 ? 16 : a.d <= 128 ? 32 : 64, sub = lane / lanes, col = lane % lanes * 4, at_once = 64 / lanes;
+  const bool mine = col < a.d;
   Found f = kNowhere;
-  for (int token = token0; token < min(token0 + tokens_each, a.tokens); ++token) {
+#pragma unroll 1
+  for (int at = blockIdx.x * each + wave; at < end; at += 4) {
+    const int token = at / q_heads, q = at - token * q_heads, head = q / a.group;
     if (f.seq < 0 || token < f.span.first || token >= f.span.first + f.span.n) f = find<T, WIDE, true>(a, token);
-    if (f.seq >= 0 && f.cuts == 1) continue;
-    for (int q = wave; q < a.group; q += 4) {
-      T* y = reinterpret_cast<T*>(a.y) + ((int64_t)token * a.kv_heads * a.group + (int64_t)head * a.group + q) * a.d;
-      if (f.seq < 0) {       // no sequence's
-        for (int c = lane * 4; c < a.d; c += 256) store4<T>(y + c, floatx4{0.f, 0.f, 0.f, 0.f}, 4, true);
-        continue;
-      }
-      const Parts parts = parts_of<T, WIDE>(a, f.many);
-      const int row = (token - f.span.first) * a.group + q, tile = row / parts.rows, r = row - tile * parts.rows;
-      float most = -INFINITY;
-      for (int cut = 0; cut < f.cuts; ++cut) {
-        const int slot = slot_of(f, a.kv_heads, tile, head, cut);
-        if (slot < parts.slots) most = fmaxf(most, parts.sums(slot, r)[0]);
-      }
-      float sum = 0.f;
-      floatx4 v = {0.f, 0.f, 0.f, 0.f};
-      for (int cut = 0; cut < f.cuts; ++cut) {
-        const int slot = slot_of(f, a.kv_heads, tile, head, cut);
-        if (slot >= parts.slots) continue;
+    T* y = reinterpret_cast<T*>(a.y) + (int64_t)at * a.d;
+    if (f.seq < 0) {       // no sequence's
+      if (sub == 0 && mine) store4<T>(y + col, floatx4{0.f, 0.f, 0.f, 0.f}, 4, true);
+      continue;
+    }
+    if (f.cuts == 1) {     // nothing of this sequence is in parts
+      const int skip = min(end, (f.span.first + f.span.n) * q_heads) - at;
+      at += (skip - 1) / 4 * 4;
+      continue;
+    }
+    const Parts parts = parts_of<T, WIDE>(a, f.many);
+    const int row = (token - f.span.first) * a.group + (q - head * a.group), tile = row / parts.rows, r = row - tile * parts.rows;
+    float most = -INFINITY, sum = 0.f;
+    floatx4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int c0 = 0; c0 < f.cuts; c0 += 64) {
+      const int n = min(f.cuts - c0, 64), slot = slot_of(f, a.kv_heads, tile, head, c0 + min(lane, n - 1));
+      float m = -INFINITY, l = 0.f;
+      if (lane < n && slot < parts.slots) {
         const float* ml = parts.sums(slot, r);
-        if (ml[1] == 0.f) continue;
-        const float factor = ml[0] == -INFINITY ? ml[1] : __builtin_amdgcn_exp2f(ml[0] - most);
-        sum = __builtin_fmaf(factor, ml[1], sum);
-        if (lane * 4 < a.d) {
-          const floatx4 x = *reinterpret_cast<const floatx4*>(parts.values(slot, r) + lane * 4);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(factor, x[i], v[i]);
-        }
+        m = ml[0];
+        l = ml[1];
       }
-      if (lane * 4 < a.d) {
+      const float now = fmaxf(most, wave_max(m)), base = now == -INFINITY ? 0.f : now;
+      const float shrink = __builtin_amdgcn_exp2f(most - base);
+      // (a part without keys has l = 0 and counts nothing; one whose scores are all NaN has no m, and l is NaN)
+      const float factor = l == 0.f ? 0.f : m == -INFINITY ? l : __builtin_amdgcn_exp2f(m - base);
+      sum = sum * shrink + wave_sum(l == 0.f ? 0.f : factor * l);
+      v *= shrink;
+      most = now;
+#pragma unroll 1
+      for (int j0 = 0; j0 < n; j0 += 4 * at_once) {
+        floatx4 x[4];
+        float by[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = sum == 0.f ? 0.f : v[i] / sum;
-        store4<T>(y + lane * 4, v, 4, true);
+        for (int k = 0; k < 4; ++k) {
+          const int j = j0 + k * at_once + sub, part = min(j, n - 1), from = slot_of(f, a.kv_heads, tile, head, c0 + part);
+          by[k] = __shfl(factor, part);
+          if (j >= n || from >= parts.slots) by[k] = 0.f;
+          x[k] = *reinterpret_cast<const floatx4*>(parts.values(min(from, parts.slots - 1), r) + (mine ? col : 0));
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = by[k] != 0.f ? __builtin_fmaf(by[k], x[k][i], v[i]) : v[i];
       }
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      for (int o = lanes; o < 64; o *= 2) v[i] += __shfl_xor(v[i], o);
+      v[i] = sum == 0.f ? 0.f : v[i] / sum;
+    }
+    if (sub == 0 && mine) store4<T>(y + col, v, 4, true);
   }
 }
 
@@ -851,10 +931,7 @@ hipError_t attend_with(const Args& a, hipStream_t stream) {
 }
 template <typename T, int DP>
 hipError_t attend_wide(const Args& a, hipStream_t stream) {
-  if constexpr (sizeof(T) == 2) {
-    if (a.d == DP) return attend_with<T, DP, true>(a, stream);
-  }
-  return attend_with<T, DP, false>(a, stream);
+  return a.d == DP ? attend_with<T, DP, true>(a, stream) : attend_with<T, DP, false>(a, stream);
 }
 template <typename T>
 hipError_t attend_as(const PagedAttentionParams& p, hipStream_t stream) {
@@ -866,8 +943,8 @@ hipError_t attend_as(const PagedAttentionParams& p, hipStream_t stream) {
 template <typename T>
 hipError_t join_as(const PagedAttentionParams& p, hipStream_t stream) {
   const Args a = args_of<T>(p);
-  const int each = p.group >= 16 ? 1 : 16 / p.group;
-  const dim3 grid((unsigned)((p.tokens + each - 1) / each) * (unsigned)p.kv_heads);
+  const int rows = p.tokens * p.kv_heads * p.group, each = std::max(4, (rows + 2047) / 2048);   // (a row a wavefront while there are few)
+  const dim3 grid((unsigned)((rows + each - 1) / each));
   if (p.d > 128) hipLaunchKernelGGL((attention_join_kernel<T, true>), grid, dim3(256), 0, stream, a, each);
   else hipLaunchKernelGGL((attention_join_kernel<T, false>), grid, dim3(256), 0, stream, a, each);
   return hipGetLastError();
