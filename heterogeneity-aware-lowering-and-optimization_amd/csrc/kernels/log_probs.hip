@@ -17,7 +17,7 @@
 namespace ohip {
 namespace {
 
-constexpr int kEach = 32, kGroups = 64, kList = 1024, kWide = 1024, kNarrow = 256;
+constexpr int kEach = 32, kGroups = 64, kList = 1024, kWide = 1024, kNarrow = 256, kManyRows = 1024;
 constexpr float kLog2e = 1.44269504f;
 typedef unsigned long long u64;
 
@@ -34,8 +34,7 @@ __device__ __forceinline__ float logit_of(const u64 k) {
 // What a part of a row, or all of it, adds up to.
 struct Sums {
   float most;    // the largest logit
-  float count;   // how often
-  float low;     // sum of exp(l - most) over the others
+  float rest;    // sum of exp(l - most) over the others
   float away;    // sum of exp(l - most) (most - l)
 };
 struct RowResult { float most, log_sum; };
@@ -44,13 +43,13 @@ __device__ __forceinline__ float log_prob_of(const RowResult& r, const float l) 
   if (!(l > -INFINITY)) return -INFINITY;
   return (l == r.most ? 0.f : l - r.most) - r.log_sum;
 }
-__device__ __forceinline__ RowResult finish_row(const LogProbsParams& p, const int row, const Sums& s) {
+// (by the first wavefront of a row's; me: thread of those)
+__device__ __forceinline__ RowResult finish_row(const LogProbsParams& p, const int row, const Sums& s, const int me) {
   const bool any = s.most > -INFINITY;
-  const float rest = (s.count - 1.f) + s.low;
-  const RowResult r = {s.most, any ? log1pf(rest) : 0.f};
-  if (threadIdx.x == 0) p.entropy[row] = any ? r.log_sum + s.away / (1.f + rest) : 0.f;
-  if ((int)threadIdx.x < p.per_row) {
-    const int64_t at = (int64_t)row * p.per_row + threadIdx.x;
+  const RowResult r = {s.most, any ? log1pf(s.rest) : 0.f};
+  if (me == 0) p.entropy[row] = any ? r.log_sum + s.away / (1.f + s.rest) : 0.f;
+  if (me < p.per_row) {
+    const int64_t at = (int64_t)row * p.per_row + me;
     const int t = p.tokens[at];
     float l = -INFINITY;
     if (t >= 0 && t < p.V) {
@@ -68,7 +67,7 @@ __device__ __forceinline__ void put_alternative(const LogProbsParams& p, const i
 }
 
 // Work space: the Sums of every part of every row, then `top` keys for each.
-__host__ __device__ inline int64_t keys_at(const LogProbsParams& p, const int parts) { return (int64_t)p.rows * parts * (int64_t)sizeof(Sums); }
+__host__ __device__ inline int64_t keys_at(const LogProbsParams& p, const int parts) { return ((int64_t)p.rows * parts * (int64_t)sizeof(Sums) + 7) / 8 * 8; }
 
 // A thread's 32 logits as they are in memory: group i are those from index first + (i NT + tid) 8 on; -inf behind the end.
 template <typename T> struct Group { unsigned w[2 * sizeof(T)]; };
@@ -78,17 +77,23 @@ template <typename T> __device__ __forceinline__ float logit_at(const Group<T>& 
   else return __uint_as_float(e & 1 ? g.w[e >> 1] & 0xffff0000u : g.w[e >> 1] << 16);
 }
 template <typename T, bool VECTOR>
+__device__ __forceinline__ Group<T> load_whole_group(const T* from) {
+  Group<T> g;
+#pragma unroll
+  for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
+    uintx4 v;
+    if constexpr (VECTOR) v = *reinterpret_cast<const uintx4*>(from + h * (16 / (int)sizeof(T)));
+    else v = reinterpret_cast<const Bytes16*>(from + h * (16 / (int)sizeof(T)))->v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g.w[4 * h + j] = v[j];
+  }
+  return g;
+}
+template <typename T, bool VECTOR>
 __device__ __forceinline__ Group<T> load_group(const T* row, const int at, const int end) {
   Group<T> g;
   if (at + 8 <= end) {
-#pragma unroll
-    for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
-      uintx4 v;
-      if constexpr (VECTOR) v = *reinterpret_cast<const uintx4*>(row + at + h * (16 / (int)sizeof(T)));
-      else v = reinterpret_cast<const Bytes16*>(row + at + h * (16 / (int)sizeof(T)))->v;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) g.w[4 * h + j] = v[j];
-    }
+    g = load_whole_group<T, VECTOR>(row + at);
   } else {
     constexpr unsigned out = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, f16_t>::value ? 0xfc00u : 0xff80u;
 #pragma unroll
@@ -115,11 +120,12 @@ template <int NT> struct Room {
 
 // Sums of parts (lane l has one; `n` of them, the first lanes), in every lane.
 __device__ __forceinline__ Sums joined(Sums s, const bool have) {
-  if (!have) s = {-INFINITY, 0.f, 0.f, 0.f};
+  if (!have) s = {-INFINITY, 0.f, 0.f};
   const float most = wave_max(s.most);
   const bool top = s.most == most;
-  const float d = fminf(most - s.most, 1e4f), f = top ? 1.f : __builtin_amdgcn_exp2f(d * -kLog2e), all = s.count + s.low;
-  return {most, wave_sum(top ? s.count : 0.f), wave_sum(top ? s.low : f * all), wave_sum(top ? s.away : f * __builtin_fmaf(d, all, s.away))};
+  const float d = fminf(most - s.most, 1e4f), f = top ? 1.f : __builtin_amdgcn_exp2f(d * -kLog2e), all = 1.f + s.rest;
+  const int first = __builtin_ctzll(__ballot(top));      // (the others' largest are terms like any other)
+  return {most, wave_sum((int)(threadIdx.x & 63) == first ? s.rest : f * all), wave_sum(top ? s.away : f * __builtin_fmaf(d, all, s.away))};
 }
 
 // The `top` best of a part whose logits reach the bound too often: the largest behind the last one, again and again.
@@ -153,8 +159,8 @@ __device__ __noinline__ void best_by_rounds(const T* logits, const int first, co
 }
 
 // Sums are of a wavefront's logits around its own largest, so that nothing is waited for before they are complete.
-// Per logit: widen, maximum, difference, its bound, exponent, exponential (four times the others), the largest's
-// exclusion (two) and two sums.
+// Per logit: widen, maximum (half an instruction), difference, its bound, exponent, exponential (as long as four others),
+// two sums.
 template <typename T, int NT, bool VECTOR, bool TOP>
 __global__ void __launch_bounds__(NT, NT == kWide ? 8 : 6) log_probs_kernel(const LogProbsParams p, const int parts, const int each) {
   constexpr int WAVES = NT / 64, LPG = NT / kGroups;
@@ -176,26 +182,41 @@ __global__ void __launch_bounds__(NT, NT == kWide ? 8 : 6) log_probs_kernel(cons
     if ((tid & (LPG - 1)) == 0) room.group[tid / LPG] = group;
     if (tid == 0) room.listed = 0;
   }
-  Sums s = {wave_max(mine), 0.f, 0.f, 0.f};
-  int equal = 0;
+  const float most = wave_max(mine);
+  float sum = 0.f, away = 0.f;
 #pragma unroll
   for (int i = 0; i < kEach / 8; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       // (a distance of 10^4 weighs nothing; -inf, NaN, and everything beside infinite logits, is as far)
-      const float x = logit_at<T>(l[i], e), d = fminf(s.most - x, 1e4f);
-      const bool top = x == s.most;
-      equal += __popcll(__ballot(top));
-      const float w = top ? 0.f : __builtin_amdgcn_exp2f(d * -kLog2e);
-      s.low += w;
-      s.away = __builtin_fmaf(w, d, s.away);
+      const float d = fminf(most - logit_at<T>(l[i], e), 1e4f), w = __builtin_amdgcn_exp2f(d * -kLog2e);
+      sum += w;
+      away = __builtin_fmaf(w, d, away);
     }
-  s.count = (float)equal;
-  s.low = wave_sum(s.low);
-  s.away = wave_sum(s.away);
+  Sums s = {most, wave_sum(sum) - 1.f, wave_sum(away)};
+  // What little is left beside the largest has lost digits to it: it is added once more without.  (A wavefront whose logits
+  // are all -inf comes here too; one with infinities has no weight of its own for them.)
+  if (!(s.rest > 3.f)) {
+    sum = 0.f;
+    int equal = 0;
+    float again = most;      // (hidden from the compiler, which would keep all 32 differences for this)
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("" : "+v"(again));
+#endif
+#pragma unroll
+    for (int i = 0; i < kEach / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = logit_at<T>(l[i], e);
+        const bool top = x == again;
+        equal += __popcll(__ballot(top));
+        sum += top ? 0.f : __builtin_amdgcn_exp2f(fminf(again - x, 1e4f) * -kLog2e);
+      }
+    s.rest = wave_sum(sum) + (float)(equal - 1);
+  }
   if (lane == 0) room.wave[wave] = s;
   __syncthreads();
-  s = joined(room.wave[lane & (WAVES - 1)], lane < WAVES);
+  const Sums of_row = joined(room.wave[lane & (WAVES - 1)], lane < WAVES);
   if constexpr (TOP) {
     // the group whose maximum has top - 1 others in front of it
     const float of_group = room.group[lane];
@@ -207,8 +228,8 @@ __global__ void __launch_bounds__(NT, NT == kWide ? 8 : 6) log_probs_kernel(cons
     }
   }
   RowResult r = {0.f, 0.f};
-  if (parts == 1) r = finish_row(p, row, s);
-  else if (tid == 0) reinterpret_cast<Sums*>(p.work)[(int64_t)row * parts + part] = s;
+  if (parts == 1) r = finish_row(p, row, of_row, tid);
+  else if (tid == 0) reinterpret_cast<Sums*>(p.work)[(int64_t)row * parts + part] = of_row;
   if constexpr (TOP) {
     u64* keys = reinterpret_cast<u64*>(reinterpret_cast<char*>(p.work) + keys_at(p, parts)) + ((int64_t)row * parts + part) * p.top;
     auto put = [&](const int place, const u64 key) {
@@ -246,6 +267,70 @@ __global__ void __launch_bounds__(NT, NT == kWide ? 8 : 6) log_probs_kernel(cons
   }
 }
 
+// Many rows without alternatives: a wavefront each, which streams its row with a running maximum a lane and waits for
+// nobody.  What the lane of the largest has added to that one's 1 has lost digits: its logits are added once more
+// by all lanes, without it.
+template <typename T, bool VECTOR>
+__global__ void __launch_bounds__(256) log_probs_stream_kernel(const LogProbsParams p) {
+  constexpr int N = 4, STEP = 64 * 8 * N;      // groups of eight a lane at a time
+  const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row >= p.rows) return;
+  const T* logits = reinterpret_cast<const T*>(p.logits) + (int64_t)row * p.V;
+  float m = -INFINITY, sum = 0.f, away = 0.f;
+  Group<T> next[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) next[i] = load_group<T, VECTOR>(logits, (i * 64 + lane) * 8, p.V);
+#pragma unroll 1
+  for (int at = 0; at < p.V; at += STEP) {
+    Group<T> l[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) l[i] = next[i];
+    if (at + 2 * STEP <= p.V) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) next[i] = load_whole_group<T, VECTOR>(logits + at + STEP + (i * 64 + lane) * 8);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) next[i] = load_group<T, VECTOR>(logits, at + STEP + (i * 64 + lane) * 8, p.V);
+    }
+    float most = m;       // (NaN is no maximum)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, logit_at<T>(l[i], e));
+    // (a distance of 10^4 weighs nothing; -inf, NaN, and everything beside infinite logits, is as far)
+    const float up = fminf(most - m, 1e4f), f = most == m ? 1.f : __builtin_amdgcn_exp2f(up * -kLog2e);
+    away = most == m ? away : f * __builtin_fmaf(up, sum, away);
+    sum *= f;
+    m = most;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float d = fminf(most - logit_at<T>(l[i], e), 1e4f), w = __builtin_amdgcn_exp2f(d * -kLog2e);
+        sum += w;
+        away = __builtin_fmaf(w, d, away);
+      }
+  }
+  const float most = wave_max(m), d = fminf(most - m, 1e4f), f = m == most ? 1.f : __builtin_amdgcn_exp2f(d * -kLog2e);
+  const int owner = __builtin_ctzll(__ballot(m == most));
+  Sums s = {most, wave_sum(lane == owner ? 0.f : f * sum), wave_sum(m == most ? away : f * __builtin_fmaf(d, sum, away))};
+  // the owner's groups, or all where infinite logits share the row
+  const bool whole = most == INFINITY;
+  const int stride = whole ? 1 : 64, first = whole ? 0 : owner;
+  float again = 0.f, equal = 0.f;
+  for (int k = lane; (k * stride + first) * 8 < p.V; k += 64) {
+    const Group<T> l = load_group<T, VECTOR>(logits, (k * stride + first) * 8, p.V);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = logit_at<T>(l, e);
+      again += x == most ? 0.f : __builtin_amdgcn_exp2f(fminf(most - x, 1e4f) * -kLog2e);
+      equal += x == most ? 1.f : 0.f;
+    }
+  }
+  s.rest += wave_sum(again) + (wave_sum(equal) - 1.f);
+  finish_row(p, row, s, lane);
+}
+
 // One workgroup a row: its parts' sums in their order, and the best of their alternatives.
 constexpr int kMostParts = (kMaxVocabulary + kWide * kEach - 1) / (kWide * kEach);
 __global__ void __launch_bounds__(256) log_probs_join_kernel(const LogProbsParams p, const int parts) {
@@ -257,7 +342,7 @@ __global__ void __launch_bounds__(256) log_probs_join_kernel(const LogProbsParam
   const int lane = threadIdx.x & 63;
   const Sums s = joined(sums[min(lane, parts - 1)], lane < parts);
   __syncthreads();
-  const RowResult r = finish_row(p, row, s);
+  const RowResult r = finish_row(p, row, s, threadIdx.x);
   for (int c = threadIdx.x; c < n; c += 256) {
     const u64 key = list[c];
     int rank = 0;
@@ -271,6 +356,13 @@ hipError_t log_probs_as(const LogProbsParams& p, const int parts, hipStream_t st
   // (parts begin at whole groups of eight, so at 16-byte boundaries where rows do)
   const int each = ((p.V + parts - 1) / parts + 7) / 8 * 8;
   const dim3 grid((unsigned)p.rows * parts);
+  // From 1024 rows on every SIMD has one to stream.  4001 x 32000 bf16: 119 us a workgroup a row.
+  if (p.top == 0 && p.rows >= kManyRows) {
+    const dim3 waves((unsigned)(p.rows + 3) / 4);
+    if (p.V % 8 == 0) hipLaunchKernelGGL((log_probs_stream_kernel<T, true>), waves, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((log_probs_stream_kernel<T, false>), waves, dim3(256), 0, stream, p);
+    return hipGetLastError();
+  }
 #define OHIP_LOG_PROBS(NT, VECTOR)                                                                                                   \
   do {                                                                                                                             \
     if (p.top > 0) hipLaunchKernelGGL((log_probs_kernel<T, NT, VECTOR, true>), grid, dim3(NT), 0, stream, p, parts, each);          \
@@ -289,7 +381,7 @@ hipError_t log_probs_as(const LogProbsParams& p, const int parts, hipStream_t st
 
 }  // namespace
 
-int log_probs_parts(const LogProbsParams& p) { return (p.V + kWide * kEach - 1) / (kWide * kEach); }
+int log_probs_parts(const LogProbsParams& p) { return p.top == 0 && p.rows >= kManyRows ? 1 : (p.V + kWide * kEach - 1) / (kWide * kEach); }
 size_t log_probs_space(const LogProbsParams& p) {
   const int parts = log_probs_parts(p);
   return (size_t)(keys_at(p, parts) + (int64_t)p.rows * parts * p.top * (int64_t)sizeof(u64));

@@ -78,6 +78,32 @@ def test_shapes(odla, shape, per_row):
     run_and_check(odla, "bf16", logits_of(shape, "bf16", 3), tokens, 3, repeats=3)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("v", [1, 9, 2048, 2056, 4095, 5001])
+def test_many_rows(odla, kind, v):
+    """1100 rows are streamed by a wavefront each: some with equal, infinite and missing logits and nearly certain tokens."""
+    announce("log probabilities of 1100 rows of %d logits, %s" % (v, kind))
+    rng = np.random.default_rng(v)
+    x = rng.standard_normal((1100, v)) * 3
+    x[0] = -np.inf
+    x[1] = 0.5
+    x[2, ::3] = np.nan
+    x[3] = np.inf
+    x[4, v // 2] = np.inf
+    x[5, v // 2] = 60.0
+    x[6, -1] = 30.0
+    x[7] = -np.inf
+    x[7, v // 3] = -5.0
+    x[8] = {"fp32": -3e38, "fp16": -65504.0, "bf16": -3e38}[kind]
+    x[9] = np.sort(x[9])                  # the maximum grows all along
+    x[10] = np.sort(x[10])[::-1]
+    x[11, ::2] = -np.inf
+    x[12] = np.nan
+    tokens = rng.integers(0, v, (1100, 2))
+    tokens[:20, 0] = v // 2
+    run_and_check(odla, kind, R.to_bits(x, kind), tokens, 0)
+
+
 def test_the_longest_row(odla):
     announce("log probabilities of 524288 logits")
     run_and_check(odla, "fp32", logits_of((2, 524288), "fp32", 3), np.array([[0, 524287], [5, 9]]), 32)
