@@ -786,8 +786,7 @@ struct PagedAttentionParams {
   DType dt = DT_F32;
 };
 size_t paged_attention_space(const PagedAttentionParams& p);
-hipError_t launch_cache_write(const PagedAttentionParams& p, hipStream_t stream);        // the new keys and values into their pages
-hipError_t launch_paged_attention(const PagedAttentionParams& p, hipStream_t stream);    // y, or parts of it in the work space
+hipError_t launch_paged_attention(const PagedAttentionParams& p, hipStream_t stream);    // the new keys and values into their pages; y, or parts of it in the work space
 hipError_t launch_attention_join(const PagedAttentionParams& p, hipStream_t stream);     // y from the parts; rows of no sequence zero
 
 // Log probabilities, entropy and the best alternatives of rows of logits (see odla_hip_LogProbs).

@@ -23,6 +23,7 @@ struct Args : PagedAttentionParams {
   unsigned page_magic; int page_shift;
   int reach;          // places of a row of the page table
   int few_slots, many_slots;
+  int writers, written;      // the first workgroups write the new tokens to their places, so many each
 };
 
 template <int CTRL, int ROWS>
@@ -148,40 +149,67 @@ __device__ __forceinline__ T* result_row(const Args& a, const SeqSpan& s, const 
 }
 
 // ------------------------------------------------------------ the new tokens --
-// A workgroup takes four tokens, a wavefront each.
-__global__ void __launch_bounds__(256) cache_write_kernel(const Args a, const int bytes) {
-  const int token = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (token >= a.tokens) return;
+// The first workgroups of the launch write the new keys and values to their places; the others take them from where they
+// are written from, so that nobody waits.  A wavefront writes one token after the other.
+__device__ __forceinline__ void write_tokens(const Args& a, const int bytes) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int end = min((int)(blockIdx.x + 1) * a.written, a.tokens);
   int seq = -1;
   SeqSpan s = {0, 0, 0, 0};
-  if (a.starts == nullptr) {
-    seq = token / (a.tokens / a.seqs);
-    s = span_of(a, seq);
-  } else {
-    for (int b0 = 0; b0 < a.seqs && seq < 0; b0 += 64) {
-      const SeqSpan m = span_of(a, b0 + lane);
-      const unsigned long long here = __ballot(token >= m.first && token < m.first + m.n);
-      if (here != 0) {
-        seq = b0 + __builtin_ctzll(here);
-        s = span_from_lane(m, __builtin_ctzll(here));
+#pragma unroll 1
+  for (int token = blockIdx.x * a.written + wave; token < end; token += 4) {
+    if (seq < 0 || token < s.first || token >= s.first + s.n) {
+      seq = -1;
+      for (int b0 = 0; b0 < a.seqs && seq < 0; b0 += 64) {
+        const SeqSpan m = span_of(a, b0 + lane);
+        const unsigned long long here = __ballot(token >= m.first && token < m.first + m.n);
+        if (here != 0) {
+          seq = b0 + __builtin_ctzll(here);
+          s = span_from_lane(m, __builtin_ctzll(here));
+        }
       }
+      if (seq < 0) continue;
+    }
+    const int place = s.cached + (token - s.first);
+    if (place >= s.len) continue;
+    const int index = fast_div(place, a.page_magic, a.page_shift);
+    const int row = cache_row(a.table[(int64_t)seq * a.table_width + index], place - index * a.page, a.page, a.pages);
+    if (row < 0) continue;
+    const uintx4* k = reinterpret_cast<const uintx4*>(reinterpret_cast<const char*>(a.k) + (int64_t)token * bytes);
+    const uintx4* v = reinterpret_cast<const uintx4*>(reinterpret_cast<const char*>(a.v) + (int64_t)token * bytes);
+    uintx4* kc = reinterpret_cast<uintx4*>(reinterpret_cast<char*>(a.k_cache) + (int64_t)row * bytes);
+    uintx4* vc = reinterpret_cast<uintx4*>(reinterpret_cast<char*>(a.v_cache) + (int64_t)row * bytes);
+    for (int i = lane; i < bytes / 16; i += 64) {
+      const uintx4 x = k[i], y = v[i];
+      kc[i] = x;
+      vc[i] = y;
     }
   }
-  if (seq < 0) return;
-  const int place = s.cached + (token - s.first);
-  if (place >= s.len) return;
-  const int index = fast_div(place, a.page_magic, a.page_shift);
-  const int row = cache_row(a.table[(int64_t)seq * a.table_width + index], place - index * a.page, a.page, a.pages);
-  if (row < 0) return;
-  const uintx4* k = reinterpret_cast<const uintx4*>(reinterpret_cast<const char*>(a.k) + (int64_t)token * bytes);
-  const uintx4* v = reinterpret_cast<const uintx4*>(reinterpret_cast<const char*>(a.v) + (int64_t)token * bytes);
-  uintx4* kc = reinterpret_cast<uintx4*>(reinterpret_cast<char*>(a.k_cache) + (int64_t)row * bytes);
-  uintx4* vc = reinterpret_cast<uintx4*>(reinterpret_cast<char*>(a.v_cache) + (int64_t)row * bytes);
-  for (int i = lane; i < bytes / 16; i += 64) {
-    const uintx4 x = k[i], y = v[i];
-    kc[i] = x;
-    vc[i] = y;
+}
+// Where the keys and values of one head of a sequence lie: in the caches up to the new tokens, which are read where they come from.
+struct Source {
+  const char *k_cache, *v_cache, *k_new, *v_new;      // (new: as if place 0 lay in front of the first new token)
+  int64_t row_bytes;
+  int fresh, end;      // the first new place, and the last one that is read
+  __device__ __forceinline__ const char* at(const char* cache, const char* fresh_ones, const int place, const int row) const {
+    const bool is = place >= fresh && place <= end;      // (row -1: any row of the cache)
+    return (is ? fresh_ones : cache) + (int64_t)(is ? place : max(row, 0)) * row_bytes;
   }
+  __device__ __forceinline__ const char* key(const int place, const int row) const { return at(k_cache, k_new, place, row); }
+  __device__ __forceinline__ const char* value(const int place, const int row) const { return at(v_cache, v_new, place, row); }
+};
+template <typename T>
+__device__ __forceinline__ Source source_of(const Args& a, const SeqSpan& s, const int head, const int hi) {
+  Source o;
+  o.row_bytes = (int64_t)a.kv_heads * a.d * (int)sizeof(T);
+  const int64_t of_head = (int64_t)head * a.d * (int)sizeof(T), first = of_head + (int64_t)(s.first - s.cached) * o.row_bytes;
+  o.k_cache = reinterpret_cast<const char*>(a.k_cache) + of_head;
+  o.v_cache = reinterpret_cast<const char*>(a.v_cache) + of_head;
+  o.k_new = reinterpret_cast<const char*>(a.k) + first;
+  o.v_new = reinterpret_cast<const char*>(a.v) + first;
+  o.end = at_least(hi, 1) - 1;       // (lookups stay in front of it)
+  o.fresh = a.k != nullptr ? s.cached : INT32_MAX;
+  return o;
 }
 
 // ------------------------------------------------------------------ few rows --
@@ -240,7 +268,7 @@ template <typename T> __device__ __forceinline__ unsigned finite_part(const unsi
 }
 // column(i): this lane's columns of its row, N times four; rows_of, row_at: as in the kernels, KT keys a tile.
 template <typename T, int KT, int N, typename RowsOf, typename RowAt, typename Column, typename Add>
-__device__ __forceinline__ void add_odd_values(const Args a, const char* vc, const int64_t row_bytes, const int t_begin, const int t_end, const int step, const int last, RowsOf rows_of,
+__device__ __forceinline__ void add_odd_values(const Args& a, const Source& src, const int t_begin, const int t_end, const int step, const int last, RowsOf rows_of,
                                             RowAt row_at, Column column, Add add) {
 #pragma unroll 1
   for (int t = t_begin; t < t_end; t += step) {
@@ -249,14 +277,13 @@ __device__ __forceinline__ void add_odd_values(const Args a, const char* vc, con
     for (int k = 0; k < KT; ++k) {
       const int row = row_at(rows_, t, k), place = t * KT + k;
       if (row < 0 || place > last || (a.window != 0 && place <= last - a.window)) continue;
-      const T* v = reinterpret_cast<const T*>(vc + row * row_bytes);
+      const T* v = reinterpret_cast<const T*>(src.value(place, row));
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        if (column(i) >= a.d) continue;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float x = Store<T>::ld(v + column(i) + j);
-          if (!__builtin_isfinite(x)) add(i, j, x);
+          const float x = Store<T>::ld(v + (column(i) < a.d ? column(i) + j : 0));      // (behind the head: columns that are not stored)
+          add(i, j, __builtin_isfinite(x) ? 0.f : x);
         }
       }
     }
@@ -265,7 +292,7 @@ __device__ __forceinline__ void add_odd_values(const Args a, const char* vc, con
 
 template <typename T, int DP> constexpr int kFewLds = (4 * 16 * (DP + 4) + 2 * 4 * 16) * (int)sizeof(float);
 template <typename T, int DP, bool WHOLE, bool TWO>
-__device__ __forceinline__ void attend_few(const Args& a, const Found& f, unsigned char* smem) {
+__device__ __forceinline__ void attend_few(const Args& a, const Found& f, const Piece& piece, unsigned char* smem) {
   using F = Few<T>;
   using S = FewShape<T, DP>;
   constexpr bool WIDE = DP > 128;
@@ -276,13 +303,10 @@ __device__ __forceinline__ void attend_few(const Args& a, const Found& f, unsign
   auto part_l = part_m + 4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, g = lane >> 4;
-  const Piece piece = piece_at(f, a.kv_heads, blockIdx.x - f.piece0);
   const int head = piece.head, r0 = piece.tile * R, rows = min(R, f.span.n * a.group - r0);
   const KeyRange seen = keys_of_rows(f.span, r0, R, a.group, a.window);
   const int t_begin = seen.lo / KT + piece.cut * f.stretch, t_end = min((seen.hi + KT - 1) / KT, f.cuts > 1 ? t_begin + f.stretch : INT32_MAX);
-  const int64_t row_bytes = (int64_t)a.kv_heads * a.d * (int)sizeof(T);
-  const char* kc = reinterpret_cast<const char*>(a.k_cache) + (int64_t)head * a.d * (int)sizeof(T);
-  const char* vc = reinterpret_cast<const char*>(a.v_cache) + (int64_t)head * a.d * (int)sizeof(T);
+  const Source src = source_of<T>(a, f.span, head, seen.hi);
   const int32_t* table = a.table + (int64_t)f.seq * a.table_width;
 
   // queries: this lane's row, and the last place that it sees
@@ -302,14 +326,13 @@ __device__ __forceinline__ void attend_few(const Args& a, const Found& f, unsign
   // waits for all keys and values requested before it.
   struct Where { int first, second, edge; };      // rows of place 0 of either page, if it went on that way, and where the second begins
   constexpr int kNone = INT32_MIN;
-  const int end = at_least(seen.hi, 1) - 1;       // (lookups stay in front of it)
   auto look_up = [&](const int t) __attribute__((always_inline)) -> Where {
     if constexpr (TWO) {
-      const int index = fast_div(at_most(t * KT, end), a.page_magic, a.page_shift), next = at_most(index + 1, fast_div(end, a.page_magic, a.page_shift));
+      const int index = fast_div(at_most(t * KT, src.end), a.page_magic, a.page_shift), next = at_most(index + 1, fast_div(src.end, a.page_magic, a.page_shift));
       const auto numbers = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)table;
       return {numbers[index], numbers[next], (index + 1) * a.page};
     } else {
-      return {table[fast_div(at_most(t * KT + (lane & (KT - 1)), end), a.page_magic, a.page_shift)], 0, 0};
+      return {table[fast_div(at_most(t * KT + (lane & (KT - 1)), src.end), a.page_magic, a.page_shift)], 0, 0};
     }
   };
   auto found = [&](const Where& w, const int t) __attribute__((always_inline)) -> Where {
@@ -336,7 +359,7 @@ __device__ __forceinline__ void attend_few(const Args& a, const Found& f, unsign
   auto load_keys = [&](const Where& rows_, const int t) __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < F::BLOCKS; ++b) {
-      const T* row = reinterpret_cast<const T*>(kc + max(row_at(rows_, t, 16 * b + l16), 0) * row_bytes);
+      const T* row = reinterpret_cast<const T*>(src.key(t * KT + 16 * b + l16, row_at(rows_, t, 16 * b + l16)));
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
         unsigned w[4];
@@ -349,7 +372,7 @@ __device__ __forceinline__ void attend_few(const Args& a, const Found& f, unsign
   auto load_values = [&](const Where& rows_, const int t) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < KEYS; ++j) {
-      const T* row = reinterpret_cast<const T*>(vc + max(row_at(rows_, t, key_of_slot(j)), 0) * row_bytes);
+      const T* row = reinterpret_cast<const T*>(src.value(t * KT + key_of_slot(j), row_at(rows_, t, key_of_slot(j))));
       constexpr int W = VW < 4 ? 2 : 4;
 #pragma unroll
       for (int w = 0; w < VW / W; ++w) load_part<T, W, WHOLE>(row, l16 * VE + w * (W * 4 / (int)sizeof(T)), a.d, &vf[j][w * W]);
@@ -448,7 +471,7 @@ __device__ __forceinline__ void attend_few(const Args& a, const Found& f, unsign
   }
 
   if (odd)
-    add_odd_values<T, KT, VE>(a, vc, row_bytes, t_begin + wave, t_end, 4, last, rows_of, row_at, [&](const int n) { return 4 * (g * VE + n); },
+    add_odd_values<T, KT, VE>(a, src, t_begin + wave, t_end, 4, last, rows_of, row_at, [&](const int n) { return 4 * (g * VE + n); },
                               [&](const int n, const int j, const float x) { o[(4 * n + j) % VE][(4 * n + j) / VE] += x; });
 
   // ---- the wavefronts' parts
@@ -556,35 +579,39 @@ __device__ __forceinline__ void request16(const char* from, unsigned char* to) {
 }
 
 // What a wavefront keeps of its 32 rows: lane l has row l % 32.
-template <int DP> struct BigRows {
-  uintx4 q[DP / 16];
-  floatx16 o[DP / 32];
+template <int DV> struct BigRows {
+  uintx4 q[DV / 16];
+  floatx16 o[DV / 32];
   float m, l;          // m in units of log 2
   int last;            // the last place that the row sees
   bool odd;            // infinite or missing values have left a tile
 };
 
+// Requests a tile of keys and values into LDS; rows: lane l, the cache's row of key l % KT.
+template <int DP, int DV, bool WHOLE>
+__device__ __forceinline__ void request_tile(const Args& a, const Source& src, unsigned char* to, const int rows, const int place0, const int lane, const int wave) {
+  using B = Big<DP>;
+#pragma unroll
+  for (int i = 0; i < B::REQUESTS; ++i) {
+    const int row = (wave * B::REQUESTS + i) * B::PER + lane / B::CHUNKS, slot = lane % B::CHUNKS, from = __shfl(rows, row);
+    // (chunks behind the end of a head's row: any of it, they meet zeros of the query or leave columns that are not stored)
+    const int k_chunk = key_slot<DP>(row, slot), v_chunk = value_slot<DP>(row, slot);
+    unsigned char* at = to + (wave * B::REQUESTS + i) * 1024;
+    if (DV == DP || k_chunk * 8 < DV) request16(src.key(place0 + row, from) + (WHOLE || k_chunk * 8 < a.d ? k_chunk * 16 : 0), at);
+    if (DV == DP || v_chunk * 8 < DV) request16(src.value(place0 + row, from) + (WHOLE || v_chunk * 8 < a.d ? v_chunk * 16 : 0), at + B::TILE);
+  }
+}
+
 // One tile of keys, out of `now`; the next one's rows of the cache are requested into `next` meanwhile (the two never
 // overlap: without saying so, every read of LDS would wait for the requests).  valid: bit k, key k is there.
-template <typename T, int DP, bool WHOLE>
-__device__ __forceinline__ void big_tile(const Args& a, unsigned char* __restrict next, unsigned char* __restrict now, const int next_rows, const bool more, const char* kc,
-                                         const char* vc, const int64_t row_bytes, const int place0, const unsigned long long valid, const bool masked, const float mult,
-                                         const int lane, const int wave, BigRows<DP>& w) {
+template <typename T, int DP, int DV, bool WHOLE>
+__device__ __forceinline__ void big_tile(const Args& a, unsigned char* __restrict next, unsigned char* __restrict now, const int next_rows, const bool more, const Source& src,
+                                         const int place0, const unsigned long long valid, const bool masked, const float mult, const int lane, const int wave,
+                                         BigRows<DV>& w) {
   using B = Big<DP>;
   constexpr int BLOCKS = B::BLOCKS;
   const int l32 = lane & 31, h = lane >> 5;
-  if (more) {
-#pragma unroll
-    for (int i = 0; i < B::REQUESTS; ++i) {
-      const int row = (wave * B::REQUESTS + i) * B::PER + lane / B::CHUNKS, slot = lane % B::CHUNKS;
-      const int64_t at = max(__shfl(next_rows, row), 0) * row_bytes;
-      // (chunks behind the end of a head's row: any of it, they meet zeros of the query or leave columns that are not stored)
-      const int k_chunk = key_slot<DP>(row, slot), v_chunk = value_slot<DP>(row, slot);
-      unsigned char* to = next + (wave * B::REQUESTS + i) * 1024;
-      request16(kc + at + (WHOLE || k_chunk * 8 < a.d ? k_chunk * 16 : 0), to);
-      request16(vc + at + (WHOLE || v_chunk * 8 < a.d ? v_chunk * 16 : 0), to + B::TILE);
-    }
-  }
+  if (more) request_tile<DP, DV, WHOLE>(a, src, next, next_rows, place0 + B::KT, lane, wave);
   floatx16 s[BLOCKS];
 #pragma unroll
   for (int b = 0; b < BLOCKS; ++b) {
@@ -592,8 +619,7 @@ __device__ __forceinline__ void big_tile(const Args& a, unsigned char* __restric
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) {
-      if (!WHOLE && c * 16 >= a.d) break;
+    for (int c = 0; c < DV / 16; ++c) {
       uintx4 k = *reinterpret_cast<const uintx4*>(row + key_slot<DP>(l32, 2 * c + h) * 16);
       if (!WHOLE && (2 * c + h) * 8 >= a.d) k = uintx4{0u, 0u, 0u, 0u};
       s[b] = mma32<T>(k, w.q[c], s[b]);
@@ -625,7 +651,7 @@ __device__ __forceinline__ void big_tile(const Args& a, unsigned char* __restric
     w.m = m;
     w.l *= shrink;
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < DV / 32; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) w.o[d][i] *= shrink;
   }
@@ -660,8 +686,9 @@ __device__ __forceinline__ void big_tile(const Args& a, unsigned char* __restric
 #pragma unroll 4
     for (int c = lane; c < B::TILE / 16; c += 64) {
       const uintx4 v = reinterpret_cast<const uintx4*>(values)[c];
+      const bool loaded = DV == DP || value_slot<DP>(c / B::CHUNKS, c % B::CHUNKS) * 8 < DV;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) most = with_exponents<T>(most, v[j]);
+      for (int j = 0; j < 4; ++j) most = with_exponents<T>(most, loaded ? v[j] : 0u);
     }
     if (__any(not_finite<T>(most))) {
       w.odd = true;
@@ -675,8 +702,7 @@ __device__ __forceinline__ void big_tile(const Args& a, unsigned char* __restric
     }
   }
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d) {
-    if (!WHOLE && d * 32 >= a.d) break;
+  for (int d = 0; d < DV / 32; ++d) {
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
@@ -688,31 +714,28 @@ __device__ __forceinline__ void big_tile(const Args& a, unsigned char* __restric
   }
 }
 
-template <typename T, int DP, bool WHOLE>
-__device__ __forceinline__ void attend_many(const Args& a, const Found& f, unsigned char* smem) {
+template <typename T, int DP, int DV, bool WHOLE>
+__device__ __forceinline__ void attend_many(const Args& a, const Found& f, const Piece& piece, unsigned char* smem) {
   using B = Big<DP>;
   constexpr bool WIDE = DP > 128;
   constexpr int R = 128, KT = B::KT;
   static_assert(R == Ways<T, WIDE>::many.rows && KT == Ways<T, WIDE>::many.keys, "as the pieces are cut");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l32 = lane & 31, h = lane >> 5;
-  const Piece piece = piece_at(f, a.kv_heads, blockIdx.x - f.piece0);
   const int head = piece.head, r0 = piece.tile * R, rows = min(R, f.span.n * a.group - r0);
   const KeyRange seen = keys_of_rows(f.span, r0, R, a.group, a.window);
   const int t_begin = seen.lo / KT + piece.cut * f.stretch, t_end = min((seen.hi + KT - 1) / KT, f.cuts > 1 ? t_begin + f.stretch : INT32_MAX);
-  const int64_t row_bytes = (int64_t)a.kv_heads * a.d * 2;
-  const char* kc = reinterpret_cast<const char*>(a.k_cache) + (int64_t)head * a.d * 2;
-  const char* vc = reinterpret_cast<const char*>(a.v_cache) + (int64_t)head * a.d * 2;
+  const Source src = source_of<T>(a, f.span, head, seen.hi);
   const int32_t* table = a.table + (int64_t)f.seq * a.table_width;
   // The scale's sign goes to the queries, and so does a scale of zero: maxima are taken of the products as they are.
   const float mult = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
-  BigRows<DP> w;
+  BigRows<DV> w;
   const int r = min(wave * 32 + l32, rows - 1), token = (r0 + r) / a.group;
   {
     const T* row = reinterpret_cast<const T*>(a.q) + ((int64_t)(f.span.first + token) * a.kv_heads * a.group + (int64_t)head * a.group + (r0 + r - token * a.group)) * a.d;
     const unsigned flip = a.scale < 0.f ? 0x80008000u : 0u, keep = a.scale == 0.f ? 0u : 0xffffffffu;
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) {
+    for (int c = 0; c < DV / 16; ++c) {
       unsigned x[4];
       load_part<T, 4, WHOLE>(row, 16 * c + 8 * h, a.d, x);
 #pragma unroll
@@ -724,15 +747,14 @@ __device__ __forceinline__ void attend_many(const Args& a, const Found& f, unsig
   w.l = 0.f;
   w.odd = false;
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
+  for (int d = 0; d < DV / 32; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) w.o[d][i] = 0.f;
   // what all rows of the tile see
   const int first_last = f.span.cached + r0 / a.group, last_last = f.span.cached + (r0 + rows - 1) / a.group;
   // (a number is looked at one tile after it was requested: what is on its way into LDS would be waited for with it)
-  const int end = at_least(seen.hi, 1) - 1;
   auto look_up = [&](const int t) __attribute__((always_inline)) -> int {
-    return table[fast_div(at_most(t * KT + (lane & (KT - 1)), end), a.page_magic, a.page_shift)];
+    return table[fast_div(at_most(t * KT + (lane & (KT - 1)), src.end), a.page_magic, a.page_shift)];
   };
   auto found = [&](const int number, const int t) __attribute__((always_inline)) -> int {
     const int place = t * KT + (lane & (KT - 1));
@@ -742,15 +764,7 @@ __device__ __forceinline__ void attend_many(const Args& a, const Found& f, unsig
   auto rows_of = [&](const int t) { return found(look_up(t), t); };
   if (t_begin < t_end) {
     int here = rows_of(t_begin), number = look_up(t_begin + 1);
-#pragma unroll
-    for (int i = 0; i < B::REQUESTS; ++i) {
-      const int row = (wave * B::REQUESTS + i) * B::PER + lane / B::CHUNKS, slot = lane % B::CHUNKS;
-      const int64_t at = max(__shfl(here, row), 0) * row_bytes;
-      const int k_chunk = key_slot<DP>(row, slot), v_chunk = value_slot<DP>(row, slot);
-      unsigned char* to = smem + (wave * B::REQUESTS + i) * 1024;
-      request16(kc + at + (WHOLE || k_chunk * 8 < a.d ? k_chunk * 16 : 0), to);
-      request16(vc + at + (WHOLE || v_chunk * 8 < a.d ? v_chunk * 16 : 0), to + B::TILE);
-    }
+    request_tile<DP, DV, WHOLE>(a, src, smem, here, t_begin * KT, lane, wave);
 #pragma unroll 1
     for (int t = t_begin; t < t_end; ++t) {
       // this tile has landed, and everybody has left the other buffer
@@ -760,12 +774,12 @@ __device__ __forceinline__ void attend_many(const Args& a, const Found& f, unsig
       const bool masked = (valid & all) != all || t * KT + KT - 1 > first_last || (a.window != 0 && t * KT <= last_last - a.window);
       const int next = found(number, t + 1), at = (t - t_begin) & 1;
       number = look_up(t + 2);
-      big_tile<T, DP, WHOLE>(a, smem + (1 - at) * B::STAGE, smem + at * B::STAGE, next, t + 1 < t_end, kc, vc, row_bytes, t * KT, valid & all, masked, mult, lane, wave, w);
+      big_tile<T, DP, DV, WHOLE>(a, smem + (1 - at) * B::STAGE, smem + at * B::STAGE, next, t + 1 < t_end, src, t * KT, valid & all, masked, mult, lane, wave, w);
       here = next;
     }
   }
   if (w.odd)
-    add_odd_values<T, KT, DP / 8>(a, vc, row_bytes, t_begin, t_end, 1, w.last, rows_of, [](const int rows_, int, const int k) { return __shfl(rows_, k); }, [&](const int n) { return 8 * n + 4 * h; },
+    add_odd_values<T, KT, DV / 8>(a, src, t_begin, t_end, 1, w.last, rows_of, [](const int rows_, int, const int k) { return __shfl(rows_, k); }, [&](const int n) { return 8 * n + 4 * h; },
                                   [&](const int n, const int j, const float x) { w.o[n / 4][n % 4 * 4 + j] += x; });
   const float sum = over_halves(w.l, [](float x, float y) { return x + y; });
   if (wave * 32 + l32 >= rows) return;
@@ -773,7 +787,7 @@ __device__ __forceinline__ void attend_many(const Args& a, const Found& f, unsig
     T* y = result_row<T>(a, f.span, head, r0 + r);
     const float by = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < DV / 32; ++d)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int col = 32 * d + 8 * i + 4 * h;
@@ -787,7 +801,7 @@ __device__ __forceinline__ void attend_many(const Args& a, const Found& f, unsig
     if (piece.slot >= parts.slots) return;
     float* to = parts.values(piece.slot, r);
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < DV / 32; ++d)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int col = 32 * d + 8 * i + 4 * h;
@@ -802,20 +816,28 @@ __device__ __forceinline__ void attend_many(const Args& a, const Found& f, unsig
 }
 
 template <typename T, int DP> constexpr int kLds = sizeof(T) == 2 && Big<DP>::LDS > kFewLds<T, DP> ? Big<DP>::LDS : kFewLds<T, DP>;
-template <typename T, int DP, bool WHOLE>
+// DV: the head size rounded up to what the tiles of many rows are multiplied for.
+template <typename T, int DP, int DV, bool WHOLE>
 __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) attend_kernel(const Args a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  const Found f = find<T, (DP > 128), false>(a, blockIdx.x);
+  if ((int)blockIdx.x < a.writers) {
+    write_tokens(a, a.kv_heads * a.d * (int)sizeof(T));
+    return;
+  }
+  const int number = blockIdx.x - a.writers;
+  const Found f = find<T, (DP > 128), false>(a, number);
   if (f.seq < 0) return;
+  const Piece piece = piece_at(f, a.kv_heads, number - f.piece0);
   if constexpr (sizeof(T) == 2) {
     if (f.many) {
-      attend_many<T, DP, WHOLE>(a, f, smem);
+      attend_many<T, DP, DV, WHOLE>(a, f, piece, smem);
       return;
     }
   }
   constexpr int KT = Few<T>::KT;
-  if (a.page >= KT || 2 * a.page == KT) attend_few<T, DP, WHOLE, true>(a, f, smem);      // (tiles begin at multiples of KT)
-  else attend_few<T, DP, WHOLE, false>(a, f, smem);
+  constexpr bool FULL = WHOLE && DV == DP;
+  if (a.page >= KT || 2 * a.page == KT) attend_few<T, DP, FULL, true>(a, f, piece, smem);      // (tiles begin at multiples of KT)
+  else attend_few<T, DP, FULL, false>(a, f, piece, smem);
 }
 
 // ------------------------------------------------------------------ the parts --
@@ -889,22 +911,35 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const Args a, const
   }
 }
 
-// Slots of a way: none where no sequence can be long enough to be cut.
-int slots_of(const PagedAttentionParams& p, const Way& w, const long long units) {
+// The most parts that the keys of one tile are cut into.
+long long most_cuts(const PagedAttentionParams& p, const Way& w) {
   const SeqSpan longest = {0, p.tokens, 0, p.table_width * p.page};
-  const long long most = (long long)key_tiles(longest, w, p.group, std::min(p.window, 1 << 30));
-  return most <= w.least ? 0 : (int)std::min((long long)most_slots(w), units * ((most + w.least - 1) / w.least));
+  return stretches(key_tiles(longest, w, p.group, std::min(p.window, 1 << 30)), w.least);
 }
+int slots_of(const PagedAttentionParams& p, const Way& w, const long long units) {
+  const long long cuts = most_cuts(p, w);
+  return cuts == 1 ? 0 : (int)std::min((long long)most_slots(w), units * cuts);
+}
+long long pieces_of(const PagedAttentionParams& p, const Way& w, const long long units) { return std::min(units + most_cut_pieces(w), units * most_cuts(p, w)); }
+template <typename T, bool WIDE> struct Units {
+  using W = Ways<T, WIDE>;
+  long long few, many;
+  explicit Units(const PagedAttentionParams& p)
+      : few(most_few_units(p.tokens, p.seqs, p.kv_heads, p.group, !W::kTwo)), many(W::kTwo ? most_many_units(p.tokens, p.seqs, p.kv_heads, p.group) : 0) {}
+};
 template <typename T, bool WIDE>
 Args args_as(const PagedAttentionParams& p) {
   using W = Ways<T, WIDE>;
+  const Units<T, WIDE> units(p);
   Args a;
   static_cast<PagedAttentionParams&>(a) = p;
   div_magic(p.page, &a.page_magic, &a.page_shift);
   a.reach = p.table_width * p.page;
   a.window = std::min(p.window, 1 << 30);   // (no place lies further back)
-  a.few_slots = slots_of(p, W::few, most_few_units(p.tokens, p.seqs, p.kv_heads, p.group, !W::kTwo));
-  a.many_slots = W::kTwo ? slots_of(p, W::many, most_many_units(p.tokens, p.seqs, p.kv_heads, p.group)) : 0;
+  a.few_slots = slots_of(p, W::few, units.few);
+  a.many_slots = slots_of(p, W::many, units.many);
+  a.written = std::max(4, (p.tokens + 127) / 128);      // (128 workgroups write a long prompt beside the others)
+  a.writers = p.k != nullptr ? (p.tokens + a.written - 1) / a.written : 0;
   return a;
 }
 template <typename T> Args args_of(const PagedAttentionParams& p) { return p.d > 128 ? args_as<T, true>(p) : args_as<T, false>(p); }
@@ -916,29 +951,33 @@ template <typename T> size_t space_of(const PagedAttentionParams& p) {
   return (size_t)(few.floats() + many.floats() + 4) * sizeof(float);
 }
 
-template <typename T, int DP, bool WHOLE>
+template <typename T, int DP, int DV, bool WHOLE>
 hipError_t attend_with(const Args& a, hipStream_t stream) {
   using W = Ways<T, (DP > 128)>;
-  long long grid = most_few_units(a.tokens, a.seqs, a.kv_heads, a.group, !W::kTwo) + (a.few_slots > 0 ? most_cut_pieces(W::few) : 0);
-  if (W::kTwo) grid += most_many_units(a.tokens, a.seqs, a.kv_heads, a.group) + (a.many_slots > 0 ? most_cut_pieces(W::many) : 0);
+  const Units<T, (DP > 128)> units(a);
+  const long long grid = a.writers + pieces_of(a, W::few, units.few) + pieces_of(a, W::many, units.many);
   static LdsLimit limit;
   if (kLds<T, DP> > 65536) {
-    const hipError_t e = limit.raise(reinterpret_cast<const void*>(&attend_kernel<T, DP, WHOLE>), kLds<T, DP>);
+    const hipError_t e = limit.raise(reinterpret_cast<const void*>(&attend_kernel<T, DP, DV, WHOLE>), kLds<T, DP>);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((attend_kernel<T, DP, WHOLE>), dim3((unsigned)grid), dim3(256), (kLds<T, DP>), stream, a);
+  hipLaunchKernelGGL((attend_kernel<T, DP, DV, WHOLE>), dim3((unsigned)grid), dim3(256), (kLds<T, DP>), stream, a);
   return hipGetLastError();
 }
-template <typename T, int DP>
+template <typename T, int DP, int DV>
 hipError_t attend_wide(const Args& a, hipStream_t stream) {
-  return a.d == DP ? attend_with<T, DP, true>(a, stream) : attend_with<T, DP, false>(a, stream);
+  return a.d == DV ? attend_with<T, DP, DV, true>(a, stream) : attend_with<T, DP, DV, false>(a, stream);
 }
 template <typename T>
 hipError_t attend_as(const PagedAttentionParams& p, hipStream_t stream) {
   const Args a = args_of<T>(p);
-  if (p.d <= 64) return attend_wide<T, 64>(a, stream);
-  if (p.d <= 128) return attend_wide<T, 128>(a, stream);
-  return attend_wide<T, 256>(a, stream);
+  if (p.d <= 64) return attend_wide<T, 64, 64>(a, stream);
+  if constexpr (sizeof(T) == 2) {
+    if (p.d <= 96) return attend_wide<T, 128, 96>(a, stream);
+    if (p.d > 128 && p.d <= 192) return attend_wide<T, 256, 192>(a, stream);
+  }
+  if (p.d <= 128) return attend_wide<T, 128, 128>(a, stream);
+  return attend_wide<T, 256, 256>(a, stream);
 }
 template <typename T>
 hipError_t join_as(const PagedAttentionParams& p, hipStream_t stream) {
@@ -953,11 +992,6 @@ hipError_t join_as(const PagedAttentionParams& p, hipStream_t stream) {
 }  // namespace
 
 size_t paged_attention_space(const PagedAttentionParams& p) { return p.dt == DT_F32 ? space_of<float>(p) : space_of<bf16_t>(p); }
-
-hipError_t launch_cache_write(const PagedAttentionParams& p, hipStream_t stream) {
-  hipLaunchKernelGGL(cache_write_kernel, dim3((unsigned)((p.tokens + 3) / 4)), dim3(256), 0, stream, args_of<float>(p), p.kv_heads * p.d * dtype_size(p.dt));
-  return hipGetLastError();
-}
 
 hipError_t launch_paged_attention(const PagedAttentionParams& p, hipStream_t stream) {
   switch (p.dt) {

@@ -4878,9 +4878,7 @@ void Planner::lower_pagedattention(int ni) {
     return p;
   };
   const std::string& name = n.out->name;
-  if (fresh)
-    emit("attend.write:" + name, {tk, tv, tt, tc, ts}, {tkc, tvc}, [=](const ExecEnv& e, hipStream_t st) { return launch_cache_write(args(e), st); }, kReads16 | kWrites16);
-  emit("attend:" + name, {tq, tkc, tvc, tt, tc, ts}, {tw, ty}, [=](const ExecEnv& e, hipStream_t st) { return launch_paged_attention(args(e), st); }, kReads16 | kWrites16);
+  emit("attend:" + name, {tq, tk, tv, tkc, tvc, tt, tc, ts}, {tkc, tvc, tw, ty}, [=](const ExecEnv& e, hipStream_t st) { return launch_paged_attention(args(e), st); }, kReads16 | kWrites16);
   emit("attend.join:" + name, {tw, tt, tc, ts}, {ty}, [=](const ExecEnv& e, hipStream_t st) { return launch_attention_join(args(e), st); }, kReads16 | kWrites16);
   set_kept(n.out, ty);
 }
