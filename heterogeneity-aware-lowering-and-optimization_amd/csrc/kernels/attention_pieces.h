@@ -60,8 +60,13 @@ OHIP_HD int most_cut_pieces(const Way& w) { return w.target + w.target / 8; }
 OHIP_HD int most_slots(const Way& w) { return 2 * most_cut_pieces(w); }
 
 // Sequences of up to kFewRows rows go in tiles of 16, others in tiles of 128 (16-bit types; fp32: all in tiles of 16).
-constexpr int kFewRows = 32;
-constexpr Way kFew16 = {16, 32, 8, 1024}, kFew32 = {16, 16, 16, 1024}, kMany = {128, 64, 8, 512}, kManyWide = {128, 32, 16, 512};   // (wide: heads above 128)
+// Two tiles of 16 would read the keys twice.  bf16, 8 heads of 128, 24 and 32 rows each, two tiles of 16 against one of 128:
+// 64 sequences of 8192 places 231 and 204 us against 203 and 176, of 512 places 44 and 45 against 30 and 32; 4 sequences of
+// 8192 places 37 and 28 against 28 and 24, of 512 places 14 and 14.5 against 16 and 16.
+// Stretches of at least 256 places: at 512 the last of these take 22 us, at 128 14.5, and the others no less.
+// 512 pieces of 128 rows are two workgroups a CU, 1024 of 16 rows four: at twice that, the 4 sequences of 8192 places take 32 us for 28.
+constexpr int kFewRows = 16;
+constexpr Way kFew16 = {16, 32, 8, 1024}, kFew32 = {16, 16, 16, 1024}, kMany = {128, 64, 4, 512}, kManyWide = {128, 32, 8, 512};   // (wide: heads above 128)
 OHIP_HD bool is_many(const SeqSpan& s, const int group) { return (long long)s.n * group > kFewRows; }
 OHIP_HD long long most_few_units(const int tokens, const int seqs, const int heads, const int group, const bool all) {
   const long long each = at_most(seqs, tokens);

@@ -356,7 +356,9 @@ hipError_t log_probs_as(const LogProbsParams& p, const int parts, hipStream_t st
   // (parts begin at whole groups of eight, so at 16-byte boundaries where rows do)
   const int each = ((p.V + parts - 1) / parts + 7) / 8 * 8;
   const dim3 grid((unsigned)p.rows * parts);
-  // From 1024 rows on every SIMD has one to stream.  4001 x 32000 bf16: 119 us a workgroup a row.
+  // From 1024 rows on every SIMD has one to stream.  bf16, a wavefront a row against a workgroup a row: 512 rows of 4096 logits
+  // 6.2 and 6.7 us, of 32000 18.7 and 12.7, of 128256 58 and 37; 1024 rows 6.1 and 9.1, 20 and 22, 63 and 63; 2048 rows 7.5
+  // and 13.4, 29 and 39, 105 and 123; 4001 rows of 32000 49 and 119.
   if (p.top == 0 && p.rows >= kManyRows) {
     const dim3 waves((unsigned)(p.rows + 3) / 4);
     if (p.V % 8 == 0) hipLaunchKernelGGL((log_probs_stream_kernel<T, true>), waves, dim3(256), 0, stream, p);
