@@ -424,3 +424,29 @@ def test_dynamic_batch(odla, batch):
     b.destroy()
     feeds["kc"].close()
     feeds["vc"].close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("d", [24, 80, 96, 192, 248])
+@pytest.mark.parametrize("junk", [np.nan, np.inf])
+def test_head_sizes_between_the_tiles(odla, kind, d, junk):
+    """Few and many rows; the places that no sequence owns, some of them in the last pages read, hold no number."""
+    announce("paged attention %s heads of %d among %s" % (kind, d, junk))
+    check(odla, Case(kind, [1, 50, 3], [70, 21, 0], 2, 3, d, page=24, seed=d, junk=junk))
+    check(odla, Case(kind, [2, 1], [300, 90], 1, 8, d, page=8, seed=d + 1, window=77, junk=junk))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows", [15, 16, 17, 32, 33, 127, 128, 129])
+@pytest.mark.parametrize("page", [8, 12, 36, 128])
+def test_around_the_tiles_of_rows(odla, kind, rows, page):
+    """Enough keys for several stretches of both ways of cutting."""
+    announce("paged attention %s %d rows, pages of %d" % (kind, rows, page))
+    check(odla, Case(kind, [rows, 1], [701, 1030], 1, 1, 64, page=page, seed=rows))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("window", [0, 150])
+def test_a_long_chunk_behind_a_long_prompt(odla, kind, window):
+    announce("paged attention %s a chunk of 410 behind 1500, window %d" % (kind, window))
+    check(odla, Case(kind, [410], [1500], 1, 4, 128, page=20, seed=window, window=window))
