@@ -767,8 +767,8 @@ __device__ __forceinline__ void attend_many(const Args& a, const Found& f, const
     request_tile<DP, DV, WHOLE>(a, src, smem, here, t_begin * KT, lane, wave);
 #pragma unroll 1
     for (int t = t_begin; t < t_end; ++t) {
-      // this tile has landed, and everybody has left the other buffer
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      // this tile has landed, and everybody has left the other buffer (the barrier alone does not wait for requests into LDS)
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __syncthreads();
       const unsigned long long valid = __ballot(here >= 0), all = KT == 64 ? ~0ull : 0xffffffffull;
       const bool masked = (valid & all) != all || t * KT + KT - 1 > first_last || (a.window != 0 && t * KT <= last_last - a.window);

@@ -450,3 +450,21 @@ def test_around_the_tiles_of_rows(odla, kind, rows, page):
 def test_a_long_chunk_behind_a_long_prompt(odla, kind, window):
     announce("paged attention %s a chunk of 410 behind 1500, window %d" % (kind, window))
     check(odla, Case(kind, [410], [1500], 1, 4, 128, page=20, seed=window, window=window))
+
+
+@pytest.mark.parametrize("kind,d", [("fp16", 96), ("bf16", 128), ("fp32", 64)])
+def test_every_execution_gives_the_same_bits(odla, kind, d):
+    """A chunk whose tiles are many, cut, and as long as the memory is far: what has not landed in LDS yet would show."""
+    announce("paged attention %s, heads of %d, 40 executions" % (kind, d))
+    c = Case(kind, [509] + [1] * 8, [2500] + [600] * 8, 4, 4, d, page=32, seed=d)
+    b = odla.HipBuilder()
+    b.output(c.record(odla, b), "y")
+    s = b.session()
+    feeds = c.feeds(odla)
+    first = s.run(feeds)["y"]
+    again = [np.array_equal(s.run(feeds)["y"], first) for _ in range(40)]
+    s.close()
+    b.destroy()
+    feeds["kc"].close()
+    feeds["vc"].close()
+    assert all(again), again
