@@ -5,7 +5,9 @@
 //
 // (no term of either cancels another, and a nearly certain token keeps its digits).
 //
-// Bound by reading the logits once: a workgroup holds its part of a row - up to 32768 logits - in registers, 32 a thread,
+// Bound by reading the logits once: 256 x 128256 fp32 with 20 alternatives, 131 MB, 29 us and 5 for the join; 4001 x 32000 bf16 without
+// any, 256 MB, 49 us, 5.2 TB/s.  One row of 32000 fp32 logits is one compute unit's: 9 us, two memory latencies and the alternatives.
+// A workgroup holds its part of a row - up to 32768 logits - in registers, 32 a thread,
 // and takes from there the largest, the sums and the alternatives.  Longer rows are several workgroups', whose parts a
 // second launch joins.
 //
@@ -370,6 +372,8 @@ hipError_t log_probs_as(const LogProbsParams& p, const int parts, hipStream_t st
     if (p.top > 0) hipLaunchKernelGGL((log_probs_kernel<T, NT, VECTOR, true>), grid, dim3(NT), 0, stream, p, parts, each);          \
     else hipLaunchKernelGGL((log_probs_kernel<T, NT, VECTOR, false>), grid, dim3(NT), 0, stream, p, parts, each);                   \
   } while (0)
+  // Short rows by 256 threads, of which a compute unit has several workgroups at once.  bf16, 5 alternatives, against 1024 threads: 8192
+  // logits 7.3 and 9.0 us for a row, 8.7 and 11 for 256, 18 and 48 for 2048; 2048 logits 8.0 and 9.4, 9.2 and 11, 20 and 50.
   if (p.V <= kNarrow * kEach) {
     if (p.V % 8 == 0) OHIP_LOG_PROBS(kNarrow, true);
     else OHIP_LOG_PROBS(kNarrow, false);

@@ -9,7 +9,8 @@
 // loaded computation owns everything it needs and compiles like a recorded one.
 //
 // File layout (little endian): "ODLAHIP3", then the sections written by
-// Writer below; every variable-length item is preceded by its 64-bit length;
+// Writer below (nodes of operators with more than two results name the others
+// behind their attributes); every variable-length item is preceded by its 64-bit length;
 // the last eight bytes are the FNV-1a hash of everything before them, so a
 // truncated or damaged file is refused before any of it is interpreted.  What
 // passes the hash is still checked record by record (validate_loaded): shapes,

@@ -938,8 +938,10 @@ odla_values odla_hip_RmsNorm(odla_value input, odla_value residual,
  * may be operands of odla_hip_PagedAttention only, several of them if wanted, and
  * are no outputs; they keep their declared type in every precision mode.  What no
  * new token is written to stays as it was.  Two executions that write the same
- * pages at the same time race; no page may be in two places that one execution
- * writes.
+ * pages at the same time race.  A place of the caches that a new token goes to
+ * belongs to that token alone in one call: it is neither another new token's nor
+ * among the places that another sequence has cached (which may share pages of
+ * their own).
  * Nothing outside the operands is read or written whatever they hold: a page
  * outside 0 .. pages - 1, or a place that the page table does not reach, is
  * neither written nor seen; cached is clamped to 0 .. P * page size and starts to
@@ -949,7 +951,9 @@ odla_values odla_hip_RmsNorm(odla_value input, odla_value residual,
  * Scores, softmax and sums are kept in 32 bits; with 16-bit operands the weights
  * are rounded to their type before they meet the values.  The last bits of a row
  * depend on the sizes of the call; the same operands give the same bits on every
- * run. */
+ * run.  Long page tables need work space for parts of rows in 32 bits, up to 1152
+ * of 128 rows of a head and 2304 of 16: beyond the static scratch's room
+ * odla_hip_ExecuteComputationStatic answers ODLA_MEM_ERROR. */
 odla_value odla_hip_PagedAttention(odla_value query, odla_value key,
                                    odla_value value, odla_value key_cache,
                                    odla_value value_cache,
