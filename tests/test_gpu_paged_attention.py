@@ -468,3 +468,49 @@ def test_every_execution_gives_the_same_bits(odla, kind, d):
     feeds["kc"].close()
     feeds["vc"].close()
     assert all(again), again
+
+
+@pytest.mark.parametrize("new", [[1, 1], [40, 1]])
+def test_caches_of_more_than_4_gib(odla, new):
+    """Pages on both sides of 2 and 4 GiB, read and written."""
+    import ctypes
+    announce("paged attention over caches of 5 GiB, %s new tokens" % new)
+    c = Case("bf16", new, [130, 200], 8, 1, 128, page=64, seed=len(new) + new[0])
+    L, small, pages = odla.load_library(), c.kc.shape[0], 41000
+    each = c.kc[0].nbytes
+    assert (pages - 1) * each > 2 ** 32
+    where = np.array([7, pages - 1, 2 ** 31 // each, 2 ** 31 // each - 1, 2 ** 32 // each, 2 ** 32 // each - 1, pages - 9, 0, 20000, 40000, 3, 33000])[:small]
+    assert len(set(where)) == small
+
+    def large(pages_of):
+        a = odla.DeviceArray.__new__(odla.DeviceArray)
+        a.L, a.shape, a.dtype, a.nbytes, a.ptr = L, (pages,) + pages_of.shape[1:], pages_of.dtype, pages * each, ctypes.c_void_p()
+        assert L.odla_AllocateDeviceMemory(ctypes.byref(a.ptr), a.nbytes) == 0
+        for i, at in enumerate(where):
+            assert L.odla_CopyMemory(ctypes.c_void_p(a.ptr.value + int(at) * each), pages_of[i].ctypes.data_as(ctypes.c_void_p), each, odla.ODLA_MEMCPY_H2D) == 0
+        return a
+
+    def pages_back(a):
+        got = np.empty_like(c.kc)
+        for i, at in enumerate(where):
+            assert L.odla_CopyMemory(got[i].ctypes.data_as(ctypes.c_void_p), ctypes.c_void_p(a.ptr.value + int(at) * each), each, odla.ODLA_MEMCPY_D2H) == 0
+        return got
+
+    want, bound, _, _ = c.want()
+    kc_want, vc_want = c.written()
+    kc, vc = large(c.kc), large(c.vc)
+    b = odla.HipBuilder()
+    kind = odla.BFLOAT16
+    try:
+        arg = lambda n, a: b.arg(n, a.shape, kind)
+        b.output(b.paged_attention(arg("q", c.q), arg("k", c.k), arg("v", c.v), arg("kc", kc), arg("vc", vc), b.arg("pt", c.table.shape, np.int32),
+                                   b.arg("n", (2,), np.int32), b.arg("s", (3,), np.int32), c.scale, 0, "y"), "y")
+        s = b.session()
+        y = s.run({"q": c.q, "k": c.k, "v": c.v, "kc": kc, "vc": vc, "pt": np.where(c.table < 0, -1, where[c.table]).astype(np.int32), "n": c.cached, "s": c.starts})["y"]
+        s.close()
+        assert np.array_equal(pages_back(kc), kc_want) and np.array_equal(pages_back(vc), vc_want)
+    finally:
+        b.destroy()
+        kc.close()
+        vc.close()
+    assert np.all(np.abs(R.values(y, "bf16") - want) <= bound)
