@@ -60,6 +60,21 @@ __device__ __forceinline__ SeqSpan span_of(const Args& a, const int b) {
   const int each = a.starts == nullptr ? a.tokens / a.seqs : 0;
   return seq_span(a.starts != nullptr ? a.starts[b] : b * each, a.starts != nullptr ? a.starts[b + 1] : (b + 1) * each, a.cached[b], a.tokens, a.reach);
 }
+// Spans of sequences b .. b + E - 1; all are requested before the first is looked at.
+template <int E>
+__device__ __forceinline__ void spans_of(const Args& a, const int b, SeqSpan (&s)[E]) {
+  const int each = a.starts == nullptr ? a.tokens / a.seqs : 0;
+  int start[E], next[E], cached[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int i = at_most(b + e, a.seqs - 1);
+    start[e] = a.starts != nullptr ? a.starts[i] : i * each;
+    next[e] = a.starts != nullptr ? a.starts[i + 1] : (i + 1) * each;
+    cached[e] = a.cached[i];
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) s[e] = b + e < a.seqs ? seq_span(start[e], next[e], cached[e], a.tokens, a.reach) : SeqSpan{0, 0, 0, 0};
+}
 __device__ __forceinline__ SeqSpan span_from_lane(const SeqSpan& s, const int lane) {
   return {__builtin_amdgcn_readlane(s.first, lane), __builtin_amdgcn_readlane(s.n, lane), __builtin_amdgcn_readlane(s.cached, lane), __builtin_amdgcn_readlane(s.len, lane)};
 }
@@ -74,42 +89,74 @@ template <typename T, bool WIDE> struct Ways {
 struct Found { int seq, cuts, stretch, tiles, piece0, slot0; bool many; SeqSpan span; };
 constexpr Found kNowhere = {-1, 1, 0, 0, 0, 0, false, {0, 0, 0, 0}};
 // The sequence with piece `key` (or, BY_TOKEN, with the new token `key`), by all lanes of a wavefront together; seq < 0: none.
-// Pieces of the sequences with many rows, which take longest, come first.
-template <typename T, bool WIDE, bool BY_TOKEN>
-__device__ __forceinline__ Found find(const Args& a, const int key) {
+// Pieces of the sequences with many rows, which take longest, come first.  E neighbouring sequences a lane.
+template <typename T, bool WIDE, bool BY_TOKEN, int E>
+__device__ __forceinline__ Found find_by(const Args& a, const int key) {
   using W = Ways<T, WIDE>;
   const int lane = threadIdx.x & 63;
-  SeqSpan s = span_of(a, lane);      // (of the first 64: kept)
-  float work[2] = {0.f, 0.f};        // few, many
-  for (int b0 = 0; b0 < a.seqs; b0 += 64) {
-    const SeqSpan t = b0 == 0 ? s : span_of(a, b0 + lane);
-    const bool many = W::kTwo && is_many(t, a.group);
-    work[0] += wave_sum(many ? 0.f : work_of(t, W::few, a.group, a.kv_heads, a.window));
-    if (W::kTwo) work[1] += wave_sum(many ? work_of(t, W::many, a.group, a.kv_heads, a.window) : 0.f);
+  SeqSpan first[E], t[E];
+  spans_of<E>(a, lane * E, first);      // (kept)
+  float few = 0.f, many = 0.f;
+#pragma unroll 1
+  for (int b0 = 0; b0 < a.seqs; b0 += 64 * E) {
+    if (b0 != 0) spans_of<E>(a, b0 + lane * E, t);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (b0 == 0) t[e] = first[e];
+      if (W::kTwo && is_many(t[e], a.group)) many += work_of(t[e], W::many, a.group, a.kv_heads, a.window);
+      else few += work_of(t[e], W::few, a.group, a.kv_heads, a.window);
+    }
   }
+  const float work[2] = {wave_sum(few), W::kTwo ? wave_sum(many) : 0.f};
   int piece0 = 0;
+#pragma unroll
   for (int way = W::kTwo ? 1 : 0; way >= 0; --way) {
+    if (work[way] == 0.f) continue;      // (every piece has a tile of keys at least)
     const Way w = way ? W::many : W::few;
     const int stretch = stretch_of(work[way], w);
     int slot0 = 0;
-    for (int b0 = 0; b0 < a.seqs; b0 += 64) {
-      const SeqSpan t = b0 == 0 ? s : span_of(a, b0 + lane);
-      const bool mine = !W::kTwo || is_many(t, a.group) == (way == 1);
-      const int cuts = stretches(key_tiles(t, w, a.group, a.window), stretch);
-      const int pieces = mine ? row_tiles(t, w, a.group) * a.kv_heads * cuts : 0, slots = cuts > 1 ? pieces : 0;
-      const int piece_end = piece0 + wave_scan(pieces), slot_end = slot0 + wave_scan(slots);
-      const unsigned long long here = BY_TOKEN ? __ballot(mine && key >= t.first && key < t.first + t.n) : __ballot(key < piece_end);
+#pragma unroll 1
+    for (int b0 = 0; b0 < a.seqs; b0 += 64 * E) {
+      if (b0 != 0) spans_of<E>(a, b0 + lane * E, t);
+      bool mine[E];
+      int cuts[E], pieces[E], slots[E], all_pieces = 0, all_slots = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (b0 == 0) t[e] = first[e];
+        mine[e] = !W::kTwo || is_many(t[e], a.group) == (way == 1);
+        cuts[e] = stretches(key_tiles(t[e], w, a.group, a.window), stretch);
+        pieces[e] = mine[e] ? row_tiles(t[e], w, a.group) * a.kv_heads * cuts[e] : 0;
+        slots[e] = cuts[e] > 1 ? pieces[e] : 0;
+        all_pieces += pieces[e];
+        all_slots += slots[e];
+      }
+      const int piece_end = piece0 + wave_scan(all_pieces), slot_end = slot0 + wave_scan(all_slots);
+      // this lane's sequence with the key, if it has one
+      int piece = piece_end - all_pieces, slot = slot_end - all_slots, which = -1, piece_of = 0, slot_of = 0, cuts_of = 0;
+      SeqSpan span = {0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const bool is = which < 0 && (BY_TOKEN ? mine[e] && key >= t[e].first && key < t[e].first + t[e].n : key < piece + pieces[e]);
+        which = is ? e : which;
+        piece_of = is ? piece : piece_of;
+        slot_of = is ? slot : slot_of;
+        cuts_of = is ? cuts[e] : cuts_of;
+        span = {is ? t[e].first : span.first, is ? t[e].n : span.n, is ? t[e].cached : span.cached, is ? t[e].len : span.len};
+        piece += pieces[e];
+        slot += slots[e];
+      }
+      const unsigned long long here = __ballot(which >= 0);
       if (here != 0) {
         const int at = __builtin_ctzll(here);
         Found f;
-        f.seq = b0 + at;
+        f.seq = b0 + at * E + __builtin_amdgcn_readlane(which, at);
         f.many = way == 1;
-        f.span = span_from_lane(t, at);
-        f.cuts = __builtin_amdgcn_readlane(cuts, at);
+        f.span = span_from_lane(span, at);
+        f.cuts = __builtin_amdgcn_readlane(cuts_of, at);
         f.stretch = stretch;
         f.tiles = row_tiles(f.span, w, a.group);
-        f.piece0 = __builtin_amdgcn_readlane(piece_end - pieces, at);
-        f.slot0 = __builtin_amdgcn_readlane(slot_end - slots, at);
+        f.piece0 = __builtin_amdgcn_readlane(piece_of, at);
+        f.slot0 = __builtin_amdgcn_readlane(slot_of, at);
         return f;
       }
       piece0 = __builtin_amdgcn_readlane(piece_end, 63);
@@ -117,6 +164,10 @@ __device__ __forceinline__ Found find(const Args& a, const int key) {
     }
   }
   return kNowhere;
+}
+template <typename T, bool WIDE, bool BY_TOKEN>
+__device__ __forceinline__ Found find(const Args& a, const int key) {
+  return a.seqs <= 64 ? find_by<T, WIDE, BY_TOKEN, 1>(a, key) : find_by<T, WIDE, BY_TOKEN, 4>(a, key);
 }
 // Pieces of a sequence: heads side by side (their keys are neighbours in memory), then stretches, then tiles of rows from
 // the last one on, which sees the most keys.  Neighbouring workgroups are on different XCDs, and a head's keys lie in few
@@ -164,14 +215,22 @@ __device__ __forceinline__ void write_tokens(const Args& a, const int bytes) {
 #pragma unroll 1
   for (int token = blockIdx.x * a.written + wave; token < end; token += 4) {
     if (seq < 0 || token < s.first || token >= s.first + s.n) {
+      // the last sequence that begins at the token or in front of it: among 64 ranges of all, then among those of one
       seq = -1;
-      for (int b0 = 0; b0 < a.seqs && seq < 0; b0 += 64) {
-        const SeqSpan m = span_of(a, b0 + lane);
-        const unsigned long long here = __ballot(token >= m.first && token < m.first + m.n);
-        if (here != 0) {
-          seq = b0 + __builtin_ctzll(here);
-          s = span_from_lane(m, __builtin_ctzll(here));
-        }
+      int lo = 0, some = a.seqs;
+#pragma unroll 1
+      while (some > 64) {
+        const int step = (some + 63) / 64, at = lane * step;
+        const bool before = at < some && (a.starts != nullptr ? a.starts[lo + at] : (lo + at) * (a.tokens / a.seqs)) <= token;
+        const int skip = at_least(__builtin_popcountll(__ballot(before)) - 1, 0) * step;      // (less than `some`, whatever the starts are)
+        lo += skip;
+        some = at_most(step, some - skip);
+      }
+      const SeqSpan m = span_of(a, lo + lane);
+      const unsigned long long here = __ballot(lane < some && token >= m.first && token < m.first + m.n);
+      if (here != 0) {
+        seq = lo + __builtin_ctzll(here);
+        s = span_from_lane(m, __builtin_ctzll(here));
       }
       if (seq < 0) continue;
     }

@@ -514,3 +514,18 @@ def test_caches_of_more_than_4_gib(odla, new):
         kc.close()
         vc.close()
     assert np.all(np.abs(R.values(y, "bf16") - want) <= bound)
+
+
+@pytest.mark.parametrize("kind,group", [("bf16", 2), ("fp32", 1)])
+@pytest.mark.parametrize("b", [63, 64, 65, 255, 256, 257, 1000, 4200])
+def test_many_sequences(odla, kind, group, b):
+    """More sequences than lanes: single tokens, none, chunks of both ways of cutting, some cut into stretches; then one token each."""
+    announce("paged attention %s of %d sequences" % (kind, b))
+    rng = np.random.default_rng(b)
+    new, cached = np.ones(b, int), rng.integers(0, 30, b)
+    new[rng.random(b) < 0.2] = 0
+    new[rng.integers(0, b, 6)] = 25
+    cached[rng.integers(0, b, 4)] = 1200
+    new[0], new[-1], cached[-1] = 0, 3, 900
+    check(odla, Case(kind, new.tolist(), cached.tolist(), 1, group, 16, page=16, seed=b, tail=2))
+    check(odla, Case(kind, [1] * b, cached.tolist(), 1, group, 16, page=16, seed=b + 1, starts=False))
