@@ -74,7 +74,13 @@ OHIP_HD long long most_few_units(const int tokens, const int seqs, const int hea
   return heads * (all ? each + (long long)tokens * group / 16 : each * (kFewRows / 16));
 }
 OHIP_HD long long most_many_units(const int tokens, const int seqs, const int heads, const int group) {
-  return (long long)tokens * group <= kFewRows ? 0 : heads * (at_most(seqs, tokens) + (long long)tokens * group / 128);
+  const long long rows = (long long)tokens * group, each = at_most(seqs, tokens), with_many = rows / (kFewRows + 1);
+  return heads * ((each < with_many ? each : with_many) + rows / 128);
+}
+// Both ways of 16-bit types together: a sequence has one tile more than whole ones of 128 rows at most.
+OHIP_HD long long most_units(const int tokens, const int seqs, const int heads, const int group) {
+  static_assert(kFewRows == 16, "a sequence of few rows is one tile");
+  return heads * (at_most(seqs, tokens) + (long long)tokens * group / 128);
 }
 
 }  // namespace ohip

@@ -1020,7 +1020,9 @@ template <typename T, int DP, int DV, bool WHOLE>
 hipError_t attend_with(const Args& a, hipStream_t stream) {
   using W = Ways<T, (DP > 128)>;
   const Units<T, (DP > 128)> units(a);
-  const long long grid = a.writers + pieces_of(a, W::few, units.few) + pieces_of(a, W::many, units.many);
+  const long long cuts = pieces_of(a, W::few, units.few) - units.few + pieces_of(a, W::many, units.many) - units.many;
+  const long long tiles = W::kTwo ? std::min(units.few + units.many, most_units(a.tokens, a.seqs, a.kv_heads, a.group)) : units.few;
+  const long long grid = a.writers + tiles + cuts;
   static LdsLimit limit;
   if (kLds<T, DP> > 65536) {
     const hipError_t e = limit.raise(reinterpret_cast<const void*>(&attend_kernel<T, DP, DV, WHOLE>), kLds<T, DP>);

@@ -76,6 +76,9 @@ int main() {
     const Way ways[] = {kFew16, kFew32, kMany, kManyWide};
     SeqSpan spans[42];
     for (int b = 0; b < seqs; ++b) spans[b] = seq_span(starts[b], starts[b + 1], rand() % (reach + 1), tokens, reach);
+    long long both = 0;
+    for (int b = 0; b < seqs; ++b) both += (long long)row_tiles(spans[b], is_many(spans[b], group) ? kMany : kFew16, group) * heads;
+    if (both > most_units(tokens, seqs, heads, group)) { printf("%lld units of both ways\n", both); return 1; }
     for (int k = 0; k < 4; ++k) {
       const Way w = ways[k];
       auto mine = [&](int b) { return k == 1 || is_many(spans[b], group) == (k >= 2); };   // (fp32: all sequences one way)
