@@ -302,7 +302,11 @@ class Planner {
   // elements on the way from where they are bound, recorded or computed.  (Their fp32 tensor is the value's main one
   // and fills no slot: readers of any other kind convert it.)
   bool kept_fp32(const _odla_value* v) const { return v != nullptr && kept_fp32_[v->index] != 0; }
-  static bool reads_fp32(const Node& n, size_t operand) {
+  bool reads_fp32(const Node& n, size_t operand) const {
+    if (n.op == OP_RMSNORM && operand == 2) {      // (the norm takes its weight in its input's type or in fp32, and no other)
+      const DType x = dtype_from_odla(n.in[0]->etype);
+      return x != DT_F32 && x != cdt_;
+    }
     return (n.op == OP_BLOCKGEMM && (operand == 1 || operand == 3)) || (n.op == OP_EXPERTS && (operand == 3 || operand == 5)) ||
            (n.op == OP_SAMPLE && operand >= 1 && operand != 2);
   }
@@ -4815,9 +4819,10 @@ void Planner::lower_rmsnorm(int ni) {
   rp.eps = n.f[0];
   rp.quantize = n.i[0] != 0;
   const int tx = get(x, L_ROWMAJOR, FORM_FLOAT);
-  const int tr = r != nullptr ? get(r, L_ROWMAJOR, FORM_FLOAT) : -1, tw = w != nullptr ? get(w, L_ROWMAJOR, FORM_FLOAT) : -1;
+  const int tr = r != nullptr ? get(r, L_ROWMAJOR, FORM_FLOAT) : -1, tw = w == nullptr ? -1 : reads_fp32(n, 2) && kept_fp32(w) ? get_fp32(w) : get(w, L_ROWMAJOR, FORM_FLOAT);
   rp.dt = T(tx).dt;
   rp.w_dt = tw >= 0 ? T(tw).dt : rp.dt;
+  if (rp.w_dt != DT_F32 && rp.w_dt != rp.dt) fail(ODLA_UNSUPPORTED_DATATYPE, "odla_hip_RmsNorm '%s': input and weight are stored in different types", n.out->name.c_str());
   if (tr >= 0 && T(tr).dt != rp.dt) fail(ODLA_UNSUPPORTED_DATATYPE, "odla_hip_RmsNorm '%s': input and residual are stored in different types", n.out->name.c_str());
   const int ty = new_tensor(rp.quantize ? DT_F8 : rp.dt, L_ROWMAJOR, n.out->shape, 0, SP_ARENA);
   const _odla_value* sum = r == nullptr ? nullptr : rp.quantize ? n.more[0] : n.out2;

@@ -907,7 +907,8 @@ odla_value odla_hip_Sample(odla_value logits, odla_value temperature,
  * epsilon is finite and not negative; a row of zeros with epsilon 0 gives NaN,
  * as the formula does, and so does a row with a NaN.  An infinity gives NaN in its
  * place and zeros beside it; so do, without the NaN, values whose squares add up
- * beyond the range of 32 bits.  The weight is stored as the precision mode says,
+ * beyond the range of 32 bits.  The weight is stored as the precision mode says
+ * (a FLOAT32 one beside an input of a 16-bit type that is not the mode's: as fp32);
  * the scales are kept as fp32 as those of odla_hip_BlockQuantize are. */
 odla_values odla_hip_RmsNorm(odla_value input, odla_value residual,
                              odla_value weight, odla_float32 epsilon,

@@ -171,3 +171,21 @@ def test_rows_do_not_depend_on_their_number(odla):
     one = run_hip(graph(odla, "bf16", (1, 2000), "bf16", True, True), {"x": feeds["x"][7:8], "r": feeds["r"][7:8], "w": feeds["w"]})
     for n in many:
         assert np.array_equal(many[n][7:8], one[n]), n
+
+
+@pytest.mark.parametrize("mode,kind", [({"fp16": True}, "bf16"), ({"bf16": True}, "fp16")])
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("constant", [False, True])
+def test_float32_weight_of_an_input_in_the_other_16_bit_type(odla, mode, kind, quantize, constant):
+    """The mode stores FLOAT32 values in one 16-bit type, the input has the other: the weight stays fp32."""
+    announce("norm of %s rows with a FLOAT32 weight, %s, 8-bit %s, constant %s" % (kind, mode, quantize, constant))
+    for shape in ((3, 384), (2, 1001)):
+        feeds = feeds_of(shape, kind, "fp32", True, shape[1])
+
+        def build(b):
+            names = (["q", "scale"] if quantize else ["y"]) + ["sum"]
+            x, r = (b.arg(n, shape, np_kind(odla, kind)) for n in "xr")
+            w = b.const("w", feeds["w"]) if constant else b.arg("w", shape[-1:])
+            for v, n in zip(b.rms_norm(x, w, r, EPSILON, odla.FLOAT8_E4M3 if quantize else np_kind(odla, kind), names), names):
+                b.output(v, n)
+        check(run_hip(build, feeds, **mode), feeds, kind, "fp32")

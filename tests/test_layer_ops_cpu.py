@@ -220,3 +220,21 @@ def test_dynamic_batch_is_recorded(odla):
     hb.output(hb.log_probs(a, hb.arg("t", (-1,), np.int32), 2)[0], "lp")
     assert hb.plan_summary()["launches"] == 4
     hb.destroy()
+
+
+@pytest.mark.parametrize("mode,kind", [({"fp16": True}, "BFLOAT16"), ({"bf16": True}, np.float16)])
+def test_weight_of_a_norm_whose_input_the_mode_does_not_store(odla, mode, kind):
+    """A FLOAT32 weight beside an input in the other 16-bit type stays fp32: one launch, four bytes an element; beside one in the
+    mode's type it takes two."""
+    room = {}
+    other = {"fp16": np.float16, "bf16": odla.BFLOAT16}[next(iter(mode))]
+    for x_kind in (getattr(odla, kind) if isinstance(kind, str) else kind, other):
+        for constant in (True, False):
+            hb = odla.HipBuilder(**mode)
+            w = hb.const("w", np.ones(3000, np.float32)) if constant else hb.arg("w", (3000,))
+            hb.output(hb.rms_norm(hb.arg("x", (2, 3000), x_kind), w)[0], "y")
+            room[x_kind is other, constant] = hb.plan_summary()
+            hb.destroy()
+    assert room[False, True]["launches"] == room[False, False]["launches"] == room[True, True]["launches"] == 1
+    assert room[True, False]["launches"] == 2           # (the cast of an argument)
+    assert room[False, True]["constant_bytes"] >= 4 * 3000 > room[True, True]["constant_bytes"] >= 2 * 3000
