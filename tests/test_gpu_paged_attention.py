@@ -149,7 +149,7 @@ def test_windows(odla, kind, window):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-def test_many_sequences(odla, kind):
+def test_sequences_of_odd_pages_beyond_a_wavefront(odla, kind):
     """More than a wavefront has lanes, some of them without new tokens."""
     announce("paged attention %s of 150 sequences" % kind)
     rng = np.random.default_rng(4)
