@@ -187,15 +187,24 @@ void drop_graph(_odla_context* ctx) {
 
 constexpr size_t kMaxParkedGraphs = 3;
 
+// Whether executions with the buffers `ext` and `other` have the same caches (true without caches).
+bool same_caches(const Plan& plan, const std::vector<const char*>& ext, const std::vector<const char*>& other) {
+  for (size_t k = 0; k < plan.inputs.size(); ++k)
+    if (plan.inputs[k].caller_only && (k >= other.size() || ext[k] != other[k])) return false;
+  return true;
+}
+
 // The captured launches hold the argument buffers they read in place.  When the
 // caller has bound other buffers, the current graph is set aside and one captured
 // for these buffers comes back, if there is one; otherwise graph_exec stays null and
 // the caller captures.
 void select_graph(_odla_context* ctx, const std::vector<const char*>& ext) {
-  if (ctx->graph_exec == nullptr || ctx->graph_ext == ext) return;
-  ctx->parked_graphs.push_back({ctx->graph_ext, ctx->graph, ctx->graph_exec});
-  ctx->graph = nullptr;
-  ctx->graph_exec = nullptr;
+  if (ctx->graph_exec != nullptr) {
+    if (ctx->graph_ext == ext) return;
+    ctx->parked_graphs.push_back({ctx->graph_ext, ctx->graph, ctx->graph_exec});
+    ctx->graph = nullptr;
+    ctx->graph_exec = nullptr;
+  }
   for (size_t i = 0; i < ctx->parked_graphs.size(); ++i) {
     if (ctx->parked_graphs[i].ext != ext) continue;
     ctx->graph = ctx->parked_graphs[i].graph;
@@ -1060,24 +1069,45 @@ odla_status execute_impl(const odla_context ctx, const odla_compute_mode mode, o
   }
 
   // 2. launch sequence: captured once into a hipGraph, replayed afterwards
-  if (ctx->use_graph && plan.steps.size() >= min_graph_steps()) {
+  bool captured = ctx->use_graph && plan.steps.size() >= min_graph_steps();
+  if (captured) {
     select_graph(ctx, ext);
     // A caller that brings new buffers every time would capture every time: after a few
-    // captures in a row this context goes back to staging copies and one graph.
+    // captures in a row this context goes back to staging copies and one graph.  Caches are not
+    // copied: where they are none that a graph is there for, executions run uncaptured until two in a row
+    // have the same caches.
     constexpr int kCaptureStreakLimit = 8;
     if (ctx->graph_exec != nullptr) {
       ctx->capture_streak = 0;
-    } else if (++ctx->capture_streak > kCaptureStreakLimit && !ctx->in_place_off) {
-      bool any = false;
-      for (const char* p : ext) any = any || p != nullptr;
-      if (any) {
-        OHIP_INFO("odla_ExecuteComputation: %d executions in a row with new device buffers; arguments and results are copied from now on", ctx->capture_streak);
-        ctx->in_place_off = true;
-        drop_graph(ctx);
-        odla_status st2 = stage_inputs(ctx, plan, ctx->arena, &ext, wait);
-        if (st2 != ODLA_SUCCESS) return st2;
+    } else if (ctx->caches_turn || ctx->capture_streak >= kCaptureStreakLimit) {
+      bool same = same_caches(plan, ext, ctx->last_ext);
+      for (const _odla_context::ParkedGraph& g : ctx->parked_graphs) same = same || (!ctx->caches_turn && same_caches(plan, ext, g.ext));
+      if (!same) {
+        if (!ctx->caches_turn)
+          OHIP_INFO("odla_ExecuteComputation: %d executions in a row with new buffers, caches among them; such executions run uncaptured from now on",
+                    ctx->capture_streak + 1);
+        ctx->caches_turn = true;
+        captured = false;
+      } else if (ctx->caches_turn) {
+        ctx->caches_turn = false;
+        ctx->capture_streak = 1;
+      } else if (!ctx->in_place_off) {
+        bool any = false;
+        for (const char* p : ext) any = any || p != nullptr;
+        if (any) {
+          OHIP_INFO("odla_ExecuteComputation: %d executions in a row with new device buffers; arguments and results are copied from now on", ctx->capture_streak + 1);
+          ctx->in_place_off = true;
+          ctx->capture_streak = 0;
+          drop_graph(ctx);
+          odla_status st2 = stage_inputs(ctx, plan, ctx->arena, &ext, wait);
+          if (st2 != ODLA_SUCCESS) return st2;
+        }
       }
+    } else {
+      ++ctx->capture_streak;
     }
+  }
+  if (captured) {
     if (ctx->graph_exec == nullptr) {
       if (hipStreamBeginCapture(ctx->stream, hipStreamCaptureModeThreadLocal) != hipSuccess) {
         OHIP_ERR("odla_ExecuteComputation: hipStreamBeginCapture failed");
@@ -1093,6 +1123,7 @@ odla_status execute_impl(const odla_context ctx, const odla_compute_mode mode, o
       }
       ctx->graph = g;
       ctx->graph_ext = ext;
+      OHIP_DEBUG("odla_ExecuteComputation: %zu launches captured", plan.steps.size());
       if (hipGraphInstantiate(&ctx->graph_exec, g, nullptr, nullptr, 0) != hipSuccess) {
         drop_graph(ctx);
         OHIP_ERR("odla_ExecuteComputation: hipGraphInstantiate failed");
@@ -1104,7 +1135,7 @@ odla_status execute_impl(const odla_context ctx, const odla_compute_mode mode, o
       return ODLA_FAILURE;
     }
   } else {
-    if (ctx->use_graph && !plan.steps.empty() && !ctx->said_uncaptured) {
+    if (ctx->use_graph && plan.steps.size() < min_graph_steps() && !plan.steps.empty() && !ctx->said_uncaptured) {
       ctx->said_uncaptured = true;
       OHIP_INFO("odla_ExecuteComputation: %zu launches per execution run uncaptured (a graph replay costs more than that few)", plan.steps.size());
     }

@@ -296,6 +296,7 @@ struct _odla_context {
   // (see host_stage); made on first use, one per context.
   char* host_stage = nullptr;
   bool host_stage_failed = false;
+  bool caches_turn = false;             // the caller binds other caches every time: no captures for them
   bool in_place_off = false;            // the caller binds new buffers every time: copy instead
   // Graphs captured for other sets of argument buffers (a caller that alternates between a
   // few device buffers replays instead of capturing again); bounded, oldest dropped first.

@@ -529,3 +529,72 @@ def test_many_sequences(odla, kind, group, b):
     new[0], new[-1], cached[-1] = 0, 3, 900
     check(odla, Case(kind, new.tolist(), cached.tolist(), 1, group, 16, page=16, seed=b, tail=2))
     check(odla, Case(kind, [1] * b, cached.tolist(), 1, group, 16, page=16, seed=b + 1, starts=False))
+
+
+class Logged:
+    """The library's messages."""
+
+    def __init__(self, odla):
+        from test_gpu_device_args import capture_log
+        self.L, self.seen = odla.load_library(), []
+        self.keep = capture_log(self.L, self.seen)
+
+    def count(self, part):
+        return sum(part in m for m in self.seen)
+
+    def close(self):
+        self.L.odla_SetLogLevel(2)
+        self.L.odla_SetLogger(None)
+
+
+def run_in_turn(odla, cases, order, new_queries=False):
+    """One context over the caches of `cases` in turn, queries in device memory: a buffer a case, or one an execution."""
+    b = odla.HipBuilder()
+    feeds = [dict(c.feeds(odla), q=odla.DeviceArray(c.q)) for c in cases]
+    b.output(cases[0].record(odla, b), "y")
+    s = b.session()
+    log, wants, extra = Logged(odla), [c.want() for c in cases], []
+    try:
+        for k, i in enumerate(order):
+            f = dict(feeds[i], pt=cases[i].table)
+            if new_queries:
+                extra.append(odla.DeviceArray(cases[i].q))
+                f["q"] = extra[-1]
+            have = R.values(s.run(f)["y"], cases[i].kind)
+            want, bound, _, _ = wants[i]
+            assert np.all(np.abs(have - want) <= bound), (k, i)
+        for c, f in [(cases[i], feeds[i]) for i in sorted(set(order))]:
+            kc, vc = c.written()
+            assert np.array_equal(f["kc"].get(), kc) and np.array_equal(f["vc"].get(), vc)
+        return log
+    finally:
+        log.close()
+        s.close()
+        b.destroy()
+        for a in [a for f in feeds for a in f.values() if isinstance(a, odla.DeviceArray)] + extra:
+            a.close()
+
+
+def test_more_caches_in_turn_than_a_context_keeps_graphs(odla, monkeypatch):
+    """A layer's computation over the caches of sixteen layers: after eight captures in a row executions run uncaptured, and
+    operands are read in place still; with the same caches twice in a row captures are worth their while again."""
+    announce("paged attention over sixteen pairs of caches in turn")
+    monkeypatch.setenv("ODLA_HIP_GRAPH_MIN_STEPS", "1")
+    cases = [Case("bf16", [1, 1, 4], [100, 7, 30], seed=s) for s in range(16)]
+    log = run_in_turn(odla, cases, list(range(16)) * 3)
+    assert log.count("copied from now on") == 0 and log.count("run uncaptured from now on") == 1
+    assert log.count("launches captured") == 8
+    assert log.count("argument 'q' is read in place") == 48
+    log = run_in_turn(odla, cases, list(range(16)) * 2 + [3] * 6 + [5, 3, 3, 5])
+    assert log.count("copied from now on") == 0 and 9 <= log.count("launches captured") <= 11
+
+
+def test_new_operands_over_one_pair_of_caches_are_copied(odla, monkeypatch):
+    """Other queries with every execution, the caches where they were: one graph over copies, as without caches."""
+    announce("paged attention, new queries with every execution")
+    monkeypatch.setenv("ODLA_HIP_GRAPH_MIN_STEPS", "1")
+    cases = [Case("bf16", [1, 1, 4], [100, 7, 30], seed=s) for s in range(2)]
+    for order, graphs in ([0] * 14, 1), ([0, 1] * 9, 2):
+        log = run_in_turn(odla, cases, order, new_queries=True)
+        assert log.count("copied from now on") == 1 and log.count("uncaptured") == 0
+        assert log.count("launches captured") == 8 + graphs
