@@ -310,8 +310,10 @@ __device__ __forceinline__ void load_part(const T* row, const int at, const int 
 }
 
 // A row's weight for a key that it does not see is zero, and zero times an infinite or missing value is none.  Where a
-// tile has such weights, such values leave it; whoever found one looks at all values of its piece once more in the end and adds
-// those to the rows that see them (what else a row's sum holds, and the weight, make no difference then).
+// tile has such weights, such values leave it; whoever found one looks at all values of its piece once more in the end and puts
+// those into the sums of the rows that see them (what else a row's sum holds, and the weight, make no difference then).  So does
+// whoever ends with a sum that is no number: a weight may be too small for its type, and so may the factor that makes up for a
+// larger maximum, and a row gets what it would get from a weight that is not zero, wherever the tiles' edges lie.
 template <typename T> constexpr unsigned kExponent = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, f16_t>::value ? 0x7c00u : 0x7f80u;
 // The largest exponents of a dword's elements so far, and whether one says infinite or missing.
 template <typename T> __device__ __forceinline__ unsigned with_exponents(const unsigned most, const unsigned w) {
@@ -331,29 +333,39 @@ template <typename T> __device__ __forceinline__ unsigned finite_part(const unsi
   if constexpr (sizeof(T) == 4) return (w & m) == m ? 0u : w;
   else return ((w & m) == m ? 0u : w & 0xffffu) | ((w >> 16 & m) == m ? 0u : w & 0xffff0000u);
 }
-// column(i): this lane's columns of its row, N times four; rows_of, row_at: as in the kernels, KT keys a tile.
-template <typename T, int KT, int N, typename RowsOf, typename RowAt, typename Column, typename Add>
-__device__ __forceinline__ void add_odd_values(const Args& a, const Source& src, const int t_begin, const int t_end, const int step, const int last, RowsOf rows_of,
-                                            RowAt row_at, Column column, Add add) {
+// column(i): this lane's columns of its row, N times four; rows_of, row_at: as in the kernels, KT keys a tile; put(i, j, x,
+// clear): the sum of column(i) + j is cleared, then has x added.
+template <typename T, int KT, int N, typename RowsOf, typename RowAt, typename Column, typename Put>
+__device__ __forceinline__ void put_odd_values(const Args& a, const Source& src, const int t_begin, const int t_end, const int step, const int last, RowsOf rows_of,
+                                            RowAt row_at, Column column, Put put) {
 #pragma unroll 1
-  for (int t = t_begin; t < t_end; t += step) {
-    const auto rows_ = rows_of(t);
+  for (int clear = 1; clear >= 0; --clear) {
 #pragma unroll 1
-    for (int k = 0; k < KT; ++k) {
-      const int row = row_at(rows_, t, k), place = t * KT + k;
-      if (row < 0 || place > last || (a.window != 0 && place <= last - a.window)) continue;
-      const T* v = reinterpret_cast<const T*>(src.value(place, row));
+    for (int t = t_begin; t < t_end; t += step) {
+      const auto rows_ = rows_of(t);
+#pragma unroll 1
+      for (int k = 0; k < KT; ++k) {
+        const int row = row_at(rows_, t, k), place = t * KT + k;
+        if (row < 0 || place > last || (a.window != 0 && place <= last - a.window)) continue;
+        const T* v = reinterpret_cast<const T*>(src.value(place, row));
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
+        for (int i = 0; i < N; ++i) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float x = Store<T>::ld(v + (column(i) < a.d ? column(i) + j : 0));      // (behind the head: columns that are not stored)
-          add(i, j, __builtin_isfinite(x) ? 0.f : x);
+          for (int j = 0; j < 4; ++j) {
+            const float x = Store<T>::ld(v + (column(i) < a.d ? column(i) + j : 0));      // (behind the head: columns that are not stored)
+            if (!__builtin_isfinite(x)) put(i, j, x, clear != 0);
+          }
+          asm volatile("" ::: "memory");      // (four at a time: this path is seldom taken and shall take no registers from the others)
         }
       }
     }
   }
 }
+// Whether a row's sums have one that is no number, although its weights' sum is (0 times it is 0 for numbers alone).
+__device__ __forceinline__ bool lost_its_number(const float zeros, const float weights) { return zeros != zeros && weights == weights; }
+// What a part's sums are joined with: its factor, but not zero (the exponential gives zero below 2^-126 in any case), so that what is no
+// number in them remains.
+constexpr float kLeastFactor = 0x1p-126f;
 
 template <typename T, int DP> constexpr int kFewLds = (4 * 16 * (DP + 4) + 2 * 4 * 16) * (int)sizeof(float);
 template <typename T, int DP, bool WHOLE, bool TWO>
@@ -535,13 +547,21 @@ __device__ __forceinline__ void attend_few(const Args& a, const Found& f, const 
     here = next;
   }
 
-  if (odd)
-    add_odd_values<T, KT, VE>(a, src, t_begin + wave, t_end, 4, last, rows_of, row_at, [&](const int n) { return 4 * (g * VE + n); },
-                              [&](const int n, const int j, const float x) { o[(4 * n + j) % VE][(4 * n + j) / VE] += x; });
+  const float own_sum = over_row(l, [](float x, float y) { return x + y; });
+  float zeros = 0.f;
+#pragma unroll
+  for (int e = 0; e < VE; ++e)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) zeros = __builtin_fmaf(o[e][i], 0.f, zeros);
+  if (odd || __any(lost_its_number(zeros, own_sum)))
+    put_odd_values<T, KT, VE>(a, src, t_begin + wave, t_end, 4, last, rows_of, row_at, [&](const int n) { return 4 * (g * VE + n); },
+                              [&](const int n, const int j, const float x, const bool clear) {
+                                const int e = (4 * n + j) % VE, i = (4 * n + j) / VE;
+                                o[e][i] = clear ? 0.f : o[e][i] + x;
+                              });
 
   // ---- the wavefronts' parts
   const int mine = threadIdx.x >> 4, column0 = (threadIdx.x & 15) * VE;
-  const float own_sum = over_row(l, [](float x, float y) { return x + y; });
   if (g == 0) { part_m[wave][l16] = m; part_l[wave][l16] = own_sum; }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -571,7 +591,7 @@ __device__ __forceinline__ void attend_few(const Args& a, const Found& f, const 
     for (int w = 0; w < 4; ++w) {
       const floatx4 x = *reinterpret_cast<const floatx4*>(&part[w][mine][column0 + e]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = factor[w] != 0.f ? __builtin_fmaf(factor[w], x[i], v[i]) : v[i];
+      for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(fmaxf(factor[w], kLeastFactor), x[i], v[i]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = by == 0.f ? 0.f : v[i] * by;
@@ -843,10 +863,15 @@ __device__ __forceinline__ void attend_many(const Args& a, const Found& f, const
       here = next;
     }
   }
-  if (w.odd)
-    add_odd_values<T, KT, DV / 8>(a, src, t_begin, t_end, 1, w.last, rows_of, [](const int rows_, int, const int k) { return __shfl(rows_, k); }, [&](const int n) { return 8 * n + 4 * h; },
-                                  [&](const int n, const int j, const float x) { w.o[n / 4][n % 4 * 4 + j] += x; });
   const float sum = over_halves(w.l, [](float x, float y) { return x + y; });
+  float zeros = 0.f;
+#pragma unroll
+  for (int d = 0; d < DV / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) zeros = __builtin_fmaf(w.o[d][i], 0.f, zeros);
+  if (w.odd || __any(lost_its_number(zeros, sum)))
+    put_odd_values<T, KT, DV / 8>(a, src, t_begin, t_end, 1, w.last, rows_of, [](const int rows_, int, const int k) { return __shfl(rows_, k); }, [&](const int n) { return 8 * n + 4 * h; },
+                                  [&](const int n, const int j, const float x, const bool clear) { w.o[n / 4][n % 4 * 4 + j] = clear ? 0.f : w.o[n / 4][n % 4 * 4 + j] + x; });
   if (wave * 32 + l32 >= rows) return;
   if (f.cuts == 1) {
     T* y = result_row<T>(a, f.span, head, r0 + r);
@@ -949,8 +974,9 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const Args a, const
       // (a part without keys has l = 0 and counts nothing; one whose scores are all NaN has no m, and l is NaN)
       const float factor = l == 0.f ? 0.f : m == -INFINITY ? l : __builtin_amdgcn_exp2f(m - base);
       sum = sum * shrink + wave_sum(l == 0.f ? 0.f : factor * l);
-      v *= shrink;
+      v *= fmaxf(shrink, kLeastFactor);
       most = now;
+      const float least = fmaxf(factor, kLeastFactor);
 #pragma unroll 1
       for (int j0 = 0; j0 < n; j0 += 4 * at_once) {
         floatx4 x[4];
@@ -958,14 +984,14 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const Args a, const
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int j = j0 + k * at_once + sub, part = min(j, n - 1), from = slot_of(f, a.kv_heads, tile, head, c0 + part);
-          by[k] = __shfl(factor, part);
-          if (j >= n || from >= parts.slots) by[k] = 0.f;
+          by[k] = __shfl(least, part);
+          if (j >= n || from >= parts.slots) by[k] = kLeastFactor;      // (the last part once more)
           x[k] = *reinterpret_cast<const floatx4*>(parts.values(min(from, parts.slots - 1), r) + (mine ? col : 0));
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = by[k] != 0.f ? __builtin_fmaf(by[k], x[k][i], v[i]) : v[i];
+          for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(by[k], x[k][i], v[i]);
       }
     }
 #pragma unroll

@@ -947,8 +947,10 @@ odla_values odla_hip_RmsNorm(odla_value input, odla_value residual,
  * outside 0 .. pages - 1, or a place that the page table does not reach, is
  * neither written nor seen; cached is clamped to 0 .. P * page size and starts to
  * 0 .. T (decreasing ones give results without meaning).  Tokens of no sequence, and
- * those that see no place at all, give zeros.  Keys and values in places that a
- * token does not see have no influence, whatever they hold.
+ * those that see no place at all (or have a score of -inf for every one), give
+ * zeros.  Keys and values in places that a token does not see have no influence,
+ * whatever they hold.  An infinite or missing value in a place that a token sees
+ * makes its element of the result infinite or NaN, however small its weight.
  * Scores, softmax and sums are kept in 32 bits; with 16-bit operands the weights
  * are rounded to their type before they meet the values.  The last bits of a row
  * depend on the sizes of the call; the same operands give the same bits on every

@@ -598,3 +598,43 @@ def test_new_operands_over_one_pair_of_caches_are_copied(odla, monkeypatch):
         log = run_in_turn(odla, cases, order, new_queries=True)
         assert log.count("copied from now on") == 1 and log.count("uncaptured") == 0
         assert log.count("launches captured") == 8 + graphs
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new,cached,window", [([1], [100], 0), ([3, 1], [5000, 70], 0), ([1], [40000], 0), ([40], [600], 0), ([150], [200], 0), ([150], [3000], 0),
+                                               ([150], [200], 120), ([5], [300], 90)])
+def test_infinite_values_count_however_small_their_weights(odla, kind, new, cached, window):
+    """With a scale of 30 nearly all weights are too small for 32 bits.  A value that is no number reaches every row that sees it all the same:
+    in tiles that all rows see and in those with a mask, in front of the maximum and behind it, in every part of a row that is cut."""
+    announce("paged attention %s, %s behind %s, window %d, infinite values of no weight" % (kind, new, cached, window))
+    rng = np.random.default_rng(cached[0] + new[0])
+    for bad in (np.inf, -np.inf, np.nan, "both"):
+        c = Case(kind, new, cached, 1, 2, 64, scale=30.0, window=window, seed=7)
+        n, total = new[0], new[0] + cached[0]
+        odd = {}      # column -> {place: value}
+        for column in (0, 7, 34, 63):
+            for value in (np.inf, -np.inf) if bad == "both" else (bad,):
+                place = int(rng.integers(max(0, cached[0] - 80) if window else 0, total))
+                odd.setdefault(column, {})[place] = value
+                bits = R.to_bits(np.full(1, value), kind)[0]
+                if place < cached[0]:
+                    c.vc[c.table[0, place // 16], place % 16, 0, column] = bits
+                else:
+                    c.v[place - cached[0], 0, column] = bits
+        y, _, _ = run(odla, c)
+        with np.errstate(invalid="ignore", over="ignore"):
+            want, bound, _, _ = c.want()
+        have = R.values(y, kind)
+        for column, values in odd.items():
+            for i in range(n):
+                p = cached[0] + i
+                seen = [v for at, v in values.items() if at <= p and (window == 0 or at > p - window)]
+                if not seen:
+                    continue
+                with np.errstate(invalid="ignore"):
+                    total_of = np.sum(seen)
+                for h in range(2):
+                    got = have[i, h, column]
+                    assert got == total_of or (np.isnan(got) and np.isnan(total_of)), (bad, column, i, h, got, total_of)
+                    want[i, h, column], bound[i, h, column], have[i, h, column] = 0, 0, 0
+        assert np.all(np.abs(have - want) <= bound), bad
