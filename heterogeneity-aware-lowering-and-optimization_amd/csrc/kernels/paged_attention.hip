@@ -3,7 +3,8 @@
 // Rows are the queries that share a head of keys: row r of a sequence is query r % group of its token r / group, so that
 // a tile of rows reads each key once for all of them.  Softmax in one pass: per row the running maximum m and
 // the sum l of exp(s - m), and o = sum exp(s - m) v, rescaled when m grows.  m follows the true maximum only when that is 2^8
-// times larger: the sums hold that, and o is seldom rescaled.
+// times larger: the sums hold that, and o is seldom rescaled.  fp16 weights are 2^7 times as large (2^15 at most), l and o with them:
+// what many distant keys add up to is not lost to the type's least number, which is 2^-32 of a row's largest weight then.
 //
 // Lengths are on the device, so the launch cannot be cut to them: every workgroup finds its piece - a tile of rows, a head
 // and a stretch of the keys - from the lengths itself (attention_pieces.h).  Long sequences with few rows are cut
@@ -23,6 +24,7 @@ namespace ohip {
 namespace {
 
 constexpr float kLog2e = 1.44269504f;
+template <typename T> constexpr float kLift = std::is_same<T, f16_t>::value ? 7.f : 0.f;
 
 struct Args : PagedAttentionParams {
   unsigned page_magic; int page_shift;
@@ -509,7 +511,7 @@ __device__ __forceinline__ void attend_few(const Args& a, const Found& f, const 
 #pragma unroll
       for (int e = 0; e < VE; ++e) o[e] *= shrink;
     }
-    const float base = m == -INFINITY ? 0.f : m;
+    const float base = (m == -INFINITY ? 0.f : m) - kLift<T>;
 #pragma unroll
     for (int j = 0; j < KEYS; ++j) {
       p[j] = __builtin_amdgcn_exp2f(p[j] - base);
@@ -740,7 +742,7 @@ __device__ __forceinline__ void big_tile(const Args& a, unsigned char* __restric
 #pragma unroll
       for (int i = 0; i < 16; ++i) w.o[d][i] *= shrink;
   }
-  const float base = w.m == -INFINITY ? 0.f : w.m;
+  const float base = (w.m == -INFINITY ? 0.f : w.m) - kLift<T>;
   uintx4 p[BLOCKS][2];
 #pragma unroll
   for (int b = 0; b < BLOCKS; ++b)

@@ -952,7 +952,8 @@ odla_values odla_hip_RmsNorm(odla_value input, odla_value residual,
  * whatever they hold.  An infinite or missing value in a place that a token sees
  * makes its element of the result infinite or NaN, however small its weight.
  * Scores, softmax and sums are kept in 32 bits; with 16-bit operands the weights
- * are rounded to their type before they meet the values.  The last bits of a row
+ * are rounded to their type before they meet the values (fp16: the least one that
+ * counts is 2^-32 of a row's largest).  The last bits of a row
  * depend on the sizes of the call; the same operands give the same bits on every
  * run.  Long page tables need work space for parts of rows in 32 bits, up to 1152
  * of 128 rows of a head and 2304 of 16: beyond the static scratch's room

@@ -638,3 +638,36 @@ def test_infinite_values_count_however_small_their_weights(odla, kind, new, cach
                     assert got == total_of or (np.isnan(got) and np.isnan(total_of)), (bad, column, i, h, got, total_of)
                     want[i, h, column], bound[i, h, column], have[i, h, column] = 0, 0, 0
         assert np.all(np.abs(have - want) <= bound), bad
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("seqs,new,heads,n", [(1, 8192, 8, 57344), (64, 1, 16, 16384)])
+def test_many_keys_of_little_weight_add_up(odla, kind, seqs, new, heads, n):
+    """A first key of weight 1 whose value is 0, and tens of thousands of weight exp(-17.75) = 2^-25.6 and value 1 behind it in the same piece: they are
+    a thousandth, which is all of the result.  An fp16 weight is off by 2^-25 of 2^7 at most there, all of them by their number times 2^-32."""
+    announce("paged attention %s, %d x %d tokens, %d keys of little weight" % (kind, seqs, new, n))
+    d, page = 8, 64
+    b = odla.HipBuilder()
+    dtype = np_kind(odla, kind)
+    pages = -(-(n + new) // page)
+    k, v = np.zeros((pages, page, heads, d)), np.ones((pages, page, heads, d))
+    k[..., 0] = -17.75
+    k[0, 0], v[0, 0] = 0, 0
+    q = np.zeros((seqs * new, heads, d))
+    q[..., 0] = 1
+    feeds = {"q": R.to_bits(q, kind), "kc": odla.DeviceArray(R.to_bits(k, kind)), "vc": odla.DeviceArray(R.to_bits(v, kind)),
+             "pt": np.tile(np.arange(pages, dtype=np.int32), (seqs, 1)), "n": np.full(seqs, n, np.int32)}      # (the new tokens' keys are there already)
+    h = {x: b.arg(x, feeds[x].shape, np.int32 if x in ("pt", "n") else dtype) for x in feeds}
+    b.output(b.paged_attention(h["q"], None, None, h["kc"], h["vc"], h["pt"], h["n"], scale=1.0, name="y"), "y")
+    s = b.session()
+    have = R.values(s.run(feeds)["y"], kind).reshape(seqs, new, heads * d)
+    s.close()
+    b.destroy()
+    feeds["kc"].close()
+    feeds["vc"].close()
+    keys = n + np.arange(new)[None, :, None]
+    total = 1 + keys * np.exp(-17.75)
+    want = keys * np.exp(-17.75) / total
+    # (exponentials of a distance of 17.75, and sums of as many terms in fp32, each off by 2^-24 of what is there; the weights' and the result's type)
+    bound = (R.EPS[kind] / 2 * (1 if kind == "fp32" else 2) + (4 * 17.75 + 8 + 2 * keys / 32) * L.ULP) * want + R.LEAST[kind] + (keys * 2.0 ** -32 / total if kind == "fp16" else 0)
+    assert np.all(np.abs(have - want) <= bound), np.max(np.abs(have - want) / bound)
