@@ -465,6 +465,10 @@ bool token_op_results(OpKind op, const std::vector<_odla_value*>& in, const int6
         results->push_back({ODLA_FLOAT32, s});
       }
       if (r != nullptr) results->push_back({in[0]->etype, xs});
+      RmsNormParams p;
+      p.rows = rows;
+      p.len = (int)last;
+      if (!rms_norm_fits(p)) return no("operand " + xs.str() + " is too large");
       return true;
     }
     case OP_PAGEDATTENTION: {
@@ -499,6 +503,12 @@ bool token_op_results(OpKind op, const std::vector<_odla_value*>& in, const int6
       if (starts != nullptr && starts->shape.numel() != seqs + 1) return no("starts " + starts->shape.str() + " must have one element more than there are sequences");
       if (starts == nullptr && tokens % seqs != 0) return no("without starts every sequence has the same number of tokens");
       if (attr[0] < 0 || attr[0] > INT32_MAX) return no("window must not be negative");
+      PagedAttentionParams p;
+      p.tokens = (int)tokens; p.seqs = (int)seqs; p.kv_heads = (int)heads; p.group = (int)group; p.d = (int)d;
+      p.page = (int)page; p.pages = (int)pages; p.table_width = (int)table->shape.d[1]; p.window = (int)attr[0];
+      p.k = k;
+      p.dt = dtype_from_odla(in[0]->etype);
+      if (!paged_attention_fits(p)) return no("query " + xs.str() + " is too large for " + std::to_string(seqs) + " sequences");
       results->push_back({in[0]->etype, xs});
       return true;
     }
@@ -509,6 +519,9 @@ bool token_op_results(OpKind op, const std::vector<_odla_value*>& in, const int6
       const int64_t n = t->shape.numel();
       if (n % rows != 0 || n / rows > kMaxTokensPerRow) return no("tokens " + t->shape.str() + " must be 1 .. 64 for every row of the logits " + xs.str());
       if (attr[0] < 0 || attr[0] > last || attr[0] > kMaxAlternatives) return no("top must be 0 .. min(V, 32)");
+      LogProbsParams p;
+      p.rows = (int)rows; p.V = (int)last; p.top = (int)attr[0];
+      if (!log_probs_fits(p)) return no("logits " + xs.str() + " are too large for alternatives");
       Shape lead;
       for (int d = 0; d + 1 < xs.rank; ++d) lead.d[lead.rank++] = xs.d[d];
       Shape top = lead;

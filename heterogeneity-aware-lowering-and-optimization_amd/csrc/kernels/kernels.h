@@ -769,6 +769,7 @@ struct RmsNormParams {
   DType dt = DT_F32, w_dt = DT_F32;
   bool quantize = false;
 };
+bool rms_norm_fits(const RmsNormParams& p);   // (a launch has less than 2^32 lanes)
 hipError_t launch_rms_norm(const RmsNormParams& p, hipStream_t stream);
 
 // Attention of new tokens over a paged cache (see odla_hip_PagedAttention).
@@ -786,6 +787,7 @@ struct PagedAttentionParams {
   DType dt = DT_F32;
 };
 size_t paged_attention_space(const PagedAttentionParams& p);
+bool paged_attention_fits(const PagedAttentionParams& p);
 hipError_t launch_paged_attention(const PagedAttentionParams& p, hipStream_t stream);    // the new keys and values into their pages; y, or parts of it in the work space
 hipError_t launch_attention_join(const PagedAttentionParams& p, hipStream_t stream);     // y from the parts; rows of no sequence zero
 
@@ -802,6 +804,7 @@ struct LogProbsParams {
 };
 int log_probs_parts(const LogProbsParams& p);           // workgroups that share a row
 size_t log_probs_space(const LogProbsParams& p);
+bool log_probs_fits(const LogProbsParams& p);
 hipError_t launch_log_probs(const LogProbsParams& p, hipStream_t stream);
 hipError_t launch_log_probs_join(const LogProbsParams& p, hipStream_t stream);   // where log_probs_parts is above 1
 

@@ -388,6 +388,7 @@ hipError_t log_probs_as(const LogProbsParams& p, const int parts, hipStream_t st
 }  // namespace
 
 int log_probs_parts(const LogProbsParams& p) { return p.top == 0 && p.rows >= kManyRows ? 1 : (p.V + kWide * kEach - 1) / (kWide * kEach); }
+bool log_probs_fits(const LogProbsParams& p) { return p.V <= kNarrow * kEach || (p.top == 0 && p.rows >= kManyRows) || (int64_t)p.rows * log_probs_parts(p) * kWide <= UINT32_MAX; }
 size_t log_probs_space(const LogProbsParams& p) {
   const int parts = log_probs_parts(p);
   return (size_t)(keys_at(p, parts) + (int64_t)p.rows * parts * p.top * (int64_t)sizeof(u64));

@@ -1045,13 +1045,19 @@ template <typename T> size_t space_of(const PagedAttentionParams& p) {
   return (size_t)(few.floats() + many.floats() + 4) * sizeof(float);
 }
 
-template <typename T, int DP, int DV, bool WHOLE>
-hipError_t attend_with(const Args& a, hipStream_t stream) {
-  using W = Ways<T, (DP > 128)>;
-  const Units<T, (DP > 128)> units(a);
+// Workgroups of the launch.
+template <typename T, bool WIDE>
+long long grid_of(const Args& a) {
+  using W = Ways<T, WIDE>;
+  const Units<T, WIDE> units(a);
   const long long cuts = pieces_of(a, W::few, units.few) - units.few + pieces_of(a, W::many, units.many) - units.many;
   const long long tiles = W::kTwo ? std::min(units.few + units.many, most_units(a.tokens, a.seqs, a.kv_heads, a.group)) : units.few;
-  const long long grid = a.writers + tiles + cuts;
+  return a.writers + tiles + cuts;
+}
+
+template <typename T, int DP, int DV, bool WHOLE>
+hipError_t attend_with(const Args& a, hipStream_t stream) {
+  const long long grid = grid_of<T, (DP > 128)>(a);
   static LdsLimit limit;
   if (kLds<T, DP> > 65536) {
     const hipError_t e = limit.raise(reinterpret_cast<const void*>(&attend_kernel<T, DP, DV, WHOLE>), kLds<T, DP>);
@@ -1087,8 +1093,14 @@ hipError_t join_as(const PagedAttentionParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
+template <typename T> bool fits_as(const PagedAttentionParams& p) {
+  const Args a = args_of<T>(p);
+  return (p.d > 128 ? grid_of<T, true>(a) : grid_of<T, false>(a)) * 256 <= UINT32_MAX;
+}
+
 }  // namespace
 
+bool paged_attention_fits(const PagedAttentionParams& p) { return p.dt == DT_F32 ? fits_as<float>(p) : fits_as<bf16_t>(p); }
 size_t paged_attention_space(const PagedAttentionParams& p) { return p.dt == DT_F32 ? space_of<float>(p) : space_of<bf16_t>(p); }
 
 hipError_t launch_paged_attention(const PagedAttentionParams& p, hipStream_t stream) {

@@ -130,6 +130,8 @@ hipError_t norm_of(const RmsNormParams& p, hipStream_t stream) {
 
 }  // namespace
 
+bool rms_norm_fits(const RmsNormParams& p) { return p.rows * (p.len <= 4096 ? 512 : 1024) <= UINT32_MAX; }
+
 hipError_t launch_rms_norm(const RmsNormParams& p, hipStream_t stream) {
   switch (p.dt) {
     case DT_F32: return norm_of<float>(p, stream);

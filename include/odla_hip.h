@@ -909,7 +909,8 @@ odla_value odla_hip_Sample(odla_value logits, odla_value temperature,
  * place and zeros beside it; so do, without the NaN, values whose squares add up
  * beyond the range of 32 bits.  The weight is stored as the precision mode says
  * (a FLOAT32 one beside an input of a 16-bit type that is not the mode's: as fp32);
- * the scales are kept as fp32 as those of odla_hip_BlockQuantize are. */
+ * the scales are kept as fp32 as those of odla_hip_BlockQuantize are.
+ * At most 65535 * 128 rows, and less than 2^22 of more than 4096 elements. */
 odla_values odla_hip_RmsNorm(odla_value input, odla_value residual,
                              odla_value weight, odla_float32 epsilon,
                              odla_element_type result_type,
@@ -931,7 +932,8 @@ odla_values odla_hip_RmsNorm(odla_value input, odla_value residual,
  *   window > 0 over the last `window` of them alone.
  * The result has the shape and type of the query; all float operands are of one
  * type.  D is a multiple of 8 up to 256, a page may have any size, B <= 65536,
- * P * page size <= 2^30, pages * page size < 2^31.
+ * P * page size <= 2^30, pages * page size < 2^31, and B * H together with T * Hq / 128
+ * (FLOAT32: T * Hq / 16) must stay below 2^24 or so: the call is refused if not.
  * key and value may both be null: the new tokens' own are in the caches already
  * (written by another operator of the computation, or by an earlier call).
  * The caches are extended where the caller has them: both are bound to 16-byte
@@ -966,7 +968,9 @@ odla_value odla_hip_PagedAttention(odla_value query, odla_value key,
                                    odla_uint32 window,
                                    const odla_value_id value_id);
 /* Log probabilities of given tokens, with the entropy and the best alternatives,
- * for every row of `logits` [.., V], V <= 524288:
+ * for every row of `logits` [.., V], V <= 524288, at most 65535 * 128 rows (with
+ * alternatives less than 2^22 of more than 8192 logits, half of that from 32769 on,
+ * and so forth):
  *   log p_i = l_i - log sum_j exp(l_j),   entropy = - sum_i p_i log p_i.
  * tokens: INT32, n = 1 .. 64 for every row (its element count is n times the
  * rows).  Results: log p of the tokens, FLOAT32 in their shape; the entropies,

@@ -238,3 +238,31 @@ def test_weight_of_a_norm_whose_input_the_mode_does_not_store(odla, mode, kind):
     assert room[False, True]["launches"] == room[False, False]["launches"] == room[True, True]["launches"] == 1
     assert room[True, False]["launches"] == 2           # (the cast of an argument)
     assert room[False, True]["constant_bytes"] >= 4 * 3000 > room[True, True]["constant_bytes"] >= 2 * 3000
+
+
+def test_calls_that_no_launch_has_room_for_are_refused(odla):
+    """A launch has less than 2^32 lanes: both sides of where the operators' launches reach that."""
+    hb = odla.HipBuilder()
+    hb.L.odla_SetLogLevel(0)
+    try:
+        bf16, n = odla.BFLOAT16, [0]
+
+        def arg(shape, kind=bf16):
+            n[0] += 1
+            return hb.arg("a%d" % n[0], shape, kind)
+
+        for rows, k, fits in ((65535 * 128, 4096, True), (2 ** 22 - 1, 4097, True), (2 ** 22, 4097, False)):
+            call = lambda: hb.rms_norm(arg((rows, k)))
+            call() if fits else refused(odla, call)
+        for rows, v, top, fits in ((65535 * 128, 8192, 1, True), (2 ** 22 - 1, 8193, 1, True), (2 ** 22, 8193, 1, False), (2 ** 22, 8193, 0, True),
+                                   (2 ** 21 - 1, 32769, 1, True), (2 ** 21, 32769, 1, False)):
+            call = lambda: hb.log_probs(arg((rows, v)), arg((rows,), np.int32), top)
+            call() if fits else refused(odla, call)
+        for seqs, heads, group, kind, fits in ((250, 65535, 1, bf16, True), (257, 65535, 1, bf16, False), (4000, 1000, 60, bf16, True), (4000, 1000, 70, np.float32, False)):
+            rows = lambda: arg((seqs, heads * 8), kind)
+            cache = lambda: arg((seqs, 1, heads, 8), kind)
+            call = lambda: hb.paged_attention(arg((seqs, heads * group * 8), kind), rows(), rows(), cache(), cache(), arg((seqs, 1), np.int32), arg((seqs,), np.int32))
+            call() if fits else refused(odla, call)
+    finally:
+        hb.L.odla_SetLogLevel(2)
+        hb.destroy()
