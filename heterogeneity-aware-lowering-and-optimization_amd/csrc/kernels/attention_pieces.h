@@ -51,7 +51,10 @@ OHIP_HD int key_tiles(const SeqSpan& s, const Way& w, const int group, const int
 OHIP_HD float work_of(const SeqSpan& s, const Way& w, const int group, const int heads, const int window) {
   return (float)row_tiles(s, w, group) * (float)heads * (float)key_tiles(s, w, group, window);
 }
-OHIP_HD int stretch_of(const float work, const Way& w) { return at_least((int)(work / (float)w.target) + 1, w.least); }
+OHIP_HD int stretch_of(const float work, const Way& w) {
+  const float each = work / (float)w.target;
+  return at_least((int)(each < 0x1p30f ? each : 0x1p30f) + 1, w.least);      // (no row has more tiles than that)
+}
 OHIP_HD int stretches(const int tiles, const int stretch) { return tiles > 0 ? (tiles - 1) / stretch + 1 : 1; }
 // Bounds over all calls of one size: pieces that come from cutting, and pieces of tiles that are cut (their parts have
 // a slot each).  (Cut: a tile of k > stretch key tiles gives at most 2 k / stretch parts.  An eighth on top: the work

@@ -106,6 +106,33 @@ int main() {
 }
 """
 
+FAR = r"""
+#include "attention_pieces.h"
+#include <cstdio>
+#include <initializer_list>
+using namespace ohip;
+int main() {
+  // the longest sequences that can be: lengths that make no sense are clamped to them
+  for (int tokens : {1, 1 << 10, 1 << 20, (1 << 25) - 1})
+    for (int heads : {1, 8, 32})
+      for (int seqs : {1, 3, 1000}) {
+        const int reach = 1 << 30;
+        const Way ways[] = {kFew16, kFew32, kMany, kManyWide};
+        for (int k = 0; k < 4; ++k) {
+          float work = 0.f;
+          const SeqSpan s = seq_span(0, 2147483647, 2147483647, tokens, reach);     // (every sequence has all tokens)
+          for (int b = 0; b < seqs; ++b) work += work_of(s, ways[k], 1, heads, 0);
+          const int stretch = stretch_of(work, ways[k]), tiles = key_tiles(s, ways[k], 1, 0), cuts = stretches(tiles, stretch);
+          const long long own = (long long)row_tiles(s, ways[k], 1) * heads, pieces = own * cuts * seqs;
+          if (stretch < ways[k].least || cuts < 1 || (cuts > 1 && pieces > most_slots(ways[k])) || pieces > own * seqs + most_cut_pieces(ways[k])) {
+            printf("way %d, %d x %d tokens, %d heads: stretch %d of %d tiles, %lld pieces\n", k, seqs, tokens, heads, stretch, tiles, pieces);
+            return 1;
+          }
+        }
+      }
+  return 0;
+}
+"""
 
 def test_what_rows_see(tmp_path):
     run_on_host(tmp_path, KEYS)
@@ -113,3 +140,7 @@ def test_what_rows_see(tmp_path):
 
 def test_pieces_and_slots_stay_within_their_bounds(tmp_path):
     run_on_host(tmp_path, PIECES)
+
+
+def test_lengths_without_sense_cut_nothing_short(tmp_path):
+    run_on_host(tmp_path, FAR)
