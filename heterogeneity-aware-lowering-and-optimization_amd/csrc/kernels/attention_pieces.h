@@ -67,8 +67,9 @@ OHIP_HD int most_slots(const Way& w) { return 2 * most_cut_pieces(w); }
 // 64 sequences of 8192 places 231 and 204 us against 203 and 176, of 512 places 44 and 45 against 30 and 32; 4 sequences of
 // 8192 places 37 and 28 against 28 and 24, of 512 places 14 and 14.5 against 16 and 16.
 // Stretches of at least 256 places: at 512 the last of these take 22 us, at 128 14.5, and the others no less.
-// 512 pieces of 128 rows are two workgroups a CU, 1024 of 16 rows four.  A chunk of 509 tokens, 4 x 4 heads of 96, behind 6000 places
-// beside 16 single tokens: 58, 53, 49 and 56 us with 256, 384, 512 and 640 pieces.
+// 512 pieces of 128 rows are two workgroups a CU, 1024 of 16 rows four.  256, 384, 512, 640 and 1024 pieces: a chunk of 509 tokens, 4 x 4
+// heads of 96, behind 6000 places beside 16 single tokens 53, 50, 48, 54 and 52 us; four chunks of up to 300, 2 x 8 heads of 64, behind
+// 8000 40, 33, 28, 32 and 33; 700 tokens, 8 x 4 heads of 128, behind 12000 beside 8 single ones 314, 251, 261, 237 and 241.
 constexpr int kFewRows = 16;
 constexpr Way kFew16 = {16, 32, 8, 1024}, kFew32 = {16, 16, 16, 1024}, kMany = {128, 64, 4, 512}, kManyWide = {128, 32, 8, 512};   // (wide: heads above 128)
 OHIP_HD bool is_many(const SeqSpan& s, const int group) { return (long long)s.n * group > kFewRows; }

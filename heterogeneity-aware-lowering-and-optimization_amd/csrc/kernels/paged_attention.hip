@@ -11,10 +11,10 @@
 // into stretches, so that there are about a thousand pieces; a stretch leaves m, l and o in fp32, and
 // a last launch joins them in the order of the stretches.
 //
-// Few rows are bound by reading the cache: 48 sequences of up to 16384 places, 8 heads of 128 for 8 queries each, bf16, 0.9 GB, 172 - 177 us
-// and 6 for the join, 5.2 TB/s (a plain read of so much reaches 6.1 - 6.8); one of 4096 places 8.5 and 5.5 us, latency.  Many
+// Few rows are bound by reading the cache: 48 sequences of up to 16384 places, 8 heads of 128 for 8 queries each, bf16, 0.9 GB, 175 us
+// and 6 for the join, 5.2 TB/s (a plain read of so much reaches 6.1 - 6.8); one of 4096 places 9.4 and 5.6 us, latency.  Many
 // rows are bound by the matrix cores and by what is done between their products: a prompt of 8192 tokens, 32 heads of 128, bf16,
-// 0.55 TFLOP, 0.67 - 0.78 ms, 700 - 820 TFLOP/s where a library product of 8192^3 reaches 1137.
+// 0.55 TFLOP, 0.66 ms, 840 TFLOP/s where a library product of 8192^3 reaches 1137.
 #include "block_common.h"
 #include "attention_pieces.h"
 

@@ -4,7 +4,7 @@
 //   s = x + r,   y = s / sqrt(mean s^2 + eps) * w,   q = e4m3(y / scale),  scale = max(max |y| / 448, 2^-126)
 //
 // Bound by memory: every operand is read and every result written once.  bf16, residual, 8-bit result: 8192 rows of 7168 values, 415 MB,
-// 85 us, 4.9 TB/s (a copy of 1 GiB 5.1); one row of 4096 values 3 us, of which a launch is 2.  A row stays in its workgroup's registers
+// 86 us, 4.8 TB/s (a copy of 1 GiB 5.1); one row of 4096 values 3 us, of which a launch is 2.  A row stays in its workgroup's registers
 // between the sum of its squares and its results, eight neighbouring values a lane, so that sixteen lanes hold a block.
 // Squares, their sum and y are fp32; s is rounded on its way out alone, so that y is not twice rounded.
 #include "block_common.h"
